@@ -368,6 +368,77 @@ int wl_layer_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, int32_t T,
 int wl_layer_batch_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, int32_t N, const int32_t *pos,
                        const int32_t *slot, int32_t slots, int32_t slot_positions, uint16_t *d_K, uint16_t *d_V);
 
+/* ---- The KV cache in 4 bits, attention over a window, sampling (no counterpart in the reference, whose
+ * cache is fp16, whose rows see every position; Sampler's draw is src/Engine.cs:353-382) ----
+ * For long contexts: a position's key and value take 9/32 of the fp16 cache's bytes, and a row may
+ * see a window of the last positions and a few first ones only. Stream-ordered on the context like
+ * the other _dev entries; row positions and sampling settings given in host arrays travel as kernel
+ * arguments, so the arrays may change on return and a capture records their values. With no rows the
+ * rows' pointers may be null.
+ *
+ * The 4-bit cache. Keys and values in two buffers of wl_kv4_bytes each, 16-byte aligned, which the caller
+ * owns (a pool of slots: that many bytes per slot, one after the other). Blocks of 32 consecutive values of a
+ * head's row hold a scale d and sixteen levels, the values (n - 8) d, n = 0..15: d = -m / 8 for m the
+ * value of largest magnitude (the first of several), rounded to 8 significant bits and to a multiple
+ * of 2^-24, |d| at most 2720; n = round to nearest even of x / d, plus 8, held to 0..15. A block with an
+ * infinity or NaN holds NaN. Per KV head, tiles of 32 positions of 18 * head_dim bytes follow each other
+ * (their inner order: windlass_amd/csrc/wl_kv4.h). head_dim is 64 or 128; other head dims are
+ * refused with WL_E_UNSUPPORTED.
+ *
+ * The window. A row at position p sees the positions j <= p with j < sinks or j > p - window; all j <= p when
+ * window is 0 (sinks is then not read). */
+
+/* Bytes of one 4-bit cache (keys or values) of `positions` positions; 0 for a shape it cannot hold. */
+int64_t wl_kv4_bytes(int32_t positions, int32_t kv_heads, int32_t head_dim);
+
+/* wl_kv_store_dev into 4-bit caches of `positions` positions: d_k, d_v [T][kv_heads * head_dim] (fp32) to
+ * positions pos0 .. pos0 + T - 1. */
+int wl_kv4_store_dev(wl_ctx *ctx, const float *d_k, const float *d_v, int32_t T, int32_t kv_heads, int32_t head_dim,
+                     void *d_K, void *d_V, int32_t positions, int32_t pos0);
+
+/* The same for N rows, row i to position pos[i] of cache slot slot[i] (host arrays, checked as
+ * wl_layer_batch_dev does). */
+int wl_kv4_store_batch_dev(wl_ctx *ctx, const float *d_k, const float *d_v, int32_t N, int32_t kv_heads,
+                           int32_t head_dim, void *d_K, void *d_V, const int32_t *pos, const int32_t *slot,
+                           int32_t slots, int32_t slot_positions);
+
+/* The values that positions pos0 .. pos0 + T - 1 of 4-bit caches hold: d_k, d_v [T][kv_heads * head_dim]. */
+int wl_kv4_read_dev(wl_ctx *ctx, const void *d_K, const void *d_V, int32_t positions, int32_t kv_heads,
+                    int32_t head_dim, int32_t pos0, int32_t T, float *d_k, float *d_v);
+
+/* wl_attention_dev over 4-bit caches of `positions` positions, with a window: d_q, d_out
+ * [T][heads * head_dim], row t at position pos0 + t. */
+int wl_kv4_attention_dev(wl_ctx *ctx, const float *d_q, int32_t T, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                         const void *d_K, const void *d_V, int32_t positions, int32_t pos0, int32_t window,
+                         int32_t sinks, float scale, float *d_out);
+
+/* The same for N rows, row i at position pos[i] of cache slot slot[i] (host arrays, checked). A row's bits do
+ * not depend on the other rows, and equal wl_kv4_attention_dev of that row alone. */
+int wl_kv4_attention_batch_dev(wl_ctx *ctx, const float *d_q, int32_t N, int32_t heads, int32_t kv_heads,
+                               int32_t head_dim, const void *d_K, const void *d_V, const int32_t *pos,
+                               const int32_t *slot, int32_t slots, int32_t slot_positions, int32_t window,
+                               int32_t sinks, float scale, float *d_out);
+
+/* wl_attention_dev (fp16 caches) with a window; any head dim. */
+int wl_attention_window_dev(wl_ctx *ctx, const float *d_q, int32_t T, int32_t heads, int32_t kv_heads,
+                            int32_t head_dim, const uint16_t *d_K, const uint16_t *d_V, int32_t pos0, int32_t window,
+                            int32_t sinks, float scale, float *d_out);
+
+/* The next token of each of `rows` rows of n logits (at most 2^24), drawn with the settings params[row]
+ * (host) and the number d_u[row] in [0, 1) (device). Tokens in order (larger logit first, of equals the
+ * lower id) with weights exp((logit - max) / temperature): the first top_k stay (0: all), of those the
+ * shortest prefix with at least top_p of their weight (1: all), of those the ones of weight at least
+ * min_p (the largest has 1); d_out[row] is the first at which the weight summed in that order passes d_u[row]
+ * times what stayed. temperature 0 is wl_argmax_dev's pick. NaN logits are never drawn; a row without
+ * a logit above -inf gives 0. Weights are formed in double and summed exactly. */
+typedef struct wl_sample_params {
+  float temperature; /* >= 0 */
+  int32_t top_k;     /* >= 0 */
+  float top_p, min_p; /* 0 .. 1 */
+} wl_sample_params;
+int wl_sample_dev(wl_ctx *ctx, const float *d_logits, int32_t rows, int64_t n, const wl_sample_params *params,
+                  const float *d_u, int32_t *d_out);
+
 /* ---- Allocation-free product (no counterpart in the reference) ----
  * For callers that cannot allocate device memory: code under HIP graph capture, tight serving
  * loops, harnesses that forbid hipMalloc. The same operation and results as wl_matmul_dev (bit

@@ -1,0 +1,337 @@
+"""The KV cache in 4 bits (wl_kv4_store_dev, _batch_dev, wl_kv4_read_dev), the attention that reads it
+(wl_kv4_attention_dev, _batch_dev) and attention over fp16 caches with a window
+(wl_attention_window_dev), against restatements in 64 bits (long_ref.py).
+
+What the cache holds is compared bit for bit. Attention's bound is long_ref's: what rounding in 32
+bits may be off, from the sizes of the scores and values."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from layer_ref import to_half_ref
+from long_ref import attention_span_ref, held_ref
+from windlass_amd._lib import check, load
+from windlass_amd.backend import Context
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+DEV = torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = Context(0)
+    yield c
+    c.close()
+
+
+def P(t):
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def dev(a):
+    t = torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+    torch.cuda.synchronize()  # the library's stream does not wait for torch's
+    return t
+
+
+def host(ctx, t):
+    ctx.sync()
+    return t.cpu().numpy()
+
+
+class Cache:
+    """4-bit caches of `slots` sequences, filled with a pattern that reads as NaN until rows are stored."""
+
+    def __init__(self, ctx, positions, KH, HD, slots=1):
+        self.ctx, self.n, self.KH, self.HD = ctx, positions, KH, HD
+        b = load().wl_kv4_bytes(positions, KH, HD)
+        assert b == KH * -(-positions // 32) * 18 * HD
+        self.K = torch.full((slots, b), 0xff, dtype=torch.uint8, device=DEV)
+        self.V = torch.full((slots, b), 0xff, dtype=torch.uint8, device=DEV)
+        torch.cuda.synchronize()
+
+    def store(self, k, v, pos0, slot=0):
+        dk, dv = dev(k), dev(v)
+        check(load().wl_kv4_store_dev(self.ctx.handle, P(dk), P(dv), len(k), self.KH, self.HD, P(self.K[slot]),
+                                      P(self.V[slot]), self.n, pos0))
+        self.ctx.sync()
+
+    def read(self, pos0, T, slot=0):
+        out = [torch.full((T, self.KH, self.HD), 7.0, device=DEV) for _ in range(2)]
+        torch.cuda.synchronize()
+        check(load().wl_kv4_read_dev(self.ctx.handle, P(self.K[slot]), P(self.V[slot]), self.n, self.KH, self.HD, pos0, T,
+                                     P(out[0]), P(out[1])))
+        return [host(self.ctx, t) for t in out]
+
+    def attention(self, q, pos0, window=0, sinks=0, scale=None, slot=0):
+        dq = dev(q)
+        out = torch.full(q.shape, 7.0, device=DEV)
+        torch.cuda.synchronize()
+        check(load().wl_kv4_attention_dev(self.ctx.handle, P(dq), q.shape[0], q.shape[1], self.KH, self.HD,
+                                          P(self.K[slot]), P(self.V[slot]), self.n, pos0, window, sinks,
+                                          scale or 1 / math.sqrt(self.HD), P(out)))
+        return host(self.ctx, out)
+
+
+def rows(rng, n, KH, HD):
+    x = rng.standard_normal((n, KH, HD), dtype=F32)
+    x[:, rng.random((KH, HD)) < 0.03] *= F32(6)
+    return x
+
+
+def bits(a):
+    return np.ascontiguousarray(a, F32).view(np.uint32)
+
+
+@pytest.mark.parametrize("KH,HD", [(1, 64), (3, 64), (8, 128), (5, 128)])
+@pytest.mark.parametrize("T,pos0,positions", [(1, 0, 1), (1, 31, 33), (70, 0, 70), (37, 29, 66), (33, 95, 200)])
+def test_store_holds_the_nearest_values(ctx, KH, HD, T, pos0, positions):
+    rng = np.random.default_rng(T * HD + KH)
+    k, v = rows(rng, T, KH, HD), rows(rng, T, KH, HD)
+    c = Cache(ctx, positions, KH, HD)
+    c.store(k, v, pos0)
+    gk, gv = c.read(pos0, T)
+    assert np.array_equal(gk, held_ref(k)) and np.array_equal(gv, held_ref(v))
+
+
+def test_blocks_of_every_size_and_kind(ctx):
+    KH, HD = 2, 64
+    rng = np.random.default_rng(5)
+    r = []
+    for e in range(-40, 18):  # largest values from below the smallest scale to past the largest
+        r.append(rng.standard_normal((KH, HD)).astype(F32) * F32(2.0 ** e))
+    x = np.stack(r)
+    x[3, 0, :32] = 0                                  # a block of zeros
+    x[4, 0, :32] = F32(-0.0)
+    x[5, 0, :32] = F32(1.25)                          # equal values
+    x[6, 0, :32] = np.where(np.arange(32) % 2, 3, -3)  # equal magnitudes: the first one's sign
+    x[7, 0, :32] = np.where(np.arange(32) < 17, 0, np.where(np.arange(32) % 2, 5, -5))
+    x[8, 0, :32] = np.arange(32) - 15.5               # ties of the rounding
+    x[9, 0, :32] = (np.arange(32) - 16) / 2
+    x[10, 1, 32:] = 1e30                              # past the largest scale
+    x[11, 1, 32:] = np.linspace(-21760, 21760, 32)
+    x[12, 0, 5] = np.inf
+    x[13, 1, 40] = np.nan
+    x[14, 1, 63] = -np.inf
+    x[15, 0, :32] = F32(1e-45)
+    c = Cache(ctx, len(x), KH, HD)
+    c.store(x, x[::-1], 0)
+    gk, gv = c.read(0, len(x))
+    assert np.array_equal(gk, held_ref(x), equal_nan=True)
+    assert np.array_equal(gv, held_ref(x[::-1]), equal_nan=True)
+    assert np.isnan(gk[12, 0, :32]).all() and np.isfinite(gk[12, 0, 32:]).all()
+
+
+def test_store_leaves_other_positions_as_they_were(ctx):
+    KH, HD, n = 2, 128, 100
+    rng = np.random.default_rng(9)
+    c = Cache(ctx, n, KH, HD)
+    k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+    c.store(k, v, 0)
+    before = c.read(0, n)
+    k2, v2 = rows(rng, 7, KH, HD), rows(rng, 7, KH, HD)
+    c.store(k2, v2, 61)
+    after = c.read(0, n)
+    for b, a, new in zip(before, after, (k2, v2)):
+        assert np.array_equal(a[:61], b[:61]) and np.array_equal(a[68:], b[68:]) and np.array_equal(a[61:68], held_ref(new))
+    raw = c.K.cpu().clone()
+    c.store(k2[:0], v2[:0], 61)  # no rows
+    assert torch.equal(raw, c.K.cpu())
+
+
+def test_batch_store_equals_single_stores(ctx):
+    KH, HD, slots, cap, N = 2, 64, 90, 70, 81  # more rows than one launch takes
+    rng = np.random.default_rng(2)
+    one, many = Cache(ctx, cap, KH, HD, slots), Cache(ctx, cap, KH, HD, slots)
+    k, v = rows(rng, N, KH, HD), rows(rng, N, KH, HD)
+    slot = rng.permutation(slots)[:N].astype(np.int32)
+    pos = rng.integers(0, cap, N).astype(np.int32)
+    dk, dv = dev(k), dev(v)
+    check(load().wl_kv4_store_batch_dev(ctx.handle, P(dk), P(dv), N, KH, HD, P(many.K), P(many.V),
+                                        pos.ctypes.data, slot.ctypes.data, slots, cap))
+    for i in range(N):
+        one.store(k[i:i + 1], v[i:i + 1], int(pos[i]), int(slot[i]))
+    ctx.sync()
+    assert torch.equal(one.K, many.K) and torch.equal(one.V, many.V)
+
+
+# rows of one call, positions before them; head counts from one per KV head to more than a wave's columns
+SHAPES = [(8, 2, 64), (8, 8, 128), (28, 4, 128), (64, 8, 128), (20, 1, 64), (5, 1, 128)]
+
+
+def kv4_case(ctx, rng, T, pos0, H, KH, HD, window, sinks, qscale=2.0):
+    n = pos0 + T
+    c = Cache(ctx, n + 5, KH, HD)  # positions past the last are never written
+    k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+    c.store(k, v, 0)
+    q = rng.standard_normal((T, H, HD), dtype=F32) * F32(qscale)
+    got = c.attention(q, pos0, window, sinks)
+    want, tol = attention_span_ref(q, held_ref(k), held_ref(v), pos0 + np.arange(T), window, sinks, 1 / math.sqrt(HD))
+    err = np.abs(got - want)
+    assert (err <= tol).all(), "worst %.3g of its bound" % float((err / tol).max())
+
+
+@pytest.mark.parametrize("H,KH,HD", SHAPES)
+@pytest.mark.parametrize("T,pos0", [(1, 0), (1, 1), (1, 31), (1, 32), (1, 700), (2, 0), (7, 333), (15, 64)])
+def test_kv4_attention_few_rows(ctx, H, KH, HD, T, pos0):
+    kv4_case(ctx, np.random.default_rng(T + pos0 + H), T, pos0, H, KH, HD, 0, 0)
+
+
+@pytest.mark.parametrize("H,KH,HD", [(8, 2, 64), (14, 2, 128), (3, 3, 128), (24, 1, 64)])
+@pytest.mark.parametrize("T,pos0", [(16, 0), (17, 3), (64, 0), (65, 100), (130, 31), (33, 900)])
+def test_kv4_attention_prompts(ctx, H, KH, HD, T, pos0):
+    kv4_case(ctx, np.random.default_rng(T + pos0 + H), T, pos0, H, KH, HD, 0, 0)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 3), (32, 0), (33, 4), (64, 64), (100, 33), (5000, 7),
+                                          (40, 5000), (2**31 - 1, 2**31 - 1)])
+@pytest.mark.parametrize("T,pos0,H,KH,HD", [(1, 0, 4, 2, 64), (1, 500, 8, 1, 128), (9, 180, 4, 4, 64), (50, 0, 4, 2, 64),
+                                            (40, 300, 6, 2, 128)])
+def test_kv4_attention_window(ctx, T, pos0, H, KH, HD, window, sinks):
+    kv4_case(ctx, np.random.default_rng(T + pos0), T, pos0, H, KH, HD, window, sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+def test_kv4_attention_long_row(ctx, window, sinks):
+    kv4_case(ctx, np.random.default_rng(8), 1, 9000, 8, 1, 128, window, sinks)
+    kv4_case(ctx, np.random.default_rng(9), 1, 2200, 16, 8, 64, window, sinks)
+
+
+def fp16_case(ctx, rng, T, pos0, H, KH, HD, window, sinks):
+    n = pos0 + T
+    k, v = to_half_ref(rows(rng, n, KH, HD)), to_half_ref(rows(rng, n, KH, HD))
+    pad = np.full((3, KH, HD), 0x7e00, np.uint16)  # positions past the last hold NaN
+    dk, dv = dev(np.concatenate([k, pad]).view(np.int16)), dev(np.concatenate([v, pad]).view(np.int16))
+    q = rng.standard_normal((T, H, HD), dtype=F32) * F32(2)
+    dq, out = dev(q), torch.full(q.shape, 7.0, device=DEV)
+    torch.cuda.synchronize()
+    check(load().wl_attention_window_dev(ctx.handle, P(dq), T, H, KH, HD, P(dk), P(dv), pos0, window, sinks,
+                                         1 / math.sqrt(HD), P(out)))
+    got = host(ctx, out)
+    want, tol = attention_span_ref(q, k.view(np.float16), v.view(np.float16), pos0 + np.arange(T), window, sinks,
+                                   1 / math.sqrt(HD))
+    err = np.abs(got - want)
+    assert (err <= tol).all(), "worst %.3g of its bound" % float((err / tol).max())
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (5, 3), (33, 4), (100, 33), (40, 5000)])
+@pytest.mark.parametrize("T,pos0,H,KH,HD", [(1, 0, 4, 2, 64), (1, 500, 8, 1, 128), (1, 3000, 4, 4, 128), (9, 180, 4, 4, 64),
+                                            (50, 0, 4, 2, 64), (40, 300, 6, 2, 128), (130, 90, 20, 1, 128),
+                                            (3, 70, 4, 2, 80), (20, 50, 3, 1, 5)])
+def test_window_attention_fp16(ctx, T, pos0, H, KH, HD, window, sinks):
+    fp16_case(ctx, np.random.default_rng(T + pos0), T, pos0, H, KH, HD, window, sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+@pytest.mark.parametrize("H,KH,HD", [(8, 2, 64), (16, 2, 128), (3, 3, 64)])
+def test_batch_rows_equal_single_rows_bitwise(ctx, H, KH, HD, window, sinks):
+    slots, cap, N = 75, 400, 70
+    rng = np.random.default_rng(H)
+    c = Cache(ctx, cap, KH, HD, slots)
+    slot = rng.permutation(slots)[:N].astype(np.int32)
+    pos = np.concatenate([[0, 31, 32, cap - 1], rng.integers(0, cap, N - 4)]).astype(np.int32)
+    for i in range(N):
+        c.store(rows(rng, pos[i] + 1, KH, HD), rows(rng, pos[i] + 1, KH, HD), 0, int(slot[i]))
+    q = rng.standard_normal((N, H, HD), dtype=F32)
+    dq, out = dev(q), torch.full(q.shape, 7.0, device=DEV)
+    torch.cuda.synchronize()
+    check(load().wl_kv4_attention_batch_dev(ctx.handle, P(dq), N, H, KH, HD, P(c.K), P(c.V), pos.ctypes.data,
+                                            slot.ctypes.data, slots, cap, window, sinks, 1 / math.sqrt(HD), P(out)))
+    got = host(ctx, out)
+    for i in range(N):
+        one = c.attention(q[i:i + 1], int(pos[i]), window, sinks, slot=int(slot[i]))
+        assert np.array_equal(bits(got[i]), bits(one[0])), i
+
+
+def test_few_rows_equal_single_rows_bitwise(ctx):
+    rng = np.random.default_rng(3)
+    for T, pos0, H, KH, HD, window in [(8, 500, 8, 2, 128, 0), (15, 1200, 4, 4, 64, 0), (5, 300, 8, 1, 64, 90)]:
+        c = Cache(ctx, pos0 + T, KH, HD)
+        c.store(rows(rng, pos0 + T, KH, HD), rows(rng, pos0 + T, KH, HD), 0)
+        q = rng.standard_normal((T, H, HD), dtype=F32)
+        got = c.attention(q, pos0, window, 4)
+        for t in range(T):
+            assert np.array_equal(bits(got[t]), bits(c.attention(q[t:t + 1], pos0 + t, window, 4)[0])), (T, t)
+
+
+@pytest.mark.parametrize("T,pos0", [(1, 400), (1, 5000), (40, 200)])
+def test_a_nan_block_reaches_only_the_rows_that_see_it(ctx, T, pos0):
+    H, KH, HD, window, sinks = 4, 2, 64, 60, 3
+    n = pos0 + T
+    rng = np.random.default_rng(1)
+    k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+    q = rng.standard_normal((T, H, HD), dtype=F32)
+    clean = Cache(ctx, n, KH, HD)
+    clean.store(k, v, 0)
+    want = clean.attention(q, pos0, window, sinks)
+    for what in "kv":
+        # a position just before the first row's window, one no row sees, and one the later rows do not
+        for at in (pos0 - window, pos0 // 2, pos0 - window + 5):
+            x, y = k.copy(), v.copy()
+            (x if what == "k" else y)[at, 0, 3] = np.inf
+            c = Cache(ctx, n, KH, HD)
+            c.store(x, y, 0)
+            got = c.attention(q, pos0, window, sinks)
+            for t in range(T):
+                sees = at < sinks or pos0 + t - window < at <= pos0 + t
+                for h in range(H):
+                    if sees and h < H // KH:
+                        assert np.isnan(got[t, h, :32]).all()
+                        assert what == "v" or np.isnan(got[t, h]).all()
+                    else:
+                        assert np.array_equal(bits(got[t, h]), bits(want[t, h])), (what, at, t, h)
+
+
+@pytest.mark.parametrize("scale", [1e-3, 0.5, -0.3, 40.0])
+def test_scales_and_large_scores(ctx, scale):
+    rng = np.random.default_rng(6)
+    for T, pos0 in [(1, 300), (20, 100)]:
+        KH, H, HD, n = 1, 4, 64, pos0 + T
+        c = Cache(ctx, n, KH, HD)
+        k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+        c.store(k, v, 0)
+        q = rng.standard_normal((T, H, HD), dtype=F32)
+        q[:, 1] *= F32(1e4)
+        q[:, 2] *= F32(1e-20)
+        q[:, 3] = 0
+        got = c.attention(q, pos0, 0, 0, scale)
+        want, tol = attention_span_ref(q, held_ref(k), held_ref(v), pos0 + np.arange(T), 0, 0, float(F32(scale)))
+        assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+def test_captured_calls_replay(ctx):
+    """A step's store, attention over both caches and the draw, captured and replayed between eager work."""
+    H, KH, HD, n = 8, 2, 128, 1500
+    rng = np.random.default_rng(4)
+    c = Cache(ctx, n, KH, HD)
+    k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+    c.store(k, v, 0)
+    h16 = dev(to_half_ref(k).view(np.int16))
+    kn, vn, q = dev(k[-1:]), dev(v[-1:]), dev(rng.standard_normal((1, H, HD), dtype=F32))
+    o4, o16 = torch.empty((1, H, HD), device=DEV), torch.empty((1, H, HD), device=DEV)
+    L, h, sc = load(), ctx.handle, 1 / math.sqrt(HD)
+
+    def step():
+        check(L.wl_kv4_store_dev(h, P(kn), P(vn), 1, KH, HD, P(c.K), P(c.V), n, n - 1))
+        check(L.wl_kv4_attention_dev(h, P(q), 1, H, KH, HD, P(c.K), P(c.V), n, n - 1, 0, 0, sc, P(o4)))
+        check(L.wl_attention_window_dev(h, P(q), 1, H, KH, HD, P(h16), P(h16), n - 1, 700, 4, sc, P(o16)))
+
+    step()
+    ctx.sync()
+    g = ctx.capture(step)
+    for i in range(4):
+        kn.copy_(torch.randn_like(kn))
+        q.copy_(torch.randn_like(q))
+        torch.cuda.synchronize()
+        step()
+        want = [bits(host(ctx, t)) for t in (o4, o16)]
+        o4.zero_()
+        o16.zero_()
+        torch.cuda.synchronize()
+        g.launch()
+        assert all(np.array_equal(bits(host(ctx, t)), w) for t, w in zip((o4, o16), want)), i
+    g.free()

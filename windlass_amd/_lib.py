@@ -29,6 +29,14 @@ SIGNATURES = {
     "wl_residual_dev": (ctypes.c_int, [P, P, P, I64, ctypes.c_float]),
     "wl_scale_dev": (ctypes.c_int, [P, P, I64, ctypes.c_float]),
     "wl_argmax_dev": (ctypes.c_int, [P, P, I32, I64, P]),
+    "wl_kv4_bytes": (I64, [I32, I32, I32]),
+    "wl_kv4_store_dev": (ctypes.c_int, [P, P, P, I32, I32, I32, P, P, I32, I32]),
+    "wl_kv4_store_batch_dev": (ctypes.c_int, [P, P, P, I32, I32, I32, P, P, P, P, I32, I32]),
+    "wl_kv4_read_dev": (ctypes.c_int, [P, P, P, I32, I32, I32, I32, I32, P, P]),
+    "wl_kv4_attention_dev": (ctypes.c_int, [P, P, I32, I32, I32, I32, P, P, I32, I32, I32, I32, F, P]),
+    "wl_kv4_attention_batch_dev": (ctypes.c_int, [P, P, I32, I32, I32, I32, P, P, P, P, I32, I32, I32, I32, F, P]),
+    "wl_attention_window_dev": (ctypes.c_int, [P, P, I32, I32, I32, I32, P, P, I32, I32, I32, F, P]),
+    "wl_sample_dev": (ctypes.c_int, [P, P, I32, I64, P, P, P]),
     "wl_embed_dev_ids": (ctypes.c_int, [P, P, P, I32, P]),
     "wl_layer_batch_dev": (ctypes.c_int, [P, P, P, I32, P, P, I32, I32, P, P]),
     "wl_embed_dev": (ctypes.c_int, [P, P, P, I32, P]),

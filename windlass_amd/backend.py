@@ -362,6 +362,16 @@ class LayerDesc(ctypes.Structure):
         ("qk_norm_full", ctypes.c_int32)]
 
 
+class SampleParams(ctypes.Structure):
+    """wl_sample_params: one row's settings (Sampler, src/Engine.cs:353-382). temperature 0 is the greedy pick;
+    top_k 0, top_p 1 and min_p 0 filter nothing."""
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        super().__init__(temperature, top_k, top_p, min_p)
+
+
 class Transformer:
     """The static operators of src/Transformer.cs that this path replaces."""
 

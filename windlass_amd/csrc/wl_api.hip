@@ -15,15 +15,18 @@
 #include <vector>
 
 #include "../../include/windlass_hip.h"
+#include "wl_attention_span.h"
 #include "wl_dequant.h"
 #include "wl_fmma.h"
 #include "wl_gemm.h"
 #include "wl_gemm_short.h"
 #include "wl_gemv.h"
 #include "wl_intdot.h"
+#include "wl_kv4.h"
 #include "wl_layer.h"
 #include "wl_moe.h"
 #include "wl_probe.h"
+#include "wl_sample.h"
 
 // Bytes of padding after every weight buffer: the GEMV reads the aligned dwords around
 // 2-byte-aligned fields and may touch up to 16 bytes past the last block.
@@ -57,7 +60,7 @@ struct wl_stage {
 // the GEMV's own store; S_LR the router's logits and the shared expert's gate, S_LM the MoE
 // FFN's output, S_LS the shared expert's).
 enum { S_X = 0, S_Y, S_H, S_MOE, S_OUT, S_AUX, S_PART, S_XB, S_QA, S_ATT,
-       S_LXN, S_LQ, S_LK, S_LV, S_LATT, S_LO, S_LG, S_LU, S_LR, S_LM, S_LS, S_ROWS, S_ARG, S_MSYNC, S_COUNT };
+       S_LXN, S_LQ, S_LK, S_LV, S_LATT, S_LO, S_LG, S_LU, S_LR, S_LM, S_LS, S_ROWS, S_ARG, S_MSYNC, S_SMP, S_COUNT };
 
 struct wl_ctx {
   int device;
@@ -1651,6 +1654,237 @@ extern "C" int wl_layer_batch_dev(wl_ctx *c, const wl_layer_desc *L, float *d_x,
   rm.slot = rows + N;
   rm.cap = slot_positions;
   return layer_run(c, L, d_x, N, 0, d_K, d_V, rm, pos, max_n, true);
+}
+
+// ------------------------------------------------- 4-bit caches, windows, sampling
+
+// The context's device is current until the end of the scope, then the caller's again.
+struct OnDevice {
+  int was = -1;
+  hipError_t e = hipSuccess;
+  explicit OnDevice(int device) {
+    int now = device;
+    e = hipGetDevice(&now);
+    if (e == hipSuccess && now != device && (e = hipSetDevice(device)) == hipSuccess) was = now;
+  }
+  ~OnDevice() {
+    if (was >= 0) hipSetDevice(was);
+  }
+};
+#define WL_ON_DEVICE(c)           \
+  OnDevice on_device((c)->device); \
+  WL_HIP(on_device.e, "hipSetDevice")
+
+static int kv4_check(const char *who, int KH, int HD, const void *K, const void *V) {
+  if (KH <= 0 || HD <= 0) return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, KH, HD);
+  if (HD != 64 && HD != 128)
+    return fail(WL_E_UNSUPPORTED, "%s: 4-bit caches hold head dims of 64 and 128, not %d", who, HD);
+  if ((int64_t)KH * HD > 1 << 24) return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, KH, HD);
+  if (((uintptr_t)K | (uintptr_t)V) & 15) return fail(WL_E_ARG, "%s: a cache is not 16-byte aligned", who);
+  return WL_OK;
+}
+
+// T rows from pos0 in a cache of `positions`.
+static int kv_rows_check(const char *who, int T, int pos0, int positions) {
+  if (T < 0 || pos0 < 0 || positions <= 0) return fail(WL_E_SHAPE, "%s: %d rows from position %d", who, T, pos0);
+  if ((int64_t)pos0 + T > positions)
+    return fail(WL_E_ARG, "The prompt and reply need %lld positions; the context is %d.", (long long)pos0 + T, positions);
+  return WL_OK;
+}
+
+static int span_check(const char *who, int heads, int kv_heads, int window, int sinks) {
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads)
+    return fail(WL_E_SHAPE, "%s: %d heads over %d KV heads", who, heads, kv_heads);
+  if (window < 0 || sinks < 0) return fail(WL_E_ARG, "%s: a window of %d and %d first positions", who, window, sinks);
+  return WL_OK;
+}
+
+// Rows of a batch call: distinct slots below `slots`, positions below `cap`.
+static int batch_check(const char *who, int N, const int32_t *pos, const int32_t *slot, int slots, int cap) {
+  if (N < 0 || slots <= 0 || cap <= 0) return fail(WL_E_SHAPE, "%s: %d rows, %d slots of %d positions", who, N, slots, cap);
+  for (int i = 0; i < N; i++) {
+    if (slot[i] < 0 || slot[i] >= slots)
+      return fail(WL_E_ARG, "Row %d's slot %d is outside 0..%d.", i, slot[i], slots - 1);
+    if (pos[i] < 0 || pos[i] >= cap)
+      return fail(WL_E_ARG, "The prompt and reply need %lld positions; the context is %d.", (long long)pos[i] + 1, cap);
+    for (int j = 0; j < i; j++)
+      if (slot[j] == slot[i]) return fail(WL_E_ARG, "A sequence can take one token per batch step.");
+  }
+  return WL_OK;
+}
+
+// f(rows, first row) for the rows of a batch, kKv4Rows at a time.
+template <class F>
+static int each_rows(int N, const int32_t *pos, const int32_t *slot, const F &f) {
+  for (int i0 = 0; i0 < N; i0 += wl::kKv4Rows) {
+    wl::KvRows R;
+    R.n = N - i0 < wl::kKv4Rows ? N - i0 : wl::kKv4Rows;
+    R.batch = 1;
+    for (int i = 0; i < R.n; i++) {
+      R.pos[i] = pos[i0 + i];
+      R.slot[i] = slot[i0 + i];
+    }
+    if (const int rc = f(R, i0)) return rc;
+  }
+  return WL_OK;
+}
+
+static wl::KvRows seq_rows(int T, int pos0) {
+  wl::KvRows R;
+  R.n = T;
+  R.pos0 = pos0;
+  return R;
+}
+
+extern "C" int64_t wl_kv4_bytes(int32_t positions, int32_t kv_heads, int32_t head_dim) {
+  return wl::kv4_bytes(positions, kv_heads, head_dim);
+}
+
+extern "C" int wl_kv4_store_dev(wl_ctx *c, const float *d_k, const float *d_v, int32_t T, int32_t kv_heads,
+                                int32_t head_dim, void *d_K, void *d_V, int32_t positions, int32_t pos0) {
+  if (!c || (T && (!d_k || !d_v)) || !d_K || !d_V) return fail(WL_E_ARG, "wl_kv4_store_dev: null argument");
+  int rc;
+  if ((rc = kv4_check("wl_kv4_store_dev", kv_heads, head_dim, d_K, d_V)) ||
+      (rc = kv_rows_check("wl_kv4_store_dev", T, pos0, positions)))
+    return rc;
+  WL_ON_DEVICE(c);
+  WL_HIP(wl::kv4_store_launch(d_k, d_v, kv_heads, head_dim, (uint8_t *)d_K, (uint8_t *)d_V, positions, 0,
+                              seq_rows(T, pos0), c->stream), "kv4 store");
+  return WL_OK;
+}
+
+extern "C" int wl_kv4_store_batch_dev(wl_ctx *c, const float *d_k, const float *d_v, int32_t N, int32_t kv_heads,
+                                      int32_t head_dim, void *d_K, void *d_V, const int32_t *pos, const int32_t *slot,
+                                      int32_t slots, int32_t slot_positions) {
+  if (!c || (N && (!d_k || !d_v || !pos || !slot)) || !d_K || !d_V)
+    return fail(WL_E_ARG, "wl_kv4_store_batch_dev: null argument");
+  int rc;
+  if ((rc = kv4_check("wl_kv4_store_batch_dev", kv_heads, head_dim, d_K, d_V)) ||
+      (rc = batch_check("wl_kv4_store_batch_dev", N, pos, slot, slots, slot_positions)))
+    return rc;
+  WL_ON_DEVICE(c);
+  const int64_t kd = (int64_t)kv_heads * head_dim;
+  return each_rows(N, pos, slot, [&](const wl::KvRows &R, int i0) -> int {
+    WL_HIP(wl::kv4_store_launch(d_k + i0 * kd, d_v + i0 * kd, kv_heads, head_dim, (uint8_t *)d_K, (uint8_t *)d_V,
+                                slot_positions, wl::kv4_bytes(slot_positions, kv_heads, head_dim), R, c->stream),
+           "kv4 store");
+    return WL_OK;
+  });
+}
+
+extern "C" int wl_kv4_read_dev(wl_ctx *c, const void *d_K, const void *d_V, int32_t positions, int32_t kv_heads,
+                               int32_t head_dim, int32_t pos0, int32_t T, float *d_k, float *d_v) {
+  if (!c || (T && (!d_k || !d_v)) || !d_K || !d_V) return fail(WL_E_ARG, "wl_kv4_read_dev: null argument");
+  int rc;
+  if ((rc = kv4_check("wl_kv4_read_dev", kv_heads, head_dim, d_K, d_V)) ||
+      (rc = kv_rows_check("wl_kv4_read_dev", T, pos0, positions)))
+    return rc;
+  WL_ON_DEVICE(c);
+  WL_HIP(wl::kv4_read_launch((const uint8_t *)d_K, (const uint8_t *)d_V, kv_heads, head_dim, positions, pos0, T, d_k, d_v,
+                             c->stream), "kv4 read");
+  return WL_OK;
+}
+
+// Attention of the rows over c16 / c4 caches, its scratch from the context.
+static int span_attention(wl_ctx *c, const float *d_q, int heads, const wl::KvCache &kc, const wl::Span &s,
+                          const wl::KvRows &R, float scale, float *d_out) {
+  const int rc = ensure(c, S_ATT, (size_t)wl::attention_span_scratch_floats(kc, heads, s, R) * sizeof(float));
+  if (rc) return rc;
+  WL_HIP(wl::attention_span_launch(d_q, heads, kc, s, R, scale, (float *)c->buf[S_ATT], d_out, c->stream), "attention");
+  return WL_OK;
+}
+
+static wl::KvCache kv4_cache(const void *K, const void *V, int KH, int HD, int positions) {
+  wl::KvCache kc;
+  kc.K = (const uint8_t *)K;
+  kc.V = (const uint8_t *)V;
+  kc.bits = 4;
+  kc.KH = KH;
+  kc.HD = HD;
+  kc.positions = positions;
+  kc.slot_bytes = wl::kv4_bytes(positions, KH, HD);
+  return kc;
+}
+
+extern "C" int wl_kv4_attention_dev(wl_ctx *c, const float *d_q, int32_t T, int32_t heads, int32_t kv_heads,
+                                    int32_t head_dim, const void *d_K, const void *d_V, int32_t positions,
+                                    int32_t pos0, int32_t window, int32_t sinks, float scale, float *d_out) {
+  if (!c || (T && (!d_q || !d_out)) || !d_K || !d_V) return fail(WL_E_ARG, "wl_kv4_attention_dev: null argument");
+  int rc;
+  if ((rc = span_check("wl_kv4_attention_dev", heads, kv_heads, window, sinks)) ||
+      (rc = kv4_check("wl_kv4_attention_dev", kv_heads, head_dim, d_K, d_V)) ||
+      (rc = kv_rows_check("wl_kv4_attention_dev", T, pos0, positions)))
+    return rc;
+  WL_ON_DEVICE(c);
+  return span_attention(c, d_q, heads, kv4_cache(d_K, d_V, kv_heads, head_dim, positions), wl::Span{window, sinks},
+                        seq_rows(T, pos0), scale, d_out);
+}
+
+extern "C" int wl_kv4_attention_batch_dev(wl_ctx *c, const float *d_q, int32_t N, int32_t heads, int32_t kv_heads,
+                                          int32_t head_dim, const void *d_K, const void *d_V, const int32_t *pos,
+                                          const int32_t *slot, int32_t slots, int32_t slot_positions, int32_t window,
+                                          int32_t sinks, float scale, float *d_out) {
+  if (!c || (N && (!d_q || !d_out || !pos || !slot)) || !d_K || !d_V)
+    return fail(WL_E_ARG, "wl_kv4_attention_batch_dev: null argument");
+  int rc;
+  if ((rc = span_check("wl_kv4_attention_batch_dev", heads, kv_heads, window, sinks)) ||
+      (rc = kv4_check("wl_kv4_attention_batch_dev", kv_heads, head_dim, d_K, d_V)) ||
+      (rc = batch_check("wl_kv4_attention_batch_dev", N, pos, slot, slots, slot_positions)))
+    return rc;
+  WL_ON_DEVICE(c);
+  const int64_t qd = (int64_t)heads * head_dim;
+  return each_rows(N, pos, slot, [&](const wl::KvRows &R, int i0) -> int {
+    return span_attention(c, d_q + i0 * qd, heads, kv4_cache(d_K, d_V, kv_heads, head_dim, slot_positions),
+                          wl::Span{window, sinks}, R, scale, d_out + i0 * qd);
+  });
+}
+
+extern "C" int wl_attention_window_dev(wl_ctx *c, const float *d_q, int32_t T, int32_t heads, int32_t kv_heads,
+                                       int32_t head_dim, const uint16_t *d_K, const uint16_t *d_V, int32_t pos0,
+                                       int32_t window, int32_t sinks, float scale, float *d_out) {
+  if (!c || (T && (!d_q || !d_K || !d_V || !d_out))) return fail(WL_E_ARG, "wl_attention_window_dev: null argument");
+  int rc;
+  if ((rc = span_check("wl_attention_window_dev", heads, kv_heads, window, sinks)) ||
+      (rc = kv_rows_check("wl_attention_window_dev", T, pos0, INT32_MAX)))
+    return rc;
+  if (head_dim <= 0 || (int64_t)kv_heads * head_dim > 1 << 24)
+    return fail(WL_E_SHAPE, "wl_attention_window_dev: %d KV heads of %d", kv_heads, head_dim);
+  WL_ON_DEVICE(c);
+  wl::KvCache kc;
+  kc.K = (const uint8_t *)d_K;
+  kc.V = (const uint8_t *)d_V;
+  kc.KH = kv_heads;
+  kc.HD = head_dim;
+  kc.positions = (int64_t)pos0 + T;
+  return span_attention(c, d_q, heads, kc, wl::Span{window, sinks}, seq_rows(T, pos0), scale, d_out);
+}
+
+extern "C" int wl_sample_dev(wl_ctx *c, const float *d_logits, int32_t rows, int64_t n, const wl_sample_params *params,
+                             const float *d_u, int32_t *d_out) {
+  if (!c || (rows && (!d_logits || !params || !d_u || !d_out))) return fail(WL_E_ARG, "wl_sample_dev: null argument");
+  if (rows < 0 || n <= 0 || n > 1 << 24) return fail(WL_E_SHAPE, "wl_sample_dev: %d rows of %lld logits", rows, (long long)n);
+  for (int i = 0; i < rows; i++) {
+    const wl_sample_params &p = params[i];
+    if (!(p.temperature >= 0.f) || p.temperature > 3.4028235e38f || p.top_k < 0 || !(p.top_p >= 0.f && p.top_p <= 1.f) ||
+        !(p.min_p >= 0.f && p.min_p <= 1.f))
+      return fail(WL_E_ARG, "wl_sample_dev: row %d: temperature %g, top_k %d, top_p %g, min_p %g", i, p.temperature,
+                  p.top_k, p.top_p, p.min_p);
+  }
+  if (rows == 0) return WL_OK;
+  WL_ON_DEVICE(c);
+  const int most = rows < wl::kSampleRows ? rows : wl::kSampleRows;
+  if (const int rc = ensure(c, S_SMP, (size_t)wl::sample_scratch_bytes(most, n))) return rc;
+  for (int r0 = 0; r0 < rows; r0 += wl::kSampleRows) {
+    const int m = rows - r0 < wl::kSampleRows ? rows - r0 : wl::kSampleRows;
+    wl::SampleSets sets = {};
+    for (int i = 0; i < m; i++) {
+      const wl_sample_params &p = params[r0 + i];
+      sets.row[i] = wl::SampleSet{p.temperature, p.top_k, p.top_p, p.min_p};
+    }
+    WL_HIP(wl::sample_launch(d_logits + (int64_t)r0 * n, m, n, sets, d_u + r0, d_out + r0, c->buf[S_SMP], c->stream),
+           "sample");
+  }
+  return WL_OK;
 }
 
 extern "C" int wl_read_peak_dev(wl_ctx *c, const void *d_src, int64_t bytes, int32_t workgroups, uint32_t *d_out) {
