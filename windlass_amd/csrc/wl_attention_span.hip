@@ -3,7 +3,7 @@
 // positions Span names).
 #include "wl_attention_span.h"
 
-#include "wl_device.h"
+#include "wl_fmma_codec.h"
 
 #pragma clang fp contract(off)
 
@@ -99,6 +99,416 @@ __global__ __launch_bounds__(256) void span_rows_kernel(const float *__restrict_
   }
 }
 
+// ------------------------------------------------------------------------------- few rows
+// Rows of up to 15 tokens and batch rows: head dims 64 and 128 on v_mfma_f32_16x16x32_f16.
+//
+// S^T = K Q^T of 16 keys: the 16 columns are eight query heads of the KV head, each row of q as two
+// fp16 parts (hi in column 2 g, lo in 2 g + 1: 22 bits of the largest value, exact products, fp32 sums),
+// which one addition of neighbouring lanes joins. O^T = V^T P^T of 32 keys: the probabilities are where the
+// scores were (lane l has keys 16 t + 4 (l / 16) + i of column l % 16), again in two parts, and V's
+// operand holds those keys in that order: 4-bit tiles are stored so, fp16 rows are paired by byte
+// permutes. So no value passes through LDS, and a lane's loads are its operands.
+//
+// A workgroup of W waves takes a run of a row's tiles (32 positions each), the waves one tile in turn, each
+// with its own running maximum, sum and output; they are added through LDS. Long rows are cut in runs by a rule
+// on the row's own tiles, so that a row's bits do not depend on the rows beside it.
+typedef float sf4 __attribute__((ext_vector_type(4)));
+constexpr float kSpUp = 0x1p14f;  // the probabilities' factor in their fp16 parts
+constexpr int kSpWaves = 4;
+constexpr int kSpRuns = 256;      // runs of a row at most
+
+// The tiles a row at p reads, in order: those of the first tokens, then the window's.
+struct SpanTiles {
+  int lead, from, n;
+  __host__ __device__ SpanTiles(const Span &s, int p) {
+    lead = (s.lead(p) + kKv4Tile - 1) / kKv4Tile;
+    from = s.first(p) / kKv4Tile;
+    from = from < lead ? lead : from;
+    n = lead + p / kKv4Tile - from + 1;
+    if (p / kKv4Tile < from) n = lead;  // the first tokens' tiles reach the row
+  }
+  __host__ __device__ int tile(int i) const { return i < lead ? i : from + (i - lead); }
+};
+
+// 16-bit pairs to fp16 values: levels at bits 4 i of both halves, their scales s and -1.5 s.
+template <int I>
+__device__ __forceinline__ uint32_t kv4_pair(uint32_t w, fh2 s, fh2 s15) {
+  const uint32_t at = I == 0 ? w << 6 : I == 1 ? w << 2 : I == 2 ? w >> 2 : w >> 6;
+  const fh2 n = as_fh2((at & 0x03c003c0u) | 0x3c003c00u);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, s, s15));
+}
+__device__ __forceinline__ fh8 as_fh8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(fh8, u32x4_t{a, b, c, d});
+}
+__device__ __forceinline__ fh2 scale15(fh2 s) { return s * fh2{(_Float16)-1.5f, (_Float16)-1.5f}; }
+
+// Tiles of 4-bit caches. hide(m): bit j set where key j of the lane (keys 16 (j / 4) + 4 kq + j % 4) is not seen:
+// its values become zeros.
+template <int HD>
+struct TileKv4 {
+  static constexpr int E = HD / 64, NB = HD / 32;
+  u32x4_t v[E], vs;
+  uint32_t k[2][4 * E / 2], ks;
+  __device__ __forceinline__ void load(const uint8_t *K, const uint8_t *V, int64_t, int64_t tile, int, int lane) {
+    const uint8_t *kt = K + tile * (18 * HD), *vt = V + tile * (18 * HD);
+    const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const uint8_t *kp = kt + (16 * t + r) * (HD / 2) + q * (HD / 8);
+      if constexpr (E == 2) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t *>(kp);
+        k[t][0] = w.x, k[t][1] = w.y, k[t][2] = w.z, k[t][3] = w.w;
+      } else {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(kp);
+        k[t][0] = w.x, k[t][1] = w.y;
+      }
+    }
+    ks = reinterpret_cast<const uint32_t *>(kt + 16 * HD)[r * NB + (E == 2 ? q : q >> 1)];
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = reinterpret_cast<const u32x4_t *>(vt)[e * 64 + lane];
+    vs = *reinterpret_cast<const u32x4_t *>(vt + 16 * HD + (q * NB + (lane & 15) * NB / 16) * 16);
+  }
+  // step i of the scores of keys 16 t ..: values q HD / 4 + 8 i .. of key r
+  __device__ __forceinline__ fh8 key(int t, int i) const {
+    const fh2 s2 = as_fh2(ks);
+    const fh2 s = t ? fh2{s2.y, s2.y} : fh2{s2.x, s2.x}, s15 = scale15(s);
+    const uint32_t w = k[t][i];
+    return as_fh8(kv4_pair<0>(w, s, s15), kv4_pair<1>(w, s, s15), kv4_pair<2>(w, s, s15), kv4_pair<3>(w, s, s15));
+  }
+  // value 4 E x + 4 e + I of the lane's eight keys
+  template <int I>
+  __device__ __forceinline__ fh8 val(int e) const {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const fh2 s = as_fh2(vs[j]);
+      o[j] = kv4_pair<I>(v[e][j], s, scale15(s));
+    }
+    return as_fh8(o[0], o[1], o[2], o[3]);
+  }
+  __device__ __forceinline__ void hide(uint32_t m) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      vs[j] &= (m >> (2 * j) & 1u ? 0u : 0xffffu) | (m >> (2 * j + 1) & 1u ? 0u : 0xffff0000u);
+  }
+  static constexpr bool kInf = false;  // every value is finite or NaN
+};
+
+// Tiles of fp16 rows [position][kv_dim]; positions past `last` are read as `last`.
+template <int HD>
+struct TileF16 {
+  static constexpr int E = HD / 64;
+  u32x4_t k[2][2 * E];
+  uint32_t v[8][2 * E];
+  __device__ __forceinline__ void load(const uint8_t *K, const uint8_t *V, int64_t stride, int64_t tile, int last,
+                                       int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    const int64_t p0 = tile * kKv4Tile;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const int64_t p = p0 + 16 * t + r < last ? p0 + 16 * t + r : last;
+      const u32x4_t *kp = reinterpret_cast<const u32x4_t *>(K + p * stride + q * (HD / 2));
+#pragma unroll
+      for (int i = 0; i < 2 * E; i++) k[t][i] = kp[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int64_t at = p0 + 16 * (j >> 2) + 4 * q + (j & 3), p = at < last ? at : last;
+      const uint8_t *vp = V + p * stride + r * (HD / 8);
+      if constexpr (E == 2) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t *>(vp);
+        v[j][0] = w.x, v[j][1] = w.y, v[j][2] = w.z, v[j][3] = w.w;
+      } else {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(vp);
+        v[j][0] = w.x, v[j][1] = w.y;
+      }
+    }
+  }
+  __device__ __forceinline__ fh8 key(int t, int i) const { return __builtin_bit_cast(fh8, k[t][i]); }
+  template <int I>
+  __device__ __forceinline__ fh8 val(int e) const {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      o[j] = __builtin_amdgcn_perm(v[2 * j + 1][2 * e + I / 2], v[2 * j][2 * e + I / 2], I & 1 ? 0x07060302u : 0x05040100u);
+    return as_fh8(o[0], o[1], o[2], o[3]);
+  }
+  __device__ __forceinline__ void hide(uint32_t m) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+      for (int i = 0; i < 2 * E; i++) v[j][i] = m >> j & 1u ? 0u : v[j][i];
+  }
+  static constexpr bool kInf = true;
+};
+
+// The runs of a launch's rows: row t's begin at off[t].
+struct SpanRuns {
+  int off[kKv4Rows + 1];
+  int most;  // of a row
+};
+
+__device__ __forceinline__ float lane_xor1(float v) {
+  return __builtin_bit_cast(float, dpp32<0xB1>(__builtin_bit_cast(uint32_t, v)));
+}
+// hi + lo of neighbouring lanes; past an infinity the low part's product with it means nothing.
+template <bool INF>
+__device__ __forceinline__ float join_parts(float v, bool low) {
+  const float o = lane_xor1(v);
+  if constexpr (INF) {
+    const float hi = low ? o : v;
+    return __builtin_isfinite(hi) ? v + o : hi;
+  }
+  return v + o;
+}
+
+template <int HD, class Tile>
+__global__ __launch_bounds__(64 * kSpWaves) void span_decode_kernel(const float *__restrict__ q, int H, KvCache c,
+                                                                    Span s, KvRows R, SpanRuns U, float scale,
+                                                                    float *__restrict__ part, float *__restrict__ out) {
+  constexpr int NK = HD / 32, ND = HD / 16, E = HD / 64, W = kSpWaves;
+  __shared__ float so[W][8][HD];
+  __shared__ float sm[W][8], sc2[8];
+  __shared__ double sl[W][8];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kq = lane >> 4, G = H / c.KH, CB = (G + 7) / 8;
+  const int unit = blockIdx.x % (c.KH * CB), run = blockIdx.x / (c.KH * CB);
+  const int kvh = unit % c.KH, cb = unit / c.KH;
+  const int t = __builtin_amdgcn_readfirstlane(
+      __popcll(__ballot(lane < R.n && U.off[lane < R.n ? lane : 0] <= run)) - 1);
+  const int runs = U.off[t + 1] - U.off[t], mine = run - U.off[t];
+  const int p = R.position(t), first = s.first(p), lead = s.lead(p);
+  const SpanTiles tl(s, p);
+  const int per = (tl.n + runs - 1) / runs, i0 = mine * per, i1 = i0 + per < tl.n ? i0 + per : tl.n;
+  const uint8_t *K, *V;
+  int64_t stride = 0;
+  if constexpr (Tile::kInf) {
+    stride = (int64_t)c.KH * HD * 2;
+    K = c.K + (int64_t)R.slot_of(t) * c.slot_bytes + kvh * (HD * 2);
+    V = c.V + (int64_t)R.slot_of(t) * c.slot_bytes + kvh * (HD * 2);
+  } else {
+    const int64_t head = (int64_t)R.slot_of(t) * c.slot_bytes + (int64_t)kvh * ((c.positions + 31) / 32) * (18 * HD);
+    K = c.K + head;
+    V = c.V + head;
+  }
+  Tile A, B;
+  int i = i0 + wv;
+  if (i < i1) A.load(K, V, stride, tl.tile(i), p, lane);
+  // the query's parts: head cb * 8 + col / 2, part col % 2, values kq HD / 4 + 8 step + 0..7
+  const bool low = col & 1;
+  const int g = cb * 8 + (col >> 1) < G ? cb * 8 + (col >> 1) : G - 1;
+  fh8 qb[NK];
+  float c2;
+  {
+    typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));
+    const float *qp = q + ((int64_t)t * H + kvh * G + g) * HD + kq * (HD / 4);
+    float x[HD / 4], m = 0.f;
+#pragma unroll
+    for (int e = 0; e < HD / 16; e++) {
+      const f4a4 w = *reinterpret_cast<const f4a4 *>(qp + 4 * e);
+      x[4 * e] = w.x, x[4 * e + 1] = w.y, x[4 * e + 2] = w.z, x[4 * e + 3] = w.w;
+    }
+#pragma unroll
+    for (int e = 0; e < HD / 4; e++) m = fabsf(x[e]) < INFINITY ? fmaxf(m, fabsf(x[e])) : m;
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    float f, inv;
+    unit_scale(m, f, inv);
+    // scores in units of log2: c2 > 0 (a negative scale negates the query)
+    c2 = fmaxf(fabsf(scale) * 1.4426950408889634f * inv, 1.1754944e-38f);
+    f = scale < 0.f ? -f : f;
+    if (scale != scale) c2 = scale;
+#pragma unroll
+    for (int e = 0; e < HD / 4; e++) {
+      const float X = x[e] * f;
+      const _Float16 a = (_Float16)X;
+      qb[e / 8][e % 8] = low ? (_Float16)(__builtin_isinf(X) ? 0.f : X - (float)a) : a;
+    }
+  }
+  sf4 O[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) O[d] = sf4{0.f, 0.f, 0.f, 0.f};
+  float M = -INFINITY;
+  double L = 0.0;
+  auto step = [&](Tile &T, int64_t tile) __attribute__((always_inline)) {
+    const int p0 = (int)tile * kKv4Tile;
+    sf4 S[2];
+#pragma unroll
+    for (int t2 = 0; t2 < 2; t2++) {
+      S[t2] = sf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < NK; k++) S[t2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.key(t2, k), qb[k], S[t2], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; e++) S[t2][e] = join_parts<Tile::kInf>(S[t2][e], low);
+    }
+    if (!(p0 + 31 <= p && (p0 >= first || p0 + 31 < lead))) {  // uniform: some position is not seen
+      uint32_t hid = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int at = p0 + 16 * (j >> 2) + 4 * kq + (j & 3);
+        if (at > p || (at >= lead && at < first)) {
+          hid |= 1u << j;
+          S[j >> 2][j & 3] = -INFINITY;
+        }
+      }
+      T.hide(hid);
+    }
+    float mt = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
+                     fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
+    if (__any(mt > M)) {
+      mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      const float Mn = fmaxf(M, mt), al = Mn > M ? __builtin_amdgcn_exp2f((M - Mn) * c2) : 1.f;
+      L *= (double)al;
+#pragma unroll
+      for (int d = 0; d < ND; d++) O[d] *= al;
+      M = Mn;
+    }
+    const float Mu = M == -INFINITY ? 0.f : M;
+    fh8 pb;
+    float ts[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float P = __builtin_amdgcn_exp2f((S[j >> 2][j & 3] - Mu) * c2);
+      ts[j & 1] += P;
+      const _Float16 a = (_Float16)(P * kSpUp);
+      pb[j] = low ? (_Float16)__builtin_fmaf(P, kSpUp, -(float)a) : a;
+    }
+    L += (double)(ts[0] + ts[1]);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      O[4 * e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<0>(e), pb, O[4 * e], 0, 0, 0);
+      O[4 * e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<1>(e), pb, O[4 * e + 1], 0, 0, 0);
+      O[4 * e + 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<2>(e), pb, O[4 * e + 2], 0, 0, 0);
+      O[4 * e + 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<3>(e), pb, O[4 * e + 3], 0, 0, 0);
+    }
+  };
+#pragma unroll 1
+  while (i < i1) {
+    if (i + W < i1) B.load(K, V, stride, tl.tile(i + W), p, lane);
+    step(A, tl.tile(i));
+    i += W;
+    if (i >= i1) break;
+    if (i + W < i1) A.load(K, V, stride, tl.tile(i + W), p, lane);
+    step(B, tl.tile(i));
+    i += W;
+  }
+  // the waves' sums under their largest maximum; row x of block d is value 4 E x + d
+  L += __shfl_xor(L, 16, 64);
+  L += __shfl_xor(L, 32, 64);
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float o = join_parts<Tile::kInf>(O[d][e], low);
+      if (!low) so[wv][col >> 1][4 * E * (4 * kq + e) + d] = o;
+    }
+  if (!low && kq == 0) {
+    sm[wv][col >> 1] = M;
+    sl[wv][col >> 1] = L;
+    sc2[col >> 1] = c2;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 8 * HD; e += 64 * W) {
+    const int gg = e / HD, d = e % HD, h = cb * 8 + gg;
+    if (h >= G) break;  // heads past the group: uniform over what follows
+    float m = sm[0][gg];
+#pragma unroll
+    for (int w = 1; w < W; w++) m = fmaxf(m, sm[w][gg]);
+    float o = 0.f;
+    double l = 0.0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const float f = __builtin_amdgcn_exp2f((sm[w][gg] - m) * sc2[gg]);
+      o += so[w][gg][d] * f;
+      l += sl[w][gg] * (double)f;
+    }
+    const int64_t row = (int64_t)t * H + kvh * G + h;
+    if (runs == 1) {
+      out[row * HD + d] = (float)((double)o * (1.0 / kSpUp) / l);
+    } else {
+      float *rec = part + (row * U.most + mine) * (HD + 4);
+      rec[d] = o;
+      if (d == 0) {
+        rec[HD] = m;
+        rec[HD + 1] = sc2[gg];
+        *reinterpret_cast<double *>(rec + HD + 2) = l;
+      }
+    }
+  }
+}
+
+// Rows of more than one run: the runs' sums under their largest maximum, in order. One wave per (row, head).
+template <int HD>
+__global__ __launch_bounds__(64) void span_join_kernel(const float *__restrict__ part, int H, SpanRuns U,
+                                                       float *__restrict__ out) {
+  const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
+  const int n = U.off[t + 1] - U.off[t];
+  if (n == 1) return;
+  const int64_t row = (int64_t)t * H + h;
+  const float *rec = part + row * U.most * (HD + 4);
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, rec[i * (HD + 4) + HD]);
+  m = wave_max_f(m);
+  float o[HD / 64] = {};
+  double l = 0.0;
+  for (int b = 0; b < n; b += 64) {
+    const int i = b + lane < n ? b + lane : n - 1;
+    const float *r = rec + i * (HD + 4);
+    const float f = b + lane < n ? __builtin_amdgcn_exp2f((r[HD] - m) * r[HD + 1]) : 0.f;
+    l += *reinterpret_cast<const double *>(r + HD + 2) * (double)f;
+    const int k = n - b < 64 ? n - b : 64;
+#pragma unroll 8
+    for (int j = 0; j < k; j++) {
+      const float w = lane_f(f, j);
+#pragma unroll
+      for (int e = 0; e < HD / 64; e++) o[e] = __builtin_fmaf(rec[(b + j) * (HD + 4) + lane + 64 * e], w, o[e]);
+    }
+  }
+  l = wave_sum_d(l);
+#pragma unroll
+  for (int e = 0; e < HD / 64; e++) out[row * HD + lane + 64 * e] = (float)((double)o[e] * (1.0 / kSpUp) / l);
+}
+
+// Runs of a row of n tiles.
+static int span_runs(int n, int units) {
+  int r = (n + kSpWaves - 1) / kSpWaves;
+  const int fill = (512 + units - 1) / units;
+  r = r > fill ? fill : r;
+  r = r > kSpRuns ? kSpRuns : r;
+  const int per = (n + r - 1) / r;
+  return (n + per - 1) / per;
+}
+
+static bool span_tiled(const KvCache &c) {
+  return c.bits == 4 || ((c.HD == 64 || c.HD == 128) && ((uintptr_t)c.K & 15) == 0 && ((uintptr_t)c.V & 15) == 0);
+}
+static bool span_decodes(const KvCache &c, const KvRows &R) { return span_tiled(c) && (R.batch || R.n < 16); }
+
+static SpanRuns span_plan(const KvCache &c, int H, const Span &s, const KvRows &R) {
+  SpanRuns U = {};
+  const int units = c.KH * ((H / c.KH + 7) / 8);
+  for (int t = 0; t < R.n; t++) {
+    const int r = span_runs(SpanTiles(s, R.position(t)).n, units);
+    U.off[t + 1] = U.off[t] + r;
+    U.most = r > U.most ? r : U.most;
+  }
+  return U;
+}
+
+template <int HD, class Tile>
+static hipError_t span_decode_launch(const float *q, int H, const KvCache &c, const Span &s, const KvRows &R, float scale,
+                                     float *part, float *out, hipStream_t st) {
+  const SpanRuns U = span_plan(c, H, s, R);
+  const int units = c.KH * ((H / c.KH + 7) / 8);
+  hipLaunchKernelGGL((span_decode_kernel<HD, Tile>), dim3((unsigned)((int64_t)U.off[R.n] * units)),
+                     dim3(64 * kSpWaves), 0, st, q, H, c, s, R, U, scale, part, out);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || U.most == 1) return e;
+  hipLaunchKernelGGL(span_join_kernel<HD>, dim3(H, R.n), dim3(64), 0, st, part, H, U, out);
+  return hipGetLastError();
+}
+
 static int64_t span_max_n(const Span &s, const KvRows &R) {
   int64_t m = 0;
   if (!R.batch) return s.seen(R.pos0 + R.n - 1);
@@ -107,12 +517,24 @@ static int64_t span_max_n(const Span &s, const KvRows &R) {
 }
 
 int64_t attention_span_scratch_floats(const KvCache &c, int H, const Span &s, const KvRows &R) {
-  return R.n > 0 ? (int64_t)R.n * H * span_max_n(s, R) : 0;
+  if (R.n <= 0) return 0;
+  if (span_decodes(c, R)) {
+    const SpanRuns U = span_plan(c, H, s, R);
+    return U.most > 1 ? (int64_t)R.n * H * U.most * (c.HD + 4) : 0;
+  }
+  return (int64_t)R.n * H * span_max_n(s, R);
 }
 
 hipError_t attention_span_launch(const float *q, int H, const KvCache &c, const Span &s, const KvRows &R, float scale,
                                  float *scratch, float *out, hipStream_t st) {
   if (R.n <= 0) return hipSuccess;
+  if (span_decodes(c, R)) {
+    if (c.bits == 4)
+      return c.HD == 64 ? span_decode_launch<64, TileKv4<64>>(q, H, c, s, R, scale, scratch, out, st)
+                        : span_decode_launch<128, TileKv4<128>>(q, H, c, s, R, scale, scratch, out, st);
+    return c.HD == 64 ? span_decode_launch<64, TileF16<64>>(q, H, c, s, R, scale, scratch, out, st)
+                      : span_decode_launch<128, TileF16<128>>(q, H, c, s, R, scale, scratch, out, st);
+  }
   hipLaunchKernelGGL(span_rows_kernel, dim3(H, R.n), dim3(256), 0, st, q, H, c, s, R, scale, scratch, span_max_n(s, R),
                      out);
   return hipGetLastError();
