@@ -113,7 +113,9 @@ __global__ __launch_bounds__(256) void span_rows_kernel(const float *__restrict_
 // with its own running maximum, sum and output; they are added through LDS. Long rows are cut in runs by a rule
 // on the row's own tiles, so that a row's bits do not depend on the rows beside it.
 typedef float sf4 __attribute__((ext_vector_type(4)));
-constexpr float kSpUp = 0x1p14f;  // the probabilities' factor in their fp16 parts
+// A running maximum is raised only by scores more than 2^6 past it, so nearly never after a wave's first tile: the
+// exponentials reach 2^6, and 2^8 of them are fp16 parts (22 bits down to 2^-22 of the row's largest, 2^-33 of it below).
+constexpr float kSpUp = 0x1p8f, kSpPast = 6.f;
 constexpr int kSpWaves = 4;
 constexpr int kSpRuns = 256;      // runs of a row at most
 
@@ -132,10 +134,16 @@ struct SpanTiles {
 
 // 16-bit pairs to fp16 values: levels at bits 4 i of both halves, their scales s and -1.5 s.
 template <int I>
-__device__ __forceinline__ uint32_t kv4_pair(uint32_t w, fh2 s, fh2 s15) {
+__device__ __forceinline__ uint32_t kv4_pair(uint32_t w, fh2 s, fh2 s15, uint32_t ones) {
   const uint32_t at = I == 0 ? w << 6 : I == 1 ? w << 2 : I == 2 ? w >> 2 : w >> 6;
-  const fh2 n = as_fh2((at & 0x03c003c0u) | 0x3c003c00u);
+  const fh2 n = as_fh2((at & 0x03c003c0u) | ones);
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, s, s15));
+}
+// Two fp16 ones, in a register: as a constant they cost the mask and the ones an instruction each.
+__device__ __forceinline__ uint32_t fp16_ones() {
+  uint32_t o;
+  asm("v_mov_b32 %0, 0x3c003c00" : "=v"(o));
+  return o;
 }
 __device__ __forceinline__ fh8 as_fh8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_bit_cast(fh8, u32x4_t{a, b, c, d});
@@ -169,20 +177,21 @@ struct TileKv4 {
     vs = *reinterpret_cast<const u32x4_t *>(vt + 16 * HD + (q * NB + (lane & 15) * NB / 16) * 16);
   }
   // step i of the scores of keys 16 t ..: values q HD / 4 + 8 i .. of key r
-  __device__ __forceinline__ fh8 key(int t, int i) const {
+  __device__ __forceinline__ fh8 key(int t, int i, uint32_t ones) const {
     const fh2 s2 = as_fh2(ks);
     const fh2 s = t ? fh2{s2.y, s2.y} : fh2{s2.x, s2.x}, s15 = scale15(s);
     const uint32_t w = k[t][i];
-    return as_fh8(kv4_pair<0>(w, s, s15), kv4_pair<1>(w, s, s15), kv4_pair<2>(w, s, s15), kv4_pair<3>(w, s, s15));
+    return as_fh8(kv4_pair<0>(w, s, s15, ones), kv4_pair<1>(w, s, s15, ones), kv4_pair<2>(w, s, s15, ones),
+                  kv4_pair<3>(w, s, s15, ones));
   }
   // value 4 E x + 4 e + I of the lane's eight keys
   template <int I>
-  __device__ __forceinline__ fh8 val(int e) const {
+  __device__ __forceinline__ fh8 val(int e, uint32_t ones) const {
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const fh2 s = as_fh2(vs[j]);
-      o[j] = kv4_pair<I>(v[e][j], s, scale15(s));
+      o[j] = kv4_pair<I>(v[e][j], s, scale15(s), ones);
     }
     return as_fh8(o[0], o[1], o[2], o[3]);
   }
@@ -192,6 +201,7 @@ struct TileKv4 {
       vs[j] &= (m >> (2 * j) & 1u ? 0u : 0xffffu) | (m >> (2 * j + 1) & 1u ? 0u : 0xffff0000u);
   }
   static constexpr bool kInf = false;  // every value is finite or NaN
+  static constexpr int kOcc = 4;  // waves per SIMD
 };
 
 // Tiles of fp16 rows [position][kv_dim]; positions past `last` are read as `last`.
@@ -224,9 +234,9 @@ struct TileF16 {
       }
     }
   }
-  __device__ __forceinline__ fh8 key(int t, int i) const { return __builtin_bit_cast(fh8, k[t][i]); }
+  __device__ __forceinline__ fh8 key(int t, int i, uint32_t) const { return __builtin_bit_cast(fh8, k[t][i]); }
   template <int I>
-  __device__ __forceinline__ fh8 val(int e) const {
+  __device__ __forceinline__ fh8 val(int e, uint32_t) const {
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; j++)
@@ -240,11 +250,12 @@ struct TileF16 {
       for (int i = 0; i < 2 * E; i++) v[j][i] = m >> j & 1u ? 0u : v[j][i];
   }
   static constexpr bool kInf = true;
+  static constexpr int kOcc = HD == 64 ? 3 : 2;
 };
 
-// The runs of a launch's rows: row t's begin at off[t].
+// The runs of a launch's rows: row t's begin at off[t], of per[t] tiles each.
 struct SpanRuns {
-  int off[kKv4Rows + 1];
+  int off[kKv4Rows + 1], per[kKv4Rows];
   int most;  // of a row
 };
 
@@ -262,24 +273,35 @@ __device__ __forceinline__ float join_parts(float v, bool low) {
   return v + o;
 }
 
+typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));  // at any float's address
+
+// A row's outputs lie in LDS and in the runs' records as the matrix cores leave them: values 16 d + 4 kq + e, for
+// value HD / 16 (4 kq + e) + d of the head. Four of them to their places in the head's row.
+template <int HD>
+__device__ __forceinline__ void span_store(float *o, int four, sf4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) o[HD / 16 * (4 * (four & 3) + e) + (four >> 2)] = v[e];
+}
+
 template <int HD, class Tile>
-__global__ __launch_bounds__(64 * kSpWaves) void span_decode_kernel(const float *__restrict__ q, int H, KvCache c,
-                                                                    Span s, KvRows R, SpanRuns U, float scale,
-                                                                    float *__restrict__ part, float *__restrict__ out) {
+__global__ __launch_bounds__(64 * kSpWaves, Tile::kOcc) void span_decode_kernel(const float *__restrict__ q, int H, int G,
+                                                                       KvCache c, Span s, KvRows R, SpanRuns U,
+                                                                       float scale, float *__restrict__ part,
+                                                                       float *__restrict__ out) {
   constexpr int NK = HD / 32, ND = HD / 16, E = HD / 64, W = kSpWaves;
-  __shared__ float so[W][8][HD];
+  __shared__ sf4 so[W][8][HD / 4 + 4];  // a head's rows 16 floats past a multiple of the banks
   __shared__ float sm[W][8], sc2[8];
   __shared__ double sl[W][8];
+  __shared__ fh8 qs[NK][64];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, kq = lane >> 4, G = H / c.KH, CB = (G + 7) / 8;
-  const int unit = blockIdx.x % (c.KH * CB), run = blockIdx.x / (c.KH * CB);
-  const int kvh = unit % c.KH, cb = unit / c.KH;
+  const int col = lane & 15, kq = lane >> 4;
+  const int kvh = blockIdx.x, run = blockIdx.y, cb = blockIdx.z;
   const int t = __builtin_amdgcn_readfirstlane(
       __popcll(__ballot(lane < R.n && U.off[lane < R.n ? lane : 0] <= run)) - 1);
-  const int runs = U.off[t + 1] - U.off[t], mine = run - U.off[t];
+  const int runs = U.off[t + 1] - U.off[t], mine = run - U.off[t], per = U.per[t];
   const int p = R.position(t), first = s.first(p), lead = s.lead(p);
   const SpanTiles tl(s, p);
-  const int per = (tl.n + runs - 1) / runs, i0 = mine * per, i1 = i0 + per < tl.n ? i0 + per : tl.n;
+  const int i0 = mine * per, i1 = i0 + per < tl.n ? i0 + per : tl.n;
   const uint8_t *K, *V;
   int64_t stride = 0;
   if constexpr (Tile::kInf) {
@@ -291,25 +313,34 @@ __global__ __launch_bounds__(64 * kSpWaves) void span_decode_kernel(const float 
     K = c.K + head;
     V = c.V + head;
   }
-  Tile A, B;
+  constexpr int NT = 2;  // tiles in registers: two or three loaded ahead were no faster, and cost a wave per SIMD
+  Tile T[NT];
   int i = i0 + wv;
-  if (i < i1) A.load(K, V, stride, tl.tile(i), p, lane);
-  // the query's parts: head cb * 8 + col / 2, part col % 2, values kq HD / 4 + 8 step + 0..7
+#pragma unroll
+  for (int a = 0; a < NT - 1; a++)
+    if (i + a * W < i1) T[a].load(K, V, stride, tl.tile(i + a * W), p, lane);
+  // the query's parts: head cb * 8 + col / 2, part col % 2, values kq HD / 4 + 8 step + 0..7. A wave makes the parts of
+  // the steps wv, wv + W, ..; all read them from LDS.
   const bool low = col & 1;
   const int g = cb * 8 + (col >> 1) < G ? cb * 8 + (col >> 1) : G - 1;
-  fh8 qb[NK];
+  const uint32_t ones = fp16_ones();
   float c2;
   {
-    typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));
     const float *qp = q + ((int64_t)t * H + kvh * G + g) * HD + kq * (HD / 4);
-    float x[HD / 4], m = 0.f;
+    sf4 x[HD / 16];
+    float m = 0.f;
 #pragma unroll
-    for (int e = 0; e < HD / 16; e++) {
-      const f4a4 w = *reinterpret_cast<const f4a4 *>(qp + 4 * e);
-      x[4 * e] = w.x, x[4 * e + 1] = w.y, x[4 * e + 2] = w.z, x[4 * e + 3] = w.w;
+    for (int e = 0; e < HD / 16; e++) x[e] = *reinterpret_cast<const f4a4 *>(qp + 4 * e);
+#pragma unroll
+    for (int e = 0; e < HD / 16; e++)
+      m = fmaxf(m, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
+    if (__any(m == INFINITY)) {  // an infinity is all in its high part, and takes no part in the scale
+      m = 0.f;
+#pragma unroll
+      for (int e = 0; e < HD / 16; e++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) m = fabsf(x[e][j]) < INFINITY ? fmaxf(m, fabsf(x[e][j])) : m;
     }
-#pragma unroll
-    for (int e = 0; e < HD / 4; e++) m = fabsf(x[e]) < INFINITY ? fmaxf(m, fabsf(x[e])) : m;
     m = fmaxf(m, __shfl_xor(m, 16, 64));
     m = fmaxf(m, __shfl_xor(m, 32, 64));
     float f, inv;
@@ -319,117 +350,143 @@ __global__ __launch_bounds__(64 * kSpWaves) void span_decode_kernel(const float 
     f = scale < 0.f ? -f : f;
     if (scale != scale) c2 = scale;
 #pragma unroll
-    for (int e = 0; e < HD / 4; e++) {
-      const float X = x[e] * f;
-      const _Float16 a = (_Float16)X;
-      qb[e / 8][e % 8] = low ? (_Float16)(__builtin_isinf(X) ? 0.f : X - (float)a) : a;
+    for (int k = 0; k < NK; k++) {
+      if (k % W != wv) continue;  // uniform
+      fh8 b;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float X = x[2 * k + e / 4][e % 4] * f;
+        const _Float16 a = (_Float16)X;
+        b[e] = low ? (_Float16)(__builtin_isinf(X) ? 0.f : X - (float)a) : a;
+      }
+      qs[k][lane] = b;
     }
   }
+  __syncthreads();
+  fh8 qb[NK];
+#pragma unroll
+  for (int k = 0; k < NK; k++) qb[k] = qs[k][lane];
   sf4 O[ND];
 #pragma unroll
   for (int d = 0; d < ND; d++) O[d] = sf4{0.f, 0.f, 0.f, 0.f};
-  float M = -INFINITY;
+  float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
+  const float past = kSpPast / c2;
   double L = 0.0;
-  auto step = [&](Tile &T, int64_t tile) __attribute__((always_inline)) {
+  auto step = [&](Tile &A, int64_t tile) __attribute__((always_inline)) {
     const int p0 = (int)tile * kKv4Tile;
     sf4 S[2];
 #pragma unroll
     for (int t2 = 0; t2 < 2; t2++) {
       S[t2] = sf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < NK; k++) S[t2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.key(t2, k), qb[k], S[t2], 0, 0, 0);
+      for (int k = 0; k < NK; k++)
+        S[t2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.key(t2, k, ones), qb[k], S[t2], 0, 0, 0);
 #pragma unroll
       for (int e = 0; e < 4; e++) S[t2][e] = join_parts<Tile::kInf>(S[t2][e], low);
     }
     if (!(p0 + 31 <= p && (p0 >= first || p0 + 31 < lead))) {  // uniform: some position is not seen
+      asm volatile("");  // a branch, not selects in every tile
       uint32_t hid = 0;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const int at = p0 + 16 * (j >> 2) + 4 * kq + (j & 3);
-        if (at > p || (at >= lead && at < first)) {
-          hid |= 1u << j;
-          S[j >> 2][j & 3] = -INFINITY;
-        }
+        const bool no = (at > p) | ((at >= lead) & (at < first));
+        hid |= (uint32_t)no << j;
+        S[j >> 2][j & 3] = no ? -INFINITY : S[j >> 2][j & 3];
       }
-      T.hide(hid);
+      A.hide(hid);
     }
     float mt = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
                      fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
-    if (__any(mt > M)) {
+    if (__any(mt > top)) {
       mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-      const float Mn = fmaxf(M, mt), al = Mn > M ? __builtin_amdgcn_exp2f((M - Mn) * c2) : 1.f;
+      const bool up = mt > top;
+      const float al = up ? __builtin_amdgcn_exp2f((M - mt) * c2) : 1.f;
       L *= (double)al;
 #pragma unroll
       for (int d = 0; d < ND; d++) O[d] *= al;
-      M = Mn;
+      M = up ? mt : M;
+      top = M + past;
     }
-    const float Mu = M == -INFINITY ? 0.f : M;
-    fh8 pb;
+    const float Mu = M == -INFINITY ? 0.f : M;  // no key of this row yet: every score is -inf
+    uint32_t pb[4];
     float ts[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float P = __builtin_amdgcn_exp2f((S[j >> 2][j & 3] - Mu) * c2);
-      ts[j & 1] += P;
-      const _Float16 a = (_Float16)(P * kSpUp);
-      pb[j] = low ? (_Float16)__builtin_fmaf(P, kSpUp, -(float)a) : a;
+    for (int j = 0; j < 4; j++) {
+      const float P0 = __builtin_amdgcn_exp2f((S[j >> 1][2 * (j & 1)] - Mu) * c2);
+      const float P1 = __builtin_amdgcn_exp2f((S[j >> 1][2 * (j & 1) + 1] - Mu) * c2);
+      ts[0] += P0;
+      ts[1] += P1;
+      const float Q0 = P0 * kSpUp, Q1 = P1 * kSpUp;
+      uint32_t hi = __builtin_bit_cast(uint32_t, fh2{(_Float16)Q0, (_Float16)Q1});
+      asm("" : "+v"(hi));  // rounded once: the compiler made the halves again for the low parts
+      const fh2 lo = {(_Float16)(Q0 - half_lo(hi)), (_Float16)(Q1 - half_hi(hi))};
+      pb[j] = low ? __builtin_bit_cast(uint32_t, lo) : hi;
     }
+    const fh8 pv = as_fh8(pb[0], pb[1], pb[2], pb[3]);
     L += (double)(ts[0] + ts[1]);
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      O[4 * e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<0>(e), pb, O[4 * e], 0, 0, 0);
-      O[4 * e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<1>(e), pb, O[4 * e + 1], 0, 0, 0);
-      O[4 * e + 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<2>(e), pb, O[4 * e + 2], 0, 0, 0);
-      O[4 * e + 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.template val<3>(e), pb, O[4 * e + 3], 0, 0, 0);
+      O[4 * e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.template val<0>(e, ones), pv, O[4 * e], 0, 0, 0);
+      O[4 * e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.template val<1>(e, ones), pv, O[4 * e + 1], 0, 0, 0);
+      O[4 * e + 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.template val<2>(e, ones), pv, O[4 * e + 2], 0, 0, 0);
+      O[4 * e + 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A.template val<3>(e, ones), pv, O[4 * e + 3], 0, 0, 0);
     }
   };
 #pragma unroll 1
   while (i < i1) {
-    if (i + W < i1) B.load(K, V, stride, tl.tile(i + W), p, lane);
-    step(A, tl.tile(i));
-    i += W;
-    if (i >= i1) break;
-    if (i + W < i1) A.load(K, V, stride, tl.tile(i + W), p, lane);
-    step(B, tl.tile(i));
-    i += W;
+#pragma unroll
+    for (int a = 0; a < NT; a++) {
+      if (i + (NT - 1) * W < i1) T[(a + NT - 1) % NT].load(K, V, stride, tl.tile(i + (NT - 1) * W), p, lane);
+      step(T[a], tl.tile(i));
+      i += W;
+      if (i >= i1) break;
+    }
   }
-  // the waves' sums under their largest maximum; row x of block d is value 4 E x + d
+  // the waves' sums under their largest maximum; of two neighbouring lanes one writes the even blocks, one the odd
   L += __shfl_xor(L, 16, 64);
   L += __shfl_xor(L, 32, 64);
 #pragma unroll
-  for (int d = 0; d < ND; d++)
+  for (int d = 0; d < ND; d += 2) {
+    sf4 o;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float o = join_parts<Tile::kInf>(O[d][e], low);
-      if (!low) so[wv][col >> 1][4 * E * (4 * kq + e) + d] = o;
+      const float a = join_parts<Tile::kInf>(O[d][e], low), b = join_parts<Tile::kInf>(O[d + 1][e], low);
+      o[e] = low ? b : a;
     }
+    so[wv][col >> 1][4 * (d + (int)low) + kq] = o;
+  }
   if (!low && kq == 0) {
     sm[wv][col >> 1] = M;
     sl[wv][col >> 1] = L;
     sc2[col >> 1] = c2;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 8 * HD; e += 64 * W) {
-    const int gg = e / HD, d = e % HD, h = cb * 8 + gg;
-    if (h >= G) break;  // heads past the group: uniform over what follows
+  for (int e = threadIdx.x; e < 2 * HD; e += 64 * W) {
+    const int gg = e / (HD / 4), four = e % (HD / 4), h = cb * 8 + gg;
+    if (h >= G) break;
     float m = sm[0][gg];
 #pragma unroll
     for (int w = 1; w < W; w++) m = fmaxf(m, sm[w][gg]);
-    float o = 0.f;
+    sf4 o = {0.f, 0.f, 0.f, 0.f};
     double l = 0.0;
 #pragma unroll
     for (int w = 0; w < W; w++) {
       const float f = __builtin_amdgcn_exp2f((sm[w][gg] - m) * sc2[gg]);
-      o += so[w][gg][d] * f;
+      o += so[w][gg][four] * f;
       l += sl[w][gg] * (double)f;
     }
     const int64_t row = (int64_t)t * H + kvh * G + h;
     if (runs == 1) {
-      out[row * HD + d] = (float)((double)o * (1.0 / kSpUp) / l);
+      const double r = (1.0 / kSpUp) / l;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = (float)((double)o[j] * r);
+      span_store<HD>(out + row * HD, four, o);
     } else {
       float *rec = part + (row * U.most + mine) * (HD + 4);
-      rec[d] = o;
-      if (d == 0) {
+      *reinterpret_cast<sf4 *>(rec + 4 * four) = o;
+      if (four == 0) {
         rec[HD] = m;
         rec[HD + 1] = sc2[gg];
         *reinterpret_cast<double *>(rec + HD + 2) = l;
@@ -438,46 +495,73 @@ __global__ __launch_bounds__(64 * kSpWaves) void span_decode_kernel(const float 
   }
 }
 
-// Rows of more than one run: the runs' sums under their largest maximum, in order. One wave per (row, head).
+// Rows of more than one run: the runs' sums under their largest maximum. A workgroup per (row, head): the
+// runs' factors once, into LDS; then HD / 4 threads to a record, the records over the groups in turn, each group's
+// sum in order and the groups' in order.
 template <int HD>
-__global__ __launch_bounds__(64) void span_join_kernel(const float *__restrict__ part, int H, SpanRuns U,
-                                                       float *__restrict__ out) {
-  const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
+__global__ __launch_bounds__(256) void span_join_kernel(const float *__restrict__ part, int H, SpanRuns U,
+                                                        float *__restrict__ out) {
+  constexpr int TH = HD / 4, NG = 256 / TH;
+  __shared__ float f[kSpRuns], sm[4];
+  __shared__ double sl[4];
+  __shared__ sf4 so[NG][TH];
+  const int h = blockIdx.x, t = blockIdx.y, tid = threadIdx.x;
   const int n = U.off[t + 1] - U.off[t];
   if (n == 1) return;
   const int64_t row = (int64_t)t * H + h;
   const float *rec = part + row * U.most * (HD + 4);
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, rec[i * (HD + 4) + HD]);
-  m = wave_max_f(m);
-  float o[HD / 64] = {};
-  double l = 0.0;
-  for (int b = 0; b < n; b += 64) {
-    const int i = b + lane < n ? b + lane : n - 1;
-    const float *r = rec + i * (HD + 4);
-    const float f = b + lane < n ? __builtin_amdgcn_exp2f((r[HD] - m) * r[HD + 1]) : 0.f;
-    l += *reinterpret_cast<const double *>(r + HD + 2) * (double)f;
-    const int k = n - b < 64 ? n - b : 64;
-#pragma unroll 8
-    for (int j = 0; j < k; j++) {
-      const float w = lane_f(f, j);
+  static_assert(kSpRuns == 256, "a thread per run");
+  const float *mine = rec + (tid < n ? tid : n - 1) * (HD + 4);
+  const float m1 = mine[HD], c2 = mine[HD + 1];
+  const double l1 = *reinterpret_cast<const double *>(mine + HD + 2);
+  float m = wave_max_f(m1);
+  if ((tid & 63) == 0) sm[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  const float f1 = tid < n ? __builtin_amdgcn_exp2f((m1 - m) * c2) : 0.f;
+  f[tid] = f1;
+  const double l = wave_sum_d(tid < n ? l1 * (double)f1 : 0.0);
+  if ((tid & 63) == 0) sl[tid >> 6] = l;
+  __syncthreads();
+  const int g = tid / TH, x = tid % TH;
+  sf4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int i = g; i < n; i += 4 * NG) {
+    sf4 v[4];
 #pragma unroll
-      for (int e = 0; e < HD / 64; e++) o[e] = __builtin_fmaf(rec[(b + j) * (HD + 4) + lane + 64 * e], w, o[e]);
+    for (int k = 0; k < 4; k++) {
+      const int r = i + k * NG < n ? i + k * NG : i;
+      v[k] = *reinterpret_cast<const sf4 *>(rec + r * (HD + 4) + 4 * x);
     }
-  }
-  l = wave_sum_d(l);
 #pragma unroll
-  for (int e = 0; e < HD / 64; e++) out[row * HD + lane + 64 * e] = (float)((double)o[e] * (1.0 / kSpUp) / l);
+    for (int k = 0; k < 4; k++)
+      if (i + k * NG < n) o += v[k] * f[i + k * NG];
+  }
+  so[g][x] = o;
+  __syncthreads();
+  if (tid < TH) {
+    sf4 s = so[0][tid];
+#pragma unroll
+    for (int k = 1; k < NG; k++) s += so[k][tid];
+    const double r = (1.0 / kSpUp) / ((sl[0] + sl[1]) + (sl[2] + sl[3]));
+    sf4 w;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = (float)((double)s[e] * r);
+    span_store<HD>(out + row * HD, tid, w);
+  }
 }
 
-// Runs of a row of n tiles.
-static int span_runs(int n, int units) {
-  int r = (n + kSpWaves - 1) / kSpWaves;
-  const int fill = (512 + units - 1) / units;
-  r = r > fill ? fill : r;
-  r = r > kSpRuns ? kSpRuns : r;
-  const int per = (n + r - 1) / r;
-  return (n + per - 1) / per;
+// Tiles of each run of a row of n tiles (a rule on the row alone). Up to 16 tiles one run, and no second launch
+// (32 heads of 64, 7 rows at 333: 6.0 us, two runs 9.2). More: two tiles a wave, where a lone row is short of waves, to
+// four from 256 tiles on, where a run's fixed work (the query's parts, the sums through LDS, its record) weighs more
+// (64 heads of 128: one row after 4,000 10.1 us, four tiles a wave 11.7; 32 rows of up to 9,001 62 us, two
+// tiles 69, one 89). And no more runs than give every CU two workgroups.
+static int span_per(int n, int units) {
+  if (n <= 16) return n;
+  int fill = (512 + units - 1) / units;
+  fill = fill > kSpRuns ? kSpRuns : fill;
+  int per = (n + 15) / 16;
+  per = per < 2 * kSpWaves ? 2 * kSpWaves : per > 4 * kSpWaves ? 4 * kSpWaves : per;
+  return per < (n + fill - 1) / fill ? (n + fill - 1) / fill : per;
 }
 
 static bool span_tiled(const KvCache &c) {
@@ -489,7 +573,9 @@ static SpanRuns span_plan(const KvCache &c, int H, const Span &s, const KvRows &
   SpanRuns U = {};
   const int units = c.KH * ((H / c.KH + 7) / 8);
   for (int t = 0; t < R.n; t++) {
-    const int r = span_runs(SpanTiles(s, R.position(t)).n, units);
+    const int n = SpanTiles(s, R.position(t)).n;
+    U.per[t] = span_per(n, units);
+    const int r = (n + U.per[t] - 1) / U.per[t];
     U.off[t + 1] = U.off[t] + r;
     U.most = r > U.most ? r : U.most;
   }
@@ -500,12 +586,12 @@ template <int HD, class Tile>
 static hipError_t span_decode_launch(const float *q, int H, const KvCache &c, const Span &s, const KvRows &R, float scale,
                                      float *part, float *out, hipStream_t st) {
   const SpanRuns U = span_plan(c, H, s, R);
-  const int units = c.KH * ((H / c.KH + 7) / 8);
-  hipLaunchKernelGGL((span_decode_kernel<HD, Tile>), dim3((unsigned)((int64_t)U.off[R.n] * units)),
-                     dim3(64 * kSpWaves), 0, st, q, H, c, s, R, U, scale, part, out);
+  const int G = H / c.KH;
+  hipLaunchKernelGGL((span_decode_kernel<HD, Tile>), dim3(c.KH, U.off[R.n], (G + 7) / 8), dim3(64 * kSpWaves), 0, st, q,
+                     H, G, c, s, R, U, scale, part, out);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || U.most == 1) return e;
-  hipLaunchKernelGGL(span_join_kernel<HD>, dim3(H, R.n), dim3(64), 0, st, part, H, U, out);
+  hipLaunchKernelGGL(span_join_kernel<HD>, dim3(H, R.n), dim3(256), 0, st, part, H, U, out);
   return hipGetLastError();
 }
 
