@@ -5,6 +5,8 @@
 
 #include "wl_fmma_codec.h"
 
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace wl {
@@ -14,25 +16,6 @@ struct F16Rows {
   int64_t kv_dim;
   __device__ float key(int64_t j, int i) const { return (float)__builtin_bit_cast(_Float16, K[j * kv_dim + i]); }
   __device__ float val(int64_t j, int i) const { return (float)__builtin_bit_cast(_Float16, V[j * kv_dim + i]); }
-};
-
-struct Kv4Rows {
-  const uint8_t *K, *V;  // the head's tiles
-  int HD;
-  __device__ float key(int64_t j, int i) const {
-    const uint8_t *t = K + j / kKv4Tile * (18 * HD);
-    const int r = (int)(j % kKv4Tile);
-    const uint32_t w = reinterpret_cast<const uint32_t *>(t)[kv4_key_word(r, i >> 3, HD)];
-    return kv4_value((w >> (16 * (i & 1) + 4 * ((i & 7) >> 1))) & 15u,
-                     reinterpret_cast<const uint16_t *>(t + 16 * HD)[kv4_key_scale(r, i >> 5, HD)]);
-  }
-  __device__ float val(int64_t j, int i) const {
-    const uint8_t *t = V + j / kKv4Tile * (18 * HD);
-    const int r = (int)(j % kKv4Tile);
-    const uint32_t w = reinterpret_cast<const uint16_t *>(t)[kv4_val_half(r, i >> 2, HD)];
-    return kv4_value((w >> (4 * (i & 3))) & 15u,
-                     reinterpret_cast<const uint16_t *>(t + 16 * HD)[kv4_val_scale(r, i >> 5, HD)]);
-  }
 };
 
 // Block-wide sum and maximum of 256 threads.
@@ -53,9 +36,9 @@ __device__ float span_max(float v, float *sh) {
   return v;
 }
 
-// One workgroup per (head, row): scores, their maximum, exponentials, sums.
-template <class C>
-__device__ void span_row(const C &c, const float *qp, int HD, int p, const Span &s, float scale, float *sp, float *op) {
+// fp16 caches of other head dims than 64 and 128: one workgroup per (head, row): scores, their maximum,
+// exponentials, sums.
+__device__ void span_row(const F16Rows &c, const float *qp, int HD, int p, const Span &s, float scale, float *sp, float *op) {
   __shared__ double shd[4];
   __shared__ float shf[4];
   const int first = s.first(p), lead = s.lead(p), n = s.seen(p);
@@ -89,14 +72,9 @@ __global__ __launch_bounds__(256) void span_rows_kernel(const float *__restrict_
   const int h = blockIdx.x, t = blockIdx.y, kvh = h / (H / c.KH), HD = c.HD;
   const int64_t row = ((int64_t)t * H + h), off = (int64_t)R.slot_of(t) * c.slot_bytes;
   const float *qp = q + row * HD;
-  if (c.bits == 4) {
-    const int64_t head = off + (int64_t)kvh * ((c.positions + kKv4Tile - 1) / kKv4Tile) * (18 * HD);
-    span_row(Kv4Rows{c.K + head, c.V + head, HD}, qp, HD, R.position(t), s, scale, scores + row * max_n, out + row * HD);
-  } else {
-    const int64_t head = off + (int64_t)kvh * HD * 2;
-    span_row(F16Rows{(const uint16_t *)(c.K + head), (const uint16_t *)(c.V + head), (int64_t)c.KH * HD}, qp, HD,
-             R.position(t), s, scale, scores + row * max_n, out + row * HD);
-  }
+  const int64_t head = off + (int64_t)kvh * HD * 2;
+  span_row(F16Rows{(const uint16_t *)(c.K + head), (const uint16_t *)(c.V + head), (int64_t)c.KH * HD}, qp, HD,
+           R.position(t), s, scale, scores + row * max_n, out + row * HD);
 }
 
 // ------------------------------------------------------------------------------- few rows
@@ -149,6 +127,14 @@ __device__ __forceinline__ fh8 as_fh8(uint32_t a, uint32_t b, uint32_t c, uint32
   return __builtin_bit_cast(fh8, u32x4_t{a, b, c, d});
 }
 __device__ __forceinline__ fh2 scale15(fh2 s) { return s * fh2{(_Float16)-1.5f, (_Float16)-1.5f}; }
+
+// Two probabilities, times kSpUp, as their fp16 parts.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint32_t &lo) {
+  hi = __builtin_bit_cast(uint32_t, fh2{(_Float16)__builtin_fmaf(a, kSpUp, 0.f), (_Float16)__builtin_fmaf(b, kSpUp, 0.f)});
+  asm("" : "+v"(hi));  // rounded once: the compiler made the halves again for the low parts
+  lo = __builtin_bit_cast(uint32_t, fh2{(_Float16)__builtin_fmaf(a, kSpUp, -half_lo(hi)),
+                                        (_Float16)__builtin_fmaf(b, kSpUp, -half_hi(hi))});  // exact but for their rounding
+}
 
 // Tiles of 4-bit caches. hide(m): bit j set where key j of the lane (keys 16 (j / 4) + 4 kq + j % 4) is not seen:
 // its values become zeros.
@@ -418,11 +404,9 @@ __global__ __launch_bounds__(64 * kSpWaves, Tile::kOcc) void span_decode_kernel(
       const float P1 = __builtin_amdgcn_exp2f((S[j >> 1][2 * (j & 1) + 1] - Mu) * c2);
       ts[0] += P0;
       ts[1] += P1;
-      const float Q0 = P0 * kSpUp, Q1 = P1 * kSpUp;
-      uint32_t hi = __builtin_bit_cast(uint32_t, fh2{(_Float16)Q0, (_Float16)Q1});
-      asm("" : "+v"(hi));  // rounded once: the compiler made the halves again for the low parts
-      const fh2 lo = {(_Float16)(Q0 - half_lo(hi)), (_Float16)(Q1 - half_hi(hi))};
-      pb[j] = low ? __builtin_bit_cast(uint32_t, lo) : hi;
+      uint32_t hi, lo;
+      split_pair(P0, P1, hi, lo);
+      pb[j] = low ? lo : hi;
     }
     const fh8 pv = as_fh8(pb[0], pb[1], pb[2], pb[3]);
     L += (double)(ts[0] + ts[1]);
@@ -564,6 +548,501 @@ static int span_per(int n, int units) {
   return per < (n + fill - 1) / fill ? (n + fill - 1) / fill : per;
 }
 
+// ------------------------------------------------------------------------------- prompts
+// Rows of 16 tokens and more on v_mfma_f32_32x32x16_f16 (head dims 64 and 128), the products and parts of
+// wl_attention.hip: S^T = K Q^T, a column per (token, query head of the KV head) in the order token * G + head,
+// 32 columns a wave, 64 keys a step, staged in LDS for the workgroup's four waves as fp16 rows of keys and, transposed,
+// rows of values in the order in which the scores' registers meet them. Two stages: a step's keys are unpacked while the
+// step before is multiplied, with one barrier between steps. A row's maximum is an integer in log2 units, so that the
+// exponential's argument is one rounding (S c2 - m), and raised only by scores more than 2^6 past it.
+constexpr int kTlK = 64, kTlW = 4, kTlCols = 32 * kTlW;
+typedef float sf16 __attribute__((ext_vector_type(16)));
+
+// The steps of a workgroup whose rows are t0 .. t1 at pos0: those of the first tokens, then the windows'.
+struct SpanSteps {
+  int lead, from, n;
+  __host__ __device__ SpanSteps(const Span &s, int first_row, int last_row) {
+    const int l = s.lead(last_row);
+    lead = (l + kTlK - 1) / kTlK;
+    from = s.first(first_row) / kTlK;
+    from = from < lead ? lead : from;
+    n = last_row / kTlK >= from ? lead + last_row / kTlK - from + 1 : lead;
+  }
+  __host__ __device__ int at(int i) const { return (i < lead ? i : from + (i - lead)) * kTlK; }
+};
+
+struct TilesArgs {
+  Span s;
+  int T, pos0, G, KH, nz, chunks, steps;  // nz workgroups of columns a KV head, chunks of `steps` steps each
+  __host__ __device__ int row0(int z) const { return pos0 + (int)((int64_t)z * kTlCols / G); }
+  __host__ __device__ int row1(int z) const {
+    const int64_t last = ((int64_t)z * kTlCols + kTlCols - 1) / G;
+    return pos0 + (int)(last < T - 1 ? last : T - 1);
+  }
+};
+
+// LDS place (halves) of value row `dim`: rows of 128 bytes, the 16-byte pieces of a row in an order of the row's own, so
+// that reads of 32 rows and writes of every eighth row both meet all banks.
+__device__ __forceinline__ int val_at(int dim, int slot) {
+  return dim * kTlK + ((((slot >> 3) ^ dim ^ (dim >> 3)) & 7) << 3 | (slot & 7));
+}
+// Keeps a value from being computed ahead of a loop into a register of its own.
+__device__ __forceinline__ int here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// A step's keys and values of one KV head from 4-bit tiles, a block of 32 key values and one of 4 x 8 values a thread.
+template <int HD>
+struct StageKv4 {
+  static constexpr int NB = HD / 32, E = HD / 64, UN = 64 * NB;  // units of 16 bytes of each
+  static constexpr bool kInf = false;
+  u32x4_t k, v, vs;
+  uint16_t ks;
+  int kkey, kblk, vt, vl, ve, vblk;
+  const uint8_t *K, *V;
+  bool doK, doV;
+  __device__ void init(const KvCache &c, int kvh, int tid) {
+    const int64_t head = (int64_t)kvh * ((c.positions + 31) / 32) * (18 * HD);
+    K = c.K + head;
+    V = c.V + head;
+    doK = HD == 128 || tid < UN;
+    doV = HD == 128 || tid >= UN;
+    const int ku = tid & (UN - 1);
+    kkey = ku / NB;
+    kblk = ku % NB;
+    vt = ku / (UN / 2);  // tile of the step
+    ve = ku / 64 % E;
+    vl = ku % 64;
+    vblk = (vl & 15) * E / 8;
+  }
+  __device__ __forceinline__ void fetch(int j0, int last) {
+    const int lt = last / 32;
+    if (doK) {
+      const int tile = (j0 + kkey) / 32 < lt ? (j0 + kkey) / 32 : lt, r = kkey & 31;
+      const uint8_t *t = K + (int64_t)tile * (18 * HD);
+      k = *reinterpret_cast<const u32x4_t *>(t + r * (HD / 2) + 16 * kblk);
+      ks = reinterpret_cast<const uint16_t *>(t + 16 * HD)[kv4_key_scale(r, kblk, HD)];
+    }
+    if (doV) {
+      const int tile = j0 / 32 + vt < lt ? j0 / 32 + vt : lt;
+      const uint8_t *t = V + (int64_t)tile * (18 * HD);
+      v = reinterpret_cast<const u32x4_t *>(t)[ve * 64 + vl];
+      vs = *reinterpret_cast<const u32x4_t *>(t + 16 * HD + ((vl >> 4) * NB + vblk) * 16);
+    }
+  }
+  // Into LDS; true where a value of a position up to `last` is NaN (it becomes zero there).
+  __device__ __forceinline__ bool stage(uint16_t *lk, uint16_t *lv, int j0, int last, uint32_t ones, bool &) {
+    constexpr int KS = HD + 8;
+    if (doK) {
+      const _Float16 h = __builtin_bit_cast(_Float16, ks);
+      const fh2 sc = {h, h}, s15 = scale15(sc);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t w = k[i];
+        *reinterpret_cast<u32x4_t *>(lk + kkey * KS + 32 * kblk + 8 * i) =
+            u32x4_t{kv4_pair<0>(w, sc, s15, ones), kv4_pair<1>(w, sc, s15, ones), kv4_pair<2>(w, sc, s15, ones),
+                    kv4_pair<3>(w, sc, s15, ones)};
+      }
+    }
+    bool bad = false;
+    if (doV) {
+      const int kq = vl >> 4, dim = 4 * E * (vl & 15) + 4 * ve, p0 = j0 + 32 * vt + 4 * kq;
+      u32x4_t sc = vs;
+      if (p0 + 19 > last) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int at = p0 + 16 * (j >> 1) + 2 * (j & 1);
+          sc[j] &= (at > last ? 0u : 0xffffu) | (at + 1 > last ? 0u : 0xffff0000u);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {  // a scale is finite or NaN
+        const bool lo = (sc[j] & 0x7c00u) == 0x7c00u, hi = (sc[j] & 0x7c000000u) == 0x7c000000u;
+        bad |= lo | hi;
+        sc[j] = lo ? sc[j] & 0xffff0000u : sc[j];
+        sc[j] = hi ? sc[j] & 0xffffu : sc[j];
+      }
+      // val_at(dim + i, slot + 16 h): dim is a multiple of 4
+      const int base = here(val_at(dim, 32 * vt + 8 * (kq & 1) + 4 * (kq >> 1)));
+      fh2 s2[4], s15[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        s2[j] = as_fh2(sc[j]);
+        s15[j] = scale15(s2[j]);
+      }
+      auto put = [&](auto I) __attribute__((always_inline)) {
+        constexpr int i = decltype(I)::value;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          *reinterpret_cast<u32x2_t *>(lv + ((base + i * kTlK) ^ (i ^ 2 * h) << 3)) =
+              u32x2_t{kv4_pair<i>(v[2 * h], s2[2 * h], s15[2 * h], ones),
+                      kv4_pair<i>(v[2 * h + 1], s2[2 * h + 1], s15[2 * h + 1], ones)};
+      };
+      put(std::integral_constant<int, 0>());
+      put(std::integral_constant<int, 1>());
+      put(std::integral_constant<int, 2>());
+      put(std::integral_constant<int, 3>());
+    }
+    return bad;
+  }
+  // NaN blocks of position p into the outputs of a lane that sees it (block d of its 32-value blocks).
+  template <class O>
+  __device__ void add_bad(int p, int, O &o) const {
+    const uint16_t *sc = reinterpret_cast<const uint16_t *>(V + (int64_t)(p / 32) * (18 * HD) + 16 * HD);
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+      if ((sc[kv4_val_scale(p % 32, d, HD)] & 0x7c00u) == 0x7c00u) o[d] += __builtin_nanf("");
+  }
+};
+
+// The same from fp16 rows.
+template <int HD>
+struct StageF16 {
+  static constexpr int U = HD / 8, KI = 64 * U / 256;
+  static constexpr bool kInf = true;
+  u32x4_t k[KI], v[4];
+  const uint16_t *K, *V;
+  int64_t kv_dim;
+  int tid, kg, dg;
+  __device__ void init(const KvCache &c, int kvh, int t) {
+    K = reinterpret_cast<const uint16_t *>(c.K) + kvh * HD;
+    V = reinterpret_cast<const uint16_t *>(c.V) + kvh * HD;
+    kv_dim = (int64_t)c.KH * HD;
+    tid = t;
+    dg = t % U;
+    kg = t / U;
+  }
+  __device__ __forceinline__ void fetch(int j0, int last) {
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+      const int e = tid + 256 * i, row = j0 + e / U < last ? j0 + e / U : last;  // past the end: the last row again, masked
+      k[i] = *reinterpret_cast<const u32x4_t *>(K + (int64_t)row * kv_dim + 8 * (e % U));
+    }
+    if (kg < 16) {
+#pragma unroll
+      for (int b = 0; b < 4; b++) {
+        const int row = j0 + 4 * kg + b < last ? j0 + 4 * kg + b : last;
+        v[b] = *reinterpret_cast<const u32x4_t *>(V + (int64_t)row * kv_dim + 8 * dg);
+      }
+    }
+  }
+  __device__ static __forceinline__ bool nonfinite(u32x4_t w) {
+    bool b = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) b |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+    return b;
+  }
+  __device__ __forceinline__ bool stage(uint16_t *lk, uint16_t *lv, int, int, uint32_t, bool &badk) {
+    constexpr int KS = HD + 8;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+      const int e = tid + 256 * i;
+      badk |= nonfinite(k[i]);
+      *reinterpret_cast<u32x4_t *>(lk + (e / U) * KS + 8 * (e % U)) = k[i];
+    }
+    if (kg < 16) {
+#pragma unroll
+      for (int b = 0; b < 4; b++) bad |= nonfinite(v[b]);
+      if (bad) {
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            v[b][i] = (v[b][i] & 0x7c00u) == 0x7c00u ? v[b][i] & 0xffff0000u : v[b][i];
+            v[b][i] = (v[b][i] & 0x7c000000u) == 0x7c000000u ? v[b][i] & 0xffffu : v[b][i];
+          }
+      }
+      // val_at(8 dg + i, slot)
+      const int base = here(val_at(8 * dg, 16 * (kg >> 2) + 8 * (kg & 1) + 4 * ((kg >> 1) & 1)));
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t a0 = __builtin_amdgcn_perm(v[1][i], v[0][i], 0x05040100u);
+        const uint32_t a1 = __builtin_amdgcn_perm(v[3][i], v[2][i], 0x05040100u);
+        const uint32_t b0 = __builtin_amdgcn_perm(v[1][i], v[0][i], 0x07060302u);
+        const uint32_t b1 = __builtin_amdgcn_perm(v[3][i], v[2][i], 0x07060302u);
+        *reinterpret_cast<u32x2_t *>(lv + ((base + 2 * i * kTlK) ^ 2 * i << 3)) = u32x2_t{a0, a1};
+        *reinterpret_cast<u32x2_t *>(lv + ((base + (2 * i + 1) * kTlK) ^ (2 * i + 1) << 3)) = u32x2_t{b0, b1};
+      }
+    }
+    return bad;
+  }
+  template <class O>
+  __device__ void add_bad(int p, int hf, O &o) const {
+    const uint16_t *vp = V + (int64_t)p * kv_dim;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const uint16_t w = vp[32 * d + 8 * (i >> 2) + 4 * hf + (i & 3)];
+        if ((w & 0x7c00u) == 0x7c00u) o[d][i] += (float)__builtin_bit_cast(_Float16, w);
+      }
+  }
+};
+
+template <int HD, class Stage>
+__global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restrict__ q, KvCache c, TilesArgs A,
+                                                            float scale, float *__restrict__ part,
+                                                            float *__restrict__ out) {
+  constexpr int NK = HD / 16, ND = HD / 32, KS = HD + 8;
+  __shared__ __attribute__((aligned(16))) uint16_t lk[2][kTlK * KS];
+  __shared__ __attribute__((aligned(16))) uint16_t lv[2][HD * kTlK];
+  __shared__ int bads[2][2][kTlW];
+  const int kvh = blockIdx.x % A.KH, ch = blockIdx.x / A.KH % A.chunks, r = blockIdx.x / A.KH / A.chunks;
+  // longest and shortest rows in turn: the workgroups that share a CU (the grid's halves) add up
+  const int z = r < (A.nz + 1) / 2 ? A.nz - 1 - r : r - (A.nz + 1) / 2;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hf = lane >> 5, col = lane & 31, G = A.G, H = G * A.KH;
+  const int last = A.row1(z);
+  const SpanSteps st(A.s, A.row0(z), last);
+  const int i0 = ch * A.steps, i1 = i0 + A.steps < st.n ? i0 + A.steps : st.n;
+  if (i0 >= i1) return;  // uniform over the workgroup
+  const int64_t NC = (int64_t)A.T * G, u = (int64_t)z * kTlCols + 32 * wv + col, uc = u < NC ? u : NC - 1;
+  const int t = (int)(uc / G), h = kvh * G + (int)(uc % G);
+  const int p = A.pos0 + t, first = A.s.first(p), lead = A.s.lead(p);
+  // the wave's rows
+  const int64_t w0 = (int64_t)z * kTlCols + 32 * wv;
+  const bool idle = w0 >= NC;
+  const int pa = A.pos0 + (int)((w0 < NC ? w0 : NC - 1) / G), pb = A.pos0 + (int)((w0 + 31 < NC ? w0 + 31 : NC - 1) / G);
+  const int firsta = A.s.first(pa), firstb = A.s.first(pb), leada = A.s.lead(pa), leadb = A.s.lead(pb);
+
+  Stage sg;
+  sg.init(c, kvh, tid);
+  sg.fetch(st.at(i0), last);
+  // the query's parts, in operand order: k = 16 i + 8 hf + 0..7
+  fh8 qh[NK], ql[NK];
+  float c2;
+  {
+    const float *qp = q + ((int64_t)t * H + h) * HD + 8 * hf;
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NK; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float a = fabsf(qp[16 * i + j]);
+        m = a < INFINITY ? fmaxf(m, a) : m;
+      }
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    float f, inv;
+    unit_scale(m, f, inv);
+    // scores in units of log2: c2 > 0 (a negative scale negates the query)
+    c2 = fmaxf(fabsf(scale) * 1.4426950408889634f * inv, 1.1754944e-38f);
+    f = scale < 0.f ? -f : f;
+    if (scale != scale) c2 = scale;
+#pragma unroll
+    for (int i = 0; i < NK; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float X = qp[16 * i + j] * f;
+        const _Float16 a = (_Float16)X;
+        qh[i][j] = a;
+        ql[i][j] = (_Float16)(__builtin_isinf(X) ? 0.f : X - (float)a);
+      }
+  }
+  sf16 O[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) O[d][i] = 0.f;
+  float M = -INFINITY, top = -INFINITY;  // log2 units; top: the score that raises it
+  double L = 0.0;
+  const uint32_t ones = fp16_ones();
+  auto stage = [&](int b, int j0) __attribute__((always_inline)) {
+    bool bk = false;
+    const bool bv = sg.stage(lk[b], lv[b], j0, last, ones, bk);
+    const bool ak = Stage::kInf && __any(bk), av = __any(bv);
+    if (lane == 0) {
+      bads[b][0][wv] = ak;
+      bads[b][1][wv] = av;
+    }
+  };
+  stage(0, st.at(i0));
+  if (i0 + 1 < i1) sg.fetch(st.at(i0 + 1), last);
+  __syncthreads();
+#pragma unroll 1
+  for (int i = i0; i < i1; i++) {
+    const int b = (i - i0) & 1, j0 = st.at(i);
+    const uint16_t *kb = lk[b], *vb = lv[b];
+    const bool badk = Stage::kInf && (bads[b][0][0] | bads[b][0][1] | bads[b][0][2] | bads[b][0][3]) != 0;
+    const bool badv = (bads[b][1][0] | bads[b][1][1] | bads[b][1][2] | bads[b][1][3]) != 0;
+    // uniform over the wave: some row of it sees some key
+    const bool on = !idle && j0 <= pb && (j0 + kTlK - 1 >= firsta || j0 < leadb);
+    float ts[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      if (on) {
+        const uint16_t *kp = kb + (32 * s + col) * KS + 8 * hf;
+        sf16 S;
+#pragma unroll
+        for (int e = 0; e < 16; e++) S[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+          S = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), ql[k], S, 0, 0, 0);
+        if (badk) {  // past an infinity the low parts' product means nothing
+          const sf16 B = S;
+#pragma unroll
+          for (int e = 0; e < 16; e++) S[e] = 0.f;
+#pragma unroll
+          for (int k = 0; k < NK; k++)
+            S = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), qh[k], S, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 16; e++) S[e] = __builtin_isfinite(S[e]) ? S[e] + B[e] : S[e];
+        } else {
+#pragma unroll
+          for (int k = 0; k < NK; k++)
+            S = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), qh[k], S, 0, 0, 0);
+        }
+        const int js = j0 + 32 * s;
+        if (!(js + 31 <= pa && (js >= firstb || js + 31 < leada))) {  // uniform: some row does not see every key
+          asm volatile("");
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const int at = js + 8 * (e >> 2) + 4 * hf + (e & 3);
+            S[e] = (at > p) | ((at >= lead) & (at < first)) ? -INFINITY : S[e];
+          }
+        }
+        float mt = S[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) mt = fmaxf(mt, S[e]);
+        mt *= c2;
+        if (__any(mt > top)) {
+          mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+          const bool up = mt > top;
+          const float Mn = up ? ceilf(mt) : M;
+          const float al = up ? __builtin_amdgcn_exp2f(M - Mn) : 1.f;
+          L *= (double)al;
+#pragma unroll
+          for (int e = 0; e < 4; e++) ts[e] *= al;
+#pragma unroll
+          for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) O[d][e] *= al;
+          M = Mn;
+          top = M + kSpPast;
+        }
+        const float Mu = M == -INFINITY ? 0.f : M;  // no key of this row yet: every score is -inf
+        const int va = here(val_at(col, 8 * hf));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float P0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * k + 2 * e], c2, -Mu));
+            const float P1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * k + 2 * e + 1], c2, -Mu));
+            ts[2 * (e & 1)] += P0;
+            ts[2 * (e & 1) + 1] += P1;
+            split_pair(P0, P1, ph[e], pl[e]);
+          }
+          const fh8 vh = as_fh8(ph[0], ph[1], ph[2], ph[3]), vl = as_fh8(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+          for (int d = 0; d < ND; d++) {
+            // val_at(32 d + col, 32 s + 16 k + 8 hf)
+            const fh8 a = *reinterpret_cast<const fh8 *>(vb + 32 * d * kTlK + (va ^ ((4 * d ^ 4 * s ^ 2 * k) & 7) << 3));
+            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, vh, O[d], 0, 0, 0);
+            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, vl, O[d], 0, 0, 0);
+          }
+        }
+      }
+      if (s == 0 && i + 1 < i1) {
+        stage(b ^ 1, st.at(i + 1));
+        if (i + 2 < i1) sg.fetch(st.at(i + 2), last);
+      }
+    }
+    if (on) {
+      L += (double)((ts[0] + ts[1]) + (ts[2] + ts[3]));
+      if (badv) {
+        for (int k = 0; k < kTlK && j0 + k <= last; k++)
+          if (j0 + k <= p && (j0 + k < lead || j0 + k >= first)) sg.add_bad(j0 + k, hf, O);
+      }
+    }
+    __syncthreads();  // the next step is staged, and this one read
+  }
+  L += __shfl_xor(L, 32, 64);
+  if (u >= NC) return;
+  const int64_t row = (int64_t)t * H + h;
+  const bool whole = A.chunks == 1;
+  float *op = whole ? out + row * HD : part + (row * A.chunks + ch) * (HD + 4);
+  const double f = whole ? 1.0 / L / kSpUp : 1.0;
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      sf4 o;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = (float)((double)O[d][4 * e + j] * f);
+      *reinterpret_cast<f4a4 *>(op + 32 * d + 8 * e + 4 * hf) = o;
+    }
+  if (!whole && hf == 0) {
+    op[HD] = M;
+    op[HD + 1] = 0.f;
+    *reinterpret_cast<double *>(op + HD + 2) = L;
+  }
+}
+
+// Rows of more than one chunk: the chunks' sums under their largest maximum, in chunk order. One wave per (row, head).
+template <int HD>
+__global__ __launch_bounds__(256) void span_tiles_join_kernel(const float *__restrict__ part, TilesArgs A,
+                                                              float *__restrict__ out) {
+  const int H = A.G * A.KH;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (int64_t)A.T * H) return;
+  const int lane = threadIdx.x & 63, t = (int)(id / H), h = (int)(id % H);
+  const int z = (int)(((int64_t)t * A.G + h % A.G) / kTlCols);
+  const int n = (SpanSteps(A.s, A.row0(z), A.row1(z)).n + A.steps - 1) / A.steps;
+  const float *rec = part + id * A.chunks * (HD + 4);
+  float m = -INFINITY;
+  for (int i = 0; i < n; i++) m = fmaxf(m, rec[i * (HD + 4) + HD]);
+  double L = 0.0;
+  float o[HD / 64] = {};
+  for (int i = 0; i < n; i++) {
+    const float *rc = rec + i * (HD + 4);
+    const float w = __builtin_amdgcn_exp2f(rc[HD] - m);
+    L += *reinterpret_cast<const double *>(rc + HD + 2) * (double)w;
+#pragma unroll
+    for (int e = 0; e < HD / 64; e++) o[e] = __builtin_fmaf(rc[lane + 64 * e], w, o[e]);
+  }
+  const double f = 1.0 / L / kSpUp;
+#pragma unroll
+  for (int e = 0; e < HD / 64; e++) out[id * HD + lane + 64 * e] = (float)((double)o[e] * f);
+}
+
+static TilesArgs tiles_plan(const KvCache &c, int H, const Span &s, const KvRows &R) {
+  TilesArgs A;
+  A.s = s;
+  A.T = R.n;
+  A.pos0 = R.pos0;
+  A.KH = c.KH;
+  A.G = H / c.KH;
+  A.nz = (int)(((int64_t)R.n * A.G + kTlCols - 1) / kTlCols);
+  int most = 0;
+  for (int z = 0; z < A.nz; z++) {
+    const int n = SpanSteps(s, A.row0(z), A.row1(z)).n;
+    most = n > most ? n : most;
+  }
+  // whole rows where the workgroups of columns alone give every CU two; otherwise cut so that they do
+  const int64_t wgs = (int64_t)c.KH * A.nz;
+  int64_t S = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
+  S = S > most ? most : S;
+  A.steps = (int)((most + S - 1) / S);
+  A.chunks = (most + A.steps - 1) / A.steps;
+  return A;
+}
+
+template <int HD, class Stage>
+static hipError_t span_tiles_launch(const float *q, int H, const KvCache &c, const Span &s, const KvRows &R, float scale,
+                                    float *part, float *out, hipStream_t st) {
+  const TilesArgs A = tiles_plan(c, H, s, R);
+  // one grid dimension: the others hold 65,535 workgroups
+  hipLaunchKernelGGL((span_tiles_kernel<HD, Stage>), dim3((unsigned)((int64_t)c.KH * A.chunks * A.nz)), dim3(256), 0, st, q,
+                     c, A, scale, part, out);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || A.chunks == 1) return e;
+  hipLaunchKernelGGL(span_tiles_join_kernel<HD>, dim3((unsigned)(((int64_t)R.n * H + 3) / 4)), dim3(256), 0, st, part, A,
+                     out);
+  return hipGetLastError();
+}
+
 static bool span_tiled(const KvCache &c) {
   return c.bits == 4 || ((c.HD == 64 || c.HD == 128) && ((uintptr_t)c.K & 15) == 0 && ((uintptr_t)c.V & 15) == 0);
 }
@@ -608,6 +1087,10 @@ int64_t attention_span_scratch_floats(const KvCache &c, int H, const Span &s, co
     const SpanRuns U = span_plan(c, H, s, R);
     return U.most > 1 ? (int64_t)R.n * H * U.most * (c.HD + 4) : 0;
   }
+  if (span_tiled(c)) {
+    const TilesArgs A = tiles_plan(c, H, s, R);
+    return A.chunks > 1 ? (int64_t)R.n * H * A.chunks * (c.HD + 4) : 0;
+  }
   return (int64_t)R.n * H * span_max_n(s, R);
 }
 
@@ -620,6 +1103,13 @@ hipError_t attention_span_launch(const float *q, int H, const KvCache &c, const 
                         : span_decode_launch<128, TileKv4<128>>(q, H, c, s, R, scale, scratch, out, st);
     return c.HD == 64 ? span_decode_launch<64, TileF16<64>>(q, H, c, s, R, scale, scratch, out, st)
                       : span_decode_launch<128, TileF16<128>>(q, H, c, s, R, scale, scratch, out, st);
+  }
+  if (span_tiled(c)) {
+    if (c.bits == 4)
+      return c.HD == 64 ? span_tiles_launch<64, StageKv4<64>>(q, H, c, s, R, scale, scratch, out, st)
+                        : span_tiles_launch<128, StageKv4<128>>(q, H, c, s, R, scale, scratch, out, st);
+    return c.HD == 64 ? span_tiles_launch<64, StageF16<64>>(q, H, c, s, R, scale, scratch, out, st)
+                      : span_tiles_launch<128, StageF16<128>>(q, H, c, s, R, scale, scratch, out, st);
   }
   hipLaunchKernelGGL(span_rows_kernel, dim3(H, R.n), dim3(256), 0, st, q, H, c, s, R, scale, scratch, span_max_n(s, R),
                      out);
