@@ -424,6 +424,23 @@ int wl_attention_window_dev(wl_ctx *ctx, const float *d_q, int32_t T, int32_t he
                             int32_t head_dim, const uint16_t *d_K, const uint16_t *d_V, int32_t pos0, int32_t window,
                             int32_t sinks, float scale, float *d_out);
 
+/* wl_layer_dev over caches of another kind, or with a window: bits is 16 (the fp16 caches of wl_layer_dev) or 4 (buffers of
+ * wl_kv4_bytes); `positions` is what the caches hold, checked against pos0 + T. With 16 bits and window 0 it is
+ * wl_layer_dev. */
+typedef struct wl_kv_opts {
+  int32_t bits;
+  int32_t window, sinks;
+  int32_t positions;
+} wl_kv_opts;
+int wl_layer_kv_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, int32_t T, int32_t pos0, void *d_K, void *d_V,
+                    const wl_kv_opts *kv);
+
+/* wl_layer_batch_dev over such caches (pools of slots; kv->positions is not read). Row i's bits equal wl_layer_kv_dev of that
+ * token alone on its sequence. */
+int wl_layer_batch_kv_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, int32_t N, const int32_t *pos,
+                          const int32_t *slot, int32_t slots, int32_t slot_positions, void *d_K, void *d_V,
+                          const wl_kv_opts *kv);
+
 /* The next token of each of `rows` rows of n logits (at most 2^24), drawn with the settings params[row]
  * (host) and the number d_u[row] in [0, 1) (device). Tokens in order (larger logit first, of equals the
  * lower id) with weights exp((logit - max) / temperature): the first top_k stay (0: all), of those the

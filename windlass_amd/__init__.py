@@ -19,6 +19,9 @@ libwindlass_hip.so (include/windlass_hip.h):
                                   loop (src/Engine.cs:356-360), every tensor resident in HBM
 - ``DeviceBatch``                 Transformer.ForwardBatch (src/Transformer.cs:127-170) and BatchEngine's
                                   stacked step (src/BatchEngine.cs:127-173): KV slots, one pass per step
+- ``SampleParams``                Sampler's settings (src/Engine.cs:353-382): ``generate`` of the two classes above
+- ``KvOpts``, ``KvCaches``        caches in 4 bits, a sliding window with first tokens that stay visible (not in the
+                                  reference): ``kv_bits``, ``window`` and ``sinks`` of DeviceTransformer
 - ``gguf.GgufModelFile``          GgufModelFile (src/Gguf.cs:104-270); ``gguf.model_config`` and
                                   ``gguf.load_device_model``: ModelConfig.From and a file's model in HBM
 
@@ -28,11 +31,11 @@ failure). There is no CPU fallback: without the built library every call raises.
 """
 from ._lib import (ArgumentOutOfRangeError, BackendError, NotSupportedError, ShapeError,
                    library_path, load)
-from .backend import (Context, FastMath, GgmlType, Graph, HostBuffer, LayerDesc, QActs, Quants, SampleParams, Stage,
-                      Transformer, WeightView, layout)
-from .model import DeviceBatch, DeviceTransformer, ModelConfig, StageStream
+from .backend import (Context, FastMath, GgmlType, Graph, HostBuffer, KvOpts, LayerDesc, QActs, Quants, SampleParams,
+                      Stage, Transformer, WeightView, layout)
+from .model import DeviceBatch, DeviceTransformer, KvCaches, ModelConfig, StageStream
 
 __all__ = ["ArgumentOutOfRangeError", "BackendError", "NotSupportedError", "ShapeError",
-           "library_path", "load", "Context", "FastMath", "GgmlType", "Graph", "HostBuffer", "LayerDesc", "QActs", "Quants", "SampleParams",
-           "Stage",
-           "Transformer", "WeightView", "layout", "DeviceBatch", "DeviceTransformer", "ModelConfig", "StageStream"]
+           "library_path", "load", "Context", "FastMath", "GgmlType", "Graph", "HostBuffer", "KvCaches", "KvOpts",
+           "LayerDesc", "QActs", "Quants", "SampleParams", "Stage", "Transformer", "WeightView", "layout", "DeviceBatch",
+           "DeviceTransformer", "ModelConfig", "StageStream"]

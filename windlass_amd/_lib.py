@@ -36,6 +36,8 @@ SIGNATURES = {
     "wl_kv4_attention_dev": (ctypes.c_int, [P, P, I32, I32, I32, I32, P, P, I32, I32, I32, I32, F, P]),
     "wl_kv4_attention_batch_dev": (ctypes.c_int, [P, P, I32, I32, I32, I32, P, P, P, P, I32, I32, I32, I32, F, P]),
     "wl_attention_window_dev": (ctypes.c_int, [P, P, I32, I32, I32, I32, P, P, I32, I32, I32, F, P]),
+    "wl_layer_kv_dev": (ctypes.c_int, [P, P, P, I32, I32, P, P, P]),
+    "wl_layer_batch_kv_dev": (ctypes.c_int, [P, P, P, I32, P, P, I32, I32, P, P, P]),
     "wl_sample_dev": (ctypes.c_int, [P, P, I32, I64, P, P, P]),
     "wl_embed_dev_ids": (ctypes.c_int, [P, P, P, I32, P]),
     "wl_layer_batch_dev": (ctypes.c_int, [P, P, P, I32, P, P, I32, I32, P, P]),

@@ -362,6 +362,13 @@ class LayerDesc(ctypes.Structure):
         ("qk_norm_full", ctypes.c_int32)]
 
 
+class KvOpts(ctypes.Structure):
+    """wl_kv_opts: a layer's cache in 16 or 4 bits, the window and first tokens its rows see (window 0: all), and
+    the positions it holds."""
+    _fields_ = [("bits", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("positions", ctypes.c_int32)]
+
+
 class SampleParams(ctypes.Structure):
     """wl_sample_params: one row's settings (Sampler, src/Engine.cs:353-382). temperature 0 is the greedy pick;
     top_k 0, top_p 1 and min_p 0 filter nothing."""

@@ -1395,8 +1395,19 @@ static int rope_angles(wl_ctx *c, const int32_t *hpos, int T, int pos0, int n, d
   return WL_OK;
 }
 
+// A layer's cache and what its rows see of it, where that is not the whole of an fp16 cache; the rows of a batch step
+// on the host.
+struct LayerKv {
+  wl::KvCache cache;
+  wl::Span span;
+  const int32_t *pos = nullptr, *slot = nullptr;
+};
+static int layer_attention_kv(wl_ctx *c, const wl_layer_desc *L, const LayerKv &kv, float *q, float *k, const float *v,
+                              int T, int pos0, int rd, double fs, const wl::RowMap &rm, float scale, float *att);
+
 static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, int32_t pos0, uint16_t *d_K,
-                     uint16_t *d_V, const wl::RowMap &rm, const int32_t *hpos, int max_n, bool each) {
+                     uint16_t *d_V, const wl::RowMap &rm, const int32_t *hpos, int max_n, bool each,
+                     const LayerKv *kv = nullptr) {
   if (!c || !L || !d_x || !d_K || !d_V) return fail(WL_E_ARG, "wl_layer_dev: null argument");
   // OLMo 2 (src/Transformer.cs:182,224-230): post-norms instead of pre-norms
   const bool post = L->d_post_attention_norm || L->d_post_ffw_norm;
@@ -1436,7 +1447,7 @@ static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, i
       (rc = ensure(c, S_LK, (size_t)T * KD * 4)) || (rc = ensure(c, S_LV, (size_t)T * KD * 4)) ||
       (rc = ensure(c, S_LATT, (size_t)T * QD * 4)) ||
       (rc = ensure(c, S_LG, (size_t)T * FF * 4)) || (rc = ensure(c, S_LU, (size_t)T * FF * 4)) ||
-      (rc = ensure(c, S_ATT, (size_t)wl::attention_scratch_floats(T, H, HD, KD, max_n, d_K, d_V, rm) * 4)))
+      (!kv && (rc = ensure(c, S_ATT, (size_t)wl::attention_scratch_floats(T, H, HD, KD, max_n, d_K, d_V, rm) * 4))))
     return rc;
   float *xn = (float *)c->buf[S_LXN], *q = (float *)c->buf[S_LQ], *k = (float *)c->buf[S_LK],
         *v = (float *)c->buf[S_LV], *att = (float *)c->buf[S_LATT],
@@ -1535,12 +1546,16 @@ static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, i
   const double fs = L->rope_freq_scale != 0.0 ? L->rope_freq_scale : 1.0;
   const float scale = L->attention_scale != 0.f ? L->attention_scale : 1.0f / (float)sqrt((double)HD);
   const float4 *tab = nullptr;
-  if (wl::rope_attention_fused(T, rm, HD, KH, rd, d_K, d_V) &&
-      (rc = rope_angles(c, hpos, T, pos0, rd, L->rope_base, fs, L->d_rope_freqs, &tab)))
-    return rc;
-  WL_HIP(wl::rope_attention_launch(q, k, v, T, H, KH, HD, rd, L->neox, pos0, L->rope_base, fs, L->d_rope_freqs, tab,
-                                   d_K, d_V, rm, scale, (float *)c->buf[S_ATT], att, max_n, c->stream),
-         "rope, kv store and attention");
+  if (kv) {
+    if ((rc = layer_attention_kv(c, L, *kv, q, k, v, T, pos0, rd, fs, rm, scale, att))) return rc;
+  } else {
+    if (wl::rope_attention_fused(T, rm, HD, KH, rd, d_K, d_V) &&
+        (rc = rope_angles(c, hpos, T, pos0, rd, L->rope_base, fs, L->d_rope_freqs, &tab)))
+      return rc;
+    WL_HIP(wl::rope_attention_launch(q, k, v, T, H, KH, HD, rd, L->neox, pos0, L->rope_base, fs, L->d_rope_freqs, tab,
+                                     d_K, d_V, rm, scale, (float *)c->buf[S_ATT], att, max_n, c->stream),
+           "rope, kv store and attention");
+  }
   if (post) {
     // o = RmsNorm(W_o att), then x += o * rs (src/Transformer.cs:223-225)
     if ((rc = ensure(c, S_LM, (size_t)T * E * 4))) return rc;
@@ -1857,6 +1872,89 @@ extern "C" int wl_attention_window_dev(wl_ctx *c, const float *d_q, int32_t T, i
   kc.HD = head_dim;
   kc.positions = (int64_t)pos0 + T;
   return span_attention(c, d_q, heads, kc, wl::Span{window, sinks}, seq_rows(T, pos0), scale, d_out);
+}
+
+// A layer's RoPE, its rows' keys and values into the cache, and their attention.
+static int layer_attention_kv(wl_ctx *c, const wl_layer_desc *L, const LayerKv &kv, float *q, float *k, const float *v,
+                              int T, int pos0, int rd, double fs, const wl::RowMap &rm, float scale, float *att) {
+  const wl::KvCache &kc = kv.cache;
+  const int H = L->heads, KH = kc.KH, HD = kc.HD;
+  const int64_t QD = (int64_t)H * HD, KD = (int64_t)KH * HD;
+  if (kc.bits == 16)
+    WL_HIP(wl::rope_kv_launch(q, k, v, T, H, KH, HD, rd, L->neox, pos0, L->rope_base, fs, L->d_rope_freqs,
+                              (uint16_t *)kc.K, (uint16_t *)kc.V, rm, c->stream), "rope and kv store");
+  auto rows = [&](const wl::KvRows &R, int i0) -> int {
+    if (kc.bits == 4)
+      WL_HIP(wl::rope_kv4_launch(q + i0 * QD, k + i0 * KD, v + i0 * KD, H, KH, HD, rd, L->neox, L->rope_base, fs,
+                                 L->d_rope_freqs, (uint8_t *)kc.K, (uint8_t *)kc.V, kc.positions, kc.slot_bytes, R,
+                                 c->stream), "rope and kv4 store");
+    return span_attention(c, q + i0 * QD, H, kc, kv.span, R, scale, att + i0 * QD);
+  };
+  return kv.pos ? each_rows(T, kv.pos, kv.slot, rows) : rows(seq_rows(T, pos0), 0);
+}
+
+// What wl_kv_opts asks for, for a layer's caches of `positions` positions (0: of fp16, not known).
+static int layer_kv(const char *who, const wl_layer_desc *L, void *d_K, void *d_V, const wl_kv_opts *o, int positions,
+                    LayerKv *kv) {
+  int rc;
+  if (o->bits != 16 && o->bits != 4) return fail(WL_E_UNSUPPORTED, "%s: a cache of %d bits", who, o->bits);
+  if ((rc = span_check(who, L->heads, L->kv_heads, o->window, o->sinks))) return rc;
+  if (L->head_dim <= 0 || (int64_t)L->kv_heads * L->head_dim > 1 << 24)
+    return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, L->kv_heads, L->head_dim);
+  if (o->bits == 4) {
+    if ((rc = kv4_check(who, L->kv_heads, L->head_dim, d_K, d_V))) return rc;
+    kv->cache = kv4_cache(d_K, d_V, L->kv_heads, L->head_dim, positions);
+  } else {
+    kv->cache.K = (const uint8_t *)d_K;
+    kv->cache.V = (const uint8_t *)d_V;
+    kv->cache.KH = L->kv_heads;
+    kv->cache.HD = L->head_dim;
+    kv->cache.positions = positions;
+    kv->cache.slot_bytes = (int64_t)positions * L->kv_heads * L->head_dim * 2;
+  }
+  kv->span = wl::Span{o->window, o->sinks};
+  return WL_OK;
+}
+
+extern "C" int wl_layer_kv_dev(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, int32_t pos0, void *d_K,
+                               void *d_V, const wl_kv_opts *o) {
+  if (!c || !L || !d_x || !d_K || !d_V || !o) return fail(WL_E_ARG, "wl_layer_kv_dev: null argument");
+  LayerKv kv;
+  int rc;
+  if ((rc = layer_kv("wl_layer_kv_dev", L, d_K, d_V, o, o->positions, &kv)) ||
+      (rc = kv_rows_check("wl_layer_kv_dev", T, pos0, o->positions)))
+    return rc;
+  WL_ON_DEVICE(c);
+  const bool plain = o->bits == 16 && !o->window;
+  return layer_run(c, L, d_x, T, pos0, (uint16_t *)d_K, (uint16_t *)d_V, wl::RowMap{}, nullptr, pos0 + T, false,
+                   plain ? nullptr : &kv);
+}
+
+extern "C" int wl_layer_batch_kv_dev(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t N, const int32_t *pos,
+                                     const int32_t *slot, int32_t slots, int32_t slot_positions, void *d_K, void *d_V,
+                                     const wl_kv_opts *o) {
+  if (!c || !L || !d_x || !pos || !slot || !d_K || !d_V || !o)
+    return fail(WL_E_ARG, "wl_layer_batch_kv_dev: null argument");
+  if (N == 0) return fail(WL_E_SHAPE, "wl_layer_batch_kv_dev: bad shape");
+  LayerKv kv;
+  int rc;
+  if ((rc = layer_kv("wl_layer_batch_kv_dev", L, d_K, d_V, o, slot_positions, &kv)) ||
+      (rc = batch_check("wl_layer_batch_kv_dev", N, pos, slot, slots, slot_positions)))
+    return rc;
+  WL_ON_DEVICE(c);
+  if (o->bits == 16 && !o->window)
+    return wl_layer_batch_dev(c, L, d_x, N, pos, slot, slots, slot_positions, (uint16_t *)d_K, (uint16_t *)d_V);
+  kv.pos = pos;
+  kv.slot = slot;
+  wl::RowMap rm;
+  if (o->bits == 16) {  // the RoPE and fp16 stores read the rows' positions and slots on the device
+    int32_t *rows;
+    if ((rc = stage_rows(c, pos, slot, N, &rows))) return rc;
+    rm.pos = rows;
+    rm.slot = rows + N;
+    rm.cap = slot_positions;
+  }
+  return layer_run(c, L, d_x, N, 0, (uint16_t *)d_K, (uint16_t *)d_V, rm, pos, 0, true, &kv);
 }
 
 extern "C" int wl_sample_dev(wl_ctx *c, const float *d_logits, int32_t rows, int64_t n, const wl_sample_params *params,

@@ -7,7 +7,7 @@
 // summed in that order passes u of the kept weight. Every step is a question about a prefix of that
 // order, so nothing is sorted but the few tokens around a prefix's end.
 //
-// Arithmetic: weights in double (a polynomial for 2^f, 2^-52), cut to whole numbers of 2^-shift (2^-45 at 128,000
+// Arithmetic: weights in double (a polynomial for 2^f), cut to whole numbers of 2^-shift (2^-45 at 128,000
 // tokens), so that sums are exact and do not depend on the order in which workgroups and atomics add them.
 //
 // Three launches. (1) Each part of 4,096 tokens of a row: its largest and least finite logit. (2) Each part: the count
@@ -52,51 +52,50 @@ __device__ __forceinline__ float sm_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// ln(2)^i / i!. Held in scalar registers past the compiler's sight: as plain constants they were moved to vector
+// registers, two instructions before each of the polynomial's.
+struct SmSeries {
+  double c[12];
+  __device__ __forceinline__ SmSeries()
+      : c{1.0, 0.6931471805599453, 0.2402265069591007, 0.055504108664821576,
+          0.009618129107628477, 0.0013333558146428441, 0.00015403530393381606, 1.5252733804059838e-05,
+          1.3215486790144305e-06, 1.0178086009239696e-07, 7.054911620801121e-09, 4.44553827187081e-10} {
+#pragma unroll
+    for (int i = 0; i < 12; i++) asm("" : "+s"(c[i]));
+  }
+};
+
 // What every launch after the first derives from the parts' records: the row's maximum and its bins.
 struct SmRow {
-  float m, R, c;
-  double per;  // log2(e) / t
+  float m, R, c;  // the maximum (of infinity: the largest finite value), the bins' reach and scale
+  double per;     // log2(e) / t; for t = 0 so large that only the maximum weighs anything
   int shift;
-  bool greedy;
   __device__ void set(float top, float low, float t, int sh) {
-    m = top;
+    m = cap(top);
     shift = sh;
-    greedy = t == 0.f;
-    per = 1.4426950408889634 / (double)t;
-    R = fminf(fminf(top - low, 64.f * t), 3.4028235e38f);
+    per = t > 0.f ? fmin(1.4426950408889634 / (double)t, 1e300) : 1e300;
+    R = fminf(fminf(m - low, 64.f * t), 3.4028235e38f);
     if (!(R > 1e-30f)) R = 0.f;  // the bins' scale stays finite; what lies lower is the last bin's
     c = R > 0.f ? (float)(kSmBins - 2) / R : 0.f;
   }
+  __device__ static float cap(float l) { return fminf(l, 3.4028235e38f); }
   __device__ int bin(float l) const {
-    const float d = l == m ? 0.f : m - l;
+    const float d = m - cap(l);
     return d > R ? kSmBins - 1 : min((int)(d * c), kSmBins - 2);
   }
-  // w in units of 2^-shift: 2^x for x = (l - m) log2(e) / t, as 2^k times 2^f, f in [0, 1): e^(f ln 2) by its series to the
-  // 14th power (the rest below 2^-52), its significand shifted.
-  __device__ u64 mass(float l) const {
-    if (l == m) return (u64)1 << shift;
-    const double x = ((double)l - (double)m) * per;
-    if (greedy || !(x > -64.0)) return 0;
-    const double k = floor(x), y = (x - k) * 0.6931471805599453;
-    double p = 1.1470745597729725e-11;  // 1 / 14!
-    p = __builtin_fma(p, y, 1.6059043836821613e-10);
-    p = __builtin_fma(p, y, 2.08767569878681e-09);
-    p = __builtin_fma(p, y, 2.505210838544172e-08);
-    p = __builtin_fma(p, y, 2.755731922398589e-07);
-    p = __builtin_fma(p, y, 2.7557319223985893e-06);
-    p = __builtin_fma(p, y, 2.48015873015873e-05);
-    p = __builtin_fma(p, y, 0.0001984126984126984);
-    p = __builtin_fma(p, y, 0.001388888888888889);
-    p = __builtin_fma(p, y, 0.008333333333333333);
-    p = __builtin_fma(p, y, 0.041666666666666664);
-    p = __builtin_fma(p, y, 0.16666666666666666);
-    p = __builtin_fma(p, y, 0.5);
-    p = __builtin_fma(p, y, 1.0);
-    p = __builtin_fma(p, y, 1.0);
-    const u64 bits = __builtin_bit_cast(u64, p);  // p in [1, 2]
+  // w in units of 2^-shift: 2^x for x = (l - m) log2(e) / t, as 2^k times 2^f, f in [-1/2, 1/2], by its series to the 11th
+  // power (the rest is below 2^-47 of it), its significand shifted.
+  __device__ __forceinline__ u64 mass(float l, const SmSeries &C) const {
+    double x = ((double)cap(l) - (double)m) * per;
+    x = fmax(x, -80.0);  // nothing is left there
+    const double k = rint(x), f = x - k;
+    double p = C.c[11];
+#pragma unroll
+    for (int i = 10; i >= 0; i--) p = __builtin_fma(p, f, C.c[i]);
+    const u64 bits = __builtin_bit_cast(u64, p);
     const u64 sig = (bits & (((u64)1 << 52) - 1)) | (u64)1 << 52;
-    const int down = 52 - shift - (int)k - ((int)(bits >> 52) - 1023);  // shift <= 61, k >= -64
-    return down >= 64 ? 0 : down >= 0 ? sig >> down : sig << -down;
+    const int down = 52 - shift - (int)k - ((int)(bits >> 52) - 1023);  // from 0 (shift <= 52)
+    return sig >> (down < 63 ? down : 63);
   }
 };
 
@@ -172,9 +171,10 @@ __global__ __launch_bounds__(256) void sample_range_kernel(const float *__restri
   }
 }
 
-__global__ __launch_bounds__(256) void sample_bins_kernel(const float *__restrict__ logits, int64_t n, SampleSets sets,
+template <int WIDE>
+__global__ __launch_bounds__(WIDE) void sample_bins_kernel(const float *__restrict__ logits, int64_t n, SampleSets sets,
                                                           int shift, SmScratch X) {
-  constexpr int N = kSmPart / 256;
+  constexpr int N = kSmPart / WIDE;
   __shared__ unsigned cn[kSmBins];
   __shared__ u64 ms[kSmBins];
   __shared__ uint16_t ids[kSmPart];
@@ -188,17 +188,20 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(const float *__restric
   float v[N];
 #pragma unroll
   for (int j = 0; j < N; j++) {
-    const int64_t i = lo + tid + 256 * j;
+    const int64_t i = lo + tid + WIDE * j;
     v[j] = i < hi ? l[i] : __builtin_nanf("");
   }
-  cn[tid] = 0;
-  ms[tid] = 0;
+  if (tid < kSmBins) {
+    cn[tid] = 0;
+    ms[tid] = 0;
+  }
   if (tid == 0) {
     mc = 0;
     mm = 0;
   }
   SmRow r;
   sm_row_of(X.rec + (int64_t)row * parts, parts, set.temperature, shift, r, sh);
+  const SmSeries C;
   const u64 least = (u64)ceil(ldexp((double)set.min_p, shift));
   unsigned at[N];  // the token's bin and its place there
   unsigned c = 0;
@@ -206,8 +209,8 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(const float *__restric
 #pragma unroll
   for (int j = 0; j < N; j++) {
     at[j] = ~0u;
+    const u64 M = r.mass(v[j], C);
     if (v[j] != v[j]) continue;
-    const u64 M = r.mass(v[j]);
     const int b = r.bin(v[j]);
     at[j] = (unsigned)b << 16 | atomicAdd(&cn[b], 1u);
     if (M) atomicAdd(&ms[b], M);
@@ -227,13 +230,15 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(const float *__restric
   }
   __syncthreads();
   const int64_t part = (int64_t)row * parts + blockIdx.x;
-  unsigned end = cn[tid];
+  unsigned end = tid < kSmBins ? cn[tid] : 0;
   u64 none = 0;
   const unsigned mine = end;
   sm_scan(end, none, sc, sm);
-  cn[tid] = end - mine;
-  X.mass[part * kSmBins + tid] = ms[tid];
-  X.end[part * kSmBins + tid] = (uint16_t)end;
+  if (tid < kSmBins) {
+    cn[tid] = end - mine;
+    X.mass[part * kSmBins + tid] = ms[tid];
+    X.end[part * kSmBins + tid] = (uint16_t)end;
+  }
   if (tid == 0) {
     X.rec[part].minp_count = mc;
     X.rec[part].minp_mass = mm;
@@ -241,12 +246,12 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(const float *__restric
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < N; j++)
-    if (at[j] != ~0u) ids[cn[at[j] >> 16] + (at[j] & 0xffffu)] = (uint16_t)(tid + 256 * j);
+    if (at[j] != ~0u) ids[cn[at[j] >> 16] + (at[j] & 0xffffu)] = (uint16_t)(tid + WIDE * j);
   __syncthreads();
   // places past the part's tokens hold nothing that is read
 #pragma unroll
-  for (int j = 0; j < kSmPart / 2048; j++)
-    reinterpret_cast<uint4 *>(X.id + part * kSmPart)[tid + 256 * j] = reinterpret_cast<const uint4 *>(ids)[tid + 256 * j];
+  for (int j = 0; j < (kSmPart / 8 + WIDE - 1) / WIDE; j++)
+    if (tid + WIDE * j < kSmPart / 8) reinterpret_cast<uint4 *>(X.id + part * kSmPart)[tid + WIDE * j] = reinterpret_cast<const uint4 *>(ids)[tid + WIDE * j];
 }
 
 // A question: the shortest prefix with at least `count` tokens, or of at least `mass`, or of more.
@@ -331,7 +336,7 @@ __device__ __forceinline__ void sm_few(SmShared &S, SmAsk a, u64 target, unsigne
   if (tid < 64) {
     const bool on = tid < (int)in;
     const u64 me = on ? S.few[tid] : ~(u64)0;
-    const u64 w = on ? r.mass(sm_value(~(uint32_t)(me >> 32))) : 0;
+    const u64 w = on ? r.mass(sm_value(~(uint32_t)(me >> 32)), SmSeries()) : 0;
     unsigned place = 1;
     u64 sum = w;
     for (int i = 0; i < (int)in; i++) {
@@ -415,7 +420,7 @@ __device__ SmPrefix sm_answer(SmShared &S, SmAsk a, u64 target, const SmView &V,
     inside([&](uint32_t key, uint32_t) {
       const uint32_t b = (hi - key) / width;
       atomicAdd(&S.sub_n[b], 1u);
-      atomicAdd(&S.sub_m[b], r.mass(sm_value(key)));
+      atomicAdd(&S.sub_m[b], r.mass(sm_value(key), SmSeries()));
     });
     __syncthreads();
     unsigned c = tid < kSmBins ? S.sub_n[tid] : 0;
@@ -450,7 +455,7 @@ __device__ SmPrefix sm_answer(SmShared &S, SmAsk a, u64 target, const SmView &V,
     return S.got;
   }
   // equal logits: the prefix takes the first `need` of them by id
-  const u64 w = r.mass(sm_value(lo));
+  const u64 w = r.mass(sm_value(lo), SmSeries());
   const u64 need64 = a == SM_COUNT ? target - c0
                      : w == 0      ? 1
                      : a == SM_MASS ? (target - m0 + w - 1) / w
@@ -499,6 +504,7 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
   __shared__ SmShared S;
   const int row = blockIdx.x, tid = threadIdx.x;
   const SampleSet set = sets.row[row];
+  const bool greedy = set.temperature == 0.f;
   const float u = us[row];
   SmView V;
   V.l = logits + (int64_t)row * n;
@@ -522,7 +528,7 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
     }
   SmRow r;
   sm_row_of(rec, parts, set.temperature, shift, r, S.f2);
-  if (r.m == -INFINITY || (r.greedy && l0 != l0)) {  // as the greedy pick
+  if (r.m == -INFINITY || (greedy && l0 != l0)) {  // as the greedy pick
     if (tid == 0) out[row] = 0;
     return;
   }
@@ -547,7 +553,7 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
   }
   const unsigned all = S.cn[kSmBins - 1];
   SmPrefix kept{all, S.ms[kSmBins - 1], 0};
-  const bool top_k = !r.greedy && set.top_k > 0 && (unsigned)set.top_k < all;
+  const bool top_k = !greedy && set.top_k > 0 && (unsigned)set.top_k < all;
   if (top_k) {
     // the bins up to the one where top_k ends, put in order where they hold few tokens
     if (tid < kSmBins && S.cn[tid] >= (unsigned)set.top_k && (tid == 0 || S.cn[tid - 1] < (unsigned)set.top_k)) S.pick = tid;
@@ -565,7 +571,7 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
       }
       __syncthreads();
       unsigned c = 0;
-      u64 m = tid < (int)in ? r.mass(sm_value(~(uint32_t)(S.few[tid] >> 32))) : 0;
+      u64 m = tid < (int)in ? r.mass(sm_value(~(uint32_t)(S.few[tid] >> 32)), SmSeries()) : 0;
       sm_scan(c, m, S.sc, S.sm);
       if (tid < (int)in) S.weight[tid] = m;  // up to and with the token
       __syncthreads();
@@ -585,7 +591,7 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
     kept = sm_answer(S, SM_COUNT, (u64)set.top_k, V, r, false);
   }
   u64 x = 0;
-  if (!r.greedy) {
+  if (!greedy) {
     if (set.top_p < 1.f) {
       const SmPrefix p = sm_answer(S, SM_MASS, sm_top_p(set.top_p, kept.mass), V, r, false);
       if (p.count < kept.count) kept = p;
@@ -610,7 +616,7 @@ hipError_t sample_launch(const float *logits, int rows, int64_t n, const SampleS
   const int parts = sample_parts(n);
   int bits = 1;
   while ((int64_t)1 << bits < n) bits++;
-  const int shift = 62 - bits;  // n weights of at most 1 stay below 2^63
+  const int shift = bits > 10 ? 62 - bits : 52;  // n weights of at most 1 stay below 2^63
   const int64_t all = (int64_t)rows * parts;
   SmScratch X;  // each array a multiple of 16 bytes from the one before
   X.mass = (u64 *)scratch;
@@ -620,7 +626,12 @@ hipError_t sample_launch(const float *logits, int rows, int64_t n, const SampleS
   hipLaunchKernelGGL(sample_range_kernel, dim3(parts, rows), dim3(256), 0, st, logits, n, X);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sample_bins_kernel, dim3(parts, rows), dim3(256), 0, st, logits, n, sets, shift, X);
+  // eight tokens a thread while there is at most a part for each CU (one row of 128,256: 6.8 us, 16 a thread 8.4), 16 where
+  // CUs take several (64 rows: 25.9 us, eight a thread 29.3)
+  if (all <= 256)
+    hipLaunchKernelGGL(sample_bins_kernel<512>, dim3(parts, rows), dim3(512), 0, st, logits, n, sets, shift, X);
+  else
+    hipLaunchKernelGGL(sample_bins_kernel<256>, dim3(parts, rows), dim3(256), 0, st, logits, n, sets, shift, X);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   hipLaunchKernelGGL(sample_pick_kernel, dim3(rows), dim3(1024), 0, st, logits, n, parts, sets, shift, X, u, out);
   return hipGetLastError();

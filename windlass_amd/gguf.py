@@ -338,9 +338,9 @@ def _vector(ctx, g, t, dev):
     return out
 
 
-def load_device_model(ctx, path, max_positions=None):
+def load_device_model(ctx, path, max_positions=None, kv_bits=16, window=0, sinks=0):
     """The model of a GGUF file in HBM: every matrix's raw blocks uploaded unchanged, the vectors
-    decoded on the GPU. Returns (DeviceTransformer, weights) - free the weights when done."""
+    decoded on the GPU; kv_bits, window and sinks as DeviceTransformer takes them. Returns (DeviceTransformer, weights) - free the weights when done."""
     import torch
     from .model import DeviceTransformer
     g = GgufModelFile.Open(path)
@@ -361,7 +361,7 @@ def load_device_model(ctx, path, max_positions=None):
         else:
             raise NotSupportedError("Tensor %s has %d dims." % (t.Name, len(t.Dims)))
     n = max_positions or int(g.Get(g.Get("general.architecture") + ".context_length", 4096))
-    return DeviceTransformer(ctx, cfg, weights, vectors, n), weights
+    return DeviceTransformer(ctx, cfg, weights, vectors, n, kv_bits=kv_bits, window=window, sinks=sinks), weights
 
 
 def _check_ffn_layouts(g, cfg):

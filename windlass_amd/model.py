@@ -14,8 +14,8 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
-from ._lib import ShapeError, check, load
-from .backend import LayerDesc
+from ._lib import NotSupportedError, ShapeError, check, load
+from .backend import KvOpts, LayerDesc, SampleParams
 
 _LAYER_TENSORS = ("attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down")
 
@@ -49,6 +49,32 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+class KvCaches:
+    """The kind of a model's KV caches, and the layer calls over them: kv_bits 16 (fp16 rows) or 4 (wl_kv4_bytes: head
+    dims 64 and 128), and the positions a row sees (window 0: all; else the last `window` and the first `sinks`)."""
+
+    def __init__(self, cfg, kv_bits=16, window=0, sinks=0):
+        if kv_bits not in (16, 4):
+            raise NotSupportedError("A KV cache of %s bits." % kv_bits)
+        if window < 0 or sinks < 0:
+            raise ShapeError("A window of %d and %d first positions." % (window, sinks))
+        if kv_bits == 4 and not load().wl_kv4_bytes(1, cfg.kv_heads, cfg.head_dim):
+            raise NotSupportedError("4-bit caches hold head dims of 64 and 128, not %d." % cfg.head_dim)
+        self.cfg, self.bits, self.window, self.sinks = cfg, kv_bits, window, sinks
+
+    def buffers(self, torch, dev, lead, positions):
+        """Caches of keys and of values for each of `lead` (a shape): [...][positions][kv_dim] halves, or bytes."""
+        if self.bits == 4:
+            n = (load().wl_kv4_bytes(positions, self.cfg.kv_heads, self.cfg.head_dim),)
+        else:
+            n = (positions, self.cfg.kv_heads * self.cfg.head_dim)
+        return [torch.zeros(tuple(lead) + n, dtype=torch.uint8 if self.bits == 4 else torch.int16, device=dev)
+                for _ in range(2)]
+
+    def opts(self, positions):
+        return KvOpts(self.bits, self.window, self.sinks, positions)
+
+
 class DeviceTransformer:
     """weights: {GGUF tensor name: WeightView} with token_embd, output (absent when tied to
     token_embd) and blk.N.{attn_q,attn_k,attn_v,attn_output,ffn_gate,ffn_up,ffn_down};
@@ -56,13 +82,14 @@ class DeviceTransformer:
     with post_norms, blk.N.post_attention_norm and blk.N.post_ffw_norm) and the optional
     blk.N.attn_{q,k,v}.bias, blk.N.attn_{q,k}_norm and rope_freqs."""
 
-    def __init__(self, ctx, cfg, weights, vectors, max_positions, stream=None):
-        """stream: a StageStream whose weights() the layer tensors of `weights` come from; the
+    def __init__(self, ctx, cfg, weights, vectors, max_positions, stream=None, kv_bits=16, window=0, sinks=0):
+        """kv_bits, window, sinks: KvCaches. stream: a StageStream whose weights() the layer tensors of `weights` come from; the
         forward then acquires and releases each layer's slot around its layer. A layer with
         blk.N.ffn_gate_inp is a MoE layer: blk.N.ffn_{gate,up,down}_exps (stacked experts), the
         router, and optionally blk.N.ffn_{gate,up,down}_shexp and ffn_gate_inp_shexp ([1][embd])."""
         import torch
         self.ctx, self.cfg, self.L, self.torch = ctx, cfg, load(), torch
+        self.kv = KvCaches(cfg, kv_bits, window, sinks)
         self.stream = stream
         self.w, self.v = weights, vectors
         self.embd_w = weights["token_embd"]
@@ -74,9 +101,8 @@ class DeviceTransformer:
         self.max_positions = max_positions
         self.dev = torch.device("cuda:%d" % ctx.device)
         self.descs = [self._desc(l) for l in range(cfg.layers)]
-        kd = cfg.kv_heads * cfg.head_dim
-        self.K = torch.zeros((cfg.layers, max_positions, kd), dtype=torch.int16, device=self.dev)
-        self.V = torch.zeros((cfg.layers, max_positions, kd), dtype=torch.int16, device=self.dev)
+        self.kv_opts = self.kv.opts(max_positions)
+        self.K, self.V = self.kv.buffers(torch, self.dev, (cfg.layers,), max_positions)
         self.logits = torch.empty((1, self.vocab), device=self.dev)
         self._tok = torch.empty(1, dtype=torch.int32, device=self.dev)
         self._xn = torch.empty((1, cfg.embd), device=self.dev)
@@ -182,8 +208,9 @@ class DeviceTransformer:
 
     def _layers_and_head(self, x, T, pos0):
         L, h, c = self.L, self.ctx.handle, ctypes.c_void_p
-        self.run_layers(lambda l, d: check(L.wl_layer_dev(h, ctypes.byref(d), c(x.data_ptr()), T, pos0,
-                                                          c(self.K[l].data_ptr()), c(self.V[l].data_ptr()))))
+        self.run_layers(lambda l, d: check(L.wl_layer_kv_dev(h, ctypes.byref(d), c(x.data_ptr()), T, pos0,
+                                                             c(self.K[l].data_ptr()), c(self.V[l].data_ptr()),
+                                                             ctypes.byref(self.kv_opts))))
         self.length = pos0 + T
         # Head (src/Transformer.cs:112-125) of the last row
         check(L.wl_rms_norm_dev(h, c(x[T - 1:].data_ptr()), 1, self.cfg.embd, c(self.v["output_norm"].data_ptr()),
@@ -192,16 +219,49 @@ class DeviceTransformer:
         self.logit_scale(self.logits, self.vocab)
         return self.logits
 
-    def sample(self):
-        """Greedy pick of self.logits on the device (src/Engine.cs:356-360); waits for it."""
-        self.sample_into(self._tok)
+    def sample(self, params=None, u=0.0):
+        """The next token after self.logits (Sampler, src/Engine.cs:353-382); waits for it: the greedy pick, or with
+        params (SampleParams) the draw of the number u in [0, 1)."""
+        if params is None:
+            self.sample_into(self._tok)
+        else:
+            d_u = self.torch.full((1,), u, device=self.dev)
+            self.torch.cuda.synchronize()  # the context's stream does not wait for torch's
+            self.sample_into(self._tok, params, d_u)
         self.ctx.sync()
         return int(self._tok.item())
 
-    def sample_into(self, d_out):
-        """The greedy pick into a device int32 element, queued (no wait)."""
-        check(self.L.wl_argmax_dev(self.ctx.handle, ctypes.c_void_p(self.logits.data_ptr()), 1, self.vocab,
-                                   ctypes.c_void_p(d_out.data_ptr())))
+    def sample_into(self, d_out, params=None, d_u=None):
+        """The greedy pick, or the draw with params and the device float d_u, into a device int32 element, queued (no
+        wait)."""
+        c = ctypes.c_void_p
+        if params is None:
+            check(self.L.wl_argmax_dev(self.ctx.handle, c(self.logits.data_ptr()), 1, self.vocab, c(d_out.data_ptr())))
+        else:
+            check(self.L.wl_sample_dev(self.ctx.handle, c(self.logits.data_ptr()), 1, self.vocab, ctypes.byref(params),
+                                       c(d_u.data_ptr()), c(d_out.data_ptr())))
+
+    def generate(self, prompt, steps, params, u, chunk=None):
+        """The prompt as greedy() runs it, then `steps` tokens drawn with params and the numbers u (steps of them, in [0,
+        1)), each fed to the next step on the device. Returns the tokens."""
+        d_u = self.torch.as_tensor(np.asarray(u, np.float32)).to(self.dev)
+        if d_u.numel() != steps:
+            raise ShapeError("%d numbers for %d tokens." % (d_u.numel(), steps))
+        ids = self.torch.empty(max(steps, 1), dtype=self.torch.int32, device=self.dev)
+        self.torch.cuda.synchronize()
+        chunk = chunk or len(prompt)
+        pos = 0
+        for i in range(0, len(prompt), chunk):
+            part = list(prompt[i:i + chunk])
+            self.forward(part, pos)
+            pos += len(part)
+        for i in range(steps):
+            if i:
+                self.forward_ids(ids[i - 1:i], pos)
+                pos += 1
+            self.sample_into(ids[i:i + 1], params, d_u[i:i + 1])
+        self.ctx.sync()
+        return [int(v) for v in ids[:steps].cpu().tolist()]
 
     def greedy(self, prompt, steps, chunk=None, keep_logits=False):
         """The prompt in chunks of `chunk` tokens (all at once when None), then `steps` greedy
@@ -320,7 +380,7 @@ class DeviceBatch:
     """Several sequences decoding together on one DeviceTransformer's weights: Transformer.
     ForwardBatch (src/Transformer.cs:127-170) and BatchEngine's stacked step
     (src/BatchEngine.cs:127-173). Each sequence owns a slot of the KV pools
-    ([layers][slots][slot_positions][kv_dim], fp16). A prompt runs as its own pass into its slot;
+    ([layers][slots][slot_positions][kv_dim] in fp16, or the model's kind: KvCaches). A prompt runs as its own pass into its slot;
     a step stacks one token of each given sequence into one pass (wl_layer_batch_dev), so every
     layer's weights are read once for all of them, and row i's bits equal that sequence's own
     one-token step."""
@@ -328,10 +388,8 @@ class DeviceBatch:
     def __init__(self, model, slots, slot_positions):
         torch = model.torch
         self.m, self.slots, self.cap = model, slots, slot_positions
-        cfg = model.cfg
-        kd = cfg.kv_heads * cfg.head_dim
-        self.K = torch.zeros((cfg.layers, slots, slot_positions, kd), dtype=torch.int16, device=model.dev)
-        self.V = torch.zeros((cfg.layers, slots, slot_positions, kd), dtype=torch.int16, device=model.dev)
+        self.K, self.V = model.kv.buffers(torch, model.dev, (model.cfg.layers, slots), slot_positions)
+        self.kv_opts = model.kv.opts(slot_positions)
         self.length = [0] * slots
         self._bufs = {}
         torch.cuda.synchronize()
@@ -370,9 +428,9 @@ class DeviceBatch:
         toks = (ctypes.c_int32 * T)(*tokens)
         check(m.L.wl_embed_dev(m.ctx.handle, m.embd_w.handle, toks, T, c(x.data_ptr())))
         m.embed_scale(x, T)
-        m.run_layers(lambda l, d: check(m.L.wl_layer_dev(m.ctx.handle, ctypes.byref(d), c(x.data_ptr()), T, pos0,
-                                                         c(self.K[l, slot].data_ptr()),
-                                                         c(self.V[l, slot].data_ptr()))))
+        m.run_layers(lambda l, d: check(m.L.wl_layer_kv_dev(m.ctx.handle, ctypes.byref(d), c(x.data_ptr()), T, pos0,
+                                                            c(self.K[l, slot].data_ptr()),
+                                                            c(self.V[l, slot].data_ptr()), ctypes.byref(self.kv_opts))))
         self.length[slot] = pos0 + T
         return self._head(x[T - 1:], 1)
 
@@ -385,9 +443,10 @@ class DeviceBatch:
         x = self._buf("x", N, m.cfg.embd)
         check(m.L.wl_embed_dev_ids(m.ctx.handle, m.embd_w.handle, c(d_ids.data_ptr()), N, c(x.data_ptr())))
         m.embed_scale(x, N)
-        m.run_layers(lambda l, d: check(m.L.wl_layer_batch_dev(m.ctx.handle, ctypes.byref(d), c(x.data_ptr()), N,
-                                                               pos, sl, self.slots, self.cap,
-                                                               c(self.K[l].data_ptr()), c(self.V[l].data_ptr()))))
+        m.run_layers(lambda l, d: check(m.L.wl_layer_batch_kv_dev(m.ctx.handle, ctypes.byref(d), c(x.data_ptr()), N,
+                                                                  pos, sl, self.slots, self.cap,
+                                                                  c(self.K[l].data_ptr()), c(self.V[l].data_ptr()),
+                                                                  ctypes.byref(self.kv_opts))))
         for s in slots:
             self.length[s] += 1
         return self._head(x, N)
@@ -415,3 +474,29 @@ class DeviceBatch:
         m.ctx.sync()
         toks = ids[:steps].cpu().numpy().T.tolist()
         return (toks, seen) if keep_logits else toks
+
+    def generate(self, prompts, steps, params, u):
+        """Each prompt in its own slot, then `steps` stacked steps with the tokens drawn on the device: params is one
+        SampleParams per sequence, u the numbers [steps][sequences] in [0, 1). Returns the tokens per sequence: what
+        DeviceTransformer.generate gives each of them alone."""
+        m, c, N = self.m, ctypes.c_void_p, len(prompts)
+        d_u = m.torch.as_tensor(np.asarray(u, np.float32).reshape(-1)).to(m.dev)
+        if len(params) != N or d_u.numel() != steps * N:
+            raise ShapeError("%d settings and %d numbers for %d sequences of %d tokens."
+                             % (len(params), d_u.numel(), N, steps))
+        ids = m.torch.empty((max(steps, 1), N), dtype=m.torch.int32, device=m.dev)
+        m.torch.cuda.synchronize()
+        ps = (SampleParams * N)(*params)
+        one = [(SampleParams * 1)(p) for p in params]
+
+        def draw(lg, rows, p, s, i):
+            check(m.L.wl_sample_dev(m.ctx.handle, c(lg.data_ptr()), rows, m.vocab, p, c(d_u[s * N + i:].data_ptr()),
+                                    c(ids[s, i:].data_ptr())))
+        for i, p in enumerate(prompts):
+            lg = self.prefill(i, list(p))
+            if steps:
+                draw(lg, 1, one[i], 0, i)
+        for s in range(1, steps):
+            draw(self.step(list(range(N)), ids[s - 1]), N, ps, s, 0)
+        m.ctx.sync()
+        return ids[:steps].cpu().numpy().T.tolist()
