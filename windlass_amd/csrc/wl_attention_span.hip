@@ -143,6 +143,7 @@ struct TileKv4 {
   static constexpr int E = HD / 64, NB = HD / 32;
   u32x4_t v[E], vs;
   uint32_t k[2][4 * E / 2], ks;
+  // nontemporal: a step reads a cache once (8B after 131,000 positions 39.0 -> 35.9 us)
   __device__ __forceinline__ void load(const uint8_t *K, const uint8_t *V, int64_t, int64_t tile, int, int lane) {
     const uint8_t *kt = K + tile * (18 * HD), *vt = V + tile * (18 * HD);
     const int r = lane & 15, q = lane >> 4;
@@ -150,16 +151,16 @@ struct TileKv4 {
     for (int t = 0; t < 2; t++) {
       const uint8_t *kp = kt + (16 * t + r) * (HD / 2) + q * (HD / 8);
       if constexpr (E == 2) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t *>(kp);
+        const u32x4_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(kp));
         k[t][0] = w.x, k[t][1] = w.y, k[t][2] = w.z, k[t][3] = w.w;
       } else {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(kp);
+        const u32x2_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t *>(kp));
         k[t][0] = w.x, k[t][1] = w.y;
       }
     }
     ks = reinterpret_cast<const uint32_t *>(kt + 16 * HD)[r * NB + (E == 2 ? q : q >> 1)];
 #pragma unroll
-    for (int e = 0; e < E; e++) v[e] = reinterpret_cast<const u32x4_t *>(vt)[e * 64 + lane];
+    for (int e = 0; e < E; e++) v[e] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(vt) + e * 64 + lane);
     vs = *reinterpret_cast<const u32x4_t *>(vt + 16 * HD + (q * NB + (lane & 15) * NB / 16) * 16);
   }
   // step i of the scores of keys 16 t ..: values q HD / 4 + 8 i .. of key r
@@ -535,17 +536,19 @@ __global__ __launch_bounds__(256) void span_join_kernel(const float *__restrict_
 }
 
 // Tiles of each run of a row of n tiles (a rule on the row alone). Up to 16 tiles one run, and no second launch
-// (32 heads of 64, 7 rows at 333: 6.0 us, two runs 9.2). More: two tiles a wave, where a lone row is short of waves, to
-// four from 256 tiles on, where a run's fixed work (the query's parts, the sums through LDS, its record) weighs more
-// (64 heads of 128: one row after 4,000 10.1 us, four tiles a wave 11.7; 32 rows of up to 9,001 62 us, two
-// tiles 69, one 89). And no more runs than give every CU two workgroups.
+// (32 heads of 64, 7 rows at 333: 6.0 us, two runs 9.2). Up to 160 tiles (5,120 positions) as many runs as give every CU a
+// workgroup, of four tiles at least, a tile a wave (64 heads of 128 after 4,000: 9.7 us, 16 tiles a run 11.7; fp16, a
+// window of 4,096: 11.4 us, eight tiles 13.0). More: four tiles a wave, where a run's fixed work (the query's parts, the
+// sums through LDS, its record) weighs more than a lone row's waves (32 rows of up to 9,001 62 us, two tiles a wave
+// 69, one 89), and no more runs than give every CU two workgroups.
 static int span_per(int n, int units) {
   if (n <= 16) return n;
-  int fill = (512 + units - 1) / units;
-  fill = fill > kSpRuns ? kSpRuns : fill;
-  int per = (n + 15) / 16;
-  per = per < 2 * kSpWaves ? 2 * kSpWaves : per > 4 * kSpWaves ? 4 * kSpWaves : per;
-  return per < (n + fill - 1) / fill ? (n + fill - 1) / fill : per;
+  const int64_t all = (int64_t)n * units;
+  int64_t per = 4 * kSpWaves, one = (all + 255) / 256, two = (all + 511) / 512;
+  if (n <= 160) per = one < kSpWaves ? kSpWaves : one < per ? one : per;
+  per = per < two ? two : per;
+  const int most = (n + kSpRuns - 1) / kSpRuns;
+  return per < most ? most : (int)per;
 }
 
 // ------------------------------------------------------------------------------- prompts
