@@ -303,6 +303,134 @@ def test_scales_and_large_scores(ctx, scale):
         assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
 
 
+@pytest.mark.parametrize("T", [1, 3, 30])
+def test_scores_past_2_to_the_26(ctx, T):
+    """Scores whose units in the last place are whole powers of e: the largest key's weight is 1 all the same."""
+    KH, H, HD, pos0 = 2, 4, 64, 200
+    n = pos0 + T
+    rng = np.random.default_rng(T)
+    k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+    q = rng.standard_normal((T, H, HD), dtype=F32) * F32(1e9)
+    c = Cache(ctx, n, KH, HD)
+    c.store(k, v, 0)
+    got = c.attention(q, pos0)
+    K, V = held_ref(k).astype(np.float64), held_ref(v)
+    for t in range(T):
+        for h in range(H):
+            s = K[:pos0 + t + 1, h // 2] @ q[t, h].astype(np.float64) / 8
+            best = np.argsort(s)[-2:]
+            assert s[best[1]] - s[best[0]] > 1e4  # nothing else weighs anything
+            assert np.array_equal(got[t, h], V[best[1], h // 2])
+
+
+@pytest.mark.parametrize("T,pos0,HD", [(1, 300, 64), (1, 5000, 128), (5, 90, 128), (40, 200, 64), (33, 100, 128)])
+def test_fp16_infinities_and_nans(ctx, T, pos0, HD):
+    """In masked places they change no bit; a visible one reaches the rows that see it, and there its own column (a
+    value) or, as a score of -inf, none."""
+    H, KH, window, sinks = 4, 2, 60, 3
+    n, G = pos0 + T, 2
+    rng = np.random.default_rng(pos0)
+    k, v = (to_half_ref(rows(rng, n, KH, HD)).view(np.float16) for _ in range(2))
+    k[:, 0, 7] = np.abs(k[:, 0, 7])
+    q = rng.standard_normal((T, H, HD), dtype=F32)
+    q[:, :, 7] = np.abs(q[:, :, 7]) + F32(0.5)
+    dq = dev(q)
+
+    def run(x, y):
+        dk, dv, out = dev(x.view(np.int16)), dev(y.view(np.int16)), torch.full(q.shape, 7.0, device=DEV)
+        torch.cuda.synchronize()
+        check(load().wl_attention_window_dev(ctx.handle, P(dq), T, H, KH, HD, P(dk), P(dv), pos0, window, sinks,
+                                             1 / math.sqrt(HD), P(out)))
+        return host(ctx, out)
+
+    want = run(k, v)
+    for what, bad in (("v", np.inf), ("v", np.nan), ("k", -np.inf), ("k", np.nan)):
+        for at in (1, pos0 - window, pos0 // 2, pos0 - window + 7, pos0):
+            x, y = k.copy(), v.copy()
+            (x if what == "k" else y)[at, 0, 7] = bad
+            got = run(x, y)
+            less, tol = attention_span_ref(q, np.where(np.isfinite(x), x, 0), np.where(np.isfinite(y), y, 0),
+                                           pos0 + np.arange(T), window, sinks, 1 / math.sqrt(HD))
+            for t in range(T):
+                sees = at <= pos0 + t and (at < sinks or at > pos0 + t - window)
+                for h in range(H):
+                    if not sees or h >= G:
+                        assert np.array_equal(bits(got[t, h]), bits(want[t, h])), (what, bad, at, t, h)
+                    elif what == "v":
+                        rest = np.arange(HD) != 7
+                        assert np.array_equal(bits(got[t, h][rest]), bits(want[t, h][rest]))
+                        assert np.isnan(got[t, h, 7]) if np.isnan(bad) else got[t, h, 7] == np.inf
+                    elif np.isnan(bad):
+                        assert np.isnan(got[t, h]).all()
+                    else:  # the key weighs nothing: the rows without it
+                        m = [j for j in range(pos0 + t + 1) if j != at and (j < sinks or j > pos0 + t - window)]
+                        s = k[m, 0].astype(np.float64) @ q[t, h] / math.sqrt(HD)
+                        p = np.exp(s - s.max())
+                        ref = (p / p.sum()) @ v[m, 0].astype(np.float64)
+                        assert (np.abs(got[t, h] - ref) <= tol[t, h]).all()
+
+
+def test_many_rows_of_another_head_dim(ctx):
+    """Scores of more than one launch's scratch."""
+    T, pos0, H, KH, HD = 3000, 3000, 4, 1, 8
+    n = pos0 + T
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn((n, KH, HD), device=DEV, generator=g).half() for _ in range(2))
+    q, out = torch.randn((T, H, HD), device=DEV, generator=g), torch.empty((T, H, HD), device=DEV)
+    torch.cuda.synchronize()
+    check(load().wl_attention_window_dev(ctx.handle, P(q), T, H, KH, HD, P(k), P(v), pos0, 0, 0, 0.3, P(out)))
+    ctx.sync()
+    K, V = k[:, 0].double(), v[:, 0].double()
+    at = torch.arange(n, device=DEV)
+    for h in range(H):
+        s = torch.mm(q[:, h].double(), K.t().contiguous()) * 0.3
+        s.masked_fill_(at > pos0 + torch.arange(T, device=DEV)[:, None], -math.inf)
+        want = torch.mm(torch.softmax(s, 1), V)
+        # long_ref's bound, with scores of at most 8 * 4.5^2 * 0.3 in size and values of at most 4.5
+        assert float((out[:, h] - want).abs().max()) <= 4.5 * (8 * 2.0**-24 * 8**0.5 * 49 + 4 * 2.0**-24 * n**0.5)
+
+
+def test_a_graph_outlives_its_scratch(ctx):
+    """A later, larger call makes the context take larger scratch; the graph's own stays with it."""
+    H, KH, HD, n = 64, 8, 128, 40000
+    rng = np.random.default_rng(8)
+    with Context(0) as own:
+        c = Cache(own, n, KH, HD)
+        k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+        c.store(k, v, 0)
+        q, out = dev(rng.standard_normal((1, H, HD), dtype=F32)), torch.zeros((1, H, HD), device=DEV)
+        logits, u, tok = dev(rng.standard_normal((2, 30000), dtype=F32)), dev(np.array([0.3, 0.8], F32)), dev(np.zeros(2, np.int32))
+        from windlass_amd.backend import SampleParams
+        ps = (SampleParams * 70)(*[SampleParams(1.0, 0, 0.9, 0.0)] * 70)
+        L, h = load(), own.handle
+
+        def step():
+            check(L.wl_kv4_attention_dev(h, P(q), 1, H, KH, HD, P(c.K), P(c.V), n, 2000, 0, 0, 0.1, P(out)))
+            check(L.wl_sample_dev(h, P(logits), 2, 30000, ps, P(u), P(tok)))
+
+        step()
+        own.sync()
+        g = own.capture(step)
+        big, many = torch.empty((15, H, HD), device=DEV).normal_(), torch.randn((70, 128000), device=DEV)
+        bo, bu, bt = torch.empty_like(big), torch.rand(70, device=DEV), torch.zeros(70, dtype=torch.int32, device=DEV)
+        for i in range(3):
+            q.normal_()
+            torch.cuda.synchronize()
+            step()
+            want = [host(own, t).copy() for t in (out, tok)]
+            check(L.wl_kv4_attention_dev(h, P(big), 15, H, KH, HD, P(c.K), P(c.V), n, n - 15, 0, 0, 0.1, P(bo)))
+            check(L.wl_sample_dev(h, P(many), 70, 128000, ps, P(bu), P(bt)))
+            own.sync()
+            junk = [torch.full((1 << 22,), float("nan"), device=DEV) for _ in range(20)]  # where freed scratch would be
+            out.zero_()
+            tok.zero_()
+            torch.cuda.synchronize()
+            g.launch()
+            assert np.array_equal(bits(host(own, out)), bits(want[0])) and np.array_equal(host(own, tok), want[1]), i
+            del junk
+        g.free()
+
+
 def test_captured_calls_replay(ctx):
     """A step's store, attention over both caches and the draw, captured and replayed between eager work."""
     H, KH, HD, n = 8, 2, 128, 1500

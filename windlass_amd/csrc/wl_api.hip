@@ -9,6 +9,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <string>
@@ -71,6 +72,9 @@ struct wl_ctx {
   int float_mma;  // wl_set_float_mma: Q4_K / Q6_K decode GEMVs on the matrix cores
   int moe_chain;  // wl_set_moe_one_launch(0): the MoE entries always run the launch chain
   bool capturing = false;  // between wl_capture_begin and wl_capture_end
+  bool captured = false;   // a capture has begun: scratch that graphs may name is kept when it grows
+  void **kept = nullptr;   // such buffers, until wl_destroy
+  int nkept = 0;
   unsigned moe_launches;  // one-launch MoE launches so far (their counter sets alternate)
   bool moe_unchecked;     // one-launch MoE launches since the err word was last read
   int moe_spin = wl::MOE_SPIN;  // polls of the one-launch MoE's bounded waits
@@ -215,6 +219,19 @@ extern "C" int wl_debug_fail_alloc(int n) {
   return WL_OK;
 }
 
+// Scratch that has grown out of use: freed, or kept to the context's end where a graph may replay calls that use it (and
+// where there is no memory to note it in, left allocated).
+static void retire(wl_ctx *c, void *p) {
+  if (!c->captured) {
+    hipFree(p);
+    return;
+  }
+  void **k = (void **)realloc(c->kept, sizeof(void *) * (size_t)(c->nkept + 1));
+  if (!k) return;
+  c->kept = k;
+  c->kept[c->nkept++] = p;
+}
+
 static int ensure(wl_ctx *c, int slot, size_t bytes) {
   if (c->cap[slot] >= bytes) return WL_OK;
   if (c->capturing)
@@ -222,7 +239,7 @@ static int ensure(wl_ctx *c, int slot, size_t bytes) {
                 "once before the capture", bytes, slot, c->cap[slot]);
   if (c->buf[slot]) {
     hipStreamSynchronize(c->stream);
-    hipFree(c->buf[slot]);
+    retire(c, c->buf[slot]);
     c->buf[slot] = nullptr;
     c->cap[slot] = 0;
   }
@@ -311,6 +328,8 @@ extern "C" void wl_destroy(wl_ctx *c) {
   hipStreamSynchronize(c->stream);
   for (void *&b : c->buf)
     if (b) hipFree(b);
+  for (int i = 0; i < c->nkept; i++) hipFree(c->kept[i]);
+  free(c->kept);
   if (c->rows_host) hipHostFree(c->rows_host);
   if (c->io_host) hipHostFree(c->io_host);
   if (c->rope.dev) hipFree(c->rope.dev);
@@ -1369,7 +1388,7 @@ static int rope_angles(wl_ctx *c, const int32_t *hpos, int T, int pos0, int n, d
     const int64_t cap = ((int64_t)top + 4095) / 4096 * 4096;
     if (R.dev) {
       hipStreamSynchronize(c->stream);
-      hipFree(R.dev);
+      retire(c, R.dev);
       R.dev = nullptr;
       R.cap = 0;
     }
@@ -1403,7 +1422,7 @@ struct LayerKv {
   const int32_t *pos = nullptr, *slot = nullptr;
 };
 static int layer_attention_kv(wl_ctx *c, const wl_layer_desc *L, const LayerKv &kv, float *q, float *k, const float *v,
-                              int T, int pos0, int rd, double fs, const wl::RowMap &rm, float scale, float *att);
+                              int T, int pos0, int rd, double fs, float scale, float *att);
 
 static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, int32_t pos0, uint16_t *d_K,
                      uint16_t *d_V, const wl::RowMap &rm, const int32_t *hpos, int max_n, bool each,
@@ -1547,7 +1566,7 @@ static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, i
   const float scale = L->attention_scale != 0.f ? L->attention_scale : 1.0f / (float)sqrt((double)HD);
   const float4 *tab = nullptr;
   if (kv) {
-    if ((rc = layer_attention_kv(c, L, *kv, q, k, v, T, pos0, rd, fs, rm, scale, att))) return rc;
+    if ((rc = layer_attention_kv(c, L, *kv, q, k, v, T, pos0, rd, fs, scale, att))) return rc;
   } else {
     if (wl::rope_attention_fused(T, rm, HD, KH, rd, d_K, d_V) &&
         (rc = rope_angles(c, hpos, T, pos0, rd, L->rope_base, fs, L->d_rope_freqs, &tab)))
@@ -1876,18 +1895,14 @@ extern "C" int wl_attention_window_dev(wl_ctx *c, const float *d_q, int32_t T, i
 
 // A layer's RoPE, its rows' keys and values into the cache, and their attention.
 static int layer_attention_kv(wl_ctx *c, const wl_layer_desc *L, const LayerKv &kv, float *q, float *k, const float *v,
-                              int T, int pos0, int rd, double fs, const wl::RowMap &rm, float scale, float *att) {
+                              int T, int pos0, int rd, double fs, float scale, float *att) {
   const wl::KvCache &kc = kv.cache;
   const int H = L->heads, KH = kc.KH, HD = kc.HD;
   const int64_t QD = (int64_t)H * HD, KD = (int64_t)KH * HD;
-  if (kc.bits == 16)
-    WL_HIP(wl::rope_kv_launch(q, k, v, T, H, KH, HD, rd, L->neox, pos0, L->rope_base, fs, L->d_rope_freqs,
-                              (uint16_t *)kc.K, (uint16_t *)kc.V, rm, c->stream), "rope and kv store");
   auto rows = [&](const wl::KvRows &R, int i0) -> int {
-    if (kc.bits == 4)
-      WL_HIP(wl::rope_kv4_launch(q + i0 * QD, k + i0 * KD, v + i0 * KD, H, KH, HD, rd, L->neox, L->rope_base, fs,
-                                 L->d_rope_freqs, (uint8_t *)kc.K, (uint8_t *)kc.V, kc.positions, kc.slot_bytes, R,
-                                 c->stream), "rope and kv4 store");
+    WL_HIP(wl::rope_cache_launch(q + i0 * QD, k + i0 * KD, v + i0 * KD, H, KH, HD, rd, L->neox, L->rope_base, fs,
+                                 L->d_rope_freqs, kc.bits, (uint8_t *)kc.K, (uint8_t *)kc.V, kc.positions, kc.slot_bytes,
+                                 R, c->stream), "rope and kv store");
     return span_attention(c, q + i0 * QD, H, kc, kv.span, R, scale, att + i0 * QD);
   };
   return kv.pos ? each_rows(T, kv.pos, kv.slot, rows) : rows(seq_rows(T, pos0), 0);
@@ -1899,7 +1914,7 @@ static int layer_kv(const char *who, const wl_layer_desc *L, void *d_K, void *d_
   int rc;
   if (o->bits != 16 && o->bits != 4) return fail(WL_E_UNSUPPORTED, "%s: a cache of %d bits", who, o->bits);
   if ((rc = span_check(who, L->heads, L->kv_heads, o->window, o->sinks))) return rc;
-  if (L->head_dim <= 0 || (int64_t)L->kv_heads * L->head_dim > 1 << 24)
+  if (L->head_dim <= 0 || L->head_dim > 16384 || (int64_t)L->kv_heads * L->head_dim > 1 << 24)
     return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, L->kv_heads, L->head_dim);
   if (o->bits == 4) {
     if ((rc = kv4_check(who, L->kv_heads, L->head_dim, d_K, d_V))) return rc;
@@ -1946,15 +1961,7 @@ extern "C" int wl_layer_batch_kv_dev(wl_ctx *c, const wl_layer_desc *L, float *d
     return wl_layer_batch_dev(c, L, d_x, N, pos, slot, slots, slot_positions, (uint16_t *)d_K, (uint16_t *)d_V);
   kv.pos = pos;
   kv.slot = slot;
-  wl::RowMap rm;
-  if (o->bits == 16) {  // the RoPE and fp16 stores read the rows' positions and slots on the device
-    int32_t *rows;
-    if ((rc = stage_rows(c, pos, slot, N, &rows))) return rc;
-    rm.pos = rows;
-    rm.slot = rows + N;
-    rm.cap = slot_positions;
-  }
-  return layer_run(c, L, d_x, N, 0, (uint16_t *)d_K, (uint16_t *)d_V, rm, pos, 0, true, &kv);
+  return layer_run(c, L, d_x, N, 0, (uint16_t *)d_K, (uint16_t *)d_V, wl::RowMap{}, pos, 0, true, &kv);
 }
 
 extern "C" int wl_sample_dev(wl_ctx *c, const float *d_logits, int32_t rows, int64_t n, const wl_sample_params *params,
@@ -1970,10 +1977,11 @@ extern "C" int wl_sample_dev(wl_ctx *c, const float *d_logits, int32_t rows, int
   }
   if (rows == 0) return WL_OK;
   WL_ON_DEVICE(c);
-  const int most = rows < wl::kSampleRows ? rows : wl::kSampleRows;
-  if (const int rc = ensure(c, S_SMP, (size_t)wl::sample_scratch_bytes(most, n))) return rc;
-  for (int r0 = 0; r0 < rows; r0 += wl::kSampleRows) {
-    const int m = rows - r0 < wl::kSampleRows ? rows - r0 : wl::kSampleRows;
+  int most = wl::kSampleRows;  // rows a launch: as many as 256 MB of scratch take
+  while (most > 1 && wl::sample_scratch_bytes(most, n) > (int64_t)256 << 20) most /= 2;
+  if (const int rc = ensure(c, S_SMP, (size_t)wl::sample_scratch_bytes(rows < most ? rows : most, n))) return rc;
+  for (int r0 = 0; r0 < rows; r0 += most) {
+    const int m = rows - r0 < most ? rows - r0 : most;
     wl::SampleSets sets = {};
     for (int i = 0; i < m; i++) {
       const wl_sample_params &p = params[r0 + i];
@@ -2007,7 +2015,7 @@ extern "C" int wl_capture_begin(wl_ctx *c) {
   if (c->capturing) return fail(WL_E_ARG, "wl_capture_begin: the context is already capturing");
   WL_HIP(hipSetDevice(c->device), "hipSetDevice");
   WL_HIP(hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal), "hipStreamBeginCapture");
-  c->capturing = true;
+  c->capturing = c->captured = true;
   return WL_OK;
 }
 

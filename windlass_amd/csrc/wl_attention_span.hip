@@ -67,14 +67,15 @@ __device__ void span_row(const F16Rows &c, const float *qp, int HD, int p, const
 }
 
 __global__ __launch_bounds__(256) void span_rows_kernel(const float *__restrict__ q, int H, KvCache c, Span s, KvRows R,
-                                                        float scale, float *__restrict__ scores, int64_t max_n,
+                                                        int t0, float scale, float *__restrict__ scores, int64_t max_n,
                                                         float *__restrict__ out) {
-  const int h = blockIdx.x, t = blockIdx.y, kvh = h / (H / c.KH), HD = c.HD;
+  const int h = blockIdx.x, t = t0 + blockIdx.y, kvh = h / (H / c.KH), HD = c.HD;
   const int64_t row = ((int64_t)t * H + h), off = (int64_t)R.slot_of(t) * c.slot_bytes;
   const float *qp = q + row * HD;
   const int64_t head = off + (int64_t)kvh * HD * 2;
   span_row(F16Rows{(const uint16_t *)(c.K + head), (const uint16_t *)(c.V + head), (int64_t)c.KH * HD}, qp, HD,
-           R.position(t), s, scale, scores + row * max_n, out + row * HD);
+           R.position(t), s, scale,
+           scores + ((int64_t)blockIdx.y * H + h) * max_n, out + row * HD);
 }
 
 // ------------------------------------------------------------------------------- few rows
@@ -556,8 +557,8 @@ static int span_per(int n, int units) {
 // wl_attention.hip: S^T = K Q^T, a column per (token, query head of the KV head) in the order token * G + head,
 // 32 columns a wave, 64 keys a step, staged in LDS for the workgroup's four waves as fp16 rows of keys and, transposed,
 // rows of values in the order in which the scores' registers meet them. Two stages: a step's keys are unpacked while the
-// step before is multiplied, with one barrier between steps. A row's maximum is an integer in log2 units, so that the
-// exponential's argument is one rounding (S c2 - m), and raised only by scores more than 2^6 past it.
+// step before is multiplied, with one barrier between steps. The exponential's argument is the score's difference from the
+// running maximum, times the scale, as above: scores of any size keep their largest near 1.
 constexpr int kTlK = 64, kTlW = 4, kTlCols = 32 * kTlW;
 typedef float sf16 __attribute__((ext_vector_type(16)));
 
@@ -848,7 +849,8 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
   for (int d = 0; d < ND; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) O[d][i] = 0.f;
-  float M = -INFINITY, top = -INFINITY;  // log2 units; top: the score that raises it
+  float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
+  const float past = kSpPast / c2;
   double L = 0.0;
   const uint32_t ones = fp16_ones();
   auto stage = [&](int b, int j0) __attribute__((always_inline)) {
@@ -882,19 +884,18 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
 #pragma unroll
         for (int k = 0; k < NK; k++)
           S = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), ql[k], S, 0, 0, 0);
-        if (badk) {  // past an infinity the low parts' product means nothing
-          const sf16 B = S;
 #pragma unroll
-          for (int e = 0; e < 16; e++) S[e] = 0.f;
+        for (int k = 0; k < NK; k++)
+          S = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), qh[k], S, 0, 0, 0);
+        if (badk) {  // past an infinity the low parts' product means nothing: there the high parts' alone
+          sf16 A;
 #pragma unroll
-          for (int k = 0; k < NK; k++)
-            S = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), qh[k], S, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 16; e++) S[e] = __builtin_isfinite(S[e]) ? S[e] + B[e] : S[e];
-        } else {
+          for (int e = 0; e < 16; e++) A[e] = 0.f;
 #pragma unroll
           for (int k = 0; k < NK; k++)
-            S = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), qh[k], S, 0, 0, 0);
+            A = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kp + 16 * k), qh[k], A, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 16; e++) S[e] = __builtin_isfinite(A[e]) ? S[e] : A[e];
         }
         const int js = j0 + 32 * s;
         if (!(js + 31 <= pa && (js >= firstb || js + 31 < leada))) {  // uniform: some row does not see every key
@@ -908,12 +909,10 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
         float mt = S[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) mt = fmaxf(mt, S[e]);
-        mt *= c2;
         if (__any(mt > top)) {
           mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
           const bool up = mt > top;
-          const float Mn = up ? ceilf(mt) : M;
-          const float al = up ? __builtin_amdgcn_exp2f(M - Mn) : 1.f;
+          const float al = up ? __builtin_amdgcn_exp2f((M - mt) * c2) : 1.f;
           L *= (double)al;
 #pragma unroll
           for (int e = 0; e < 4; e++) ts[e] *= al;
@@ -921,8 +920,8 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
           for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int e = 0; e < 16; e++) O[d][e] *= al;
-          M = Mn;
-          top = M + kSpPast;
+          M = up ? mt : M;
+          top = M + past;
         }
         const float Mu = M == -INFINITY ? 0.f : M;  // no key of this row yet: every score is -inf
         const int va = here(val_at(col, 8 * hf));
@@ -931,8 +930,8 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
           uint32_t ph[4], pl[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float P0 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * k + 2 * e], c2, -Mu));
-            const float P1 = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8 * k + 2 * e + 1], c2, -Mu));
+            const float P0 = __builtin_amdgcn_exp2f((S[8 * k + 2 * e] - Mu) * c2);
+            const float P1 = __builtin_amdgcn_exp2f((S[8 * k + 2 * e + 1] - Mu) * c2);
             ts[2 * (e & 1)] += P0;
             ts[2 * (e & 1) + 1] += P1;
             split_pair(P0, P1, ph[e], pl[e]);
@@ -978,7 +977,7 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
     }
   if (!whole && hf == 0) {
     op[HD] = M;
-    op[HD + 1] = 0.f;
+    op[HD + 1] = c2;
     *reinterpret_cast<double *>(op + HD + 2) = L;
   }
 }
@@ -1000,7 +999,7 @@ __global__ __launch_bounds__(256) void span_tiles_join_kernel(const float *__res
   float o[HD / 64] = {};
   for (int i = 0; i < n; i++) {
     const float *rc = rec + i * (HD + 4);
-    const float w = __builtin_amdgcn_exp2f(rc[HD] - m);
+    const float w = __builtin_amdgcn_exp2f((rc[HD] - m) * rc[HD + 1]);
     L += *reinterpret_cast<const double *>(rc + HD + 2) * (double)w;
 #pragma unroll
     for (int e = 0; e < HD / 64; e++) o[e] = __builtin_fmaf(rc[lane + 64 * e], w, o[e]);
@@ -1084,6 +1083,12 @@ static int64_t span_max_n(const Span &s, const KvRows &R) {
   return m;
 }
 
+// Rows of the plain kernel's launches: their scores take at most 256 MB, where one row's do.
+static int span_rows_step(int H, const Span &s, const KvRows &R) {
+  const int64_t one = (int64_t)H * span_max_n(s, R), fit = ((int64_t)64 << 20) / one;
+  return (int)(fit < 1 ? 1 : fit > 32768 ? 32768 : fit < R.n ? fit : R.n);
+}
+
 int64_t attention_span_scratch_floats(const KvCache &c, int H, const Span &s, const KvRows &R) {
   if (R.n <= 0) return 0;
   if (span_decodes(c, R)) {
@@ -1094,7 +1099,7 @@ int64_t attention_span_scratch_floats(const KvCache &c, int H, const Span &s, co
     const TilesArgs A = tiles_plan(c, H, s, R);
     return A.chunks > 1 ? (int64_t)R.n * H * A.chunks * (c.HD + 4) : 0;
   }
-  return (int64_t)R.n * H * span_max_n(s, R);
+  return (int64_t)span_rows_step(H, s, R) * H * span_max_n(s, R);
 }
 
 hipError_t attention_span_launch(const float *q, int H, const KvCache &c, const Span &s, const KvRows &R, float scale,
@@ -1114,9 +1119,15 @@ hipError_t attention_span_launch(const float *q, int H, const KvCache &c, const 
     return c.HD == 64 ? span_tiles_launch<64, StageF16<64>>(q, H, c, s, R, scale, scratch, out, st)
                       : span_tiles_launch<128, StageF16<128>>(q, H, c, s, R, scale, scratch, out, st);
   }
-  hipLaunchKernelGGL(span_rows_kernel, dim3(H, R.n), dim3(256), 0, st, q, H, c, s, R, scale, scratch, span_max_n(s, R),
-                     out);
-  return hipGetLastError();
+  const int step = span_rows_step(H, s, R);
+  for (int t0 = 0; t0 < R.n; t0 += step) {
+    const int n = R.n - t0 < step ? R.n - t0 : step;
+    hipLaunchKernelGGL(span_rows_kernel, dim3(H, n), dim3(256), 0, st, q, H, c, s, R, t0, scale, scratch, span_max_n(s, R),
+                       out);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace wl

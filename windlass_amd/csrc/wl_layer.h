@@ -30,11 +30,12 @@ hipError_t rope_launch(float *x, int64_t ldx, int T, int heads, int hd, int n, i
 hipError_t rope_kv_launch(float *q, float *k, const float *v, int T, int H, int KH, int hd, int n, int neox,
                           int pos0, double base, double freq_scale, const float *freqs, uint16_t *Kc, uint16_t *Vc,
                           const RowMap &rm, hipStream_t st);
-// A layer's RoPE on q (in place) and k, and the 4-bit stores of k and v (wl_kv4.h; caches of `positions` positions,
-// slot_bytes apart), with the bits of the two apart; k is left as it was or rotated. One launch up to 64 rows.
-hipError_t rope_kv4_launch(float *q, float *k, const float *v, int H, int KH, int hd, int n, int neox, double base,
-                           double freq_scale, const float *freqs, uint8_t *K4, uint8_t *V4, int64_t positions,
-                           int64_t slot_bytes, const KvRows &rows, hipStream_t st);
+// A layer's RoPE on q (in place) and k, and the stores of k and v into caches of 16 or 4 bits (wl_kv4.h) of `positions`
+// positions, slot_bytes apart, with the bits of the operations apart; k is left as it was or rotated. One launch up to 64
+// rows (hd at most 16,384: a head's values lie in LDS).
+hipError_t rope_cache_launch(float *q, float *k, const float *v, int H, int KH, int hd, int n, int neox, double base,
+                             double freq_scale, const float *freqs, int bits, uint8_t *K, uint8_t *V, int64_t positions,
+                             int64_t slot_bytes, const KvRows &rows, hipStream_t st);
 hipError_t kv_store_launch(const float *k, const float *v, int64_t n, uint16_t *K, uint16_t *V, hipStream_t st);
 // Floats of scratch attention_launch needs for these operands; max_n: the most positions a row
 // attends to (pos0 + T for one sequence).

@@ -281,34 +281,44 @@ __global__ __launch_bounds__(256) void rope_qkv_kernel(RopeRow R) {
     for (int j = first; j < KD; j += step) R.column(t, crow, j);
 }
 
-// RoPE and the 4-bit stores of up to kRopeItemRows rows: one wave per head of q, k and v. Every pair's angle by its own
-// thread, as rope_items_kernel takes it; a key head is rotated in LDS and its blocks held from there.
-__global__ __launch_bounds__(64) void rope_kv4_kernel(RopeRow R, uint8_t *__restrict__ K4, uint8_t *__restrict__ V4,
-                                                      int64_t tiles, int64_t slot_bytes, KvRows rows) {
-  __shared__ float x[128];
+// RoPE and the cache stores of up to kRopeItemRows rows, their positions and slots in the arguments: one wave per head of q,
+// k and v. Every pair's angle by its own thread, as rope_items_kernel takes it; a key head is rotated in LDS and held from
+// there, in blocks of 4 bits or as ToHalf gives it.
+__global__ __launch_bounds__(64) void rope_cache_kernel(RopeRow R, int bits, uint8_t *__restrict__ K,
+                                                        uint8_t *__restrict__ V, int64_t positions, int64_t slot_bytes,
+                                                        KvRows rows) {
+  extern __shared__ float x[];  // hd
   const int head = blockIdx.x, t = blockIdx.y, lane = threadIdx.x, half = R.n / 2;
   const int p = rows.position(t);
-  const bool val = head >= R.H + R.KH;
-  float c = 0.f, s = 0.f, y0, y1;
-  int a, b;
-  if (!val) rope_cs(p, lane < half ? lane : 0, half, R.theta_scale, R.freq_scale, R.freqs, c, s);
-  if (head < R.H) {
-    if (lane < half) rope_pair(R.q + (int64_t)t * R.ldq + (int64_t)head * R.hd, lane, R.n, R.neox, c, s, y0, y1, a, b);
+  const bool isq = head < R.H, val = head >= R.H + R.KH;
+  const int kvh = val ? head - R.H - R.KH : head - R.H;
+  float *qh = R.q + (int64_t)t * R.ldq + (int64_t)head * R.hd;
+  if (!isq) {
+    const float *row = (val ? R.v : R.k) + ((int64_t)t * R.KH + kvh) * R.hd;
+    for (int i = lane; i < R.hd; i += 64) x[i] = row[i];
+    __syncthreads();
+  }
+  if (!val)
+    for (int i0 = 0; i0 < half; i0 += 64) {  // every lane runs the angle product (uniform trip count)
+      float c, s, y0, y1;
+      int a, b;
+      rope_cs(p, i0 + lane < half ? i0 + lane : 0, half, R.theta_scale, R.freq_scale, R.freqs, c, s);
+      if (i0 + lane < half) rope_pair(isq ? qh : x, i0 + lane, R.n, R.neox, c, s, y0, y1, a, b);
+    }
+  if (isq) return;
+  __syncthreads();
+  uint8_t *cache = (val ? V : K) + rows.slot_of(t) * slot_bytes;
+  if (bits == 16) {
+    uint16_t *o = reinterpret_cast<uint16_t *>(cache) + ((int64_t)p * R.KH + kvh) * R.hd;
+    for (int i = lane; i < R.hd; i += 64) o[i] = to_half(x[i]);
     return;
   }
-  const int kvh = val ? head - R.H - R.KH : head - R.H;
-  const float *row = (val ? R.v : R.k) + ((int64_t)t * R.KH + kvh) * R.hd;
-  for (int i = lane; i < R.hd; i += 64) x[i] = row[i];
-  __syncthreads();
-  if (!val && lane < half) rope_pair(x, lane, R.n, R.neox, c, s, y0, y1, a, b);
-  __syncthreads();
   if (lane >= R.hd / 8) return;  // 8 or 16 lanes: whole blocks
   float w[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) w[i] = x[8 * lane + i];
-  kv4_put(w, val, lane,
-          (val ? V4 : K4) + rows.slot_of(t) * slot_bytes + ((int64_t)kvh * tiles + p / kKv4Tile) * (18 * R.hd),
-          p % kKv4Tile, R.hd);
+  const int64_t tile = (int64_t)kvh * ((positions + kKv4Tile - 1) / kKv4Tile) + p / kKv4Tile;
+  kv4_put(w, val, lane, cache + tile * (18 * R.hd), p % kKv4Tile, R.hd);
 }
 
 // ToHalf (src/Transformer.cs:342-348) of one token's keys and values.
@@ -1039,20 +1049,23 @@ hipError_t rope_kv_launch(float *q, float *k, const float *v, int T, int H, int 
                            freqs, Kc, Vc, rm.slot, rm.cap}, T, st);
 }
 
-hipError_t rope_kv4_launch(float *q, float *k, const float *v, int H, int KH, int hd, int n, int neox, double base,
-                           double freq_scale, const float *freqs, uint8_t *K4, uint8_t *V4, int64_t positions,
-                           int64_t slot_bytes, const KvRows &rows, hipStream_t st) {
+hipError_t rope_cache_launch(float *q, float *k, const float *v, int H, int KH, int hd, int n, int neox, double base,
+                             double freq_scale, const float *freqs, int bits, uint8_t *K, uint8_t *V, int64_t positions,
+                             int64_t slot_bytes, const KvRows &rows, hipStream_t st) {
   if (rows.n <= 0) return hipSuccess;
   const RopeRow R{q, (int64_t)H * hd, H, k, v, KH, hd, n, neox, rows.pos0, nullptr, pow(base, -2.0 / n), freq_scale, freqs,
                   nullptr, nullptr, nullptr, 0};
-  if (rows.n <= kRopeItemRows) {
-    hipLaunchKernelGGL(rope_kv4_kernel, dim3(H + 2 * KH, rows.n), dim3(64), 0, st, R, K4, V4,
-                       (positions + kKv4Tile - 1) / kKv4Tile, slot_bytes, rows);
+  if (rows.n <= kRopeItemRows) {  // every batch's rows
+    hipLaunchKernelGGL(rope_cache_kernel, dim3(H + 2 * KH, rows.n), dim3(64), (size_t)hd * 4, st, R, bits, K, V, positions,
+                       slot_bytes, rows);
     return hipGetLastError();
   }
-  const hipError_t e = rope_rows(R, rows.n, st);  // rows of one sequence
+  if (bits == 16)
+    return rope_kv_launch(q, k, v, rows.n, H, KH, hd, n, neox, rows.pos0, base, freq_scale, freqs,
+                          reinterpret_cast<uint16_t *>(K), reinterpret_cast<uint16_t *>(V), RowMap{}, st);
+  const hipError_t e = rope_rows(R, rows.n, st);
   if (e != hipSuccess) return e;
-  return kv4_store_launch(k, v, KH, hd, K4, V4, positions, slot_bytes, rows, st);
+  return kv4_store_launch(k, v, KH, hd, K, V, positions, slot_bytes, rows, st);
 }
 
 hipError_t kv_store_launch(const float *k, const float *v, int64_t n, uint16_t *K, uint16_t *V, hipStream_t st) {
