@@ -474,7 +474,8 @@ int wl_matmul_dev_noalloc(wl_ctx *ctx, const wl_weight *w, int32_t expert, const
  * is recorded, not run, and wl_capture_end returns the recording as one graph. wl_graph_launch
  * replays it on the context's stream: the same kernels with the same arguments (the same device
  * buffers, the same weights), enqueued by one host call. A call that would grow the context's
- * scratch during a capture fails with WL_E_ARG (run the same calls once before capturing), and
+ * scratch during a capture fails with WL_E_ARG (run the same calls once before capturing); scratch
+ * that later calls outgrow is kept until wl_destroy, since a recording may use it; and
  * the MoE entries take their launch chain while capturing (the same bits as one launch).
  * Host-buffer entries synchronise and must not be called while capturing. */
 typedef struct wl_graph wl_graph;

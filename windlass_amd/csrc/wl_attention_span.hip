@@ -91,6 +91,13 @@ __global__ __launch_bounds__(256) void span_rows_kernel(const float *__restrict_
 // A workgroup of W waves takes a run of a row's tiles (32 positions each), the waves one tile in turn, each
 // with its own running maximum, sum and output; they are added through LDS. Long rows are cut in runs by a rule
 // on the row's own tiles, so that a row's bits do not depend on the rows beside it.
+//
+// What bounds it: a 4-bit position of a head is 2.25 HD bytes for 4 HD G products. One row after 131,000 (8B, 151 MB) takes
+// 33.8 us and the join 4, against 24.8 for reading the bytes: the loads wait 43% of the wave cycles and the unpacking
+// keeps the VALU 54% busy. 32 rows of up to 9,001 (70B, 249 MB): 60.4 us, VALU 67%, matrix cores 9%; short contexts are
+// two launches' latency (70B after 4,000: 6.0 and 3.1 us). Measured and not kept: the last workgroup of a row joining its
+// runs (with fences 770 us for the 32 rows; with device-scope stores 66.9 against 61.6, and 41.7 against 35.5 for the long
+// row), records loaded ahead in the join (62.5 -> 66), eight waves a workgroup.
 typedef float sf4 __attribute__((ext_vector_type(4)));
 // A running maximum is raised only by scores more than 2^6 past it, so nearly never after a wave's first tile: the
 // exponentials reach 2^6, and 2^8 of them are fp16 parts (22 bits down to 2^-22 of the row's largest, 2^-33 of it below).
@@ -559,6 +566,13 @@ static int span_per(int n, int units) {
 // rows of values in the order in which the scores' registers meet them. Two stages: a step's keys are unpacked while the
 // step before is multiplied, with one barrier between steps. The exponential's argument is the score's difference from the
 // running maximum, times the scale, as above: scores of any size keep their largest near 1.
+//
+// What bounds it: both products twice (two parts), 206 GFLOP for 2,048 tokens of the 8B model's 32 heads after 2,048, in
+// 214 us: 960 TFLOP/s, where a library's product of 4,096 x 4,096 matrices reaches 1,100. The matrix cores are busy 38%
+// of the cycles and the VALU 48%, with two waves a SIMD that seldom overlap them; 254 registers leave no room for a second
+// tile of scores, and kernels that kept one (the scores of 32 keys beside the exponentials of the 32 before) spilled and
+// took 297-308 us. Rows cut in two and more chunks where whole rows fill the CUs: 282 us; 2 and 4 chunks for a window of
+// 1,500 rows, whose 376 workgroups are one and two a CU: 114 and 131 us against 102.
 constexpr int kTlK = 64, kTlW = 4, kTlCols = 32 * kTlW;
 typedef float sf16 __attribute__((ext_vector_type(16)));
 
@@ -600,7 +614,7 @@ __device__ __forceinline__ int here(int v) {
 template <int HD>
 struct StageKv4 {
   static constexpr int NB = HD / 32, E = HD / 64, UN = 64 * NB;  // units of 16 bytes of each
-  static constexpr bool kInf = false;
+  static constexpr bool kInf = false, kPrio = false;
   u32x4_t k, v, vs;
   uint16_t ks;
   int kkey, kblk, vt, vl, ve, vblk;
@@ -705,6 +719,9 @@ template <int HD>
 struct StageF16 {
   static constexpr int U = HD / 8, KI = 64 * U / 256;
   static constexpr bool kInf = true;
+  // exponentials and the products after them before the other wave's work: a window of 1,500 rows 102 -> 97 us (with 4-bit
+  // tiles, whose staging is the VALU's, 214 -> 221)
+  static constexpr bool kPrio = true;
   u32x4_t k[KI], v[4];
   const uint16_t *K, *V;
   int64_t kv_dim;
@@ -906,6 +923,7 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
             S[e] = (at > p) | ((at >= lead) & (at < first)) ? -INFINITY : S[e];
           }
         }
+        if constexpr (Stage::kPrio) __builtin_amdgcn_s_setprio(1);
         float mt = S[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) mt = fmaxf(mt, S[e]);
@@ -946,6 +964,7 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
           }
         }
       }
+      if constexpr (Stage::kPrio) __builtin_amdgcn_s_setprio(0);
       if (s == 0 && i + 1 < i1) {
         stage(b ^ 1, st.at(i + 1));
         if (i + 2 < i1) sg.fetch(st.at(i + 2), last);
