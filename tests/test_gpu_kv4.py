@@ -431,6 +431,30 @@ def test_a_graph_outlives_its_scratch(ctx):
         g.free()
 
 
+def test_kept_scratch_stays_small():
+    """Once anything was captured, scratch that a longer context outgrows is kept: all of it stays below three times the
+    last's 130 MB and half as much again (one call's growth at a time would keep 40 sizes, 2.6 GB)."""
+    H, KH, HD, n, T = 64, 8, 128, 1 << 17, 15
+    with Context(0) as own:
+        L, h = load(), own.handle
+        K, V = [torch.zeros(L.wl_kv4_bytes(n, KH, HD), dtype=torch.uint8, device=DEV) for _ in range(2)]
+        q, out = torch.randn((T, H, HD), device=DEV), torch.empty((T, H, HD), device=DEV)
+        torch.cuda.synchronize()
+
+        def at(pos):
+            check(L.wl_kv4_attention_dev(h, P(q), T, H, KH, HD, P(K), P(V), n, pos, 0, 0, 0.1, P(out)))
+
+        at(1000)
+        own.sync()
+        own.capture(lambda: at(1000)).free()
+        before = torch.cuda.mem_get_info()[0]
+        for i in range(1, 41):
+            at(i * (n - T) // 40)
+        own.sync()
+        last = T * H * 256 * (HD + 4) * 4
+        assert before - torch.cuda.mem_get_info()[0] < 3 * 1.5 * last + (64 << 20)
+
+
 def test_captured_calls_replay(ctx):
     """A step's store, attention over both caches and the draw, captured and replayed between eager work."""
     H, KH, HD, n = 8, 2, 128, 1500

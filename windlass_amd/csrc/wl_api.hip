@@ -237,14 +237,27 @@ static int ensure(wl_ctx *c, int slot, size_t bytes) {
   if (c->capturing)
     return fail(WL_E_ARG, "a captured call needs %zu bytes of scratch slot %d, which holds %zu: run the same calls "
                 "once before the capture", bytes, slot, c->cap[slot]);
+  size_t want = bytes < 4096 ? 4096 : bytes;
+  const size_t least = want;
   if (c->buf[slot]) {
+    // half as much again where growth repeats as positions go on (each allocation waits for the stream), and where what is
+    // outgrown is kept: so that all of it stays below two of the last
+    if (c->captured || slot == S_ATT) {
+      const size_t more = c->cap[slot] / 2, grown = c->cap[slot] + (more < (size_t)256 << 20 ? more : (size_t)256 << 20);
+      want = want < grown ? grown : want;
+    }
     hipStreamSynchronize(c->stream);
     retire(c, c->buf[slot]);
     c->buf[slot] = nullptr;
     c->cap[slot] = 0;
   }
-  size_t want = bytes < 4096 ? 4096 : bytes;
-  if (dev_alloc(&c->buf[slot], want) != hipSuccess) {
+  hipError_t e = dev_alloc(&c->buf[slot], want);
+  if (e != hipSuccess && want > least) {
+    (void)hipGetLastError();  // or the next launch's check reports it
+    e = dev_alloc(&c->buf[slot], want = least);
+  }
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
     c->buf[slot] = nullptr;
     return fail(WL_E_NOMEM, "cannot allocate %zu bytes of device scratch", want);
   }

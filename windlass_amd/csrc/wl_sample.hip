@@ -181,7 +181,7 @@ __global__ __launch_bounds__(WIDE) void sample_bins_kernel(const float *__restri
   constexpr int N = kSmPart / WIDE;
   __shared__ unsigned cn[kSmBins];
   __shared__ u64 ms[kSmBins];
-  __shared__ uint16_t ids[kSmPart];
+  __shared__ __attribute__((aligned(16))) uint16_t ids[kSmPart];
   __shared__ float sh[2];
   __shared__ unsigned mc, sc[4];
   __shared__ u64 mm, sm[4];
@@ -255,7 +255,8 @@ __global__ __launch_bounds__(WIDE) void sample_bins_kernel(const float *__restri
   // places past the part's tokens hold nothing that is read
 #pragma unroll
   for (int j = 0; j < (kSmPart / 8 + WIDE - 1) / WIDE; j++)
-    if (tid + WIDE * j < kSmPart / 8) reinterpret_cast<uint4 *>(X.id + part * kSmPart)[tid + WIDE * j] = reinterpret_cast<const uint4 *>(ids)[tid + WIDE * j];
+    if (tid + WIDE * j < kSmPart / 8)
+      reinterpret_cast<uint4 *>(X.id + part * kSmPart)[tid + WIDE * j] = reinterpret_cast<const uint4 *>(ids)[tid + WIDE * j];
 }
 
 // A question: the shortest prefix with at least `count` tokens, or of at least `mass`, or of more.
