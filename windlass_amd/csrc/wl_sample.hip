@@ -524,6 +524,15 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
     S.cn[tid] = 0;
     S.ms[tid] = 0;
   }
+  // four threads a bin, each a quarter of the parts; the counts come as running sums
+  unsigned c = 0;
+  u64 m = 0;
+  const int b = tid & (kSmBins - 1);
+#pragma unroll 8
+  for (int p = tid / kSmBins; p < parts; p += 4) {
+    c += V.end[(int64_t)p * kSmBins + b];
+    m += masses[(int64_t)p * kSmBins + b];
+  }
   unsigned mpc = 0;
   u64 mpm = 0;
   if (set.min_p > 0.f)
@@ -538,15 +547,6 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
     return;
   }
   {
-    // four threads a bin, each a quarter of the parts; the counts come as running sums
-    unsigned c = 0;
-    u64 m = 0;
-    const int b = tid & (kSmBins - 1);
-#pragma unroll 8
-    for (int p = tid / kSmBins; p < parts; p += 4) {
-      c += V.end[(int64_t)p * kSmBins + b];
-      m += masses[(int64_t)p * kSmBins + b];
-    }
     atomicAdd(&S.cn[b], c);
     atomicAdd(&S.ms[b], m);
     __syncthreads();
