@@ -121,6 +121,18 @@ def test_masked_and_non_finite_logits(ctx):
         compare(ctx, l, rng, [s] * len(l))
 
 
+@pytest.mark.parametrize("masked", [0.0, 0.5, 0.97])
+def test_counts_past_the_bins(ctx, masked):
+    """A low temperature leaves most tokens below the bins' reach: top_k ends among them, or among masked ones."""
+    rng = np.random.default_rng(int(masked * 100))
+    n, ks = 50001, [20, 300, 1400, 5000, 26000, 45000, 50000]
+    l = peaked(rng, 3 * len(ks), n)
+    l[rng.random(l.shape) < masked] = -np.inf
+    l[2::3] = np.rint(l[2::3] * F32(2)) / F32(2)  # many equal
+    l[:, 17] = np.finfo(F32).min
+    compare(ctx, l, rng, [dict(temperature=t, top_k=k, top_p=p) for k in ks for t, p in [(0.002, 1.0), (0.03, 0.9), (0.3, 0.99)]])
+
+
 def test_numbers_outside_the_range(ctx):
     l = np.array([[1.0, 5.0, 3.0, 3.0]] * 4, F32)
     got = sample(ctx, l, [-1.0, np.nan, 1.0, np.inf], [dict(top_k=3)] * 4)

@@ -14,11 +14,13 @@
 // and weight of its tokens in 256 bins of equal width below the row's maximum (64 t wide at most, weights below e^-64
 // in the last bin), its tokens' places by bin, and what has w >= min_p. (3) One workgroup a row adds the parts'
 // bins and answers the questions: a prefix's end lies in one bin, whose tokens it gathers and narrows down by their
-// bits; with top_k of few tokens it gathers the whole prefix and puts that in order.
+// bits, and equal ones by their ids; with top_k of few tokens it gathers the whole prefix and puts that in order.
 //
-// What bounds it: a row of 128,256 is read from HBM in launch 1 and from the caches after (64 rows, 33 MB: 6.4 us), then
-// 64 rows' bins take 25.4 us (LDS atomics, the double polynomial and their latency) and their questions 20 (a workgroup a
-// row, each question a few dependent loads). One row is three dependent launches: 2.5, 6.5 and 10.4 us.
+// What bounds it: a row of 128,256 is read from HBM in launch 1 and from the caches after (64 rows, 33 MB: 6.2 us), then
+// 64 rows' bins take 24.2 us (50 VALU instructions a token, and LDS atomics that meet: two or four copies of the bins, votes
+// for the last bin and no min_p sums where none is asked each gained less than a microsecond or lost) and their questions
+// 16.6 (a workgroup a row: chains of LDS and cache latencies, 2.5 to 6 us a question). One row is three dependent launches:
+// 2.4, 6.6 and 6.3 us.
 #include "wl_sample.h"
 
 #include "wl_device.h"
@@ -29,7 +31,7 @@
 
 namespace wl {
 
-constexpr int kSmBins = 256, kSmPart = 4096, kSmList = 4096, kSmFew = 64, kSmPrefix = 256, kSmGroup = 64;
+constexpr int kSmBins = 256, kSmPart = 4096, kSmList = 4096, kSmFew = 256, kSmGroup = 64;
 typedef unsigned long long u64;
 
 // A part's record.
@@ -87,6 +89,14 @@ struct SmRow {
     const float d = m - cap(l);
     return d > R ? kSmBins - 1 : min((int)(d * c), kSmBins - 2);
   }
+  // Bounds of the keys of a bin's logits: its edges, past what bin() rounds.
+  __device__ void keys(int b, uint32_t &lo, uint32_t &hi) const {
+    const double step = (double)R * (1.0 / (kSmBins - 2));  // 1 / c, but for c's rounding
+    const double up = (double)min(b, kSmBins - 2) * step * (1.0 - 0x1p-20), down = (double)(b + 1) * step * (1.0 + 0x1p-20);
+    hi = b ? sm_key((float)((double)m - up)) + 1 : m < 3.4028235e38f ? sm_key(m) : sm_key(INFINITY);
+    lo = sm_key(-INFINITY);
+    if (b < kSmBins - 1) lo = sm_key(fmaxf((float)((double)m - down), -3.4028235e38f)) - 1;
+  }
   // w in units of 2^-shift: 2^x for x = (l - m) log2(e) / t, as 2^k times 2^f, f in [-1/2, 1/2], by its series to the 11th
   // power (the rest is below 2^-47 of it), its significand shifted.
   __device__ __forceinline__ u64 mass(float l, const SmSeries &C) const {
@@ -123,19 +133,52 @@ __device__ __forceinline__ void sm_row_of(const SmPart *__restrict__ part, int p
   r.set(sh[0], sh[1], t, shift);
 }
 
+// Running sums over a wave's lanes (all of them active): within rows of 16 by lane shifts, then the rows' sums. A general
+// shuffle goes through LDS, and each of its six steps costs that latency (one row's draw 15.7 us, with these 15.1).
+template <int CTRL>
+__device__ __forceinline__ unsigned sm_dpp(unsigned v) {
+  return dpp32<CTRL>(v);
+}
+template <int CTRL>
+__device__ __forceinline__ u64 sm_dpp(u64 v) {
+  return (u64)dpp32<CTRL>((uint32_t)(v >> 32)) << 32 | dpp32<CTRL>((uint32_t)v);
+}
+__device__ __forceinline__ unsigned sm_lane(unsigned v, int l) { return (unsigned)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ u64 sm_lane(u64 v, int l) {
+  return (u64)sm_lane((unsigned)(v >> 32), l) << 32 | sm_lane((unsigned)v, l);
+}
+template <class T>
+__device__ __forceinline__ T sm_running(T v) {
+  v += sm_dpp<0x111>(v);  // row_shr 1, 2, 4, 8: zeros from before the row
+  v += sm_dpp<0x112>(v);
+  v += sm_dpp<0x114>(v);
+  v += sm_dpp<0x118>(v);
+  const T a = sm_lane(v, 15), b = a + sm_lane(v, 31), c = b + sm_lane(v, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row == 0 ? T(0) : row == 1 ? a : row == 2 ? b : c);
+}
+// The sum over 4 (by = 2) or 16 (by = 4) neighbouring lanes, in each of them.
+template <class T>
+__device__ __forceinline__ T sm_sum(T v, int by) {
+  v += sm_dpp<0xB1>(v);  // quad_perm 1,0,3,2
+  v += sm_dpp<0x4E>(v);  // quad_perm 2,3,0,1
+  if (by == 4) {
+    v += sm_dpp<0x124>(v);  // row_ror 4, 8
+    v += sm_dpp<0x128>(v);
+  }
+  return v;
+}
+
 // Running sums over the bins of 256 threads (all of the workgroup call it; sh holds 4 of each).
 __device__ __forceinline__ void sm_scan(unsigned &c, u64 &m, unsigned *sc, u64 *sm) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const unsigned a = __shfl_up(c, s, 64);
-    const u64 b = __shfl_up(m, s, 64);
-    c += lane >= s ? a : 0;
-    m += lane >= s ? b : 0;
-  }
-  if (lane == 63 && wv < 4) {
-    sc[wv] = c;
-    sm[wv] = m;
+  if (wv < 4) {
+    c = sm_running(c);
+    m = sm_running(m);
+    if (lane == 63) {
+      sc[wv] = c;
+      sm[wv] = m;
+    }
   }
   __syncthreads();
 #pragma unroll
@@ -273,13 +316,14 @@ struct SmShared {
   unsigned sub_n[kSmBins];
   u64 sub_m[kSmBins];
   u64 list[kSmList];  // ~key, id of gathered tokens
-  u64 few[kSmPrefix], weight[kSmPrefix];
+  u64 few[kSmFew], weight[kSmFew];
+  unsigned minp_count;  // the row's tokens with w >= min_p, and their weight
+  u64 minp_mass;
   unsigned from[kSmGroup + 1];  // of a group of parts: where each part's gathered tokens begin
   uint16_t off[kSmGroup];       // and the first in the part's order
   unsigned used;
   int pick;
-  uint32_t lo, hi;
-  unsigned wave[16], sc[4];
+  unsigned sc[4];
   u64 sm[4];
   SmPrefix got;
   float f2[2];
@@ -309,12 +353,7 @@ __device__ __forceinline__ void sm_each(SmShared &S, const SmView &V, int b0, in
         first = b0 ? V.end[(int64_t)p * kSmBins + b0 - 1] : 0;
         last = V.end[(int64_t)p * kSmBins + b1];
       }
-      unsigned sum = last - first;
-#pragma unroll
-      for (int s = 1; s < 64; s <<= 1) {
-        const unsigned a = __shfl_up(sum, s, 64);
-        sum += tid >= s ? a : 0;
-      }
+      const unsigned sum = sm_running(last - first);
       S.off[tid] = (uint16_t)first;
       S.from[tid + 1] = sum;
       if (tid == 0) S.from[0] = 0;
@@ -334,105 +373,88 @@ __device__ __forceinline__ void sm_each(SmShared &S, const SmView &V, int b0, in
   }
 }
 
-// Few tokens (at most 64) of S.few in a wave's lanes: each one's place among them and the weight up to it.
+// The answer among few tokens (at most 256, in S.few, after c0 tokens of weight m0): 16 or 4 threads a token count those up
+// to it and add their weights.
 __device__ __forceinline__ void sm_few(SmShared &S, SmAsk a, u64 target, unsigned in, unsigned c0, u64 m0,
                                        const SmRow &r) {
-  const int tid = threadIdx.x;
-  if (tid < 64) {
-    const bool on = tid < (int)in;
-    const u64 me = on ? S.few[tid] : ~(u64)0;
-    const u64 w = on ? r.mass(sm_value(~(uint32_t)(me >> 32)), SmSeries()) : 0;
-    unsigned place = 1;
-    u64 sum = w;
-    for (int i = 0; i < (int)in; i++) {
-      const u64 o = S.few[i];
-      const u64 ow = __shfl(w, i, 64);
-      place += o < me ? 1u : 0u;
-      sum += o < me ? ow : 0;
+  const int tid = threadIdx.x, by = in <= 64 ? 4 : 2;  // log2 of them
+  if (tid < (int)in) S.weight[tid] = r.mass(sm_value(~(uint32_t)(S.few[tid] >> 32)), SmSeries());
+  __syncthreads();
+  const unsigned i = tid >> by, k0 = tid & ((1 << by) - 1);
+  if (i < in) {
+    const u64 me = S.few[i];
+    unsigned place = 0;
+    u64 sum = 0;
+#pragma unroll 4
+    for (unsigned k = k0; k < in; k += 1 << by) {
+      const bool up = S.few[k] <= me;
+      place += up ? 1u : 0u;
+      sum += up ? S.weight[k] : 0;
     }
-    const bool y = on && sm_yes(a, target, c0 + place, m0 + sum);
-    if (y && !sm_yes(a, target, c0 + place - 1, m0 + sum - w)) S.got = SmPrefix{c0 + place, m0 + sum, (int)(uint32_t)me};
+    place = sm_sum(place, by);
+    sum = sm_sum(sum, by);
+    if (k0 == 0 && sm_yes(a, target, c0 + place, m0 + sum) && !sm_yes(a, target, c0 + place - 1, m0 + sum - S.weight[i]))
+      S.got = SmPrefix{c0 + place, m0 + sum, (int)(uint32_t)me};
   }
   __syncthreads();
 }
 
 // The prefix that answers (a, target): every thread of the workgroup calls it and gets the answer.
-__device__ SmPrefix sm_answer(SmShared &S, SmAsk a, u64 target, const SmView &V, const SmRow &r, bool token) {
+__device__ __forceinline__ SmPrefix sm_answer(SmShared &S, SmAsk a, u64 target, const SmView &V, const SmRow &r) {
   const int tid = threadIdx.x, nt = blockDim.x;
   __syncthreads();
   if (tid < kSmBins) {
     const bool y = sm_yes(a, target, S.cn[tid], S.ms[tid]);
     if (y && (tid == 0 || !sm_yes(a, target, S.cn[tid - 1], S.ms[tid - 1]))) S.pick = tid;
   }
-  if (tid == 0) {
-    S.lo = 0xffffffffu;
-    S.hi = 0;
-    S.used = 0;
-  }
+  if (tid == 0) S.used = 0;
   __syncthreads();
   const int bin = S.pick;
   unsigned c0 = bin ? S.cn[bin - 1] : 0, in = S.cn[bin] - c0;
   u64 m0 = bin ? S.ms[bin - 1] : 0;
   // a whole bin's prefix needs no token of it
-  if (a == SM_COUNT && !token && c0 + in == target) return SmPrefix{c0 + in, S.ms[bin], 0};
-  if (in <= kSmFew) {
-    sm_each(S, V, bin, bin, [&](uint32_t key, uint32_t id) { S.few[atomicAdd(&S.used, 1u)] = (u64)~key << 32 | id; });
-    sm_few(S, a, target, in, c0, m0, r);
-    return S.got;
-  }
-  const bool listed = in <= kSmList;
-  {
-    uint32_t lo = 0xffffffffu, hi = 0;
-    sm_each(S, V, bin, bin, [&](uint32_t key, uint32_t id) {
-      if (listed) S.list[atomicAdd(&S.used, 1u)] = (u64)~key << 32 | id;
-      lo = min(lo, key);
-      hi = max(hi, key);
-    });
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) {
-      lo = min(lo, (uint32_t)__shfl_xor((int)lo, s, 64));
-      hi = max(hi, (uint32_t)__shfl_xor((int)hi, s, 64));
-    }
-    if ((tid & 63) == 0) {
-      atomicMin(&S.lo, lo);
-      atomicMax(&S.hi, hi);
-    }
-  }
-  __syncthreads();
-  uint32_t lo = S.lo, hi = S.hi;
-  const unsigned have = in;
-  // every token of the bin whose key lies in [lo, hi]
-  auto inside = [&](auto f) {
-    if (listed) {
-      for (unsigned i = tid; i < have; i += nt) {
-        const uint32_t key = ~(uint32_t)(S.list[i] >> 32);
-        if (key >= lo && key <= hi) f(key, (uint32_t)S.list[i]);
-      }
-    } else {
+  if (a == SM_COUNT && c0 + in == target) return SmPrefix{c0 + in, S.ms[bin], 0};
+  // narrowed down to few by the keys, 256 steps at a time, and equal logits by their ids
+  uint32_t lo, hi, id0 = 0, id1 = 0xffffffffu;
+  r.keys(bin, lo, hi);
+  const uint32_t floor = sm_key(S.f2[1]);  // the least finite logit
+  bool listed = false;
+  unsigned have = 0;
+  auto inside = [&](uint32_t key, uint32_t id) { return key >= lo && key <= hi && id >= id0 && id <= id1; };
+  for (;;) {
+    if (!listed && in <= kSmList) {
       sm_each(S, V, bin, bin, [&](uint32_t key, uint32_t id) {
-        if (key >= lo && key <= hi) f(key, id);
+        if (inside(key, id)) S.list[atomicAdd(&S.used, 1u)] = (u64)~key << 32 | id;
       });
+      listed = true;
+      have = in;
     }
-  };
-  while (in > kSmFew && lo < hi) {
-    __syncthreads();
+    if (in <= kSmFew) break;
+    const bool keys = lo < hi;
+    if (!keys && id1 >= V.n) id1 = (uint32_t)V.n - 1;
+    // -inf, which would spread the steps, is the last step's
+    const uint32_t range = keys ? hi - (floor > lo && floor <= hi ? floor : lo) : id1 - id0;
+    const int wide = range >> 8 ? 24 - __clz((int)range) : 0;  // log2 of a step
     if (tid < kSmBins) {
       S.sub_n[tid] = 0;
       S.sub_m[tid] = 0;
     }
     __syncthreads();
-    const uint32_t width = (hi - lo) / kSmBins + 1;
-    inside([&](uint32_t key, uint32_t) {
-      const uint32_t b = (hi - key) / width;
+    auto count = [&](uint32_t key, uint32_t id) {
+      if (!inside(key, id)) return;
+      const uint32_t b = min((keys ? hi - key : id - id0) >> wide, (uint32_t)kSmBins - 1);
       atomicAdd(&S.sub_n[b], 1u);
       atomicAdd(&S.sub_m[b], r.mass(sm_value(key), SmSeries()));
-    });
+    };
+    if (listed)
+      for (unsigned i = tid; i < have; i += nt) count(~(uint32_t)(S.list[i] >> 32), (uint32_t)S.list[i]);
+    else
+      sm_each(S, V, bin, bin, count);
     __syncthreads();
     unsigned c = tid < kSmBins ? S.sub_n[tid] : 0;
     u64 m = tid < kSmBins ? S.sub_m[tid] : 0;
     sm_scan(c, m, S.sc, S.sm);
-    __syncthreads();
-    if (tid < kSmBins) {
+    if (tid < kSmBins) {  // each thread its own; the ones before it below
       S.sub_n[tid] = c;
       S.sub_m[tid] = m;
     }
@@ -442,54 +464,30 @@ __device__ SmPrefix sm_answer(SmShared &S, SmAsk a, u64 target, const SmView &V,
       if (y && (tid == 0 || !sm_yes(a, target, c0 + S.sub_n[tid - 1], m0 + S.sub_m[tid - 1]))) S.pick = tid;
     }
     __syncthreads();
-    const int b = S.pick;
+    const uint32_t b = (uint32_t)S.pick, step = (uint32_t)1 << wide;
     const unsigned cb = b ? S.sub_n[b - 1] : 0;
     in = S.sub_n[b] - cb;
     c0 += cb;
     m0 += b ? S.sub_m[b - 1] : 0;
-    hi -= (uint32_t)b * width;
-    lo = hi - lo >= width ? hi - width + 1 : lo;
-  }
-  __syncthreads();
-  if (in <= kSmFew) {
-    if (tid == 0) S.used = 0;
-    __syncthreads();
-    inside([&](uint32_t key, uint32_t id) { S.few[atomicAdd(&S.used, 1u)] = (u64)~key << 32 | id; });
-    __syncthreads();
-    sm_few(S, a, target, in, c0, m0, r);
-    return S.got;
-  }
-  // equal logits: the prefix takes the first `need` of them by id
-  const u64 w = r.mass(sm_value(lo), SmSeries());
-  const u64 need64 = a == SM_COUNT ? target - c0
-                     : w == 0      ? 1
-                     : a == SM_MASS ? (target - m0 + w - 1) / w
-                                    : (target - m0) / w + 1;
-  const unsigned need = need64 < 1 ? 1 : need64 > in ? in : (unsigned)need64;
-  SmPrefix g{c0 + need, m0 + need * w, 0};
-  if (token) {
-    unsigned before = 0;
-    for (int64_t i0 = 0; i0 < V.n && before < need; i0 += nt) {
-      const int64_t i = i0 + tid;
-      const float v = i < V.n ? V.l[i] : 0.f;
-      const bool y = i < V.n && v == v && sm_key(v) == lo;
-      const u64 vote = __ballot(y);
-      if ((tid & 63) == 0) S.wave[tid >> 6] = (unsigned)__popcll(vote);
-      __syncthreads();
-      unsigned at = before, all = 0;
-      for (int k = 0; k < nt / 64; k++) {
-        if (k < (tid >> 6)) at += S.wave[k];
-        all += S.wave[k];
-      }
-      at += (unsigned)__popcll(vote & ((1ull << (tid & 63)) - 1));
-      if (y && at + 1 == need) S.got.token = (int)i;
-      before += all;
-      __syncthreads();
+    const bool end = b == kSmBins - 1;
+    if (keys) {
+      hi -= b << wide;
+      lo = !end && hi - lo >= step ? hi - step + 1 : lo;
+    } else {
+      id0 += b << wide;
+      id1 = !end && id1 - id0 >= step ? id0 + step - 1 : id1;
     }
     __syncthreads();
-    g.token = S.got.token;
   }
-  return g;
+  if (tid == 0) S.used = 0;
+  __syncthreads();
+  for (unsigned i = tid; i < have; i += nt) {
+    const u64 t = S.list[i];
+    if (inside(~(uint32_t)(t >> 32), (uint32_t)t)) S.few[atomicAdd(&S.used, 1u)] = t;
+  }
+  __syncthreads();
+  sm_few(S, a, target, in, c0, m0, r);
+  return S.got;
 }
 
 // The weight that top_p of `mass` asks for, and the one that u of it passes.
@@ -533,13 +531,23 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
     c += V.end[(int64_t)p * kSmBins + b];
     m += masses[(int64_t)p * kSmBins + b];
   }
-  unsigned mpc = 0;
-  u64 mpm = 0;
-  if (set.min_p > 0.f)
-    for (int p = 0; p < parts; p++) {
-      mpc += rec[p].minp_count;
-      mpm += rec[p].minp_mass;
+  if (set.min_p > 0.f && tid >= 64 && tid < 128) {  // beside the first wave's reading of the range
+    unsigned n_ = 0;
+    u64 m_ = 0;
+    for (int p = tid - 64; p < parts; p += 64) {
+      n_ += rec[p].minp_count;
+      m_ += rec[p].minp_mass;
     }
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) {
+      n_ += __shfl_xor(n_, x, 64);
+      m_ += __shfl_xor(m_, x, 64);
+    }
+    if (tid == 64) {
+      S.minp_count = n_;
+      S.minp_mass = m_;
+    }
+  }
   SmRow r;
   sm_row_of(rec, parts, set.temperature, shift, r, S.f2);
   if (r.m == -INFINITY || (greedy && l0 != l0)) {  // as the greedy pick
@@ -566,13 +574,20 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
     __syncthreads();
     const int bin = S.pick;
     const unsigned in = S.cn[bin];
-    if (in <= kSmPrefix) {
-      sm_each(S, V, 0, bin, [&](uint32_t key, uint32_t id) { S.list[atomicAdd(&S.used, 1u)] = (u64)~key << 32 | id; });
-      if (tid < (int)in) {  // to its place, by counting those before it
-        const u64 me = S.list[tid];
+    if (in <= kSmFew) {
+      // each bin's tokens together, then each token to its place among its bin's, four threads a token
+      if (tid <= bin) S.sub_n[tid] = tid ? S.cn[tid - 1] : 0;
+      sm_each(S, V, 0, bin, [&](uint32_t key, uint32_t id) {
+        S.list[atomicAdd(&S.sub_n[r.bin(sm_value(key))], 1u)] = (u64)~key << 32 | id;
+      });
+      if (tid >> 2 < (int)in) {
+        const u64 me = S.list[tid >> 2];
+        const int b = r.bin(sm_value(~(uint32_t)(me >> 32)));
+        const unsigned from = b ? S.cn[b - 1] : 0, to = S.cn[b];
         unsigned place = 0;
-        for (unsigned i = 0; i < in; i++) place += S.list[i] < me ? 1u : 0u;
-        S.few[place] = me;
+        for (unsigned i = from + (tid & 3); i < to; i += 4) place += S.list[i] < me ? 1u : 0u;
+        place = sm_sum(place, 2);
+        if ((tid & 3) == 0) S.few[from + place] = me;
       }
       __syncthreads();
       unsigned c = 0;
@@ -587,25 +602,34 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
         __syncthreads();
         count = (unsigned)S.pick;
       }
-      if (set.min_p > 0.f && mpc < count) count = mpc;
+      if (set.min_p > 0.f && S.minp_count < count) count = S.minp_count;
       const u64 x = sm_draw(u, S.weight[count - 1]);
       if (tid < (int)count && S.weight[tid] > x && (tid == 0 || S.weight[tid - 1] <= x))
         out[row] = (int)(uint32_t)S.few[tid];
       return;
     }
-    kept = sm_answer(S, SM_COUNT, (u64)set.top_k, V, r, false);
   }
-  u64 x = 0;
-  if (!greedy) {
-    if (set.top_p < 1.f) {
-      const SmPrefix p = sm_answer(S, SM_MASS, sm_top_p(set.top_p, kept.mass), V, r, false);
-      if (p.count < kept.count) kept = p;
+  // the questions in turn, in one copy of the code (a launch runs it once or twice: most of its time is the fetching)
+#pragma unroll 1
+  for (int q = 0; q < 3; q++) {
+    SmAsk a = SM_OVER;
+    u64 x = 0;
+    if (q == 0) {
+      if (!top_k) continue;
+      a = SM_COUNT;
+      x = (u64)set.top_k;
+    } else if (q == 1) {
+      if (greedy || !(set.top_p < 1.f)) continue;
+      a = SM_MASS;
+      x = sm_top_p(set.top_p, kept.mass);
+    } else if (!greedy) {
+      if (set.min_p > 0.f && S.minp_count < kept.count) kept = SmPrefix{S.minp_count, S.minp_mass, 0};
+      x = sm_draw(u, kept.mass);
     }
-    if (set.min_p > 0.f && mpc < kept.count) kept = SmPrefix{mpc, mpm, 0};
-    x = sm_draw(u, kept.mass);
+    const SmPrefix p = sm_answer(S, a, x, V, r);
+    if (q == 2 && tid == 0) out[row] = p.token;
+    if (p.count < kept.count) kept = p;
   }
-  const SmPrefix d = sm_answer(S, SM_OVER, x, V, r, true);
-  if (tid == 0) out[row] = d.token;
 }
 
 static int sample_parts(int64_t n) { return (int)((n + kSmPart - 1) / kSmPart); }
