@@ -201,6 +201,47 @@ def test_kv4_attention_long_row(ctx, window, sinks):
     kv4_case(ctx, np.random.default_rng(9), 1, 2200, 16, 8, 64, window, sinks)
 
 
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("slots", [1, 3])
+def test_offsets_past_32_bits(ctx, slots, T):
+    """Caches of 4.6 GB each, whose last slot's window and first positions are compared with a short cache's."""
+    H, KH, HD, n, last = 16, 8, 128, 8 * 10**6 // slots, 60
+    rng = np.random.default_rng(T)
+    c = Cache(ctx, n, KH, HD, slots)
+    k, v = rows(rng, 3 + last, KH, HD), rows(rng, 3 + last, KH, HD)
+    q = rng.standard_normal((T, H, HD), dtype=F32)
+    c.store(k[:3], v[:3], 0, slots - 1)
+    c.store(k[3:], v[3:], n - last, slots - 1)
+    gk, gv = c.read(n - last, last, slots - 1)
+    assert np.array_equal(gk, held_ref(k[3:])) and np.array_equal(gv, held_ref(v[3:]))
+    got = c.attention(q, n - T, 30, 3, slot=slots - 1)
+    want, tol = attention_span_ref(q, held_ref(k), held_ref(v), 3 + last - T + np.arange(T), 30, 3, 1 / math.sqrt(HD))
+    assert (np.abs(got - want) <= tol).all()
+    if T == 1:
+        dq, out, pos, slot = dev(q), torch.empty((1, H, HD), device=DEV), np.array([n - 1], np.int32), np.array([slots - 1], np.int32)
+        check(load().wl_kv4_attention_batch_dev(ctx.handle, P(dq), 1, H, KH, HD, P(c.K), P(c.V), pos.ctypes.data,
+                                                slot.ctypes.data, slots, n, 30, 3, 1 / math.sqrt(HD), P(out)))
+        assert np.array_equal(bits(host(ctx, out)), bits(got))
+
+
+@pytest.mark.parametrize("T", [1, 20])
+def test_fp16_offsets_past_32_bits(ctx, T):
+    H, KH, HD, n, last = 16, 8, 128, 22 * 10**5, 60  # 4.5 GB each
+    rng = np.random.default_rng(T)
+    k, v = to_half_ref(rows(rng, 3 + last, KH, HD)), to_half_ref(rows(rng, 3 + last, KH, HD))
+    K, V = [torch.full((n, KH * HD), 0x7e00, dtype=torch.int16, device=DEV) for _ in range(2)]
+    for t, x in ((K, k), (V, v)):
+        x = torch.from_numpy(x.view(np.int16).reshape(3 + last, -1)).to(DEV)
+        t[:3], t[n - last:] = x[:3], x[3:]
+    q = rng.standard_normal((T, H, HD), dtype=F32)
+    dq, out = dev(q), torch.empty((T, H, HD), device=DEV)
+    check(load().wl_attention_window_dev(ctx.handle, P(dq), T, H, KH, HD, P(K), P(V), n - T, 30, 3, 1 / math.sqrt(HD),
+                                         P(out)))
+    want, tol = attention_span_ref(q, k.view(np.float16), v.view(np.float16), 3 + last - T + np.arange(T), 30, 3,
+                                   1 / math.sqrt(HD))
+    assert (np.abs(host(ctx, out) - want) <= tol).all()
+
+
 def fp16_case(ctx, rng, T, pos0, H, KH, HD, window, sinks):
     n = pos0 + T
     k, v = to_half_ref(rows(rng, n, KH, HD)), to_half_ref(rows(rng, n, KH, HD))

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from long_ref import sample_ref
-from windlass_amd._lib import check, load
+from windlass_amd._lib import ShapeError, check, load
 from windlass_amd.backend import Context, SampleParams
 
 pytestmark = pytest.mark.gpu
@@ -71,6 +71,13 @@ SETS = [dict(), dict(temperature=0.0), dict(temperature=0.7, top_k=40, top_p=0.9
 def test_every_setting(ctx, n):
     rng = np.random.default_rng(n)
     compare(ctx, peaked(rng, len(SETS), n), rng, SETS)
+
+
+def test_the_longest_rows(ctx):
+    rng = np.random.default_rng(24)
+    compare(ctx, peaked(rng, 2, 1 << 24), rng, [dict(temperature=0.7, top_k=300, top_p=0.95), dict(min_p=0.2)])
+    with pytest.raises(ShapeError):
+        sample(ctx, np.zeros((1, (1 << 24) + 1), F32), [0.5], [dict()])
 
 
 @pytest.mark.parametrize("rows", [1, 2, 64, 65, 131])
