@@ -571,7 +571,7 @@ static int span_per(int n, int units) {
 // 214 us: 960 TFLOP/s, where a library's product of 4,096 x 4,096 matrices reaches 1,100. The matrix cores are busy 38%
 // of the cycles and the VALU 48%, with two waves a SIMD that seldom overlap them; 254 registers leave no room for a second
 // tile of scores, and kernels that kept one (the scores of 32 keys beside the exponentials of the 32 before) spilled and
-// took 297-308 us. Rows cut in two and more chunks where whole rows fill the CUs: 282 us; 2 and 4 chunks for a window of
+// took 297-308 us; the next step's unpacking among a chain's products, 225-245 us, for the same reason. Rows cut in two and more chunks where whole rows fill the CUs: 282 us; 2 and 4 chunks for a window of
 // 1,500 rows, whose 376 workgroups are one and two a CU: 114 and 131 us against 102.
 constexpr int kTlK = 64, kTlW = 4, kTlCols = 32 * kTlW;
 typedef float sf16 __attribute__((ext_vector_type(16)));
@@ -955,13 +955,15 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
             split_pair(P0, P1, ph[e], pl[e]);
           }
           const fh8 vh = as_fh8(ph[0], ph[1], ph[2], ph[3]), vl = as_fh8(pl[0], pl[1], pl[2], pl[3]);
+          fh8 a[ND];  // an output's two parts apart from each other: 214 -> 213 us, the window 97.4 -> 96.0
 #pragma unroll
           for (int d = 0; d < ND; d++) {
             // val_at(32 d + col, 32 s + 16 k + 8 hf)
-            const fh8 a = *reinterpret_cast<const fh8 *>(vb + 32 * d * kTlK + (va ^ ((4 * d ^ 4 * s ^ 2 * k) & 7) << 3));
-            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, vh, O[d], 0, 0, 0);
-            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, vl, O[d], 0, 0, 0);
+            a[d] = *reinterpret_cast<const fh8 *>(vb + 32 * d * kTlK + (va ^ ((4 * d ^ 4 * s ^ 2 * k) & 7) << 3));
+            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[d], vh, O[d], 0, 0, 0);
           }
+#pragma unroll
+          for (int d = 0; d < ND; d++) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[d], vl, O[d], 0, 0, 0);
         }
       }
       if constexpr (Stage::kPrio) __builtin_amdgcn_s_setprio(0);
