@@ -604,6 +604,9 @@ struct TilesArgs {
 __device__ __forceinline__ int val_at(int dim, int slot) {
   return dim * kTlK + ((((slot >> 3) ^ dim ^ (dim >> 3)) & 7) << 3 | (slot & 7));
 }
+// Bits 15 and 31 set where a half of w is an infinity or NaN: its exponent's ones carry.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; }
+constexpr uint32_t kNotFinite = 0x80008000u;
 // Keeps a value from being computed ahead of a loop into a register of its own.
 __device__ __forceinline__ int here(int v) {
   asm volatile("" : "+v"(v));
@@ -667,19 +670,18 @@ struct StageKv4 {
     if (doV) {
       const int kq = vl >> 4, dim = 4 * E * (vl & 15) + 4 * ve, p0 = j0 + 32 * vt + 4 * kq;
       u32x4_t sc = vs;
-      if (p0 + 19 > last) {
+      const uint32_t odd = not_finite(sc.x) | not_finite(sc.y) | not_finite(sc.z) | not_finite(sc.w);
+      if (j0 + kTlK - 1 > last || __any(odd & kNotFinite)) {  // uniform over the wave, and rare
+        asm volatile("");
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 4; j++) {  // a scale is finite or NaN; past `last` it may be anything
           const int at = p0 + 16 * (j >> 1) + 2 * (j & 1);
           sc[j] &= (at > last ? 0u : 0xffffu) | (at + 1 > last ? 0u : 0xffff0000u);
+          const bool lo = (sc[j] & 0x7c00u) == 0x7c00u, hi = (sc[j] & 0x7c000000u) == 0x7c000000u;
+          bad |= lo | hi;
+          sc[j] = lo ? sc[j] & 0xffff0000u : sc[j];
+          sc[j] = hi ? sc[j] & 0xffffu : sc[j];
         }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {  // a scale is finite or NaN
-        const bool lo = (sc[j] & 0x7c00u) == 0x7c00u, hi = (sc[j] & 0x7c000000u) == 0x7c000000u;
-        bad |= lo | hi;
-        sc[j] = lo ? sc[j] & 0xffff0000u : sc[j];
-        sc[j] = hi ? sc[j] & 0xffffu : sc[j];
       }
       // val_at(dim + i, slot + 16 h): dim is a multiple of 4
       const int base = here(val_at(dim, 32 * vt + 8 * (kq & 1) + 4 * (kq >> 1)));
@@ -748,24 +750,25 @@ struct StageF16 {
       }
     }
   }
-  __device__ static __forceinline__ bool nonfinite(u32x4_t w) {
-    bool b = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) b |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
-    return b;
+  __device__ static __forceinline__ uint32_t odd(u32x4_t w) {
+    return not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
   }
   __device__ __forceinline__ bool stage(uint16_t *lk, uint16_t *lv, int, int, uint32_t, bool &badk) {
     constexpr int KS = HD + 8;
     bool bad = false;
+    uint32_t oddk = 0;
 #pragma unroll
     for (int i = 0; i < KI; i++) {
       const int e = tid + 256 * i;
-      badk |= nonfinite(k[i]);
+      oddk |= odd(k[i]);
       *reinterpret_cast<u32x4_t *>(lk + (e / U) * KS + 8 * (e % U)) = k[i];
     }
+    badk = (oddk & kNotFinite) != 0;
     if (kg < 16) {
+      uint32_t oddv = 0;
 #pragma unroll
-      for (int b = 0; b < 4; b++) bad |= nonfinite(v[b]);
+      for (int b = 0; b < 4; b++) oddv |= odd(v[b]);
+      bad = (oddv & kNotFinite) != 0;
       if (bad) {
 #pragma unroll
         for (int b = 0; b < 4; b++)
