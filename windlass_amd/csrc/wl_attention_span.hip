@@ -568,8 +568,8 @@ static int span_per(int n, int units) {
 // running maximum, times the scale, as above: scores of any size keep their largest near 1.
 //
 // What bounds it: both products twice (two parts), 206 GFLOP for 2,048 tokens of the 8B model's 32 heads after 2,048, in
-// 214 us: 960 TFLOP/s, where a library's product of 4,096 x 4,096 matrices reaches 1,100. The matrix cores are busy 38%
-// of the cycles and the VALU 48%, with two waves a SIMD that seldom overlap them; 254 registers leave no room for a second
+// 205-214 us on the cards measured: 960 to 1,005 TFLOP/s, where a library's product of 4,096 x 4,096 matrices reaches 1,100. The matrix cores are busy 40%
+// of the cycles and the VALU 50%, with two waves a SIMD that seldom overlap them; 254 registers leave no room for a second
 // tile of scores, and kernels that kept one (the scores of 32 keys beside the exponentials of the 32 before) spilled and
 // took 297-308 us; the next step's unpacking among a chain's products, 225-245 us, for the same reason. Rows cut in two and more chunks where whole rows fill the CUs: 282 us; 2 and 4 chunks for a window of
 // 1,500 rows, whose 376 workgroups are one and two a CU: 114 and 131 us against 102.
@@ -721,8 +721,8 @@ template <int HD>
 struct StageF16 {
   static constexpr int U = HD / 8, KI = 64 * U / 256;
   static constexpr bool kInf = true;
-  // exponentials and the products after them before the other wave's work: a window of 1,500 rows 102 -> 97 us (with 4-bit
-  // tiles, whose staging is the VALU's, 214 -> 221)
+  // exponentials and the products after them before the other wave's work: a window of 1,500 rows 93.5 -> 88.8 us (with 4-bit
+  // tiles, whose staging is the VALU's, 205 -> 211)
   static constexpr bool kPrio = true;
   u32x4_t k[KI], v[4];
   const uint16_t *K, *V;
