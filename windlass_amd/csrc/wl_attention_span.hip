@@ -268,6 +268,12 @@ __device__ __forceinline__ float join_parts(float v, bool low) {
   return v + o;
 }
 
+// What sums under the maximum M weigh under a larger one. Scores of -inf alone leave M at -inf and sums of zeros (or NaN, from
+// a NaN score): a factor of zero, also where no other sums have a maximum, and 0 / 0 is such a row's output.
+__device__ __forceinline__ float weight_of(float M, float m, float c2) {
+  return M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - m) * c2);
+}
+
 typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));  // at any float's address
 
 // A row's outputs lie in LDS and in the runs' records as the matrix cores leave them: values 16 d + 4 kq + e, for
@@ -466,7 +472,7 @@ __global__ __launch_bounds__(64 * kSpWaves, Tile::kOcc) void span_decode_kernel(
     double l = 0.0;
 #pragma unroll
     for (int w = 0; w < W; w++) {
-      const float f = __builtin_amdgcn_exp2f((sm[w][gg] - m) * sc2[gg]);
+      const float f = weight_of(sm[w][gg], m, sc2[gg]);
       o += so[w][gg][four] * f;
       l += sl[w][gg] * (double)f;
     }
@@ -511,7 +517,7 @@ __global__ __launch_bounds__(256) void span_join_kernel(const float *__restrict_
   if ((tid & 63) == 0) sm[tid >> 6] = m;
   __syncthreads();
   m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  const float f1 = tid < n ? __builtin_amdgcn_exp2f((m1 - m) * c2) : 0.f;
+  const float f1 = tid < n ? weight_of(m1, m, c2) : 0.f;
   f[tid] = f1;
   const double l = wave_sum_d(tid < n ? l1 * (double)f1 : 0.0);
   if ((tid & 63) == 0) sl[tid >> 6] = l;
