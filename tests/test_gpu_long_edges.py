@@ -1,13 +1,14 @@
 """Edges of attention over 4-bit caches and windows. Bounds are long_ref's, or stand at the test."""
 import ctypes
+import math
 
 import numpy as np
 import pytest
 import torch
 
 from layer_ref import to_half_ref
-from long_ref import attention_span_ref
-from test_gpu_kv4 import P, bits, dev, host, rows
+from long_ref import attention_span_ref, held_ref
+from test_gpu_kv4 import Cache, P, bits, dev, host, rows
 from test_gpu_long_models import E, H, KH, Layer, caches, same
 from windlass_amd._lib import check, load
 from windlass_amd.backend import Context, KvOpts
@@ -98,3 +99,49 @@ def test_layer_rows_with_keys_at_minus_infinity(ctx, N):
                                            cap, P(kk), P(vv), ctypes.byref(o)))
     assert np.isfinite(host(ctx, x)).all() and same(ctx, x, y)
     l.free()
+
+
+# a scale of zero, and queries so small that the scores' unit is the smallest there is
+@pytest.mark.parametrize("scale,qsize", [(0.0, 1.0), (0.1, 1e-35), (-0.1, 1e-37), (0.1, 1e-42)])
+@pytest.mark.parametrize("kind", [4, 16])
+@pytest.mark.parametrize("T,pos0,H,KH,HD,window,sinks", [(40, 300, 6, 2, 128, 100, 0), (130, 500, 4, 4, 64, 70, 3),
+                                                         (70, 10, 8, 1, 128, 33, 5), (1, 900, 4, 2, 64, 700, 4),
+                                                         (9, 300, 8, 2, 128, 40, 0), (1, 3000, 8, 1, 64, 0, 0)])
+def test_equal_scores(ctx, T, pos0, H, KH, HD, window, sinks, kind, scale, qsize):
+    """Scores that differ by nothing: every visible position weighs the same, wherever a row's first one lies in a step."""
+    rng = np.random.default_rng(T + pos0)
+    n = pos0 + T
+    q = rng.standard_normal((T, H, HD)).astype(F32) * F32(qsize)
+    if kind == 4:
+        k, v = rows(rng, n, KH, HD), rows(rng, n, KH, HD)
+        c = Cache(ctx, n, KH, HD)
+        c.store(k, v, 0)
+        k, v = held_ref(k), held_ref(v)
+        dq, out = dev(q), torch.full(q.shape, 7.0, device=DEV)
+        torch.cuda.synchronize()
+        check(load().wl_kv4_attention_dev(ctx.handle, P(dq), T, H, KH, HD, P(c.K), P(c.V), n, pos0, window, sinks,
+                                          ctypes.c_float(scale), P(out)))
+        got = host(ctx, out)
+    else:
+        k, v = halves(rng, n, KH, HD), halves(rng, n, KH, HD)
+        got = window16(ctx, q, k, v, pos0, window, sinks, scale)
+    want, tol = attention_span_ref(q, k, v, pos0 + np.arange(T), window, sinks, float(F32(scale)))
+    err = np.abs(got - want)
+    assert (err <= tol).all(), "worst %.3g of its bound" % float((err / tol).max())
+
+
+@pytest.mark.parametrize("T", [1, 4])
+def test_small_queries_beside_a_head_without_a_maximum(ctx, T):
+    """Two heads of one KV head, their queries of 1e-35: a first tile of keys at -inf for one of them is at +inf for the other,
+    whose output is NaN; the first weighs the other positions the same."""
+    H, KH, HD, pos0 = 2, 1, 64, 200
+    rng = np.random.default_rng(T)
+    k, v = halves(rng, pos0 + T, KH, HD), halves(rng, pos0 + T, KH, HD)
+    k[:32, 0, 7] = -np.inf
+    q = rng.standard_normal((T, H, HD), dtype=F32)
+    q[:, 0, 7], q[:, 1, 7] = F32(1.0), F32(-1.0)
+    got = window16(ctx, q * F32(1e-35), k, v, pos0, 0, 0, 0.1)
+    assert np.isnan(got[:, 1]).all()
+    want = np.stack([v[32:pos0 + t + 1, 0].astype(np.float64).mean(0) for t in range(T)])
+    u = 2.0 ** -24
+    assert (np.abs(got[:, 0] - want) <= np.abs(v.astype(F32)).max() * (4 * u * math.sqrt(pos0 + T) + 4 * u)).all()

@@ -102,6 +102,9 @@ typedef float sf4 __attribute__((ext_vector_type(4)));
 // A running maximum is raised only by scores more than 2^6 past it, so nearly never after a wave's first tile: the
 // exponentials reach 2^6, and 2^8 of them are fp16 parts (22 bits down to 2^-22 of the row's largest, 2^-33 of it below).
 constexpr float kSpUp = 0x1p8f, kSpPast = 6.f;
+// In the scores' units: finite where those are the smallest there are, so that a lane without a key yet keeps -inf as what
+// raises its maximum.
+__device__ __forceinline__ float past_of(float c2) { return fminf(kSpPast / c2, 3.4028235e38f); }
 constexpr int kSpWaves = 4;
 constexpr int kSpRuns = 256;      // runs of a row at most
 
@@ -371,7 +374,7 @@ __global__ __launch_bounds__(64 * kSpWaves, Tile::kOcc) void span_decode_kernel(
 #pragma unroll
   for (int d = 0; d < ND; d++) O[d] = sf4{0.f, 0.f, 0.f, 0.f};
   float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
-  const float past = kSpPast / c2;
+  const float past = past_of(c2);
   double L = 0.0;
   auto step = [&](Tile &A, int64_t tile) __attribute__((always_inline)) {
     const int p0 = (int)tile * kKv4Tile;
@@ -876,7 +879,7 @@ __global__ __launch_bounds__(256, 2) void span_tiles_kernel(const float *__restr
 #pragma unroll
     for (int i = 0; i < 16; i++) O[d][i] = 0.f;
   float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
-  const float past = kSpPast / c2;
+  const float past = past_of(c2);
   double L = 0.0;
   const uint32_t ones = fp16_ones();
   auto stage = [&](int b, int j0) __attribute__((always_inline)) {
