@@ -232,6 +232,15 @@ static void retire(wl_ctx *c, void *p) {
   c->kept[c->nkept++] = p;
 }
 
+// The least that an outgrown buffer of `bytes` grows to. Half as much again where what is outgrown is kept: so that all of it
+// stays below two of the last (but where memory has run out, and a call takes just what it needs). And where growth repeats as
+// positions go on, each allocation waiting for the stream: there 256 MB more at most.
+static size_t half_more(const wl_ctx *c, size_t bytes, bool repeats) {
+  const size_t most = (size_t)256 << 20;
+  if (c->captured) return bytes + bytes / 2;
+  return repeats ? bytes + (bytes / 2 < most ? bytes / 2 : most) : bytes;
+}
+
 static int ensure(wl_ctx *c, int slot, size_t bytes) {
   if (c->cap[slot] >= bytes) return WL_OK;
   if (c->capturing)
@@ -240,12 +249,8 @@ static int ensure(wl_ctx *c, int slot, size_t bytes) {
   size_t want = bytes < 4096 ? 4096 : bytes;
   const size_t least = want;
   if (c->buf[slot]) {
-    // half as much again where growth repeats as positions go on (each allocation waits for the stream), and where what is
-    // outgrown is kept: so that all of it stays below two of the last
-    if (c->captured || slot == S_ATT) {
-      const size_t more = c->cap[slot] / 2, grown = c->cap[slot] + (more < (size_t)256 << 20 ? more : (size_t)256 << 20);
-      want = want < grown ? grown : want;
-    }
+    const size_t grown = half_more(c, c->cap[slot], slot == S_ATT);
+    want = want < grown ? grown : want;
     hipStreamSynchronize(c->stream);
     retire(c, c->buf[slot]);
     c->buf[slot] = nullptr;
@@ -1398,7 +1403,8 @@ static int rope_angles(wl_ctx *c, const int32_t *hpos, int T, int pos0, int n, d
     if (c->capturing)
       return fail(WL_E_ARG, "a captured call needs RoPE angles of %d positions, the table holds %lld: run the same "
                   "calls once before the capture", top, (long long)R.cap);
-    const int64_t cap = ((int64_t)top + 4095) / 4096 * 4096;
+    const int64_t least = ((int64_t)top + 4095) / 4096 * 4096, grown = (int64_t)half_more(c, (size_t)R.cap, false);
+    int64_t cap = least > grown ? least : grown;
     if (R.dev) {
       hipStreamSynchronize(c->stream);
       retire(c, R.dev);
@@ -1406,8 +1412,15 @@ static int rope_angles(wl_ctx *c, const int32_t *hpos, int T, int pos0, int n, d
       R.cap = 0;
     }
     void *d = nullptr;
-    if (dev_alloc(&d, (size_t)cap * wl::kRopePairs * sizeof(float4)) != hipSuccess)
+    hipError_t e = dev_alloc(&d, (size_t)cap * wl::kRopePairs * sizeof(float4));
+    if (e != hipSuccess && cap > least) {
+      (void)hipGetLastError();
+      e = dev_alloc(&d, (size_t)(cap = least) * wl::kRopePairs * sizeof(float4));
+    }
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
       return fail(WL_E_NOMEM, "cannot allocate the RoPE table of %lld positions", (long long)cap);
+    }
     R.dev = (float4 *)d;
     R.cap = cap;
     R.have.assign((size_t)cap, 0);
