@@ -447,8 +447,8 @@ int wl_layer_batch_kv_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, i
  * shortest prefix with at least top_p of their weight (1: all), of those the ones of weight at least
  * min_p (the largest has 1); d_out[row] is the first at which the weight summed in that order passes d_u[row]
  * times what stayed. temperature 0 is wl_argmax_dev's pick. NaN logits are never drawn; a row without
- * a logit above -inf gives 0. Weights are formed in double, cut to whole numbers of 2^-45 at 128,000 logits (2^-38 at
- * 2^24), and summed exactly: the same token whatever the other rows. */
+ * a logit above -inf gives 0. Weights are formed in double, cut to whole numbers of a unit (2^-46 at 128,000 logits;
+ * past 2^18 of the row's own weight: all that is cut off is below 2^-29 of the weight at 128,000 logits, 2^-25 at 2^24), and summed exactly: the same token whatever the other rows. */
 typedef struct wl_sample_params {
   float temperature; /* >= 0 */
   int32_t top_k;     /* >= 0 */

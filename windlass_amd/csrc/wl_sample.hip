@@ -7,8 +7,12 @@
 // summed in that order passes u of the kept weight. Every step is a question about a prefix of that
 // order, so nothing is sorted but the few tokens around a prefix's end.
 //
-// Arithmetic: weights in double (a polynomial for 2^f), cut to whole numbers of 2^-shift (2^-45 at 128,000
-// tokens), so that sums are exact and do not depend on the order in which workgroups and atomics add them.
+// Arithmetic: weights in double (a polynomial for 2^f), cut to whole numbers of 2^-shift, so that sums are exact and do not
+// depend on the order in which workgroups and atomics add them. Up to 2^18 tokens a unit that leaves the sum of n weights of 1
+// at 2^63 at most: what is cut off is below n 2^(bits of n - 63), 2^-29 of the weight at 128,000 tokens. Longer rows bound their
+// weight first, each part's tokens at the part's largest, at most 4,096 times the weight: n 2^-49 of it is cut off at most,
+// 2^-25 at 2^24 (with the unit of n weights of 1, one logit 20 above 2^24 others of deviation 2 lost them more than half of
+// what they weigh together). Bounding every row took one row of 128,256 from 15.0 to 15.2 us, 64 rows from 46.8 to 47.9.
 //
 // Three launches. (1) Each part of 4,096 tokens of a row: its largest and least finite logit. (2) Each part: the count
 // and weight of its tokens in 256 bins of equal width below the row's maximum (64 t wide at most, weights below e^-64
@@ -76,15 +80,24 @@ struct SmRow {
   float m, R, c;  // the maximum (of infinity: the largest finite value), the bins' reach and scale
   double per;     // log2(e) / t; for t = 0 so large that only the maximum weighs anything
   int shift;
-  __device__ void set(float top, float low, float t, int sh) {
+  __device__ void set(float top, float low, float t) {
     m = cap(top);
-    shift = sh;
     per = t > 0.f ? fmin(1.4426950408889634 / (double)t, 1e300) : 1e300;
     R = fminf(fminf(m - low, 64.f * t), 3.4028235e38f);
     if (!(R > 1e-30f)) R = 0.f;  // the bins' scale stays finite; what lies lower is the last bin's
     c = R > 0.f ? (float)(kSmBins - 2) / R : 0.f;
   }
   __device__ static float cap(float l) { return fminf(l, 3.4028235e38f); }
+  // The weight of a part's largest logit. In 32 bits: off by 2^-16 of it at most, and nothing below 2^-126.
+  __device__ float largest(float part_top) const {
+    return __builtin_amdgcn_exp2f((float)fmax(((double)cap(part_top) - (double)m) * per, -200.0));
+  }
+  // At most 2^63 units: n weights of 1, or kSmPart times the parts' largest weights, which add up to `sum`, and 1% for its rounding.
+  __device__ void unit(int64_t n, bool bounded, float sum) {
+    int e = 32 - __clz((int)n - 1);
+    if (bounded) frexpf(1.01f * sum * (float)kSmPart, &e);
+    shift = e > 11 ? 63 - e : 52;
+  }
   __device__ int bin(float l) const {
     const float d = m - cap(l);
     return d > R ? kSmBins - 1 : min((int)(d * c), kSmBins - 2);
@@ -113,24 +126,41 @@ struct SmRow {
   }
 };
 
-__device__ __forceinline__ void sm_row_of(const SmPart *__restrict__ part, int parts, float t, int shift, SmRow &r,
+// The sum over a wave, the same in every lane.
+__device__ __forceinline__ float wave_sum_f(float v) {
+  v += __builtin_bit_cast(float, dpp32<0xB1>(__builtin_bit_cast(uint32_t, v)));  // as wave_max_f
+  v += __builtin_bit_cast(float, dpp32<0x4E>(__builtin_bit_cast(uint32_t, v)));
+  v += __builtin_bit_cast(float, dpp32<0x124>(__builtin_bit_cast(uint32_t, v)));
+  v += __builtin_bit_cast(float, dpp32<0x128>(__builtin_bit_cast(uint32_t, v)));
+  return (lane_f(v, 0) + lane_f(v, 16)) + (lane_f(v, 32) + lane_f(v, 48));
+}
+
+__device__ __forceinline__ void sm_row_of(const SmPart *__restrict__ part, int parts, int64_t n, float t, SmRow &r,
                                           float *sh) {
-  // every thread of the workgroup; sh holds 2 floats
+  // every thread of the workgroup; sh holds 3 floats
+  const bool bounded = parts > 64;
   if (threadIdx.x < 64) {
-    float top = -INFINITY, low = INFINITY;
+    float top = -INFINITY, low = INFINITY, sum = 0.f;
     for (int i = threadIdx.x; i < parts; i += 64) {
       top = fmaxf(top, part[i].top);
       low = fminf(low, part[i].low);
     }
     top = wave_max_f(top);
     low = -wave_max_f(-low);
+    if (bounded) {
+      r.set(top, low, t);
+      for (int i = threadIdx.x; i < parts; i += 64) sum += r.largest(part[i].top);
+      sum = wave_sum_f(sum);
+    }
     if (threadIdx.x == 0) {
       sh[0] = top;
       sh[1] = low;
+      sh[2] = sum;
     }
   }
   __syncthreads();
-  r.set(sh[0], sh[1], t, shift);
+  r.set(sh[0], sh[1], t);
+  r.unit(n, bounded, sh[2]);
 }
 
 // Running sums over a wave's lanes (all of them active): within rows of 16 by lane shifts, then the rows' sums. A general
@@ -220,12 +250,12 @@ __global__ __launch_bounds__(256) void sample_range_kernel(const float *__restri
 
 template <int WIDE>
 __global__ __launch_bounds__(WIDE) void sample_bins_kernel(const float *__restrict__ logits, int64_t n, SampleSets sets,
-                                                          int shift, SmScratch X) {
+                                                          SmScratch X) {
   constexpr int N = kSmPart / WIDE;
   __shared__ unsigned cn[kSmBins];
   __shared__ u64 ms[kSmBins];
   __shared__ __attribute__((aligned(16))) uint16_t ids[kSmPart];
-  __shared__ float sh[2];
+  __shared__ float sh[3];
   __shared__ unsigned mc, sc[4];
   __shared__ u64 mm, sm[4];
   const int row = blockIdx.y, parts = gridDim.x, tid = threadIdx.x;
@@ -247,9 +277,9 @@ __global__ __launch_bounds__(WIDE) void sample_bins_kernel(const float *__restri
     mm = 0;
   }
   SmRow r;
-  sm_row_of(X.rec + (int64_t)row * parts, parts, set.temperature, shift, r, sh);
+  sm_row_of(X.rec + (int64_t)row * parts, parts, n, set.temperature, r, sh);
   const SmSeries C;
-  const u64 least = (u64)ceil(ldexp((double)set.min_p, shift));
+  const u64 least = (u64)ceil(ldexp((double)set.min_p, r.shift));
   unsigned at[N];  // the token's bin and its place there
   unsigned c = 0;
   u64 m = 0;
@@ -326,7 +356,7 @@ struct SmShared {
   unsigned sc[4];
   u64 sm[4];
   SmPrefix got;
-  float f2[2];
+  float f3[3];
 };
 
 __device__ __forceinline__ bool sm_yes(SmAsk a, u64 target, unsigned c, u64 m) {
@@ -417,7 +447,7 @@ __device__ __forceinline__ SmPrefix sm_answer(SmShared &S, SmAsk a, u64 target, 
   // narrowed down to few by the keys, 256 steps at a time, and equal logits by their ids
   uint32_t lo, hi, id0 = 0, id1 = 0xffffffffu;
   r.keys(bin, lo, hi);
-  const uint32_t floor = sm_key(S.f2[1]);  // the least finite logit
+  const uint32_t floor = sm_key(S.f3[1]);  // the least finite logit
   bool listed = false;
   unsigned have = 0;
   auto inside = [&](uint32_t key, uint32_t id) { return key >= lo && key <= hi && id >= id0 && id <= id1; };
@@ -502,7 +532,7 @@ __device__ __forceinline__ u64 sm_draw(float u, u64 mass) {
 }
 
 __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restrict__ logits, int64_t n, int parts,
-                                                           SampleSets sets, int shift, SmScratch X,
+                                                           SampleSets sets, SmScratch X,
                                                            const float *__restrict__ us, int *__restrict__ out) {
   __shared__ SmShared S;
   const int row = blockIdx.x, tid = threadIdx.x;
@@ -549,7 +579,7 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(const float *__restri
     }
   }
   SmRow r;
-  sm_row_of(rec, parts, set.temperature, shift, r, S.f2);
+  sm_row_of(rec, parts, n, set.temperature, r, S.f3);
   if (r.m == -INFINITY || (greedy && l0 != l0)) {  // as the greedy pick
     if (tid == 0) out[row] = 0;
     return;
@@ -643,9 +673,6 @@ hipError_t sample_launch(const float *logits, int rows, int64_t n, const SampleS
                          void *scratch, hipStream_t st) {
   if (rows <= 0) return hipSuccess;
   const int parts = sample_parts(n);
-  int bits = 1;
-  while ((int64_t)1 << bits < n) bits++;
-  const int shift = bits > 10 ? 62 - bits : 52;  // n weights of at most 1 stay below 2^63
   const int64_t all = (int64_t)rows * parts;
   SmScratch X;  // each array a multiple of 16 bytes from the one before
   X.mass = (u64 *)scratch;
@@ -658,11 +685,11 @@ hipError_t sample_launch(const float *logits, int rows, int64_t n, const SampleS
   // eight tokens a thread while there is at most a part for each CU (one row of 128,256: 6.8 us, 16 a thread 8.4), 16 where
   // CUs take several (64 rows: 25.9 us, eight a thread 29.3)
   if (all <= 256)
-    hipLaunchKernelGGL(sample_bins_kernel<512>, dim3(parts, rows), dim3(512), 0, st, logits, n, sets, shift, X);
+    hipLaunchKernelGGL(sample_bins_kernel<512>, dim3(parts, rows), dim3(512), 0, st, logits, n, sets, X);
   else
-    hipLaunchKernelGGL(sample_bins_kernel<256>, dim3(parts, rows), dim3(256), 0, st, logits, n, sets, shift, X);
+    hipLaunchKernelGGL(sample_bins_kernel<256>, dim3(parts, rows), dim3(256), 0, st, logits, n, sets, X);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL(sample_pick_kernel, dim3(rows), dim3(1024), 0, st, logits, n, parts, sets, shift, X, u, out);
+  hipLaunchKernelGGL(sample_pick_kernel, dim3(rows), dim3(1024), 0, st, logits, n, parts, sets, X, u, out);
   return hipGetLastError();
 }
 
