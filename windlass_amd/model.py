@@ -108,7 +108,7 @@ class DeviceTransformer:
         self._xn = torch.empty((1, cfg.embd), device=self.dev)
         self._x = {}
         self.length = 0
-        torch.cuda.synchronize()  # the context's stream does not wait for torch's
+        torch.cuda.synchronize(self.dev)  # the context's stream does not wait for torch's
 
     def _desc(self, l):
         c, p, v = self.cfg, "blk.%d." % l, self.v
@@ -226,7 +226,7 @@ class DeviceTransformer:
             self.sample_into(self._tok)
         else:
             d_u = self.torch.full((1,), u, device=self.dev)
-            self.torch.cuda.synchronize()  # the context's stream does not wait for torch's
+            self.torch.cuda.synchronize(self.dev)  # the context's stream does not wait for torch's
             self.sample_into(self._tok, params, d_u)
         self.ctx.sync()
         return int(self._tok.item())
@@ -248,7 +248,7 @@ class DeviceTransformer:
         if d_u.numel() != steps:
             raise ShapeError("%d numbers for %d tokens." % (d_u.numel(), steps))
         ids = self.torch.empty(max(steps, 1), dtype=self.torch.int32, device=self.dev)
-        self.torch.cuda.synchronize()
+        self.torch.cuda.synchronize(self.dev)
         chunk = chunk or len(prompt)
         pos = 0
         for i in range(0, len(prompt), chunk):
@@ -392,7 +392,7 @@ class DeviceBatch:
         self.kv_opts = model.kv.opts(slot_positions)
         self.length = [0] * slots
         self._bufs = {}
-        torch.cuda.synchronize()
+        torch.cuda.synchronize(model.dev)
 
     def _buf(self, kind, rows, cols):
         """A device float32 buffer kept for the object's life: the library's queued work may still
@@ -485,7 +485,7 @@ class DeviceBatch:
             raise ShapeError("%d settings and %d numbers for %d sequences of %d tokens."
                              % (len(params), d_u.numel(), N, steps))
         ids = m.torch.empty((max(steps, 1), N), dtype=m.torch.int32, device=m.dev)
-        m.torch.cuda.synchronize()
+        m.torch.cuda.synchronize(m.dev)
         ps = (SampleParams * N)(*params)
         one = [(SampleParams * 1)(p) for p in params]
 
