@@ -49,6 +49,15 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _fits(prompt, steps, pos0, positions):
+    """Refuses an empty prompt, and one that with its reply (the last token is not fed back) passes the positions."""
+    if not prompt:
+        raise ShapeError("No tokens to run.")
+    need = pos0 + prompt + max(steps - 1, 0)
+    if need > positions:
+        raise ShapeError("The prompt and reply need %d positions; the context is %d." % (need, positions))
+
+
 class KvCaches:
     """The kind of a model's KV caches, and the layer calls over them: kv_bits 16 (fp16 rows) or 4 (wl_kv4_bytes: head
     dims 64 and 128), and the positions a row sees (window 0: all; else the last `window` and the first `sinks`)."""
@@ -243,24 +252,28 @@ class DeviceTransformer:
 
     def generate(self, prompt, steps, params, u, chunk=None):
         """The prompt as greedy() runs it, then `steps` tokens drawn with params and the numbers u (steps of them, in [0,
-        1)), each fed to the next step on the device. Returns the tokens."""
+        1)), each fed to the next step on the device. Returns the tokens. A prompt and reply that the context does not hold
+        are refused before anything runs."""
         d_u = self.torch.as_tensor(np.asarray(u, np.float32)).to(self.dev)
         if d_u.numel() != steps:
             raise ShapeError("%d numbers for %d tokens." % (d_u.numel(), steps))
+        _fits(len(prompt), steps, 0, self.max_positions)
         ids = self.torch.empty(max(steps, 1), dtype=self.torch.int32, device=self.dev)
         self.torch.cuda.synchronize(self.dev)
         chunk = chunk or len(prompt)
         pos = 0
-        for i in range(0, len(prompt), chunk):
-            part = list(prompt[i:i + chunk])
-            self.forward(part, pos)
-            pos += len(part)
-        for i in range(steps):
-            if i:
-                self.forward_ids(ids[i - 1:i], pos)
-                pos += 1
-            self.sample_into(ids[i:i + 1], params, d_u[i:i + 1])
-        self.ctx.sync()
+        try:
+            for i in range(0, len(prompt), chunk):
+                part = list(prompt[i:i + chunk])
+                self.forward(part, pos)
+                pos += len(part)
+            for i in range(steps):
+                if i:
+                    self.forward_ids(ids[i - 1:i], pos)
+                    pos += 1
+                self.sample_into(ids[i:i + 1], params, d_u[i:i + 1])
+        finally:
+            self.ctx.sync()  # also after a failure: what is queued uses ids and d_u
         return [int(v) for v in ids[:steps].cpu().tolist()]
 
     def greedy(self, prompt, steps, chunk=None, keep_logits=False):
@@ -478,12 +491,16 @@ class DeviceBatch:
     def generate(self, prompts, steps, params, u):
         """Each prompt in its own slot, then `steps` stacked steps with the tokens drawn on the device: params is one
         SampleParams per sequence, u the numbers [steps][sequences] in [0, 1). Returns the tokens per sequence: what
-        DeviceTransformer.generate gives each of them alone."""
+        DeviceTransformer.generate gives each of them alone. What the slots do not hold is refused before anything runs."""
         m, c, N = self.m, ctypes.c_void_p, len(prompts)
         d_u = m.torch.as_tensor(np.asarray(u, np.float32).reshape(-1)).to(m.dev)
         if len(params) != N or d_u.numel() != steps * N:
             raise ShapeError("%d settings and %d numbers for %d sequences of %d tokens."
                              % (len(params), d_u.numel(), N, steps))
+        if N > self.slots:
+            raise ShapeError("%d sequences for %d slots." % (N, self.slots))
+        for i, p in enumerate(prompts):
+            _fits(len(p), steps, self.length[i], self.cap)
         ids = m.torch.empty((max(steps, 1), N), dtype=m.torch.int32, device=m.dev)
         m.torch.cuda.synchronize(m.dev)
         ps = (SampleParams * N)(*params)
@@ -492,11 +509,13 @@ class DeviceBatch:
         def draw(lg, rows, p, s, i):
             check(m.L.wl_sample_dev(m.ctx.handle, c(lg.data_ptr()), rows, m.vocab, p, c(d_u[s * N + i:].data_ptr()),
                                     c(ids[s, i:].data_ptr())))
-        for i, p in enumerate(prompts):
-            lg = self.prefill(i, list(p))
-            if steps:
-                draw(lg, 1, one[i], 0, i)
-        for s in range(1, steps):
-            draw(self.step(list(range(N)), ids[s - 1]), N, ps, s, 0)
-        m.ctx.sync()
+        try:
+            for i, p in enumerate(prompts):
+                lg = self.prefill(i, list(p))
+                if steps:
+                    draw(lg, 1, one[i], 0, i)
+            for s in range(1, steps):
+                draw(self.step(list(range(N)), ids[s - 1]), N, ps, s, 0)
+        finally:
+            m.ctx.sync()  # also after a failure: what is queued uses ids and d_u
         return ids[:steps].cpu().numpy().T.tolist()
