@@ -77,7 +77,7 @@ def test_large_kept_scratch_stays_small():
 
 
 def test_kept_rope_tables_stay_small():
-    """Angles of 64 pairs, 1 KB a position, to 131,000 positions, 4,096 more at a time."""
+    """Angles of 64 pairs, 1 KB a position, to 131,000 positions, 4,096 more at a time: no recording names their table."""
     cap, step = 1 << 17, 4096
     with Context(0) as own:
         l = Layer(own, 64, 64, 0)

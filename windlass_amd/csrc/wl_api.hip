@@ -232,7 +232,7 @@ static void retire(wl_ctx *c, void *p) {
   c->kept[c->nkept++] = p;
 }
 
-// The least that an outgrown buffer of `bytes` grows to. Half as much again where what is outgrown is kept: so that all of it
+// The least that outgrown scratch of `bytes` grows to. Half as much again where what is outgrown is kept: so that all of it
 // stays below two of the last (but where memory has run out, and a call takes just what it needs). And where growth repeats as
 // positions go on, each allocation waiting for the stream: there 256 MB more at most.
 static size_t half_more(const wl_ctx *c, size_t bytes, bool repeats) {
@@ -1400,27 +1400,16 @@ static int rope_angles(wl_ctx *c, const int32_t *hpos, int T, int pos0, int n, d
     if (p + 1 > top) top = p + 1;
   }
   if (top > R.cap) {
-    if (c->capturing)
-      return fail(WL_E_ARG, "a captured call needs RoPE angles of %d positions, the table holds %lld: run the same "
-                  "calls once before the capture", top, (long long)R.cap);
-    const int64_t least = ((int64_t)top + 4095) / 4096 * 4096, grown = (int64_t)half_more(c, (size_t)R.cap, false);
-    int64_t cap = least > grown ? least : grown;
-    if (R.dev) {
+    const int64_t cap = ((int64_t)top + 4095) / 4096 * 4096;
+    if (R.dev) {  // no recording names it
       hipStreamSynchronize(c->stream);
-      retire(c, R.dev);
+      hipFree(R.dev);
       R.dev = nullptr;
       R.cap = 0;
     }
     void *d = nullptr;
-    hipError_t e = dev_alloc(&d, (size_t)cap * wl::kRopePairs * sizeof(float4));
-    if (e != hipSuccess && cap > least) {
-      (void)hipGetLastError();
-      e = dev_alloc(&d, (size_t)(cap = least) * wl::kRopePairs * sizeof(float4));
-    }
-    if (e != hipSuccess) {
-      (void)hipGetLastError();
+    if (dev_alloc(&d, (size_t)cap * wl::kRopePairs * sizeof(float4)) != hipSuccess)
       return fail(WL_E_NOMEM, "cannot allocate the RoPE table of %lld positions", (long long)cap);
-    }
     R.dev = (float4 *)d;
     R.cap = cap;
     R.have.assign((size_t)cap, 0);
@@ -1594,7 +1583,9 @@ static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, i
   if (kv) {
     if ((rc = layer_attention_kv(c, L, *kv, q, k, v, T, pos0, rd, fs, scale, att))) return rc;
   } else {
-    if (wl::rope_attention_fused(T, rm, HD, KH, rd, d_K, d_V) &&
+    // A recording takes no angles from the table, which calls between its replays may fill for other settings: they are made
+    // in the launches, with the same bits.
+    if (!c->capturing && wl::rope_attention_fused(T, rm, HD, KH, rd, d_K, d_V) &&
         (rc = rope_angles(c, hpos, T, pos0, rd, L->rope_base, fs, L->d_rope_freqs, &tab)))
       return rc;
     WL_HIP(wl::rope_attention_launch(q, k, v, T, H, KH, HD, rd, L->neox, pos0, L->rope_base, fs, L->d_rope_freqs, tab,
