@@ -476,7 +476,8 @@ int wl_matmul_dev_noalloc(wl_ctx *ctx, const wl_weight *w, int32_t expert, const
  * replays it on the context's stream: the same kernels with the same arguments (the same device
  * buffers, the same weights), enqueued by one host call. A call that would grow the context's
  * scratch during a capture fails with WL_E_ARG (run the same calls once before capturing); scratch
- * that later calls outgrow is kept until wl_destroy, since a recording may use it; and
+ * that later calls outgrow is kept until wl_destroy, since a recording may use it; token ids,
+ * positions and slots given in host arrays are recorded by value; and
  * the MoE entries take their launch chain while capturing (the same bits as one launch).
  * Host-buffer entries synchronise and must not be called while capturing. */
 typedef struct wl_graph wl_graph;

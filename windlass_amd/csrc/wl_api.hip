@@ -1330,6 +1330,12 @@ static int stage_rows(wl_ctx *c, const int32_t *a, const int32_t *b, int n, int3
   int rc;
   if ((rc = ensure(c, S_ROWS, (size_t)words * sizeof(int32_t)))) return rc;
   int32_t *rows = (int32_t *)c->buf[S_ROWS];
+  if (c->capturing) {  // recorded by value: by a replay the ring below holds other rows
+    WL_HIP(wl::put_ints_launch(a, n, rows, c->stream), "row copy");
+    if (b) WL_HIP(wl::put_ints_launch(b, n, rows + n, c->stream), "row copy");
+    *d_rows = rows;
+    return WL_OK;
+  }
   if ((size_t)words > c->rows_ints) {  // grow the pinned ring (after every queued copy from it)
     WL_HIP(hipStreamSynchronize(c->stream), "row staging");
     if (c->rows_host) hipHostFree(c->rows_host);

@@ -36,6 +36,8 @@ hipError_t rope_kv_launch(float *q, float *k, const float *v, int T, int H, int 
 hipError_t rope_cache_launch(float *q, float *k, const float *v, int H, int KH, int hd, int n, int neox, double base,
                              double freq_scale, const float *freqs, int bits, uint8_t *K, uint8_t *V, int64_t positions,
                              int64_t slot_bytes, const KvRows &rows, hipStream_t st);
+// n int32 of host memory to device memory as kernel arguments: in a capture their values are recorded.
+hipError_t put_ints_launch(const int32_t *host, int n, int32_t *dev, hipStream_t st);
 hipError_t kv_store_launch(const float *k, const float *v, int64_t n, uint16_t *K, uint16_t *V, hipStream_t st);
 // Floats of scratch attention_launch needs for these operands; max_n: the most positions a row
 // attends to (pos0 + T for one sequence).

@@ -321,6 +321,14 @@ __global__ __launch_bounds__(64) void rope_cache_kernel(RopeRow R, int bits, uin
   kv4_put(w, val, lane, cache + tile * (18 * R.hd), p % kKv4Tile, R.hd);
 }
 
+constexpr int kPutInts = 256;
+struct PutInts {
+  int32_t v[kPutInts];
+};
+__global__ __launch_bounds__(kPutInts) void put_ints_kernel(PutInts a, int n, int32_t *__restrict__ dev) {
+  if ((int)threadIdx.x < n) dev[threadIdx.x] = a.v[threadIdx.x];
+}
+
 // ToHalf (src/Transformer.cs:342-348) of one token's keys and values.
 __global__ void kv_store_kernel(const float *__restrict__ k, const float *__restrict__ v, int64_t n,
                                 uint16_t *__restrict__ K, uint16_t *__restrict__ V) {
@@ -1066,6 +1074,17 @@ hipError_t rope_cache_launch(float *q, float *k, const float *v, int H, int KH, 
   const hipError_t e = rope_rows(R, rows.n, st);
   if (e != hipSuccess) return e;
   return kv4_store_launch(k, v, KH, hd, K, V, positions, slot_bytes, rows, st);
+}
+
+hipError_t put_ints_launch(const int32_t *host, int n, int32_t *dev, hipStream_t st) {
+  for (int i = 0; i < n; i += kPutInts) {
+    PutInts a;
+    const int m = n - i < kPutInts ? n - i : kPutInts;
+    for (int j = 0; j < kPutInts; j++) a.v[j] = j < m ? host[i + j] : 0;
+    hipLaunchKernelGGL(put_ints_kernel, dim3(1), dim3(kPutInts), 0, st, a, m, dev + i);
+    if (const hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t kv_store_launch(const float *k, const float *v, int64_t n, uint16_t *K, uint16_t *V, hipStream_t st) {
