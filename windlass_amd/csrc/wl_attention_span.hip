@@ -43,8 +43,8 @@ __device__ void span_row(const F16Rows &c, const float *qp, int HD, int p, const
   __shared__ float shf[4];
   const int first = s.first(p), lead = s.lead(p), n = s.seen(p);
   float mx = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int64_t j = i < lead ? i : first + (i - lead);
+  for (unsigned i = threadIdx.x; i < (unsigned)n; i += 256) {  // a step past the last position may pass 2^31
+    const int64_t j = i < (unsigned)lead ? i : first + (i - lead);
     float d = 0.f;
     for (int e = 0; e < HD; e++) d += qp[e] * c.key(j, e);
     d *= scale;
@@ -53,7 +53,7 @@ __device__ void span_row(const F16Rows &c, const float *qp, int HD, int p, const
   }
   mx = span_max(mx, shf);
   double sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) {
+  for (unsigned i = threadIdx.x; i < (unsigned)n; i += 256) {
     const float e = (float)exp((double)(sp[i] - mx));
     sp[i] = e;
     sum += (double)e;
@@ -108,11 +108,14 @@ __device__ __forceinline__ float past_of(float c2) { return fminf(kSpPast / c2, 
 constexpr int kSpWaves = 4;
 constexpr int kSpRuns = 256;      // runs of a row at most
 
+// Units that hold n positions; n up to 2^31 - 1, which no rounding up may pass.
+__host__ __device__ constexpr int units_of(int n, int unit) { return n / unit + (n % unit != 0); }
+
 // The tiles a row at p reads, in order: those of the first tokens, then the window's.
 struct SpanTiles {
   int lead, from, n;
   __host__ __device__ SpanTiles(const Span &s, int p) {
-    lead = (s.lead(p) + kKv4Tile - 1) / kKv4Tile;
+    lead = units_of(s.lead(p), kKv4Tile);
     from = s.first(p) / kKv4Tile;
     from = from < lead ? lead : from;
     n = lead + p / kKv4Tile - from + 1;
@@ -589,8 +592,7 @@ typedef float sf16 __attribute__((ext_vector_type(16)));
 struct SpanSteps {
   int lead, from, n;
   __host__ __device__ SpanSteps(const Span &s, int first_row, int last_row) {
-    const int l = s.lead(last_row);
-    lead = (l + kTlK - 1) / kTlK;
+    lead = units_of(s.lead(last_row), kTlK);
     from = s.first(first_row) / kTlK;
     from = from < lead ? lead : from;
     n = last_row / kTlK >= from ? lead + last_row / kTlK - from + 1 : lead;
