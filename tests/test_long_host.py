@@ -38,3 +38,9 @@ def test_first_tokens_up_to_the_last_position(T, window):
     assert want > 8 * T * 68  # more than one run of a row
     assert scratch(T, top, 8, 1, 64, window, 2**31 - 1) == want
     assert scratch(T, 40, 8, 1, 64, window, 2**31 - 1) == scratch(T, 40, 8, 1, 64, 0, 0)
+
+
+def test_no_bytes_for_caches_that_no_call_takes():
+    f = load().wl_kv4_bytes
+    assert f(2**31 - 1, 1 << 18, 64) == 2**26 * 2**18 * 18 * 64 and f(33, 1 << 17, 128) == 2 * 2**17 * 18 * 128
+    assert f(1, (1 << 18) + 1, 64) == f(1, (1 << 17) + 1, 128) == f(2**31 - 1, 2**31 - 1, 128) == f(64, 2**31 - 1, 64) == 0

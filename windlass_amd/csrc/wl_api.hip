@@ -1736,7 +1736,7 @@ static int kv4_check(const char *who, int KH, int HD, const void *K, const void 
   if (KH <= 0 || HD <= 0) return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, KH, HD);
   if (HD != 64 && HD != 128)
     return fail(WL_E_UNSUPPORTED, "%s: 4-bit caches hold head dims of 64 and 128, not %d", who, HD);
-  if ((int64_t)KH * HD > 1 << 24) return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, KH, HD);
+  if ((int64_t)KH * HD > wl::kKv4Row) return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, KH, HD);
   if (((uintptr_t)K | (uintptr_t)V) & 15) return fail(WL_E_ARG, "%s: a cache is not 16-byte aligned", who);
   return WL_OK;
 }

@@ -29,9 +29,11 @@ namespace wl {
 constexpr int kKv4Tile = 32;   // positions per tile
 constexpr int kKv4Rows = 64;   // rows of a batch call that one launch takes
 
-// Bytes of one cache; 0 for head dims other than 64 and 128.
+constexpr int kKv4Row = 1 << 24;  // values of a position's keys at most
+
+// Bytes of one cache; 0 for head dims other than 64 and 128, and for more KV heads than the calls take.
 inline int64_t kv4_bytes(int64_t positions, int64_t kv_heads, int hd) {
-  if (positions <= 0 || kv_heads <= 0 || (hd != 64 && hd != 128)) return 0;
+  if (positions <= 0 || kv_heads <= 0 || (hd != 64 && hd != 128) || kv_heads * hd > kKv4Row) return 0;
   return kv_heads * ((positions + kKv4Tile - 1) / kKv4Tile) * 18 * hd;
 }
 
