@@ -100,3 +100,12 @@ def test_nothing_stays_queued_after_a_failure(fails, after):
     with pytest.raises(ArgumentOutOfRangeError):
         b.generate([[1, 2], [3]], 5, [SampleParams()] * 2, [0.5] * 10)
     assert m.log[-1] == "sync"
+
+
+@pytest.mark.parametrize("kw", [dict(window=-1), dict(sinks=-1), dict(window=1 << 31), dict(window=1 << 32), dict(sinks=1 << 32)])
+def test_windows_past_32_bits_are_refused(kw):
+    """2^32 would reach the library as 0: no window."""
+    cfg = ModelConfig(layers=1, embd=4, heads=1, kv_heads=1, head_dim=64)
+    assert KvCaches(cfg, window=(1 << 31) - 1, sinks=(1 << 31) - 1).opts(5).window == (1 << 31) - 1
+    with pytest.raises(ShapeError):
+        KvCaches(cfg, **kw)

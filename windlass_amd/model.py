@@ -65,7 +65,7 @@ class KvCaches:
     def __init__(self, cfg, kv_bits=16, window=0, sinks=0):
         if kv_bits not in (16, 4):
             raise NotSupportedError("A KV cache of %s bits." % kv_bits)
-        if window < 0 or sinks < 0:
+        if not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):
             raise ShapeError("A window of %d and %d first positions." % (window, sinks))
         if kv_bits == 4 and not load().wl_kv4_bytes(1, cfg.kv_heads, cfg.head_dim):
             raise NotSupportedError("4-bit caches hold head dims of 64 and 128, not %d." % cfg.head_dim)
