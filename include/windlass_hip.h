@@ -386,7 +386,8 @@ int wl_layer_batch_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, int3
  * refused with WL_E_UNSUPPORTED.
  *
  * The window. A row at position p sees the positions j <= p with j < sinks or j > p - window; all j <= p when
- * window is 0 (sinks is then not read). */
+ * window is 0 (sinks is then not read). It saves the time of the positions that a row does not see: a cache holds
+ * every position all the same. */
 
 /* Bytes of one 4-bit cache (keys or values) of `positions` positions; 0 for a shape it cannot hold. */
 int64_t wl_kv4_bytes(int32_t positions, int32_t kv_heads, int32_t head_dim);
@@ -419,7 +420,8 @@ int wl_kv4_attention_batch_dev(wl_ctx *ctx, const float *d_q, int32_t N, int32_t
                                const int32_t *slot, int32_t slots, int32_t slot_positions, int32_t window,
                                int32_t sinks, float scale, float *d_out);
 
-/* wl_attention_dev (fp16 caches) with a window; any head dim. */
+/* wl_attention_dev (fp16 caches) with a window; any head dim. A visible value that is infinite or NaN makes its
+ * column of the rows that see it infinite or NaN; a score of -inf weighs nothing, and a row of only such scores is NaN. */
 int wl_attention_window_dev(wl_ctx *ctx, const float *d_q, int32_t T, int32_t heads, int32_t kv_heads,
                             int32_t head_dim, const uint16_t *d_K, const uint16_t *d_V, int32_t pos0, int32_t window,
                             int32_t sinks, float scale, float *d_out);

@@ -93,9 +93,9 @@ __global__ __launch_bounds__(256) void span_rows_kernel(const float *__restrict_
 // on the row's own tiles, so that a row's bits do not depend on the rows beside it.
 //
 // What bounds it: a 4-bit position of a head is 2.25 HD bytes for 4 HD G products. One row after 131,000 (8B, 151 MB) takes
-// 33.8 us and the join 4, against 24.8 for reading the bytes: the loads wait 43% of the wave cycles and the unpacking
-// keeps the VALU 54% busy. 32 rows of up to 9,001 (70B, 249 MB): 60.4 us, VALU 67%, matrix cores 9%; short contexts are
-// two launches' latency (70B after 4,000: 6.0 and 3.1 us). Measured and not kept: the last workgroup of a row joining its
+// 32.2 us and the join 4.7, against 24.8 for reading the bytes: the loads wait 44% of the wave cycles and the unpacking
+// keeps the VALU 57% busy. 32 rows of up to 9,001 (70B, 249 MB): 59.3 us, VALU 69%, matrix cores 9%; short contexts are
+// two launches' latency (70B after 4,000: 6.3 and 3.8 us). Measured and not kept: the last workgroup of a row joining its
 // runs (with fences 770 us for the 32 rows; with device-scope stores 66.9 against 61.6, and 41.7 against 35.5 for the long
 // row), records loaded ahead in the join (62.5 -> 66), eight waves a workgroup.
 typedef float sf4 __attribute__((ext_vector_type(4)));
@@ -559,8 +559,10 @@ __global__ __launch_bounds__(256) void span_join_kernel(const float *__restrict_
 // (32 heads of 64, 7 rows at 333: 6.0 us, two runs 9.2). Up to 160 tiles (5,120 positions) as many runs as give every CU a
 // workgroup, of four tiles at least, a tile a wave (64 heads of 128 after 4,000: 9.7 us, 16 tiles a run 11.7; fp16, a
 // window of 4,096: 11.4 us, eight tiles 13.0). More: four tiles a wave, where a run's fixed work (the query's parts, the
-// sums through LDS, its record) weighs more than a lone row's waves (32 rows of up to 9,001 62 us, two tiles a wave
-// 69, one 89), and no more runs than give every CU two workgroups.
+// sums through LDS, its record) weighs more than a lone row's waves (32 rows of up to 9,001 65 us, two tiles a wave
+// 73, one 93; 8 rows of 8B 21.0, 22.3, 28.4), and no more runs than give every CU two workgroups. A lone row of 8 KV heads
+// pays for it between 5,120 and 10,000 positions: 11.9 us at 5,200 and 12.1 at 8,000, two tiles a wave 10.1-10.8; at
+// 12,000 and 16,000 12.2 and 12.4, two tiles 12.6 and 12.7.
 static int span_per(int n, int units) {
   if (n <= 16) return n;
   const int64_t all = (int64_t)n * units;
@@ -581,7 +583,7 @@ static int span_per(int n, int units) {
 //
 // What bounds it: both products twice (two parts), 206 GFLOP for 2,048 tokens of the 8B model's 32 heads after 2,048, in
 // 205-214 us on the cards measured: 960 to 1,005 TFLOP/s, where a library's product of 4,096 x 4,096 matrices reaches 1,100. The matrix cores are busy 40%
-// of the cycles and the VALU 50%, with two waves a SIMD that seldom overlap them; 254 registers leave no room for a second
+// of the cycles and the VALU 48%, with two waves a SIMD that seldom overlap them; 254 registers leave no room for a second
 // tile of scores, and kernels that kept one (the scores of 32 keys beside the exponentials of the 32 before) spilled and
 // took 297-308 us; the next step's unpacking among a chain's products, 225-245 us, for the same reason. Rows cut in two and more chunks where whole rows fill the CUs: 282 us; 2 and 4 chunks for a window of
 // 1,500 rows, whose 376 workgroups are one and two a CU: 114 and 131 us against 102.
@@ -1057,7 +1059,9 @@ static TilesArgs tiles_plan(const KvCache &c, int H, const Span &s, const KvRows
     const int n = SpanSteps(s, A.row0(z), A.row1(z)).n;
     most = n > most ? n : most;
   }
-  // whole rows where the workgroups of columns alone give every CU two; otherwise cut so that they do
+  // Whole rows where the workgroups of columns alone give every CU one; fewer are cut so that they give two (8B after 2,000:
+  // 500 rows 66 us, whole 104; a window of 1,024 49, whole 66; but 1,500 rows, whole, 175, cut 199). Just below the border
+  // cutting costs more than it gives: 992 rows 140 us, whole 124, the window's 87, whole 68.
   const int64_t wgs = (int64_t)c.KH * A.nz;
   int64_t S = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
   S = S > most ? most : S;

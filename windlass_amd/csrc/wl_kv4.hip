@@ -1,8 +1,8 @@
 // wl_kv4.hip - rows of keys and values into the 4-bit caches and back (wl_kv4.h).
 //
 // What bounds it: 8 bytes read and 1.125 written per key and value pair. A decode step's row is a launch's latency (1.7-2.5
-// us of GPU time); a prompt's rows HBM (2,000 rows of 8 heads of 128, 18.7 MB each way: stored in 7.8 us, read back in
-// 6.3, 2.4 and 3.0 TB/s, half of it the launch's ends). Four lanes share a block because its largest value is a maximum
+// us of GPU time); a prompt's rows HBM (2,000 rows of 8 heads of 128, 18.7 MB each way: stored in 7.2 us, read back in
+// 6.3, 2.6 and 3.0 TB/s, half of it the launch's ends). Four lanes share a block because its largest value is a maximum
 // over 32; 16 bytes a lane and load keep the reads whole.
 #include "wl_kv4.h"
 

@@ -20,11 +20,11 @@
 // bins and answers the questions: a prefix's end lies in one bin, whose tokens it gathers and narrows down by their
 // bits, and equal ones by their ids; with top_k of few tokens it gathers the whole prefix and puts that in order.
 //
-// What bounds it: a row of 128,256 is read from HBM in launch 1 and from the caches after (64 rows, 33 MB: 6.2 us), then
-// 64 rows' bins take 24.2 us (50 VALU instructions a token, and LDS atomics that meet: two or four copies of the bins, votes
+// What bounds it: a row of 128,256 is read from HBM in launch 1 and from the caches after (64 rows, 33 MB: 6.6 us), then
+// 64 rows' bins take 23.0 us (50 VALU instructions a token, and LDS atomics that meet: two or four copies of the bins, votes
 // for the last bin and no min_p sums where none is asked each gained less than a microsecond or lost) and their questions
-// 16.6 (a workgroup a row: chains of LDS and cache latencies, 2.5 to 6 us a question). One row is three dependent launches:
-// 2.4, 6.6 and 6.3 us.
+// 17.1 (a workgroup a row: chains of LDS and cache latencies, 2.5 to 6 us a question). One row is three dependent launches:
+// 2.6, 6.8 and 6.3 us.
 #include "wl_sample.h"
 
 #include "wl_device.h"

@@ -340,8 +340,8 @@ def _vector(ctx, g, t, dev):
 
 def load_device_model(ctx, path, max_positions=None, kv_bits=16, window=0, sinks=0):
     """The model of a GGUF file in HBM: every matrix's raw blocks uploaded unchanged, the vectors
-    decoded on the GPU; kv_bits, window and sinks as DeviceTransformer takes them. Returns
-    (DeviceTransformer, weights) - free the weights when done."""
+    decoded on the GPU; kv_bits, window and sinks as DeviceTransformer takes them (a file's own
+    attention.sliding_window is not read). Returns (DeviceTransformer, weights) - free the weights when done."""
     import torch
     from .model import DeviceTransformer
     g = GgufModelFile.Open(path)

@@ -60,7 +60,8 @@ def _fits(prompt, steps, pos0, positions):
 
 class KvCaches:
     """The kind of a model's KV caches, and the layer calls over them: kv_bits 16 (fp16 rows) or 4 (wl_kv4_bytes: head
-    dims 64 and 128), and the positions a row sees (window 0: all; else the last `window` and the first `sinks`)."""
+    dims 64 and 128), and the positions a row sees (window 0: all; else the last `window` and the first `sinks`), the same
+    in every layer. The caches hold every position whatever the window."""
 
     def __init__(self, cfg, kv_bits=16, window=0, sinks=0):
         if kv_bits not in (16, 4):
