@@ -443,6 +443,81 @@ int wl_layer_batch_kv_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, i
                           const int32_t *slot, int32_t slots, int32_t slot_positions, void *d_K, void *d_V,
                           const wl_kv_opts *kv);
 
+/* ---- KV caches in pages, attention of sequences that share them (no counterpart in the reference, whose
+ * batch engine gives every sequence a slot for the longest context) ----
+ * A pool of pages holds the keys and values of many sequences in fp16: a sequence takes the pages that it needs, several
+ * share those of a common beginning, and a row may attend to chosen pages only. Stream-ordered on the context like the other
+ * _dev entries, with their rules for host arrays: entries' arrays may change on return, and a capture records their values.
+ *
+ * The pool. d_K and d_V hold wl_page_bytes for each page, 16-byte aligned, in an order of their own (windlass_amd/csrc/
+ * wl_paged.h), which the caller owns, and so the table: d_table[sequence][table_pages] (device) names the page of a
+ * sequence's positions page * j .. page * j + page - 1. An id outside 0 .. pages - 1 is no page: nothing is stored there, and no
+ * row sees its positions. Sequences may share pages that no call writes to any more. head_dim is 64 or 128; other head dims
+ * are refused with WL_E_UNSUPPORTED.
+ * d_bounds (or null) holds wl_page_bounds_bytes for each page: the smallest and the largest key of each channel, fp16
+ * [kv_heads][2][head_dim], over the page's positions up to the last that was stored last (a NaN where one of them is).
+ *
+ * Entries. Entry i of n is rows[i] rows (rows null: one each) of sequence seq[i], at positions pos[i] and on, in host
+ * arrays; q, k, v and outputs hold the entries' rows one after the other. An entry may have no rows, and with no rows at all
+ * the rows' pointers may be null. */
+typedef struct wl_pages {
+  void *d_K, *d_V, *d_bounds;
+  const int32_t *d_table;
+  int32_t pages, page; /* page: 16, 32, 64, 128 or 256 positions */
+  int32_t kv_heads, head_dim;
+  int32_t sequences, table_pages;
+} wl_pages;
+typedef struct wl_page_rows {
+  int32_t n;
+  const int32_t *seq, *pos, *rows;
+} wl_page_rows;
+
+/* Bytes of a page's keys (and of its values), and of its bounds; 0 for a shape that a pool cannot hold. */
+int64_t wl_page_bytes(int32_t page, int32_t kv_heads, int32_t head_dim);
+int64_t wl_page_bounds_bytes(int32_t kv_heads, int32_t head_dim);
+
+/* Ids (host; -1: no page) into the table: entries first .. first + n - 1 of a sequence. p->d_table is written here. */
+int wl_paged_assign_dev(wl_ctx *ctx, const wl_pages *p, int32_t seq, int32_t first, int32_t n, const int32_t *ids);
+
+/* wl_rope_dev's rotation of q [rows][heads * head_dim] into d_q_out (which may be d_q) and of k, and k and v
+ * [rows][kv_heads * head_dim] into the pages, in one launch; with d_bounds also the bounds of the pages written to. rope_dims 0
+ * rotates nothing; heads 0 (and null d_q, d_q_out) leaves the queries out. d_k and d_v stay as they were. The entries'
+ * sequences are distinct, and no page that is written to belongs to two of them. */
+int wl_paged_store_dev(wl_ctx *ctx, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
+                       const float *d_k, const float *d_v, int32_t rope_dims, int32_t neox, double base,
+                       double freq_scale, const float *d_freqs, float *d_q_out);
+
+/* The values that positions pos0 .. pos0 + T - 1 of a sequence hold: d_k, d_v [T][kv_heads * head_dim] (zeros where there
+ * is no page). */
+int wl_paged_read_dev(wl_ctx *ctx, const wl_pages *p, int32_t seq, int32_t pos0, int32_t T, float *d_k, float *d_v);
+
+/* wl_attention_dev over pages: d_q, d_out [rows][heads * head_dim], each row over positions 0 .. its own of its sequence. A
+ * score of -inf weighs nothing; a row without a score above -inf (or that sees no page) gives zeros. A visible value that is
+ * infinite or NaN makes its column of the rows that see it infinite or NaN.
+ * prefix > 0 (whole pages): the entries' sequences have the same pages for the positions below it, which are read from the
+ * first entry's and once for all rows; every pos[i] is at least prefix. With prefix 0 a row's bits do not depend on the other
+ * entries; with one they differ from those in the last places. */
+int wl_paged_attention_dev(wl_ctx *ctx, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
+                           int32_t prefix, float scale, float *d_out);
+
+/* Attention of each row and KV head to some of its pages: of the pages up to its own, the `first` first and the
+ * `recent` last (its own among them), and of the others the `top` of largest score (of equals the lower): the largest, over
+ * the query heads of the KV head, of the sum over channels of max(q lo, q hi) with the page's bounds lo and hi: no score
+ * q k of the page is larger. Formed in double; a score that is infinite or NaN comes before all others, and what has no
+ * page is not taken. d_blocks (or null) [rows][kv_heads][first + recent + top] receives the pages taken (their numbers within
+ * the sequence, rising; -1 after the last). Scores below 0 and a negative scale change nothing in the choice. */
+typedef struct wl_sparse_opts {
+  int32_t first, recent, top; /* recent >= 1 */
+} wl_sparse_opts;
+int wl_paged_sparse_dev(wl_ctx *ctx, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
+                        const wl_sparse_opts *o, float scale, float *d_out, int32_t *d_blocks);
+
+/* wl_layer_dev over pages: d_x [rows][embd] of the entries' rows (distinct sequences, no prefix or sparse choice by default:
+ * 0 and null; not both). Where every entry has one row the products run as wl_layer_batch_dev's, so that without a prefix a
+ * row's bits equal those of its call alone; otherwise all rows are one prompt's. */
+int wl_layer_paged_dev(wl_ctx *ctx, const wl_layer_desc *layer, float *d_x, const wl_pages *p, const wl_page_rows *r,
+                       int32_t prefix, const wl_sparse_opts *o);
+
 /* The next token of each of `rows` rows of n logits (at most 2^24), drawn with the settings params[row]
  * (host) and the number d_u[row] in [0, 1) (device). Tokens in order (larger logit first, of equals the
  * lower id) with weights exp((logit - max) / temperature): the first top_k stay (0: all), of those the

@@ -22,6 +22,9 @@ libwindlass_hip.so (include/windlass_hip.h):
 - ``SampleParams``                Sampler's settings (src/Engine.cs:353-382): ``generate`` of the two classes above
 - ``KvOpts``, ``KvCaches``        caches in 4 bits, a sliding window with first tokens that stay visible (not in the
                                   reference): ``kv_bits``, ``window`` and ``sinks`` of DeviceTransformer
+- ``Pages``, ``PageRows``,
+  ``SparseOpts``, ``PagedBatch``  caches in pages that sequences share, a common beginning read once, attention to
+                                  chosen pages (not in the reference)
 - ``gguf.GgufModelFile``          GgufModelFile (src/Gguf.cs:104-270); ``gguf.model_config`` and
                                   ``gguf.load_device_model``: ModelConfig.From and a file's model in HBM
 
@@ -31,11 +34,11 @@ failure). There is no CPU fallback: without the built library every call raises.
 """
 from ._lib import (ArgumentOutOfRangeError, BackendError, NotSupportedError, ShapeError,
                    library_path, load)
-from .backend import (Context, FastMath, GgmlType, Graph, HostBuffer, KvOpts, LayerDesc, QActs, Quants, SampleParams,
-                      Stage, Transformer, WeightView, layout)
-from .model import DeviceBatch, DeviceTransformer, KvCaches, ModelConfig, StageStream
+from .backend import (Context, FastMath, GgmlType, Graph, HostBuffer, KvOpts, LayerDesc, PageRows, Pages, QActs, Quants,
+                      SampleParams, SparseOpts, Stage, Transformer, WeightView, layout)
+from .model import DeviceBatch, DeviceTransformer, KvCaches, ModelConfig, PagedBatch, StageStream
 
 __all__ = ["ArgumentOutOfRangeError", "BackendError", "NotSupportedError", "ShapeError",
            "library_path", "load", "Context", "FastMath", "GgmlType", "Graph", "HostBuffer", "KvCaches", "KvOpts",
-           "LayerDesc", "QActs", "Quants", "SampleParams", "Stage", "Transformer", "WeightView", "layout", "DeviceBatch",
-           "DeviceTransformer", "ModelConfig", "StageStream"]
+           "LayerDesc", "PageRows", "Pages", "QActs", "Quants", "SampleParams", "SparseOpts", "Stage", "Transformer", "WeightView", "layout", "DeviceBatch",
+           "DeviceTransformer", "ModelConfig", "PagedBatch", "StageStream"]

@@ -38,6 +38,14 @@ SIGNATURES = {
     "wl_attention_window_dev": (ctypes.c_int, [P, P, I32, I32, I32, I32, P, P, I32, I32, I32, F, P]),
     "wl_layer_kv_dev": (ctypes.c_int, [P, P, P, I32, I32, P, P, P]),
     "wl_layer_batch_kv_dev": (ctypes.c_int, [P, P, P, I32, P, P, I32, I32, P, P, P]),
+    "wl_page_bytes": (I64, [I32, I32, I32]),
+    "wl_page_bounds_bytes": (I64, [I32, I32]),
+    "wl_paged_assign_dev": (ctypes.c_int, [P, P, I32, I32, I32, P]),
+    "wl_paged_store_dev": (ctypes.c_int, [P, P, P, P, I32, P, P, I32, I32, ctypes.c_double, ctypes.c_double, P, P]),
+    "wl_paged_read_dev": (ctypes.c_int, [P, P, I32, I32, I32, P, P]),
+    "wl_paged_attention_dev": (ctypes.c_int, [P, P, P, P, I32, I32, F, P]),
+    "wl_paged_sparse_dev": (ctypes.c_int, [P, P, P, P, I32, P, F, P, P]),
+    "wl_layer_paged_dev": (ctypes.c_int, [P, P, P, P, P, I32, P]),
     "wl_sample_dev": (ctypes.c_int, [P, P, I32, I64, P, P, P]),
     "wl_embed_dev_ids": (ctypes.c_int, [P, P, P, I32, P]),
     "wl_layer_batch_dev": (ctypes.c_int, [P, P, P, I32, P, P, I32, I32, P, P]),

@@ -369,6 +369,30 @@ class KvOpts(ctypes.Structure):
                 ("positions", ctypes.c_int32)]
 
 
+class Pages(ctypes.Structure):
+    """wl_pages: a pool of pages of keys and values, the table of the sequences' pages, and their shapes."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_K", "d_V", "d_bounds", "d_table")] + [
+        (n, ctypes.c_int32) for n in ("pages", "page", "kv_heads", "head_dim", "sequences", "table_pages")]
+
+
+class PageRows(ctypes.Structure):
+    """wl_page_rows: a call's entries, rows[i] rows (one each when rows is None) of sequence seq[i] from position pos[i]."""
+    _fields_ = [("n", ctypes.c_int32)] + [(n, ctypes.POINTER(ctypes.c_int32)) for n in ("seq", "pos", "rows")]
+
+    def __init__(self, seq, pos, rows=None):
+        n = len(seq)
+        if len(pos) != n or (rows is not None and len(rows) != n):
+            raise ShapeError("Entries of %d sequences, %d positions and %s rows." % (n, len(pos), rows and len(rows)))
+        a = ctypes.c_int32 * n
+        super().__init__(n, a(*seq), a(*pos), None if rows is None else a(*rows))  # ctypes keeps the arrays alive
+
+
+class SparseOpts(ctypes.Structure):
+    """wl_sparse_opts: the pages a row attends to: the `first` first, the `recent` last, and the `top` others of largest
+    score."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("first", "recent", "top")]
+
+
 class SampleParams(ctypes.Structure):
     """wl_sample_params: one row's settings (Sampler, src/Engine.cs:353-382). temperature 0 is the greedy pick;
     top_k 0, top_p 1 and min_p 0 filter nothing."""

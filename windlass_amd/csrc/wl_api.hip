@@ -26,6 +26,7 @@
 #include "wl_kv4.h"
 #include "wl_layer.h"
 #include "wl_moe.h"
+#include "wl_paged.h"
 #include "wl_probe.h"
 #include "wl_sample.h"
 
@@ -56,12 +57,13 @@ struct wl_stage {
 
 // S_PART holds the K-chunk partials of split GEMV rows, S_XB the bf16 copy of x for the GEMM,
 // S_QA the 8-bit activations of the integer path, S_MSYNC the one-launch MoE's counters
-// (allocated and zeroed once; every launch leaves them zero).
+// (allocated and zeroed once; every launch leaves them zero), S_SEL the pages' scores and S_BLK the pages chosen.
 // S_L* are wl_layer_dev's activations (S_LO: wl_matmul_add_dev's product when the add is not
 // the GEMV's own store; S_LR the router's logits and the shared expert's gate, S_LM the MoE
 // FFN's output, S_LS the shared expert's).
 enum { S_X = 0, S_Y, S_H, S_MOE, S_OUT, S_AUX, S_PART, S_XB, S_QA, S_ATT,
-       S_LXN, S_LQ, S_LK, S_LV, S_LATT, S_LO, S_LG, S_LU, S_LR, S_LM, S_LS, S_ROWS, S_ARG, S_MSYNC, S_SMP, S_COUNT };
+       S_LXN, S_LQ, S_LK, S_LV, S_LATT, S_LO, S_LG, S_LU, S_LR, S_LM, S_LS, S_ROWS, S_ARG, S_MSYNC, S_SMP,
+       S_SEL, S_BLK, S_COUNT };
 
 struct wl_ctx {
   int device;
@@ -1445,9 +1447,19 @@ struct LayerKv {
 static int layer_attention_kv(wl_ctx *c, const wl_layer_desc *L, const LayerKv &kv, float *q, float *k, const float *v,
                               int T, int pos0, int rd, double fs, float scale, float *att);
 
+// A layer's cache in pages, and the call's entries.
+struct LayerPaged {
+  const wl_pages *p;
+  const wl_page_rows *r;
+  int prefix;
+  const wl_sparse_opts *sparse;
+};
+static int layer_attention_paged(wl_ctx *c, const wl_layer_desc *L, const LayerPaged &pg, float *q, const float *k,
+                                 const float *v, int rd, double fs, float scale, float *att);
+
 static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, int32_t pos0, uint16_t *d_K,
                      uint16_t *d_V, const wl::RowMap &rm, const int32_t *hpos, int max_n, bool each,
-                     const LayerKv *kv = nullptr) {
+                     const LayerKv *kv = nullptr, const LayerPaged *pg = nullptr) {
   if (!c || !L || !d_x || !d_K || !d_V) return fail(WL_E_ARG, "wl_layer_dev: null argument");
   // OLMo 2 (src/Transformer.cs:182,224-230): post-norms instead of pre-norms
   const bool post = L->d_post_attention_norm || L->d_post_ffw_norm;
@@ -1487,7 +1499,7 @@ static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, i
       (rc = ensure(c, S_LK, (size_t)T * KD * 4)) || (rc = ensure(c, S_LV, (size_t)T * KD * 4)) ||
       (rc = ensure(c, S_LATT, (size_t)T * QD * 4)) ||
       (rc = ensure(c, S_LG, (size_t)T * FF * 4)) || (rc = ensure(c, S_LU, (size_t)T * FF * 4)) ||
-      (!kv && (rc = ensure(c, S_ATT, (size_t)wl::attention_scratch_floats(T, H, HD, KD, max_n, d_K, d_V, rm) * 4))))
+      (!kv && !pg && (rc = ensure(c, S_ATT, (size_t)wl::attention_scratch_floats(T, H, HD, KD, max_n, d_K, d_V, rm) * 4))))
     return rc;
   float *xn = (float *)c->buf[S_LXN], *q = (float *)c->buf[S_LQ], *k = (float *)c->buf[S_LK],
         *v = (float *)c->buf[S_LV], *att = (float *)c->buf[S_LATT],
@@ -1586,7 +1598,9 @@ static int layer_run(wl_ctx *c, const wl_layer_desc *L, float *d_x, int32_t T, i
   const double fs = L->rope_freq_scale != 0.0 ? L->rope_freq_scale : 1.0;
   const float scale = L->attention_scale != 0.f ? L->attention_scale : 1.0f / (float)sqrt((double)HD);
   const float4 *tab = nullptr;
-  if (kv) {
+  if (pg) {
+    if ((rc = layer_attention_paged(c, L, *pg, q, k, v, rd, fs, scale, att))) return rc;
+  } else if (kv) {
     if ((rc = layer_attention_kv(c, L, *kv, q, k, v, T, pos0, rd, fs, scale, att))) return rc;
   } else {
     // A recording takes no angles from the table, which calls between its replays may fill for other settings: they are made
@@ -1985,6 +1999,278 @@ extern "C" int wl_layer_batch_kv_dev(wl_ctx *c, const wl_layer_desc *L, float *d
   kv.pos = pos;
   kv.slot = slot;
   return layer_run(c, L, d_x, N, 0, (uint16_t *)d_K, (uint16_t *)d_V, wl::RowMap{}, pos, 0, true, &kv);
+}
+
+// ------------------------------------------------- caches in pages
+
+extern "C" int64_t wl_page_bytes(int32_t page, int32_t kv_heads, int32_t head_dim) {
+  if (page < 16 || page > 256 || (page & (page - 1)) || kv_heads <= 0 || (head_dim != 64 && head_dim != 128) ||
+      (int64_t)kv_heads * head_dim > wl::kPgValues)
+    return 0;
+  return (int64_t)page * kv_heads * head_dim * 2;
+}
+
+extern "C" int64_t wl_page_bounds_bytes(int32_t kv_heads, int32_t head_dim) {
+  return wl_page_bytes(16, kv_heads, head_dim) / 8;
+}
+
+// The pool of a call, as the kernels take it.
+static int paged_pool(const char *who, const wl_pages *p, wl::PagePool *o) {
+  if (!p->d_K || !p->d_V || !p->d_table) return fail(WL_E_ARG, "%s: null argument", who);
+  if (p->kv_heads <= 0 || p->head_dim <= 0 || (int64_t)p->kv_heads * p->head_dim > wl::kPgValues)
+    return fail(WL_E_SHAPE, "%s: %d KV heads of %d", who, p->kv_heads, p->head_dim);
+  if (p->head_dim != 64 && p->head_dim != 128)
+    return fail(WL_E_UNSUPPORTED, "%s: pages hold head dims of 64 and 128, not %d", who, p->head_dim);
+  if (!wl_page_bytes(p->page, p->kv_heads, p->head_dim))
+    return fail(WL_E_SHAPE, "%s: a page of %d positions is not 16, 32, 64, 128 or 256", who, p->page);
+  if (p->pages <= 0 || p->sequences <= 0 || p->table_pages <= 0)
+    return fail(WL_E_SHAPE, "%s: %d pages, a table of %d x %d", who, p->pages, p->sequences, p->table_pages);
+  if (((uintptr_t)p->d_K | (uintptr_t)p->d_V | (uintptr_t)p->d_bounds) & 15)
+    return fail(WL_E_ARG, "%s: a pool is not 16-byte aligned", who);
+  if ((uintptr_t)p->d_table & 3) return fail(WL_E_ARG, "%s: the table is not 4-byte aligned", who);
+  o->K = (uint16_t *)p->d_K;
+  o->V = (uint16_t *)p->d_V;
+  o->bounds = (uint16_t *)p->d_bounds;
+  o->table = p->d_table;
+  o->pages = p->pages;
+  o->page = p->page;
+  o->shift = __builtin_ctz((unsigned)p->page);
+  o->KH = p->kv_heads;
+  o->HD = p->head_dim;
+  o->width = p->table_pages;
+  return WL_OK;
+}
+
+// The entries of a call: their sequences (distinct, where they are written to) and positions within the table.
+static int paged_rows(const char *who, const wl_pages *p, const wl_page_rows *r, bool distinct, int *rows) {
+  if (r->n < 0) return fail(WL_E_SHAPE, "%s: %d entries", who, r->n);
+  if (r->n && (!r->seq || !r->pos)) return fail(WL_E_ARG, "%s: null argument", who);
+  const int64_t most = std::min((int64_t)p->page * p->table_pages, (int64_t)INT32_MAX);
+  int64_t all = 0;
+  for (int i = 0; i < r->n; i++) {
+    const int t = r->rows ? r->rows[i] : 1;
+    if (t < 0) return fail(WL_E_SHAPE, "%s: entry %d has %d rows", who, i, t);
+    if (r->seq[i] < 0 || r->seq[i] >= p->sequences)
+      return fail(WL_E_ARG, "Entry %d's sequence %d is outside 0..%d.", i, r->seq[i], p->sequences - 1);
+    if (r->pos[i] < 0 || (int64_t)r->pos[i] + t > most)
+      return fail(WL_E_ARG, "The prompt and reply need %lld positions; the context is %lld.", (long long)r->pos[i] + t,
+                  (long long)most);
+    all += t;
+  }
+  if (all > 1 << 24) return fail(WL_E_SHAPE, "%s: %lld rows", who, (long long)all);
+  if (distinct) {
+    std::vector<int32_t> s(r->seq, r->seq + r->n);
+    std::sort(s.begin(), s.end());
+    if (std::adjacent_find(s.begin(), s.end()) != s.end())
+      return fail(WL_E_ARG, "%s: a sequence can be one entry of a call that stores.", who);
+  }
+  *rows = (int)all;
+  return WL_OK;
+}
+
+static int paged_heads(const char *who, int heads, int kv_heads, int head_dim) {
+  if (heads <= 0 || heads % kv_heads || (int64_t)heads * head_dim > wl::kPgValues)
+    return fail(WL_E_SHAPE, "%s: %d heads over %d KV heads", who, heads, kv_heads);
+  return WL_OK;
+}
+
+static int paged_prefix(const char *who, const wl_pages *p, const wl_page_rows *r, int prefix) {
+  if (prefix < 0 || prefix % p->page)
+    return fail(WL_E_ARG, "%s: a prefix of %d positions is not whole pages of %d", who, prefix, p->page);
+  for (int i = 0; i < r->n; i++)
+    if (r->pos[i] < prefix)
+      return fail(WL_E_ARG, "%s: entry %d begins at %d, within the prefix of %d", who, i, r->pos[i], prefix);
+  return WL_OK;
+}
+
+static int paged_sparse(const char *who, const wl_pages *p, const wl_sparse_opts *o) {
+  if (!p->d_bounds) return fail(WL_E_ARG, "%s: the pages have no bounds", who);
+  if (o->first < 0 || o->recent < 1 || o->top < 0 || (int64_t)o->first + o->recent + o->top > 1 << 20)
+    return fail(WL_E_ARG, "%s: the %d first, %d last and %d other pages", who, o->first, o->recent, o->top);
+  return WL_OK;
+}
+
+// f(rows, first row) for a call's entries, kPgRows and `most` rows at a time; entries without rows are left out.
+template <class F>
+static int each_page_rows(const wl_page_rows *r, int most, const F &f) {
+  wl::PageRows R;
+  R.row0[0] = 0;
+  int r0 = 0;
+  auto flush = [&]() -> int {
+    const int rc = R.n ? f(R, r0) : WL_OK;
+    r0 += R.row0[R.n];
+    R.n = 0;
+    return rc;
+  };
+  for (int i = 0; i < r->n; i++) {
+    const int T = r->rows ? r->rows[i] : 1;
+    for (int t = 0; t < T;) {
+      const int m = std::min(T - t, most - R.row0[R.n]);
+      R.seq[R.n] = r->seq[i];
+      R.pos[R.n] = r->pos[i] + t;
+      R.row0[R.n + 1] = R.row0[R.n] + m;
+      R.n++;
+      t += m;
+      if (R.n == wl::kPgRows || R.row0[R.n] == most)
+        if (const int rc = flush()) return rc;
+    }
+  }
+  return flush();
+}
+
+extern "C" int wl_paged_assign_dev(wl_ctx *c, const wl_pages *p, int32_t seq, int32_t first, int32_t n, const int32_t *ids) {
+  if (!c || !p || (n && !ids)) return fail(WL_E_ARG, "wl_paged_assign_dev: null argument");
+  wl::PagePool pool;
+  if (const int rc = paged_pool("wl_paged_assign_dev", p, &pool)) return rc;
+  if (seq < 0 || seq >= p->sequences) return fail(WL_E_ARG, "Sequence %d is outside 0..%d.", seq, p->sequences - 1);
+  if (n < 0 || first < 0 || (int64_t)first + n > p->table_pages)
+    return fail(WL_E_ARG, "wl_paged_assign_dev: entries %d..%lld of %d", first, (long long)first + n - 1, p->table_pages);
+  for (int i = 0; i < n; i++)
+    if (ids[i] < -1 || ids[i] >= p->pages) return fail(WL_E_ARG, "Page %d is outside 0..%d.", ids[i], p->pages - 1);
+  WL_ON_DEVICE(c);
+  WL_HIP(wl::put_ints_launch(ids, n, const_cast<int32_t *>(p->d_table) + (int64_t)seq * p->table_pages + first, c->stream),
+         "page table");
+  return WL_OK;
+}
+
+static int paged_store(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
+                       const float *d_k, const float *d_v, const wl::PageRope &rope, float *d_q_out) {
+  const int64_t qd = (int64_t)heads * pool.HD, kd = (int64_t)pool.KH * pool.HD;
+  return each_page_rows(r, 1 << 20, [&](const wl::PageRows &R, int r0) -> int {
+    WL_HIP(wl::paged_store_launch(pool, R, heads ? d_q + r0 * qd : nullptr, heads, d_k + r0 * kd, d_v + r0 * kd, rope,
+                                  heads ? d_q_out + r0 * qd : nullptr, c->stream), "paged store");
+    return WL_OK;
+  });
+}
+
+extern "C" int wl_paged_store_dev(wl_ctx *c, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
+                                  const float *d_k, const float *d_v, int32_t rope_dims, int32_t neox, double base,
+                                  double freq_scale, const float *d_freqs, float *d_q_out) {
+  if (!c || !p || !r) return fail(WL_E_ARG, "wl_paged_store_dev: null argument");
+  wl::PagePool pool;
+  int rc, rows;
+  if ((rc = paged_pool("wl_paged_store_dev", p, &pool)) || (rc = paged_rows("wl_paged_store_dev", p, r, true, &rows)) ||
+      (heads && (rc = paged_heads("wl_paged_store_dev", heads, p->kv_heads, p->head_dim))))
+    return rc;
+  if (rope_dims < 0 || rope_dims > p->head_dim || rope_dims % 2)
+    return fail(WL_E_SHAPE, "wl_paged_store_dev: %d rotated of %d per head", rope_dims, p->head_dim);
+  if (rows && (!d_k || !d_v || (heads && (!d_q || !d_q_out)))) return fail(WL_E_ARG, "wl_paged_store_dev: null argument");
+  WL_ON_DEVICE(c);
+  return paged_store(c, pool, r, d_q, heads, d_k, d_v, wl::page_rope(rope_dims, neox, base, freq_scale, d_freqs), d_q_out);
+}
+
+extern "C" int wl_paged_read_dev(wl_ctx *c, const wl_pages *p, int32_t seq, int32_t pos0, int32_t T, float *d_k, float *d_v) {
+  if (!c || !p || (T && (!d_k || !d_v))) return fail(WL_E_ARG, "wl_paged_read_dev: null argument");
+  wl::PagePool pool;
+  int rc, rows;
+  const wl_page_rows r = {1, &seq, &pos0, &T};
+  if ((rc = paged_pool("wl_paged_read_dev", p, &pool)) || (rc = paged_rows("wl_paged_read_dev", p, &r, false, &rows)))
+    return rc;
+  WL_ON_DEVICE(c);
+  WL_HIP(wl::paged_read_launch(pool, seq, pos0, T, d_k, d_v, c->stream), "paged read");
+  return WL_OK;
+}
+
+static int paged_attention(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
+                           int prefix, float scale, float *d_out) {
+  const int64_t qd = (int64_t)heads * pool.HD;
+  return each_page_rows(r, 1 << 20, [&](const wl::PageRows &R, int r0) -> int {
+    const int64_t floats = wl::paged_attention_scratch_floats(pool, R, heads, prefix, 0);
+    if (const int rc = ensure(c, S_ATT, (size_t)floats * sizeof(float))) return rc;
+    WL_HIP(wl::paged_attention_launch(pool, R, d_q + r0 * qd, heads, prefix, nullptr, 0, scale, (float *)c->buf[S_ATT],
+                                      d_out + r0 * qd, c->stream), "paged attention");
+    return WL_OK;
+  });
+}
+
+extern "C" int wl_paged_attention_dev(wl_ctx *c, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
+                                      int32_t prefix, float scale, float *d_out) {
+  if (!c || !p || !r) return fail(WL_E_ARG, "wl_paged_attention_dev: null argument");
+  wl::PagePool pool;
+  int rc, rows;
+  if ((rc = paged_pool("wl_paged_attention_dev", p, &pool)) ||
+      (rc = paged_rows("wl_paged_attention_dev", p, r, false, &rows)) ||
+      (rc = paged_heads("wl_paged_attention_dev", heads, p->kv_heads, p->head_dim)) ||
+      (rc = paged_prefix("wl_paged_attention_dev", p, r, prefix)))
+    return rc;
+  if (rows && (!d_q || !d_out)) return fail(WL_E_ARG, "wl_paged_attention_dev: null argument");
+  WL_ON_DEVICE(c);
+  return paged_attention(c, pool, r, d_q, heads, prefix, scale, d_out);
+}
+
+// Rows of a choice of pages at a time: as many as 256 MB of scores and of pages chosen take.
+static int sparse_rows(const wl::PagePool &pool, const wl_page_rows *r, const wl::PageSelect &s) {
+  int64_t pages = s.most();
+  for (int i = 0; i < r->n; i++)
+    pages = std::max(pages, ((int64_t)r->pos[i] + (r->rows ? r->rows[i] : 1) + pool.page - 1) >> pool.shift);
+  return (int)std::clamp(((int64_t)32 << 20) / (pages * pool.KH), (int64_t)1, (int64_t)32768);
+}
+
+static int paged_sparse_attention(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
+                                  const wl_sparse_opts *o, float scale, float *d_out, int32_t *d_blocks) {
+  const int64_t qd = (int64_t)heads * pool.HD;
+  const wl::PageSelect s{o->first, o->recent, o->top};
+  return each_page_rows(r, sparse_rows(pool, r, s), [&](const wl::PageRows &R, int r0) -> int {
+    int rc;
+    const size_t blocks = (size_t)R.row0[R.n] * pool.KH * s.most();
+    if ((rc = ensure(c, S_SEL, (size_t)wl::paged_select_scratch_bytes(pool, R, s))) ||
+        (!d_blocks && (rc = ensure(c, S_BLK, blocks * sizeof(int32_t)))) ||
+        (rc = ensure(c, S_ATT, (size_t)wl::paged_attention_scratch_floats(pool, R, heads, 0, s.most()) * sizeof(float))))
+      return rc;
+    int32_t *b = d_blocks ? d_blocks + (int64_t)r0 * pool.KH * s.most() : (int32_t *)c->buf[S_BLK];
+    WL_HIP(wl::paged_select_launch(pool, R, d_q + r0 * qd, heads, s, c->buf[S_SEL], b, c->stream), "page choice");
+    WL_HIP(wl::paged_attention_launch(pool, R, d_q + r0 * qd, heads, 0, b, s.most(), scale, (float *)c->buf[S_ATT],
+                                      d_out + r0 * qd, c->stream), "paged attention");
+    return WL_OK;
+  });
+}
+
+extern "C" int wl_paged_sparse_dev(wl_ctx *c, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
+                                   const wl_sparse_opts *o, float scale, float *d_out, int32_t *d_blocks) {
+  if (!c || !p || !r || !o) return fail(WL_E_ARG, "wl_paged_sparse_dev: null argument");
+  wl::PagePool pool;
+  int rc, rows;
+  if ((rc = paged_pool("wl_paged_sparse_dev", p, &pool)) ||
+      (rc = paged_rows("wl_paged_sparse_dev", p, r, false, &rows)) ||
+      (rc = paged_heads("wl_paged_sparse_dev", heads, p->kv_heads, p->head_dim)) ||
+      (rc = paged_sparse("wl_paged_sparse_dev", p, o)))
+    return rc;
+  if (rows && (!d_q || !d_out)) return fail(WL_E_ARG, "wl_paged_sparse_dev: null argument");
+  WL_ON_DEVICE(c);
+  return paged_sparse_attention(c, pool, r, d_q, heads, o, scale, d_out, d_blocks);
+}
+
+// A layer's RoPE, its rows' keys and values into their pages, and their attention.
+static int layer_attention_paged(wl_ctx *c, const wl_layer_desc *L, const LayerPaged &pg, float *q, const float *k,
+                                 const float *v, int rd, double fs, float scale, float *att) {
+  wl::PagePool pool;
+  int rc;
+  if ((rc = paged_pool("wl_layer_paged_dev", pg.p, &pool)) ||
+      (rc = paged_store(c, pool, pg.r, q, L->heads, k, v, wl::page_rope(rd, L->neox, L->rope_base, fs, L->d_rope_freqs), q)))
+    return rc;
+  return pg.sparse ? paged_sparse_attention(c, pool, pg.r, q, L->heads, pg.sparse, scale, att, nullptr)
+                   : paged_attention(c, pool, pg.r, q, L->heads, pg.prefix, scale, att);
+}
+
+extern "C" int wl_layer_paged_dev(wl_ctx *c, const wl_layer_desc *L, float *d_x, const wl_pages *p, const wl_page_rows *r,
+                                  int32_t prefix, const wl_sparse_opts *o) {
+  if (!c || !L || !d_x || !p || !r) return fail(WL_E_ARG, "wl_layer_paged_dev: null argument");
+  wl::PagePool pool;
+  int rc, rows;
+  if ((rc = paged_pool("wl_layer_paged_dev", p, &pool)) || (rc = paged_rows("wl_layer_paged_dev", p, r, true, &rows)) ||
+      (rc = paged_heads("wl_layer_paged_dev", L->heads, p->kv_heads, p->head_dim)) ||
+      (rc = paged_prefix("wl_layer_paged_dev", p, r, prefix)) || (o && (rc = paged_sparse("wl_layer_paged_dev", p, o))))
+    return rc;
+  if (L->kv_heads != p->kv_heads || L->head_dim != p->head_dim)
+    return fail(WL_E_SHAPE, "wl_layer_paged_dev: %d KV heads of %d; the pages hold %d of %d", L->kv_heads, L->head_dim,
+                p->kv_heads, p->head_dim);
+  if (o && prefix) return fail(WL_E_ARG, "wl_layer_paged_dev: a prefix and a choice of pages");
+  if (rows == 0) return fail(WL_E_SHAPE, "wl_layer_paged_dev: bad shape");
+  bool each = true;
+  for (int i = 0; i < r->n && r->rows; i++) each = each && r->rows[i] <= 1;
+  WL_ON_DEVICE(c);
+  const LayerPaged pg{p, r, prefix, o};
+  return layer_run(c, L, d_x, rows, 0, pool.K, pool.V, wl::RowMap{}, nullptr, 0, each, nullptr, &pg);
 }
 
 extern "C" int wl_sample_dev(wl_ctx *c, const float *d_logits, int32_t rows, int64_t n, const wl_sample_params *params,

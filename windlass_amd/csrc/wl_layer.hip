@@ -15,6 +15,7 @@
 #include "wl_frag.h"
 
 #include "wl_device.h"
+#include "wl_rope.h"
 
 #include <math.h>
 
@@ -153,24 +154,6 @@ __global__ __launch_bounds__(1024) void rms_norm_frag_kernel(const float *__rest
                                                              const float *__restrict__ w, float eps, int ord,
                                                              uint16_t *__restrict__ xf) {
   rms_row(x + (int64_t)blockIdx.x * dim, dim, w, eps, true, PutFrag{xf, (int)blockIdx.x, dim, ord});
-}
-
-// The angle of rotated pair i at a position: RopeTable's running product in double
-// (src/Transformer.cs:396-414) taken to step i, divided by the pair's frequency factor when the
-// model has them (rope_freqs.weight, `half` of them). The product is the same sequence for every
-// pair, so a wave runs it once for all its lanes (the trip count `half` is uniform) and each lane
-// keeps the value after its own i steps: every lane gets the bits the sequential table has
-// without a divergent loop of up to 63 dependent multiplies per lane.
-__device__ __forceinline__ void rope_cs(int p, int i, int half, double theta_scale, double freq_scale,
-                                        const float *__restrict__ freqs, float &c, float &s) {
-  double theta = (double)p * freq_scale, mine = theta;
-  for (int k = 1; k < half; k++) {
-    theta *= theta_scale;
-    if (k == i) mine = theta;
-  }
-  const double a = freqs && i < half ? mine / (double)freqs[i] : mine;
-  c = (float)cos(a);
-  s = (float)sin(a);
 }
 
 // Rope (src/Transformer.cs:416-431) on pair i of one head: (2i, 2i+1), or (i, i + n/2) NeoX.

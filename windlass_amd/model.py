@@ -14,8 +14,8 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
-from ._lib import NotSupportedError, ShapeError, check, load
-from .backend import KvOpts, LayerDesc, SampleParams
+from ._lib import ArgumentOutOfRangeError, NotSupportedError, ShapeError, check, load
+from .backend import KvOpts, LayerDesc, PageRows, Pages, SampleParams
 
 _LAYER_TENSORS = ("attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down")
 
@@ -520,3 +520,160 @@ class DeviceBatch:
         finally:
             m.ctx.sync()  # also after a failure: what is queued uses ids and d_u
         return ids[:steps].cpu().numpy().T.tolist()
+
+
+class PagedBatch(DeviceBatch):
+    """A DeviceBatch whose sequences take pages of a pool as they grow, and share those of a common beginning, instead of a
+    slot for the longest context each (wl_layer_paged_dev). `pages` pages of `page` positions for all sequences together,
+    in every layer; a sequence holds up to slot_positions. Without sharing, a step's rows have the bits of the sequence's
+    own step. With sparse (SparseOpts) the steps' rows attend to pages chosen by their bounds; prompts see every position.
+    The pages are fp16 ones, and a model with 4-bit caches or a window is refused."""
+
+    def __init__(self, model, pages, slots, slot_positions, page=64, sparse=None):
+        torch, c = model.torch, model.cfg
+        if model.kv.bits != 16 or model.kv.window:
+            raise NotSupportedError("Pages of a model with %d-bit caches and a window of %d." % (model.kv.bits, model.kv.window))
+        L = load()
+        size = L.wl_page_bytes(page, c.kv_heads, c.head_dim)
+        if not size:
+            raise NotSupportedError("Pages of %d positions of %d heads of %d." % (page, c.kv_heads, c.head_dim))
+        if not (0 < pages < 1 << 31 and slots > 0 and 0 < slot_positions < 1 << 31):
+            raise ShapeError("%d pages, %d sequences of %d positions." % (pages, slots, slot_positions))
+        self.m, self.slots, self.cap, self.page, self.sparse = model, slots, slot_positions, page, sparse
+        width = (slot_positions + page - 1) // page
+        self.K, self.V = (torch.zeros((c.layers, pages * size), dtype=torch.uint8, device=model.dev) for _ in range(2))
+        self.bounds = None
+        if sparse:
+            b = L.wl_page_bounds_bytes(c.kv_heads, c.head_dim)
+            self.bounds = torch.zeros((c.layers, pages * b), dtype=torch.uint8, device=model.dev)
+        self.table = torch.full((slots, width), -1, dtype=torch.int32, device=model.dev)
+        self.desc = [Pages(_ptr(self.K[l]), _ptr(self.V[l]), None if self.bounds is None else _ptr(self.bounds[l]),
+                           _ptr(self.table), pages, page, c.kv_heads, c.head_dim, slots, width) for l in range(c.layers)]
+        self.free_pages = list(range(pages - 1, -1, -1))
+        self.users = [0] * pages               # sequences that hold a page
+        self.held = [[] for _ in range(slots)]  # a sequence's pages
+        self.length = [0] * slots
+        self._bufs = {}
+        torch.cuda.synchronize(model.dev)
+
+    def _need(self, slot, n):
+        """Pages that the sequence lacks for n positions."""
+        return max(0, (n + self.page - 1) // self.page - len(self.held[slot]))
+
+    def _slots(self, slots):
+        if len(set(slots)) != len(slots) or any(not 0 <= s < self.slots for s in slots):
+            raise ArgumentOutOfRangeError("Sequences %s of %d." % (list(slots), self.slots))
+
+    def _grow(self, slots, counts):
+        """Room for `counts` more positions of each sequence, or an error that leaves everything as it was."""
+        self._slots(slots)
+        for s, n in zip(slots, counts):
+            if n <= 0 or self.length[s] + n > self.cap:
+                raise ShapeError("The prompt and reply need %d positions; the context is %d." % (self.length[s] + n, self.cap))
+        need = [self._need(s, self.length[s] + n) for s, n in zip(slots, counts)]
+        if sum(need) > len(self.free_pages):
+            raise ShapeError("%d more pages are needed; %d are free." % (sum(need), len(self.free_pages)))
+        for s, n in zip(slots, need):
+            if n:
+                self._hold(s, self.free_pages[:-n - 1:-1])
+                del self.free_pages[-n:]
+
+    def _hold(self, slot, ids):
+        if not ids:
+            return
+        check(self.m.L.wl_paged_assign_dev(self.m.ctx.handle, ctypes.byref(self.desc[0]), slot, len(self.held[slot]), len(ids),
+                                           (ctypes.c_int32 * len(ids))(*ids)))
+        self.held[slot] += ids
+        for i in ids:
+            self.users[i] += 1
+
+    def share(self, src, dst, positions):
+        """The empty sequence dst begins with the first `positions` (whole pages) of src: the same pages."""
+        self._slots([src, dst])
+        if positions % self.page or not 0 <= positions <= min(self.length[src], self.cap):
+            raise ShapeError("%d positions to share are not whole pages of %d, or more than %d."
+                             % (positions, self.page, self.length[src]))
+        if self.length[dst] or self.held[dst]:
+            raise ShapeError("Sequence %d holds %d positions." % (dst, self.length[dst]))
+        self._hold(dst, self.held[src][:positions // self.page])
+        self.length[dst] = positions
+
+    def release(self, slot):
+        """Forgets a sequence; pages that no other holds are free again."""
+        self._slots([slot])
+        for i in self.held[slot]:
+            self.users[i] -= 1
+            if not self.users[i]:
+                self.free_pages.append(i)
+        self.held[slot], self.length[slot] = [], 0
+
+    def _shared(self, slots):
+        """The positions at the beginning that all of the sequences have in the same pages."""
+        if len(slots) < 2:
+            return 0
+        n = 0
+        for ids in zip(*(self.held[s] for s in slots)):
+            if any(i != ids[0] for i in ids):
+                break
+            n += 1
+        return n * self.page
+
+    def _pass(self, x, slots, counts, prefix, sparse):
+        m, c = self.m, ctypes.c_void_p
+        r = PageRows(slots, [self.length[s] for s in slots], counts)
+        o = ctypes.byref(sparse) if sparse else None
+        m.run_layers(lambda l, d: check(m.L.wl_layer_paged_dev(m.ctx.handle, ctypes.byref(d), c(x.data_ptr()),
+                                                               ctypes.byref(self.desc[l]), ctypes.byref(r), prefix, o)))
+        for s, n in zip(slots, counts):
+            self.length[s] += n
+
+    def prefill(self, slot, tokens):
+        """The prompt of the sequence in `slot` from its current length; the device logits of its last token [1][vocab]."""
+        m, c, T = self.m, ctypes.c_void_p, len(tokens)
+        self._grow([slot], [T])
+        x = self._buf("x", T, m.cfg.embd)
+        check(m.L.wl_embed_dev(m.ctx.handle, m.embd_w.handle, (ctypes.c_int32 * T)(*tokens), T, c(x.data_ptr())))
+        m.embed_scale(x, T)
+        self._pass(x, [slot], [T], 0, None)
+        return self._head(x[T - 1:], 1)
+
+    def step(self, slots, d_ids):
+        """One stacked decode step (DeviceBatch.step); pages that all of the sequences share at their beginning are read
+        once."""
+        m, c, N = self.m, ctypes.c_void_p, len(slots)
+        self._grow(slots, [1] * N)
+        x = self._buf("x", N, m.cfg.embd)
+        check(m.L.wl_embed_dev_ids(m.ctx.handle, m.embd_w.handle, c(d_ids.data_ptr()), N, c(x.data_ptr())))
+        m.embed_scale(x, N)
+        self._pass(x, list(slots), [1] * N, 0 if self.sparse else self._shared(slots), self.sparse)
+        return self._head(x, N)
+
+    def generate(self, prompts, steps, params, u, shared=0):
+        """DeviceBatch.generate; with `shared`, the prompts' first `shared` tokens are the same: whole pages of them run once,
+        in the first sequence, and the others hold its pages. The sequences are then empty before."""
+        N = len(prompts)
+        for p in prompts:
+            if shared < 0 or shared > len(p) or list(p[:shared]) != list(prompts[0][:shared]):
+                raise ShapeError("The prompts' first %d tokens are not the same." % shared)
+        k = min([shared] + [len(p) - 1 for p in prompts]) // self.page * self.page if N > 1 else 0  # each runs a token of its own
+        if N > self.slots:
+            raise ShapeError("%d sequences for %d slots." % (N, self.slots))
+        if k and any(self.length[:N]):
+            raise ShapeError("A shared beginning for sequences that hold positions.")
+        if len(params) != N or np.size(u) != steps * N:
+            raise ShapeError("%d settings and %d numbers for %d sequences of %d tokens." % (len(params), np.size(u), N, steps))
+        for i, p in enumerate(prompts):
+            _fits(len(p), steps, self.length[i], self.cap)
+        need = sum(self._need(i, self.length[i] + len(p) + max(steps - 1, 0)) for i, p in enumerate(prompts))
+        need -= max(0, N - 1) * (k // self.page)
+        if need > len(self.free_pages):
+            raise ShapeError("%d more pages are needed; %d are free." % (need, len(self.free_pages)))
+        if k:
+            try:
+                self.prefill(0, list(prompts[0][:k]))
+                for i in range(1, N):
+                    self.share(0, i, k)
+            except BaseException:
+                self.m.ctx.sync()
+                raise
+        return super().generate([list(p[k:]) for p in prompts], steps, params, u)
