@@ -2090,6 +2090,9 @@ static int paged_sparse(const char *who, const wl_pages *p, const wl_sparse_opts
   return WL_OK;
 }
 
+// Rows of a launch: a (row, head) pair is a workgroup of one of them.
+static int paged_most_rows(int heads) { return std::max(1, (1 << 24) / std::max(heads, 1)); }
+
 // f(rows, first row) for a call's entries, kPgRows and `most` rows at a time; entries without rows are left out.
 template <class F>
 static int each_page_rows(const wl_page_rows *r, int most, const F &f) {
@@ -2136,7 +2139,7 @@ extern "C" int wl_paged_assign_dev(wl_ctx *c, const wl_pages *p, int32_t seq, in
 static int paged_store(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
                        const float *d_k, const float *d_v, const wl::PageRope &rope, float *d_q_out) {
   const int64_t qd = (int64_t)heads * pool.HD, kd = (int64_t)pool.KH * pool.HD;
-  return each_page_rows(r, 1 << 20, [&](const wl::PageRows &R, int r0) -> int {
+  return each_page_rows(r, paged_most_rows(heads), [&](const wl::PageRows &R, int r0) -> int {
     WL_HIP(wl::paged_store_launch(pool, R, heads ? d_q + r0 * qd : nullptr, heads, d_k + r0 * kd, d_v + r0 * kd, rope,
                                   heads ? d_q_out + r0 * qd : nullptr, c->stream), "paged store");
     return WL_OK;
@@ -2174,7 +2177,7 @@ extern "C" int wl_paged_read_dev(wl_ctx *c, const wl_pages *p, int32_t seq, int3
 static int paged_attention(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
                            int prefix, float scale, float *d_out) {
   const int64_t qd = (int64_t)heads * pool.HD;
-  return each_page_rows(r, 1 << 20, [&](const wl::PageRows &R, int r0) -> int {
+  return each_page_rows(r, paged_most_rows(heads), [&](const wl::PageRows &R, int r0) -> int {
     const int64_t floats = wl::paged_attention_scratch_floats(pool, R, heads, prefix, 0);
     if (const int rc = ensure(c, S_ATT, (size_t)floats * sizeof(float))) return rc;
     WL_HIP(wl::paged_attention_launch(pool, R, d_q + r0 * qd, heads, prefix, nullptr, 0, scale, (float *)c->buf[S_ATT],
@@ -2210,7 +2213,7 @@ static int paged_sparse_attention(wl_ctx *c, const wl::PagePool &pool, const wl_
                                   const wl_sparse_opts *o, float scale, float *d_out, int32_t *d_blocks) {
   const int64_t qd = (int64_t)heads * pool.HD;
   const wl::PageSelect s{o->first, o->recent, o->top};
-  return each_page_rows(r, sparse_rows(pool, r, s), [&](const wl::PageRows &R, int r0) -> int {
+  return each_page_rows(r, std::min(sparse_rows(pool, r, s), paged_most_rows(heads)), [&](const wl::PageRows &R, int r0) -> int {
     int rc;
     const size_t blocks = (size_t)R.row0[R.n] * pool.KH * s.most();
     if ((rc = ensure(c, S_SEL, (size_t)wl::paged_select_scratch_bytes(pool, R, s))) ||

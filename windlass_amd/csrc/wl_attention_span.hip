@@ -3,7 +3,7 @@
 // positions Span names).
 #include "wl_attention_span.h"
 
-#include "wl_fmma_codec.h"
+#include "wl_attention_parts.h"
 
 #include <type_traits>
 
@@ -98,13 +98,6 @@ __global__ __launch_bounds__(256) void span_rows_kernel(const float *__restrict_
 // two launches' latency (70B after 4,000: 6.3 and 3.8 us). Measured and not kept: the last workgroup of a row joining its
 // runs (with fences 770 us for the 32 rows; with device-scope stores 66.9 against 61.6, and 41.7 against 35.5 for the long
 // row), records loaded ahead in the join (62.5 -> 66), eight waves a workgroup.
-typedef float sf4 __attribute__((ext_vector_type(4)));
-// A running maximum is raised only by scores more than 2^6 past it, so nearly never after a wave's first tile: the
-// exponentials reach 2^6, and 2^8 of them are fp16 parts (22 bits down to 2^-22 of the row's largest, 2^-33 of it below).
-constexpr float kSpUp = 0x1p8f, kSpPast = 6.f;
-// In the scores' units: finite where those are the smallest there are, so that a lane without a key yet keeps -inf as what
-// raises its maximum.
-__device__ __forceinline__ float past_of(float c2) { return fminf(kSpPast / c2, 3.4028235e38f); }
 constexpr int kSpWaves = 4;
 constexpr int kSpRuns = 256;      // runs of a row at most
 
@@ -137,18 +130,7 @@ __device__ __forceinline__ uint32_t fp16_ones() {
   asm("v_mov_b32 %0, 0x3c003c00" : "=v"(o));
   return o;
 }
-__device__ __forceinline__ fh8 as_fh8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __builtin_bit_cast(fh8, u32x4_t{a, b, c, d});
-}
 __device__ __forceinline__ fh2 scale15(fh2 s) { return s * fh2{(_Float16)-1.5f, (_Float16)-1.5f}; }
-
-// Two probabilities, times kSpUp, as their fp16 parts.
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t &hi, uint32_t &lo) {
-  hi = __builtin_bit_cast(uint32_t, fh2{(_Float16)__builtin_fmaf(a, kSpUp, 0.f), (_Float16)__builtin_fmaf(b, kSpUp, 0.f)});
-  asm("" : "+v"(hi));  // rounded once: the compiler made the halves again for the low parts
-  lo = __builtin_bit_cast(uint32_t, fh2{(_Float16)__builtin_fmaf(a, kSpUp, -half_lo(hi)),
-                                        (_Float16)__builtin_fmaf(b, kSpUp, -half_hi(hi))});  // exact but for their rounding
-}
 
 // Tiles of 4-bit caches. hide(m): bit j set where key j of the lane (keys 16 (j / 4) + 4 kq + j % 4) is not seen:
 // its values become zeros.
@@ -273,14 +255,6 @@ __device__ __forceinline__ float join_parts(float v, bool low) {
   }
   return v + o;
 }
-
-// What sums under the maximum M weigh under a larger one. Scores of -inf alone leave M at -inf and sums of zeros (or NaN, from
-// a NaN score): a factor of zero, also where no other sums have a maximum, and 0 / 0 is such a row's output.
-__device__ __forceinline__ float weight_of(float M, float m, float c2) {
-  return M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((M - m) * c2);
-}
-
-typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));  // at any float's address
 
 // A row's outputs lie in LDS and in the runs' records as the matrix cores leave them: values 16 d + 4 kq + e, for
 // value HD / 16 (4 kq + e) + d of the head. Four of them to their places in the head's row.

@@ -1,74 +1,798 @@
-// wl_paged_attention.hip - attention over KV caches in pages (wl_paged.h).
+// wl_paged_attention.hip - attention over KV caches in pages (wl_paged.h): over all positions of a row's sequence, over a prefix
+// that the rows of many sequences share, and over chosen pages.
+//
+// A column is a (row, query head of the KV head) pair, row * G + head within its entry, its query as two fp16 parts (22 bits of
+// its largest value). S^T = K Q^T and O^T = V^T P^T, the probabilities in two parts as well; a page holds both operands as the
+// matrix cores take them, so that keys and values go from memory (or LDS) to the products as they lie. Rows of few columns take
+// paged_few_kernel (16 columns, the waves one tile of 32 positions in turn), others paged_many_kernel (32 columns a wave, the
+// positions staged in LDS). Both cut long rows in runs, whose outputs, maxima and sums paged_join_kernel adds; a shared prefix is
+// one such launch over the rows of all entries, without a mask, and its runs are added beside those of each entry's own.
 #include "wl_paged.h"
 
+#include "wl_attention_parts.h"
 #include "wl_paged_device.h"
+
+#include <algorithm>
 
 #pragma clang fp contract(off)
 
 namespace wl {
 
-// One wave per row and head, a lane per position for the scores and per channel for the outputs.
-template <int HD>
-__global__ __launch_bounds__(64) void paged_attention_kernel(PagePool P, PageRows R, const float *__restrict__ q, int H,
-                                                             int prefix, const int32_t *__restrict__ blocks, int most,
-                                                             float scale, float *__restrict__ out) {
-  __shared__ float qs[HD];
-  const int h = blockIdx.x, row = blockIdx.y, lane = threadIdx.x, kvh = h / (H / P.KH);
-  const int i = entry_of(R.row0, R.n, row);
-  const int p = R.pos[i] + row - R.row0[i];
-  const int64_t at = ((int64_t)row * H + h) * HD;
-  for (int d = lane; d < HD; d += 64) qs[d] = q[at + d];
-  __syncthreads();
-  float M = -INFINITY, O[HD / 64] = {};
-  double L = 0.0;
-  const int nb = blocks ? most : (p >> P.shift) + 1;
-  for (int b = 0; b < nb; b++) {
-    const int j = blocks ? blocks[((int64_t)row * P.KH + kvh) * most + b] : b;
-    if (j < 0) break;
-    const int id = P.id((j << P.shift) < prefix ? R.seq[0] : R.seq[i], j);
-    if (id < 0) continue;
-    const uint16_t *K = P.K + P.at(id, kvh), *V = P.V + P.at(id, kvh);
-    for (int o0 = 0; o0 < P.page; o0 += 64) {
-      const int off = o0 + lane;
-      const bool in = off < P.page && (j << P.shift) + off <= p;
-      float s = 0.f;
-      if (in)
-        for (int d = 0; d < HD; d++) s += qs[d] * (float)__builtin_bit_cast(_Float16, K[pg_key(off, d, HD)]);
-      s = in ? s * scale : -INFINITY;
-      float m = s;
-      for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-      m = fmaxf(m, M);
-      const float al = M == -INFINITY ? 0.f : expf(M - m), w = s == -INFINITY ? 0.f : expf(s - m);
-      M = m;
-      double l = w;
-      for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x, 64);
-      L = L * al + l;
-      for (int e = 0; e < HD / 64; e++) O[e] *= al;
-      const unsigned long long seen = __ballot(in);
-      for (int x = 0; x < 64; x++)
-        if (seen >> x & 1) {
-          const float wx = __shfl(w, x, 64);
-          for (int e = 0; e < HD / 64; e++)
-            O[e] += wx * (float)__builtin_bit_cast(_Float16, V[pg_val(o0 + x, lane + 64 * e, HD)]);
-        }
-    }
-  }
-  for (int e = 0; e < HD / 64; e++) out[at + lane + 64 * e] = L == 0.0 ? 0.f : (float)((double)O[e] / L);
+typedef float sf16 __attribute__((ext_vector_type(16)));
+
+constexpr int kFewCols = 16, kFewWaves = 4;
+constexpr int kManyWaves = 4, kManyCols = 32 * kManyWaves, kManyUnits = 4;  // units of a step
+constexpr int kPgRuns = 256;  // of a row at most
+constexpr uint32_t kNowhere = 0xfffffff0u;  // the position of a unit that no row sees
+
+// A launch's items: entry i's begin at off[i], column block by column block, `per` tiles or steps each. Its rows' records, a run
+// after the other for each (row, head), begin H * rec[i] records into `part`; alone: a row of one run is the output itself.
+struct PagedPlan {
+  int off[kPgRows + 1], per[kPgRows], rec[kPgRows];
+  int inc, base;  // a row's positions end at pos + row * inc; units before base are not read
+  int alone;
+};
+
+// What a column needs of its query: the factor of its parts, and of its scores in units of log2.
+__device__ __forceinline__ void query_scale(float m, float scale, float &f, float &c2) {
+  float inv;
+  unit_scale(m, f, inv);
+  // c2 > 0: a negative scale negates the query
+  c2 = fmaxf(fabsf(scale) * 1.4426950408889634f * inv, 1.1754944e-38f);
+  f = scale < 0.f ? -f : f;
+  if (scale != scale) c2 = scale;
+}
+__device__ __forceinline__ void query_parts(float x, float f, _Float16 &hi, _Float16 &lo) {
+  const float X = x * f;
+  hi = (_Float16)X;
+  lo = (_Float16)(__builtin_isinf(X) ? 0.f : X - (float)hi);  // an infinity is all in its high part
 }
 
-int64_t paged_attention_scratch_floats(const PagePool &, const PageRows &, int, int, int) { return 0; }
+// Bits 15 and 31 set where a half of w is an infinity or NaN: its exponent's ones carry.
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+
+// Of a lane's eight values of a channel, positions at .. at + 7: those that no column sees (past pb) become zeros, and of those
+// that some do not see (past pa) the infinite and NaN ones; true where one of these was seen by some.
+__device__ __forceinline__ bool clear_unseen(u32x4_t &w, uint32_t at, uint32_t pa, uint32_t pb) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t a = at + 2 * j, b = a + 1;
+    const uint32_t odd = odd_halves(w[j]);
+    const uint32_t all = (a <= pa ? 0xffffu : 0u) | (b <= pa ? 0xffff0000u : 0u);
+    const uint32_t some = (a <= pb ? 0xffffu : 0u) | (b <= pb ? 0xffff0000u : 0u);
+    const uint32_t drop = ((odd >> 15) * 0xffffu & ~all) | ~some;
+    bad |= (odd >> 15) * 0xffffu & ~all & some;
+    w[j] &= ~drop;
+  }
+  return bad != 0;
+}
+
+// ------------------------------------------------------------------------------- few columns
+
+// The keys of a tile are loaded again once its scores are made, and its values once they are multiplied: half a tile is in flight
+// all the time, and a SIMD holds three waves.
+template <int HD>
+struct FewTile {
+  static constexpr int NK = HD / 32, ND = HD / 16;
+  u32x4_t k[2][NK], v[ND];
+  uint32_t up[2];  // the positions of the units' first values
+  // a, b: halves before the tile's two units
+  __device__ __forceinline__ void keys(const PagePool &P, int64_t a, int64_t b, int lane) {
+    const int m = lane & 15, kq = lane >> 4;
+    const uint16_t *kp = P.K + (m < 8 ? a : b) + kq * 64 + (m & 7) * 8;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int i = 0; i < NK; i++)
+        k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(kp + t * 8 * HD + i * 256));
+  }
+  __device__ __forceinline__ void values(const PagePool &P, int64_t a, int64_t b, int lane) {
+    const int m = lane & 15, kq = lane >> 4;
+    const uint16_t *vp = P.V + (kq < 2 ? a : b) + (kq & 1) * 8 * HD + m * 8;
+#pragma unroll
+    for (int d = 0; d < ND; d++) v[d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(vp + d * 128));
+  }
+};
+
+template <int HD, bool SPARSE>
+__global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_kernel(PagePool P, PageRows R, PagedPlan U,
+                                                                      const float *__restrict__ q, int G,
+                                                                      const int32_t *__restrict__ blocks, int nblocks,
+                                                                      float scale, float *__restrict__ part,
+                                                                      float *__restrict__ out) {
+  constexpr int NK = HD / 32, ND = HD / 16, W = kFewWaves;
+  __shared__ sf4 so[W][kFewCols][HD / 4 + 1];
+  __shared__ float sm[W][kFewCols], sc2[kFewCols];
+  __shared__ double sl[W][kFewCols];
+  __shared__ fh8 qs[2][NK][64];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kq = lane >> 4, KH = P.KH, H = G * KH, us = P.shift - 4;
+  const int kvh = blockIdx.x % KH, item = blockIdx.x / KH;
+  int i, row0, T, pos, cb, run, runs, per;
+  if constexpr (SPARSE) {
+    const int nb = (G + kFewCols - 1) / kFewCols;
+    runs = U.off[1];
+    per = U.per[0];
+    run = item % runs;
+    cb = item / runs % nb;
+    row0 = item / runs / nb;
+    i = entry_of(R.row0, R.n, row0);
+    T = 1;
+    pos = R.pos[i] + row0 - R.row0[i];
+  } else {
+    i = entry_of(U.off, R.n, item);
+    row0 = R.row0[i];
+    T = R.rows(i);
+    pos = R.pos[i];
+    per = U.per[i];
+    runs = (U.off[i + 1] - U.off[i]) / ((T * G + kFewCols - 1) / kFewCols);
+    run = (item - U.off[i]) % runs;
+    cb = (item - U.off[i]) / runs;
+  }
+  const int NC = T * G, c0 = cb * kFewCols, c = c0 + col < NC ? c0 + col : NC - 1;
+  const int t = c / G, h = kvh * G + c % G;
+  const int p = pos + t * U.inc, pa = pos + c0 / G * U.inc;
+  const int pb = pos + (c0 + kFewCols - 1 < NC ? c0 + kFewCols - 1 : NC - 1) / G * U.inc;
+  int nu;  // units
+  if constexpr (SPARSE) nu = ((pos >> P.shift) + 1 < nblocks ? (pos >> P.shift) + 1 : nblocks) << us;
+  else nu = (pb >> 4) - U.base + 1;
+  const int nt = (nu + 1) / 2, i0 = run * per, i1 = i0 + per < nt ? i0 + per : nt;
+
+  // The wave's units, 64 (32 tiles) at a time: lane 2 k + x has unit x of its k-th tile.
+  int64_t off;
+  uint32_t up;
+  auto units = [&](int first) __attribute__((always_inline)) {
+    const int tile = first + W * (lane >> 1), j = 2 * tile + (lane & 1);
+    off = 0;
+    up = kNowhere;
+    if (tile >= i1 || j >= nu) return;
+    int b, u;
+    if constexpr (SPARSE) {
+      b = blocks[((int64_t)row0 * KH + kvh) * nblocks + (j >> us)];
+      if (b < 0) return;
+      u = (b << us) + (j & ((1 << us) - 1));
+    } else {
+      u = U.base + j;
+      b = u >> us;
+    }
+    const int id = P.id(R.seq[i], b);
+    if (id < 0) return;
+    off = P.at(id, kvh) + (int64_t)(u & ((1 << us) - 1)) * 16 * HD;
+    up = 16u * (uint32_t)u;
+  };
+  auto lane64 = [](int64_t v, int l) __attribute__((always_inline)) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, l));
+  };
+  FewTile<HD> a;
+  int64_t oa, ob;  // the next tile's units
+  uint32_t ua, ub;
+  auto next_tile = [&](int k) __attribute__((always_inline)) {
+    oa = lane64(off, 2 * k);
+    ob = lane64(off, 2 * k + 1);
+    ua = (uint32_t)__builtin_amdgcn_readlane((int)up, 2 * k);
+    ub = (uint32_t)__builtin_amdgcn_readlane((int)up, 2 * k + 1);
+  };
+  int tile = i0 + wv, k = 0;
+  units(tile);
+  if (tile < i1) {
+    next_tile(0);
+    a.keys(P, oa, ob, lane);
+    a.values(P, oa, ob, lane);
+  }
+
+  // the columns' parts: a wave makes those of the steps wv, wv + W, ..; all read them from LDS
+  float c2;
+  {
+    const float *qp = q + ((int64_t)(row0 + t) * H + h) * HD + kq * 8;
+    sf4 x[2 * NK];
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2 * NK; e++) x[e] = *reinterpret_cast<const f4a4 *>(qp + e / 2 * 32 + e % 2 * 4);
+#pragma unroll
+    for (int e = 0; e < 2 * NK; e++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) m = fabsf(x[e][j]) < INFINITY ? fmaxf(m, fabsf(x[e][j])) : m;
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    float f;
+    query_scale(m, scale, f, c2);
+#pragma unroll
+    for (int s = 0; s < NK; s++) {
+      if (s % W != wv) continue;  // uniform
+      fh8 a, b;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        _Float16 hi, lo;
+        query_parts(x[2 * s + e / 4][e % 4], f, hi, lo);
+        a[e] = hi;
+        b[e] = lo;
+      }
+      qs[0][s][lane] = a;
+      qs[1][s][lane] = b;
+    }
+  }
+  __syncthreads();
+  sf4 O[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) O[d] = sf4{0.f, 0.f, 0.f, 0.f};
+  float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
+  const float past = past_of(c2);
+  double L = 0.0;
+#pragma unroll 1
+  for (; tile < i1; tile += W) {
+    a.up[0] = ua;
+    a.up[1] = ub;
+    const bool more = tile + W < i1;  // uniform
+    if (more) {
+      if (++k == 32) {
+        k = 0;
+        units(tile + W);
+      }
+      next_tile(k);
+    }
+    fh8 qh[NK], ql[NK];  // read again for each tile: in registers they were spilled
+#pragma unroll
+    for (int s = 0; s < NK; s++) {
+      ql[s] = qs[1][s][lane];
+      qh[s] = qs[0][s][lane];
+    }
+    sf4 S[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      S[x] = sf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NK; s++) {
+        S[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.k[x][s]), ql[s], S[x], 0, 0, 0);
+        S[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.k[x][s]), qh[s], S[x], 0, 0, 0);
+      }
+    }
+    const uint32_t at = (kq >> 1 ? a.up[1] : a.up[0]) + 8 * (kq & 1);  // of the lane's eight positions
+    bool bad = false;
+    if (a.up[0] + 15 > (uint32_t)pa || a.up[1] + 15 > (uint32_t)pa) {  // uniform: some column does not see every position
+      asm volatile("");  // a branch, not selects in every tile
+#pragma unroll
+      for (int j = 0; j < 8; j++) S[j >> 2][j & 3] = at + j > (uint32_t)p ? -INFINITY : S[j >> 2][j & 3];
+#pragma unroll
+      for (int d = 0; d < ND; d++) bad |= clear_unseen(a.v[d], at, pa, pb);
+      bad = __any(bad);
+    }
+    float mt = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
+                     fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
+    if (__any(mt > top)) {
+      mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      const bool raise = mt > top;
+      const float al = raise ? __builtin_amdgcn_exp2f((M - mt) * c2) : 1.f;
+      L *= (double)al;
+#pragma unroll
+      for (int d = 0; d < ND; d++) O[d] *= al;
+      M = raise ? mt : M;
+      top = M + past;
+    }
+    const float Mu = M == -INFINITY ? 0.f : M;  // no position of this column yet: every score is -inf
+    float e[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f((S[j >> 2][j & 3] - Mu) * c2);
+    float ts = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    if (__any(ts != ts)) {  // past an infinity the low parts' product means nothing: a score of -inf may be NaN here
+      asm volatile("");
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        sf4 A1 = sf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NK; s++)
+          A1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.k[x][s]), qh[s], A1, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; j++) e[4 * x + j] = A1[j] == -INFINITY && S[x][j] != S[x][j] ? 0.f : e[4 * x + j];
+      }
+      ts = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    }
+    if (more) a.keys(P, oa, ob, lane);
+    L += (double)ts;
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) split_pair(e[2 * j], e[2 * j + 1], ph[j], pl[j]);
+    const fh8 eh = as_fh8(ph[0], ph[1], ph[2], ph[3]), el = as_fh8(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+    for (int d = 0; d < ND; d++) O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.v[d]), el, O[d], 0, 0, 0);
+#pragma unroll
+    for (int d = 0; d < ND; d++) O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.v[d]), eh, O[d], 0, 0, 0);
+    if (bad) {  // infinite and NaN values into the columns that see them
+      for (int x = 0; x < 32; x++) {
+        const uint32_t w = (x >> 4 ? a.up[1] : a.up[0]) + (x & 15);
+        if (w <= (uint32_t)pa || w > (uint32_t)pb) continue;  // uniform
+        const uint16_t *vp = P.V + P.at(P.id(R.seq[i], (int)(w >> P.shift)), kvh);
+        const int o = (int)(w & (P.page - 1));
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint16_t y = vp[pg_val(o, 16 * d + 4 * kq + j, HD)];
+            if ((y & 0x7c00u) == 0x7c00u && w <= (uint32_t)p) O[d][j] += (float)__builtin_bit_cast(_Float16, y);
+          }
+      }
+    }
+    if (more) a.values(P, oa, ob, lane);
+  }
+  // the waves' sums under their largest maximum
+  L += __shfl_xor(L, 16, 64);
+  L += __shfl_xor(L, 32, 64);
+#pragma unroll
+  for (int d = 0; d < ND; d++) so[wv][col][4 * d + kq] = O[d];
+  if (kq == 0) {
+    sm[wv][col] = M;
+    sl[wv][col] = L;
+    sc2[col] = c2;
+  }
+  __syncthreads();
+  const bool whole = U.alone && runs == 1;
+  for (int e = threadIdx.x; e < kFewCols * HD / 4; e += 64 * W) {
+    const int g = e / (HD / 4), four = e % (HD / 4), cc = c0 + g;
+    if (cc >= NC) break;
+    float m = sm[0][g];
+#pragma unroll
+    for (int w = 1; w < W; w++) m = fmaxf(m, sm[w][g]);
+    sf4 o = {0.f, 0.f, 0.f, 0.f};
+    double l = 0.0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const float f = weight_of(sm[w][g], m, sc2[g]);
+      o += so[w][g][four] * f;
+      l += sl[w][g] * (double)f;
+    }
+    const int64_t at = (int64_t)(cc / G) * H + kvh * G + cc % G, row = (int64_t)row0 * H + at;
+    if (whole) {
+      const double r = (1.0 / kSpUp) / l;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = l == 0.0 ? 0.f : (float)((double)o[j] * r);
+      *reinterpret_cast<f4a4 *>(out + row * HD + 4 * four) = o;
+    } else {
+      const int64_t from = SPARSE ? (int64_t)row0 * H * runs : (int64_t)U.rec[i] * H;
+      float *rec = part + (from + at * runs + run) * (HD + 4);
+      *reinterpret_cast<sf4 *>(rec + 4 * four) = o;
+      if (four == 0) {
+        rec[HD] = m;
+        rec[HD + 1] = sc2[g];
+        *reinterpret_cast<double *>(rec + HD + 2) = l;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- many columns
+
+// 16 bytes a lane from memory to LDS, lane after lane from `to` on; complete after landed(). The compiler's own form made
+// every read of LDS after it wait for it, also reads of the buffer before.
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
+__device__ __forceinline__ void to_lds(const uint16_t *from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <int HD>
+__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool P, PageRows R, PagedPlan U,
+                                                                        const float *__restrict__ q, int G, float scale,
+                                                                        float *__restrict__ part, float *__restrict__ out) {
+  constexpr int NK = HD / 16, ND = HD / 32, UN = 16 * HD;  // halves of a unit
+  __shared__ __attribute__((aligned(1024))) uint16_t lk[2][kManyUnits * UN], lv[2][kManyUnits * UN];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hf = lane >> 5, col = lane & 31, KH = P.KH, H = G * KH, us = P.shift - 4;
+  const int kvh = blockIdx.x % KH, item = blockIdx.x / KH;
+  const int i = entry_of(U.off, R.n, item), row0 = R.row0[i], T = R.rows(i), pos = R.pos[i], per = U.per[i];
+  const int64_t NC = (int64_t)T * G;
+  const int nz = (int)((NC + kManyCols - 1) / kManyCols), runs = (U.off[i + 1] - U.off[i]) / nz;
+  const int run = (item - U.off[i]) % runs, r = (item - U.off[i]) / runs;
+  // longest and shortest rows in turn: the workgroups that share a CU (the grid's halves) add up
+  const int z = r < (nz + 1) / 2 ? nz - 1 - r : r - (nz + 1) / 2;
+  const int64_t z0 = (int64_t)z * kManyCols, w0 = z0 + 32 * wv, u = w0 + col, uc = u < NC ? u : NC - 1;
+  auto position = [&](int64_t c) __attribute__((always_inline)) { return pos + (int)((c < NC ? c : NC - 1) / G) * U.inc; };
+  const int t = (int)(uc / G), h = kvh * G + (int)(uc % G), p = pos + t * U.inc;
+  const int pa = position(w0), pb = position(w0 + 31), last = position(z0 + kManyCols - 1);
+  const bool idle = w0 >= NC;
+  const int nu = (last >> 4) - U.base + 1, ns = (nu + kManyUnits - 1) / kManyUnits;
+  const int i0 = run * per, i1 = i0 + per < ns ? i0 + per : ns;
+
+  // The pages of 16 steps: lane l has unit l of theirs; those of the 16 after them are loaded ahead.
+  auto page_of = [&](int first) __attribute__((always_inline)) {
+    const int j = kManyUnits * first + lane;
+    return j < nu && first < i1 ? P.id(R.seq[i], (U.base + j) >> us) : -1;
+  };
+  int ids = page_of(i0), ahead = page_of(i0 + 16);
+  uint64_t there = __ballot(ids >= 0);
+  // step s into buffer b, a unit a wave; returns which units are there
+  auto stage = [&](int b, int s) __attribute__((always_inline)) {
+    const int x = s - i0;
+    if (x && (x & 15) == 0) {  // uniform
+      ids = ahead;
+      ahead = page_of(s + 16);
+      there = __ballot(ids >= 0);
+    }
+    const int l = (x & 15) * kManyUnits, id = __builtin_amdgcn_readlane(ids, l + wv);
+    const int unit = U.base + kManyUnits * s + wv;
+    const int64_t off = P.at(id < 0 ? 0 : id, kvh) + (int64_t)(unit & ((1 << us) - 1)) * UN;
+    // keys lie in LDS as [HD / 8][16 rows of the products][8]
+    const uint16_t *kp = P.K + off + (lane >> 3 & 1) * 8 * HD + (lane >> 4) * 64 + (lane & 7) * 8;
+    const uint16_t *vp = P.V + off + lane * 8;
+    const uint32_t ko = (uint32_t)(uintptr_t)(lds_u16 *)(lk[b] + wv * UN);
+    const uint32_t vo = (uint32_t)(uintptr_t)(lds_u16 *)(lv[b] + wv * UN);
+#pragma unroll
+    for (int c = 0; c < UN / 512; c++) {
+      to_lds(kp + c * 256, ko + c * 1024);
+      to_lds(vp + c * 512, vo + c * 1024);
+    }
+    return (int)(there >> l) & 15;
+  };
+  int have = i0 < i1 ? stage(0, i0) : 0;
+  // the columns' parts, in operand order: k = 16 i + 8 hf + 0..7
+  fh8 qh[NK], ql[NK];
+  float c2;
+  {
+    const float *qp = q + ((int64_t)(row0 + t) * H + h) * HD + 8 * hf;
+    float m = 0.f;
+#pragma unroll
+    for (int s = 0; s < NK; s++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float a = fabsf(qp[16 * s + j]);
+        m = a < INFINITY ? fmaxf(m, a) : m;
+      }
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    float f;
+    query_scale(m, scale, f, c2);
+#pragma unroll
+    for (int s = 0; s < NK; s++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        _Float16 hi, lo;
+        query_parts(qp[16 * s + j], f, hi, lo);
+        qh[s][j] = hi;
+        ql[s][j] = lo;
+      }
+  }
+  sf16 O[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) O[d][e] = 0.f;
+  float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
+  const float past = past_of(c2);
+  double L = 0.0;
+  landed();
+  __syncthreads();
+#pragma unroll 1
+  for (int s = i0; s < i1; s++) {
+    const int b = (s - i0) & 1, here = have;
+    if (s + 1 < i1) have = stage(b ^ 1, s + 1);
+    const uint32_t s0 = 16u * (uint32_t)(U.base + kManyUnits * s);  // the step's first position
+    const bool on = !idle && s0 <= (uint32_t)pb;
+    if (on) {
+      float ts = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        const uint16_t *kb = lk[b] + (2 * x + (col >> 4)) * UN + hf * 128 + (col & 15) * 8;
+        sf16 S;
+#pragma unroll
+        for (int e = 0; e < 16; e++) S[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+          const fh8 a = *reinterpret_cast<const fh8 *>(kb + 256 * k);
+          S = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], S, 0, 0, 0);
+          S = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], S, 0, 0, 0);
+        }
+        const uint32_t p0 = s0 + 32 * x;
+        const bool cut = p0 + 31 > (uint32_t)pa || (here >> (2 * x) & 3) != 3;  // uniform: some column does not see all
+        uint32_t up[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) up[k] = here >> (2 * x + k) & 1 ? p0 + 16 * k : kNowhere;
+        if (cut) {
+          asm volatile("");
+#pragma unroll
+          for (int e = 0; e < 16; e++) S[e] = up[e >> 3] + 8 * hf + (e & 7) > (uint32_t)p ? -INFINITY : S[e];
+        }
+        float mt = S[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) mt = fmaxf(mt, S[e]);
+        if (__any(mt > top)) {
+          mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+          const bool raise = mt > top;
+          const float al = raise ? __builtin_amdgcn_exp2f((M - mt) * c2) : 1.f;
+          L *= (double)al;
+          ts *= al;
+#pragma unroll
+          for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) O[d][e] *= al;
+          M = raise ? mt : M;
+          top = M + past;
+        }
+        const float Mu = M == -INFINITY ? 0.f : M;  // no position of this column yet: every score is -inf
+        float tx[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const float w = __builtin_amdgcn_exp2f((S[e] - Mu) * c2);
+          tx[e & 3] += w;
+          S[e] = w;
+        }
+        float tt = (tx[0] + tx[1]) + (tx[2] + tx[3]);
+        if (__any(tt != tt)) {  // past an infinity the low parts' product means nothing: a score of -inf may be NaN here
+          asm volatile("");
+          sf16 A;
+#pragma unroll
+          for (int e = 0; e < 16; e++) A[e] = 0.f;
+#pragma unroll
+          for (int k = 0; k < NK; k++)
+            A = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kb + 256 * k), qh[k], A, 0, 0, 0);
+          tt = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            S[e] = A[e] == -INFINITY && S[e] != S[e] ? 0.f : S[e];
+            tt += S[e];
+          }
+        }
+        ts += tt;
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) split_pair(S[8 * k + 2 * e], S[8 * k + 2 * e + 1], ph[e], pl[e]);
+          const fh8 eh = as_fh8(ph[0], ph[1], ph[2], ph[3]), el = as_fh8(pl[0], pl[1], pl[2], pl[3]);
+          const uint16_t *vb = lv[b] + (2 * x + k) * UN + hf * 8 * HD + col * 8;
+          u32x4_t a[ND];
+#pragma unroll
+          for (int d = 0; d < ND; d++) a[d] = *reinterpret_cast<const u32x4_t *>(vb + 256 * d);
+          if (cut) {
+            asm volatile("");
+#pragma unroll
+            for (int d = 0; d < ND; d++) bad |= clear_unseen(a[d], up[k] + 8 * hf, pa, pb);
+          }
+#pragma unroll
+          for (int d = 0; d < ND; d++) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fh8, a[d]), eh, O[d], 0, 0, 0);
+#pragma unroll
+          for (int d = 0; d < ND; d++) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fh8, a[d]), el, O[d], 0, 0, 0);
+        }
+        if (__any(bad)) {  // infinite and NaN values into the columns that see them
+          for (int y = 0; y < 32; y++) {
+            const uint32_t w = (y >> 4 ? up[1] : up[0]) + (y & 15);
+            if (w <= (uint32_t)pa || w > (uint32_t)pb) continue;  // uniform
+            const uint16_t *vp = lv[b] + (2 * x + (y >> 4)) * UN;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                const uint16_t o = vp[pg_val(y & 15, 32 * d + 8 * (e >> 2) + 4 * hf + (e & 3), HD)];
+                if ((o & 0x7c00u) == 0x7c00u && w <= (uint32_t)p) O[d][e] += (float)__builtin_bit_cast(_Float16, o);
+              }
+          }
+        }
+      }
+      L += (double)ts;
+    }
+    landed();
+    __syncthreads();  // the next step is there, and this one read
+  }
+  L += __shfl_xor(L, 32, 64);
+  if (u >= NC) return;
+  const int64_t at = (int64_t)t * H + h;
+  const bool whole = U.alone && runs == 1;
+  float *op = whole ? out + ((int64_t)row0 * H + at) * HD : part + ((int64_t)U.rec[i] * H + at * runs + run) * (HD + 4);
+  const double f = whole ? 1.0 / L / kSpUp : 1.0;
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      sf4 o;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = whole && L == 0.0 ? 0.f : (float)((double)O[d][4 * e + j] * f);
+      *reinterpret_cast<f4a4 *>(op + 32 * d + 8 * e + 4 * hf) = o;
+    }
+  if (!whole && hf == 0) {
+    op[HD] = M;
+    op[HD + 1] = c2;
+    *reinterpret_cast<double *>(op + HD + 2) = L;
+  }
+}
+
+// ------------------------------------------------------------------------------- runs
+
+// The runs of a row of each entry (1 and alone: the output itself), where its records are, and the prefix' runs of every row.
+struct PagedRuns {
+  int n[kPgRows], rec[kPgRows];
+  int pre, pre_rec, alone, sparse;
+};
+
+// The records of a row's runs under their largest maximum. A workgroup per (row, head): the runs' factors once, into LDS; then
+// HD / 4 threads to a record, the records over the groups in turn, each group's sum in order and the groups' in order.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(const float *__restrict__ part, int H, PageRows R, PagedRuns U,
+                                                         float *__restrict__ out) {
+  constexpr int TH = HD / 4, NG = 256 / TH;
+  __shared__ float f[kPgRuns], sm[4];
+  __shared__ double sl[4];
+  __shared__ sf4 so[NG][TH];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, i = U.sparse ? 0 : entry_of(R.row0, R.n, (int)(row / H));
+  const int own = U.n[i], n = U.pre + own;
+  if (own == 1 && U.alone) return;
+  const float *pre = part + ((int64_t)U.pre_rec * H + row * U.pre) * (HD + 4);
+  const float *ours = part + ((int64_t)U.rec[i] * H + (row - (U.sparse ? 0 : (int64_t)R.row0[i] * H)) * own) * (HD + 4);
+  auto record = [&](int k) { return k < U.pre ? pre + k * (HD + 4) : ours + (k - U.pre) * (HD + 4); };
+  static_assert(kPgRuns == 256, "a thread per run");
+  const float *mine = record(tid < n ? tid : n - 1);
+  const float m1 = mine[HD], c2 = mine[HD + 1];
+  const double l1 = *reinterpret_cast<const double *>(mine + HD + 2);
+  float m = wave_max_f(m1);
+  if ((tid & 63) == 0) sm[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  const float f1 = tid < n ? weight_of(m1, m, c2) : 0.f;
+  f[tid] = f1;
+  const double l = wave_sum_d(tid < n ? l1 * (double)f1 : 0.0);
+  if ((tid & 63) == 0) sl[tid >> 6] = l;
+  __syncthreads();
+  const int g = tid / TH, x = tid % TH;
+  sf4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int j = g; j < n; j += 4 * NG) {
+    sf4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const sf4 *>(record(j + k * NG < n ? j + k * NG : j) + 4 * x);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (j + k * NG < n) o += v[k] * f[j + k * NG];
+  }
+  so[g][x] = o;
+  __syncthreads();
+  if (tid < TH) {
+    sf4 s = so[0][tid];
+#pragma unroll
+    for (int k = 1; k < NG; k++) s += so[k][tid];
+    const double all = (sl[0] + sl[1]) + (sl[2] + sl[3]), r = (1.0 / kSpUp) / all;
+#pragma unroll
+    for (int e = 0; e < 4; e++) s[e] = all == 0.0 ? 0.f : (float)((double)s[e] * r);
+    *reinterpret_cast<f4a4 *>(out + row * HD + 4 * tid) = s;
+  }
+}
+
+// ------------------------------------------------------------------------------- plans
+
+static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Columns that paged_few_kernel takes.
+static bool is_few(int64_t columns) { return columns <= 64; }
+
+// Tiles of each run of a row of n tiles, of `units` workgroups a run (a rule on the entry alone).
+static int few_per(int n, int units) {
+  if (n <= 16) return n;
+  const int64_t all = (int64_t)n * units;
+  int64_t per = 4 * kFewWaves, one = (all + 255) / 256, two = (all + 511) / 512;
+  if (n <= 160) per = one < kFewWaves ? kFewWaves : one < per ? one : per;
+  per = per < two ? two : per;
+  const int most = ceil_div(n, kPgRuns / 2);
+  return per < most ? most : (int)per;
+}
+
+// Steps of each run of an entry whose longest columns take n steps, in nz workgroups of columns a KV head.
+static int many_per(int n, int64_t wgs) {
+  int64_t S = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
+  S = S > n ? n : S;
+  S = S > kPgRuns / 2 ? kPgRuns / 2 : S;
+  return ceil_div(n, S);
+}
+
+// The launches of a call: the prefix (few or many columns), the entries of few columns, those of many.
+struct PagedLaunches {
+  PagedPlan pre, few, many;
+  PageRows all;  // the rows of the prefix, as one entry
+  bool pre_few = false;
+  PagedRuns runs;
+  int records = 0;  // of a head
+};
+
+static void paged_launches(const PagePool &p, const PageRows &r, int H, int prefix, int chosen_pages, PagedLaunches &L) {
+  const int G = H / p.KH, rows = r.row0[r.n], base = prefix / kPgUnit;
+  L.runs.pre = L.runs.pre_rec = 0;
+  L.runs.alone = L.few.alone = L.many.alone = !prefix;
+  L.runs.sparse = chosen_pages > 0;
+  L.few.inc = L.many.inc = 1;
+  L.few.base = L.many.base = base;
+  L.few.off[0] = L.many.off[0] = 0;
+  if (chosen_pages) {  // rows one by one, all with as many runs
+    const int n = ceil_div((int64_t)chosen_pages << (p.shift - 4), 2);
+    L.few.per[0] = few_per(n, p.KH * ceil_div(G, kFewCols));
+    L.few.off[1] = L.runs.n[0] = ceil_div(n, L.few.per[0]);
+    L.few.rec[0] = L.runs.rec[0] = 0;
+    if (L.runs.n[0] > 1) L.records = rows * L.runs.n[0];
+    return;
+  }
+  if (prefix) {
+    const int64_t NC = (int64_t)rows * G;
+    L.all.n = 1;
+    L.all.seq[0] = r.seq[0];
+    L.all.pos[0] = prefix - 1;
+    L.all.row0[0] = 0;
+    L.all.row0[1] = rows;
+    L.pre_few = is_few(NC);
+    const int blocks = ceil_div(NC, L.pre_few ? kFewCols : kManyCols);
+    const int n = ceil_div(prefix / kPgUnit, L.pre_few ? 2 : kManyUnits);
+    L.pre.per[0] = L.pre_few ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
+    L.runs.pre = ceil_div(n, L.pre.per[0]);
+    L.pre.off[0] = L.pre.inc = L.pre.base = L.pre.rec[0] = L.pre.alone = 0;
+    L.pre.off[1] = L.runs.pre * blocks;
+    L.records = rows * L.runs.pre;
+  }
+  for (int i = 0; i < r.n; i++) {
+    const int T = r.rows(i);
+    L.few.off[i + 1] = L.few.off[i];
+    L.many.off[i + 1] = L.many.off[i];
+    L.few.rec[i] = L.many.rec[i] = L.runs.rec[i] = L.records;
+    L.runs.n[i] = 1;
+    if (!T) continue;
+    const int64_t NC = (int64_t)T * G;
+    const int units = ((r.pos[i] + T - 1) >> 4) - base + 1;
+    const bool f = is_few(NC);
+    PagedPlan &U = f ? L.few : L.many;
+    const int blocks = ceil_div(NC, f ? kFewCols : kManyCols), n = ceil_div(units, f ? 2 : kManyUnits);
+    U.per[i] = f ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
+    L.runs.n[i] = ceil_div(n, U.per[i]);
+    U.off[i + 1] += L.runs.n[i] * blocks;
+    if (L.runs.n[i] > 1 || prefix) L.records += T * L.runs.n[i];
+  }
+}
+
+// Pages of a choice that any row of a call has: of a short context fewer than the choice takes.
+static int chosen(const PagePool &p, const PageRows &r, int most) {
+  int n = 1;
+  for (int i = 0; i < r.n; i++)
+    if (r.rows(i)) n = std::max(n, ((r.pos[i] + r.rows(i) - 1) >> p.shift) + 1);
+  return std::min(n, most);
+}
+
+int64_t paged_attention_scratch_floats(const PagePool &p, const PageRows &r, int H, int prefix, int most) {
+  if (r.row0[r.n] <= 0) return 0;
+  PagedLaunches L;
+  paged_launches(p, r, H, prefix, most ? chosen(p, r, most) : 0, L);
+  return (int64_t)L.records * H * (p.HD + 4);
+}
+
+template <int HD>
+static hipError_t paged_attend(const PagePool &p, const PageRows &r, const float *q, int H, int prefix, const int32_t *blocks,
+                               int most, float scale, float *part, float *out, hipStream_t st) {
+  PagedLaunches L;
+  paged_launches(p, r, H, prefix, most ? chosen(p, r, most) : 0, L);
+  const int G = H / p.KH, rows = r.row0[r.n];
+  hipError_t e = hipSuccess;
+  auto few = [&](const PageRows &R, const PagedPlan &U, int items) {
+    hipLaunchKernelGGL((paged_few_kernel<HD, false>), dim3((unsigned)items * p.KH), dim3(64 * kFewWaves), 0, st, p, R, U, q,
+                       G, nullptr, 0, scale, part, out);
+    e = hipGetLastError();
+  };
+  auto many = [&](const PageRows &R, const PagedPlan &U, int items) {
+    hipLaunchKernelGGL(paged_many_kernel<HD>, dim3((unsigned)items * p.KH), dim3(64 * kManyWaves), 0, st, p, R, U, q, G,
+                       scale, part, out);
+    e = hipGetLastError();
+  };
+  if (blocks) {
+    const int64_t items = (int64_t)rows * ceil_div(G, kFewCols) * L.few.off[1];
+    hipLaunchKernelGGL((paged_few_kernel<HD, true>), dim3((unsigned)(items * p.KH)), dim3(64 * kFewWaves), 0, st, p, r, L.few,
+                       q, G, blocks, most, scale, part, out);
+    e = hipGetLastError();
+  } else {
+    if (prefix) (L.pre_few ? few(L.all, L.pre, L.pre.off[1]) : many(L.all, L.pre, L.pre.off[1]));
+    if (e == hipSuccess && L.many.off[r.n]) many(r, L.many, L.many.off[r.n]);
+    if (e == hipSuccess && L.few.off[r.n]) few(r, L.few, L.few.off[r.n]);
+  }
+  if (e != hipSuccess || !L.records) return e;
+  hipLaunchKernelGGL(paged_join_kernel<HD>, dim3((unsigned)((int64_t)rows * H)), dim3(256), 0, st, part, H, r, L.runs, out);
+  return hipGetLastError();
+}
 
 hipError_t paged_attention_launch(const PagePool &p, const PageRows &r, const float *q, int H, int prefix,
-                                  const int32_t *blocks, int most, float scale, float *, float *out, hipStream_t st) {
-  const int rows = r.row0[r.n];
-  if (rows <= 0) return hipSuccess;
-  if (p.HD == 64)
-    hipLaunchKernelGGL(paged_attention_kernel<64>, dim3(H, rows), dim3(64), 0, st, p, r, q, H, prefix, blocks, most, scale,
-                       out);
-  else
-    hipLaunchKernelGGL(paged_attention_kernel<128>, dim3(H, rows), dim3(64), 0, st, p, r, q, H, prefix, blocks, most, scale,
-                       out);
-  return hipGetLastError();
+                                  const int32_t *blocks, int most, float scale, float *scratch, float *out, hipStream_t st) {
+  if (r.row0[r.n] <= 0) return hipSuccess;
+  return p.HD == 64 ? paged_attend<64>(p, r, q, H, prefix, blocks, most, scale, scratch, out, st)
+                    : paged_attend<128>(p, r, q, H, prefix, blocks, most, scale, scratch, out, st);
 }
 
 }  // namespace wl
