@@ -690,18 +690,18 @@ struct PagedLaunches {
   int records = 0;  // of a head
 };
 
-static void paged_launches(const PagePool &p, const PageRows &r, int H, int prefix, int chosen_pages, PagedLaunches &L) {
+// most, chosen: the pages that a row may take, and those that any row of the call has.
+static void paged_launches(const PagePool &p, const PageRows &r, int H, int prefix, int most, int chosen, PagedLaunches &L) {
   const int G = H / p.KH, rows = r.row0[r.n], base = prefix / kPgUnit;
   L.runs.pre = L.runs.pre_rec = 0;
   L.runs.alone = L.few.alone = L.many.alone = !prefix;
-  L.runs.sparse = chosen_pages > 0;
+  L.runs.sparse = most > 0;
   L.few.inc = L.many.inc = 1;
   L.few.base = L.many.base = base;
   L.few.off[0] = L.many.off[0] = 0;
-  if (chosen_pages) {  // rows one by one, all with as many runs
-    const int n = ceil_div((int64_t)chosen_pages << (p.shift - 4), 2);
-    L.few.per[0] = few_per(n, p.KH * ceil_div(G, kFewCols));
-    L.few.off[1] = L.runs.n[0] = ceil_div(n, L.few.per[0]);
+  if (most) {  // rows one by one, cut by a rule on the choice alone, all with as many runs
+    L.few.per[0] = few_per(ceil_div((int64_t)most << (p.shift - 4), 2), p.KH * ceil_div(G, kFewCols));
+    L.few.off[1] = L.runs.n[0] = ceil_div(ceil_div((int64_t)chosen << (p.shift - 4), 2), L.few.per[0]);
     L.few.rec[0] = L.runs.rec[0] = 0;
     if (L.runs.n[0] > 1) L.records = rows * L.runs.n[0];
     return;
@@ -752,7 +752,7 @@ static int chosen(const PagePool &p, const PageRows &r, int most) {
 int64_t paged_attention_scratch_floats(const PagePool &p, const PageRows &r, int H, int prefix, int most) {
   if (r.row0[r.n] <= 0) return 0;
   PagedLaunches L;
-  paged_launches(p, r, H, prefix, most ? chosen(p, r, most) : 0, L);
+  paged_launches(p, r, H, prefix, most, chosen(p, r, most), L);
   return (int64_t)L.records * H * (p.HD + 4);
 }
 
@@ -760,7 +760,7 @@ template <int HD>
 static hipError_t paged_attend(const PagePool &p, const PageRows &r, const float *q, int H, int prefix, const int32_t *blocks,
                                int most, float scale, float *part, float *out, hipStream_t st) {
   PagedLaunches L;
-  paged_launches(p, r, H, prefix, most ? chosen(p, r, most) : 0, L);
+  paged_launches(p, r, H, prefix, most, chosen(p, r, most), L);
   const int G = H / p.KH, rows = r.row0[r.n];
   hipError_t e = hipSuccess;
   auto few = [&](const PageRows &R, const PagedPlan &U, int items) {

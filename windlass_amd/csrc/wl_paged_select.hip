@@ -1,97 +1,260 @@
 // wl_paged_select.hip - the pages that a row and KV head attends to, by a bound of their scores (wl_paged.h).
+//
+// The score of a page is the largest, over the heads g of the group, of sum_d max(q_gd, 0) hi_d + min(q_gd, 0) lo_d: a product
+// of the heads' [2 HD] halves with the pages', in 64 bits on v_mfma_f64_16x16x4_f64, since which page is taken must not hang on
+// a rounding (a product of a 24-bit query and an 11-bit bound is exact, a sum of 256 of them off by 2^-45 of its terms). Scores
+// are kept as whole numbers of the same order, and the pages taken are those from a border (score, page) on, found by
+// histograms of a narrowing range.
 #include "wl_paged.h"
 
 #include "wl_paged_device.h"
+
+#include <algorithm>
 
 #pragma clang fp contract(off)
 
 namespace wl {
 
-// One workgroup per row and KV head: the scores, then the pages one after the other.
-__global__ __launch_bounds__(256) void paged_select_kernel(PagePool P, PageRows R, const float *__restrict__ q, int H,
-                                                           PageSelect S, double *__restrict__ scores, int64_t width,
-                                                           int32_t *__restrict__ blocks) {
-  __shared__ double best[256];
-  __shared__ int at[256];
-  const int kvh = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, HD = P.HD, G = H / P.KH;
-  const int i = entry_of(R.row0, R.n, row);
-  const int cur = (R.pos[i] + row - R.row0[i]) >> P.shift;
-  const int from = S.first < cur + 1 ? S.first : cur + 1;
-  const int to = S.recent > cur + 1 - from ? from : cur + 1 - S.recent;
-  double *sc = scores + ((int64_t)row * P.KH + kvh) * width;
-  int32_t *o = blocks + ((int64_t)row * P.KH + kvh) * S.most();
-  const float *qp = q + ((int64_t)row * H + kvh * G) * HD;
-  for (int j = from + tid; j < to; j += 256) {
-    const int id = P.id(R.seq[i], j);
-    double m = -INFINITY;
-    if (id >= 0) {
-      const uint16_t *b = P.bounds + ((int64_t)id * P.KH + kvh) * 2 * HD;
-      for (int g = 0; g < G; g++) {
-        double s = 0.0;
-        for (int d = 0; d < HD; d++) {
-          const double x = qp[g * HD + d];
-          const double l = (double)(float)__builtin_bit_cast(_Float16, b[d]);
-          const double h = (double)(float)__builtin_bit_cast(_Float16, b[HD + d]);
-          s += fmax(x, 0.0) * h + fmin(x, 0.0) * l;
-        }
-        s = __builtin_isfinite(s) ? s : INFINITY;
-        m = s > m ? s : m;
-      }
-    }
-    sc[j] = m;
+constexpr int kScorePages = 64;  // of a workgroup, 16 a wave
+
+// Pages from .. to - 1 are open to choice for a row whose own page is cur.
+struct OpenPages {
+  int from, to;
+  __host__ __device__ OpenPages(const PageSelect &s, int cur) {
+    from = s.first < cur + 1 ? s.first : cur + 1;
+    to = s.recent > cur + 1 - from ? from : cur + 1 - s.recent;
   }
-  __syncthreads();
-  // the largest, `top` times; taken pages become NaN
-  for (int k = 0; k < S.top; k++) {
-    double m = -INFINITY;
-    int a = -1;
-    for (int j = from + tid; j < to; j += 256)
-      if (sc[j] > m) {
-        m = sc[j];
-        a = j;
-      }
-    best[tid] = m;
-    at[tid] = a;
-    __syncthreads();
-    if (tid == 0) {
-      for (int t = 1; t < 256; t++)
-        if (at[t] >= 0 && (a < 0 || best[t] > m || (best[t] == m && at[t] < a))) {
-          m = best[t];
-          a = at[t];
-        }
-      at[0] = a;
-      if (a >= 0) sc[a] = __builtin_nan("");
-    }
-    __syncthreads();
-    if (at[0] < 0) break;  // uniform
-    __syncthreads();
-  }
-  __syncthreads();
-  if (tid == 0) {
-    int n = 0;
-    for (int j = 0; j <= cur; j++)
-      if (j < from || j >= to || sc[j] != sc[j]) o[n++] = j;
-    for (; n < S.most(); n++) o[n] = -1;
-  }
+};
+
+// Entry i's items begin at off[i], per[i] workgroups for each of its rows.
+struct ScorePlan {
+  int off[kPgRows + 1], per[kPgRows];
+};
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// A whole number in the order of x, a score that is not finite as +inf; 0 is no page.
+__device__ __forceinline__ uint64_t score_key(double x) {
+  x = __builtin_isfinite(x) ? x : INFINITY;
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-static int64_t select_width(const PagePool &p, const PageRows &r) {
+// A wave makes the scores of 16 pages: operand column l % 16 is a page, row l % 16 a head (past the group's last the last again),
+// and lane l has the channels l / 16 * HD / 4 on of both, so that its loads are whole and the largest of a column is the page's
+// score in whatever order the rows come out.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageRows R, ScorePlan U, PageSelect S,
+                                                          const float *__restrict__ q, int G, uint64_t *__restrict__ keys,
+                                                          int64_t width) {
+  constexpr int N = HD / 4;
+  const int lane = threadIdx.x & 63, x = lane & 15, k = lane >> 4;
+  const int kvh = blockIdx.x % P.KH, item = blockIdx.x / P.KH, H = G * P.KH;
+  const int i = entry_of(U.off, R.n, item), t = (item - U.off[i]) / U.per[i], row = R.row0[i] + t;
+  const OpenPages o(S, (R.pos[i] + t) >> P.shift);
+  const int j = o.from + (item - U.off[i]) % U.per[i] * kScorePages + (threadIdx.x >> 6) * 16 + x;
+  const int id = j < o.to ? P.id(R.seq[i], j) : -1;
+  const uint16_t *b = P.bounds + ((int64_t)(id < 0 ? 0 : id) * P.KH + kvh) * 2 * HD + k * N;
+  fh8 lo[N / 8], hi[N / 8];
+#pragma unroll
+  for (int e = 0; e < N / 8; e++) {
+    lo[e] = *reinterpret_cast<const fh8 *>(b + 8 * e);
+    hi[e] = *reinterpret_cast<const fh8 *>(b + HD + 8 * e);
+  }
+  double best = -INFINITY;
+  for (int g0 = 0; g0 < G; g0 += 16) {
+    const int g = g0 + x < G ? g0 + x : G - 1;
+    const float *qp = q + ((int64_t)row * H + kvh * G + g) * HD + k * N;
+    f64x4 a0 = {0.0, 0.0, 0.0, 0.0}, a1 = a0;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const float v = qp[e];
+      // a NaN goes with both
+      const double up = (double)(v < 0.f ? 0.f : v), down = (double)(v > 0.f ? 0.f : v);
+      a0 = __builtin_amdgcn_mfma_f64_16x16x4f64(up, (double)(float)hi[e / 8][e % 8], a0, 0, 0, 0);
+      a1 = __builtin_amdgcn_mfma_f64_16x16x4f64(down, (double)(float)lo[e / 8][e % 8], a1, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const double s = a0[e] + a1[e];
+      best = fmax(best, __builtin_isfinite(s) ? s : INFINITY);
+    }
+  }
+  best = fmax(best, __shfl_xor(best, 16, 64));
+  best = fmax(best, __shfl_xor(best, 32, 64));
+  if (k == 0 && j < o.to) keys[((int64_t)row * P.KH + kvh) * width + j - o.from] = id < 0 ? 0 : score_key(best);
+}
+
+// Sum over the workgroup's 256 threads up to and with this one, and of all.
+__device__ __forceinline__ int block_scan(int v, int *sh, int &all) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int o = __shfl_up(v, m, 64);
+    v += lane >= m ? o : 0;
+  }
+  __syncthreads();
+  if (lane == 63) sh[w] = v;
+  __syncthreads();
+  all = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  return v + (w > 0 ? sh[0] : 0) + (w > 1 ? sh[1] : 0) + (w > 2 ? sh[2] : 0);
+}
+
+// A workgroup per row and KV head. Thread t has pages t * m .. of the m = ceil(n / 256) each has, in registers up to kOwn of them.
+template <int kOwn>
+__global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageRows R, PageSelect S,
+                                                         const uint64_t *__restrict__ keys, int64_t width,
+                                                         int32_t *__restrict__ blocks) {
+  constexpr int BINS = 1024;
+  __shared__ int bins[BINS], sh[4], pick[3];
+  __shared__ uint64_t ends[2][4];
+  const int kvh = blockIdx.x % P.KH, row = blockIdx.x / P.KH, tid = threadIdx.x;
+  const int i = entry_of(R.row0, R.n, row);
+  const int cur = (R.pos[i] + row - R.row0[i]) >> P.shift;
+  const OpenPages o(S, cur);
+  const int n = o.to - o.from, m = (n + 255) / 256;
+  const uint64_t *kp = keys + ((int64_t)row * P.KH + kvh) * width;
+  int32_t *out = blocks + ((int64_t)row * P.KH + kvh) * S.most();
+  uint64_t mine[kOwn > 0 ? kOwn : 1];
+  if constexpr (kOwn > 0) {
+#pragma unroll
+    for (int e = 0; e < kOwn; e++) mine[e] = e < m && tid * m + e < n ? kp[tid * m + e] : 0;
+  }
+  // f(key, page) over the thread's pages that are there
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (kOwn > 0) {
+#pragma unroll
+      for (int e = 0; e < kOwn; e++)
+        if (mine[e]) f(mine[e], tid * m + e);
+    } else {
+      for (int e = 0; e < m && (int64_t)tid * m + e < n; e++)
+        if (const uint64_t v = kp[tid * m + e]) f(v, tid * m + e);
+    }
+  };
+  int all = 0;
+  uint64_t lo = ~0ull, hi = 0;
+  each([&](uint64_t v, int) {
+    all++;
+    lo = v < lo ? v : lo;
+    hi = v > hi ? v : hi;
+  });
+#pragma unroll
+  for (int x = 32; x; x >>= 1) {
+    const uint64_t a = __shfl_xor(lo, x, 64), b = __shfl_xor(hi, x, 64);
+    lo = a < lo ? a : lo;
+    hi = b > hi ? b : hi;
+  }
+  if ((tid & 63) == 0) {
+    ends[0][tid >> 6] = lo;
+    ends[1][tid >> 6] = hi;
+  }
+  (void)block_scan(all, sh, all);  // its barriers also order the ends
+  for (int w = 0; w < 4; w++) {
+    lo = ends[0][w] < lo ? ends[0][w] : lo;
+    hi = ends[1][w] > hi ? ends[1][w] : hi;
+  }
+  // The border: pages of a key above `key`, and those of that key up to page `upto`. `need` of the pages in lo .. hi (by key, then,
+  // among equal keys, by page from the last) are taken, and all above hi.
+  uint64_t key = 0;
+  int upto = -1, need = S.top;
+  if (need >= all) {
+    key = 0;
+  } else if (need == 0) {
+    key = ~0ull;
+  } else {
+    bool ties = false;
+    for (;;) {
+      const uint64_t span = hi - lo;
+      const int shift = span >> 10 ? 54 - __builtin_clzll(span) : 0;  // span >> shift is below 1024
+      for (int e = tid; e < BINS; e += 256) bins[e] = 0;
+      __syncthreads();
+      each([&](uint64_t v, int page) {
+        const uint64_t w = ties ? ~(uint32_t)page : v;
+        if ((!ties || v == key) && w >= lo && w <= hi) atomicAdd(&bins[(w - lo) >> shift], 1);
+      });
+      __syncthreads();
+      // from the top: thread t has bins 1023 - 4 t down to 1020 - 4 t
+      int c[4], sum = 0, total;
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum += c[e] = bins[BINS - 1 - 4 * tid - e];
+      int before = block_scan(sum, sh, total) - sum;
+      if (before < need && before + sum >= need) {  // one thread
+        int e = 0;
+        while (before + c[e] < need) before += c[e++];
+        pick[0] = BINS - 1 - 4 * tid - e;
+        pick[1] = before;
+        pick[2] = c[e];
+      }
+      __syncthreads();
+      need -= pick[1];
+      const int in = pick[2];
+      lo += (uint64_t)pick[0] << shift;
+      const uint64_t bin = (1ull << shift) - 1;
+      hi = hi - lo < bin ? hi : lo + bin;
+      if (in == need) {  // the whole bin
+        if (ties) upto = (int)~(uint32_t)lo;
+        else key = lo - 1;
+        break;
+      }
+      if (shift == 0) {  // equal keys: by page, which ends with one page a bin
+        ties = true;
+        key = lo;
+        lo = ~(uint32_t)(n - 1);
+        hi = 0xffffffffu;
+      }
+    }
+  }
+  auto taken = [&](uint64_t v, int page) { return v > key || (v == key && page <= upto); };
+  int count = 0, total;
+  each([&](uint64_t v, int page) { count += taken(v, page); });
+  int at = o.from + block_scan(count, sh, total) - count;
+  each([&](uint64_t v, int page) {
+    if (taken(v, page)) out[at++] = o.from + page;
+  });
+  for (int e = tid; e < o.from; e += 256) out[e] = e;
+  const int rest = o.from + total, last = rest + cur + 1 - o.to;
+  for (int e = rest + tid; e < S.most(); e += 256) out[e] = e < last ? o.to + e - rest : -1;
+}
+
+// Pages open to choice of any row of a call.
+static int64_t open_width(const PagePool &p, const PageRows &r, const PageSelect &s) {
   int64_t w = 1;
   for (int i = 0; i < r.n; i++)
-    if (r.rows(i)) w = w > ((r.pos[i] + r.rows(i) - 1) >> p.shift) + 1 ? w : ((r.pos[i] + r.rows(i) - 1) >> p.shift) + 1;
+    if (r.rows(i)) {
+      const OpenPages o(s, (r.pos[i] + r.rows(i) - 1) >> p.shift);
+      w = std::max(w, (int64_t)o.to - o.from);
+    }
   return w;
 }
 
-int64_t paged_select_scratch_bytes(const PagePool &p, const PageRows &r, const PageSelect &) {
-  return (int64_t)r.row0[r.n] * p.KH * select_width(p, r) * 8;
+int64_t paged_select_scratch_bytes(const PagePool &p, const PageRows &r, const PageSelect &s) {
+  return (int64_t)r.row0[r.n] * p.KH * open_width(p, r, s) * 8;
 }
 
 hipError_t paged_select_launch(const PagePool &p, const PageRows &r, const float *q, int H, const PageSelect &s,
                                void *scratch, int32_t *blocks, hipStream_t st) {
-  const int rows = r.row0[r.n];
+  const int rows = r.row0[r.n], G = H / p.KH;
   if (rows <= 0) return hipSuccess;
-  hipLaunchKernelGGL(paged_select_kernel, dim3(p.KH, rows), dim3(256), 0, st, p, r, q, H, s, (double *)scratch,
-                     select_width(p, r), blocks);
+  const int64_t width = open_width(p, r, s);
+  uint64_t *keys = (uint64_t *)scratch;
+  ScorePlan U;
+  U.off[0] = 0;
+  for (int i = 0; i < r.n; i++) {
+    const int T = r.rows(i);
+    const OpenPages o(s, T ? (r.pos[i] + T - 1) >> p.shift : 0);
+    U.per[i] = T ? std::max(0, (o.to - o.from + kScorePages - 1) / kScorePages) : 0;
+    U.off[i + 1] = U.off[i] + T * U.per[i];
+  }
+  if (U.off[r.n]) {
+    const dim3 grid((unsigned)((int64_t)U.off[r.n] * p.KH));
+    if (p.HD == 64) hipLaunchKernelGGL(paged_score_kernel<64>, grid, dim3(256), 0, st, p, r, U, s, q, G, keys, width);
+    else hipLaunchKernelGGL(paged_score_kernel<128>, grid, dim3(256), 0, st, p, r, U, s, q, G, keys, width);
+    if (const hipError_t e = hipGetLastError()) return e;
+  }
+  const dim3 grid((unsigned)(rows * p.KH));
+  if (width <= 256 * 4) hipLaunchKernelGGL(paged_take_kernel<4>, grid, dim3(256), 0, st, p, r, s, keys, width, blocks);
+  else if (width <= 256 * 16) hipLaunchKernelGGL(paged_take_kernel<16>, grid, dim3(256), 0, st, p, r, s, keys, width, blocks);
+  else hipLaunchKernelGGL(paged_take_kernel<0>, grid, dim3(256), 0, st, p, r, s, keys, width, blocks);
   return hipGetLastError();
 }
 
