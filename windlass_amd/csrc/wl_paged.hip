@@ -10,110 +10,265 @@
 
 namespace wl {
 
+constexpr int kPgUnitRows = 8;  // rows of a sequence from which units pay
+
 struct StoreArgs {
   PagePool p;
   PageRope e;
   const float *q, *k, *v;
   float *qr;
-  int H;
+  int H, parts, each;  // parts of a row or unit, query heads each
 };
 
 __device__ __forceinline__ uint16_t half_of(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+__device__ __forceinline__ uint32_t halves_of(float x, float y) { return half_of(x) | (uint32_t)half_of(y) << 16; }
 
-// A workgroup per row.
-__global__ __launch_bounds__(256) void paged_store_kernel(StoreArgs A, PageRows R) {
-  __shared__ float2 angle[64];
-  const int row = blockIdx.x, tid = threadIdx.x, HD = A.p.HD, KH = A.p.KH, half = A.e.n / 2;
-  const int i = entry_of(R.row0, R.n, row);
-  const int p = R.pos[i] + row - R.row0[i];
-  const int id = A.p.id(R.seq[i], p >> A.p.shift), off = p & (A.p.page - 1);
-  if (tid < 64) {
-    float c = 1.f, s = 0.f;
-    if (half) rope_cs(p, tid < half ? tid : 0, half, A.e.theta_scale, A.e.freq_scale, A.e.freqs, c, s);
-    if (tid < half) angle[tid] = make_float2(c, s);
+// The two values of a head that lane pair x turns: (2 x, 2 x + 1), or (x, x + n / 2) among a NeoX head's first n; what is not
+// rotated goes in twos.
+struct Pair {
+  int a, b;
+  bool turns;
+  __device__ Pair(const PageRope &e, int x) : turns(x < e.n / 2) {
+    a = e.neox && turns ? x : 2 * x;
+    b = e.neox && turns ? x + e.n / 2 : 2 * x + 1;
   }
+  __device__ __forceinline__ float2 load(const float *h) const { return make_float2(h[a], h[b]); }
+  __device__ __forceinline__ float2 turn(float2 v, float c, float s) const {
+    return turns ? make_float2(v.x * c - v.y * s, v.x * s + v.y * c) : v;
+  }
+};
+
+// The smaller or larger of each; a NaN stays.
+__device__ __forceinline__ fh8 least(fh8 a, fh8 b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ fh8 most(fh8 a, fh8 b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ fh8 lane_swap(fh8 v, int m) {
+  u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+#pragma unroll
+  for (int e = 0; e < 4; e++) w[e] = __shfl_xor(w[e], m, 64);
+  return __builtin_bit_cast(fh8, w);
+}
+
+// Few rows of each sequence: a wave per part of a row, `each` query heads or the keys and values of one KV head (two of 64), a
+// lane per pair, so that the heads of a part share its angles. With one row of each sequence the
+// waves of the keys also make their page's bounds.
+template <int HD>
+__global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U) {
+  constexpr int NP = HD / 2, HS = 64 / NP, HMAX = 8;  // pairs, heads at once, query heads a part at most (in steps of HS)
+  __shared__ double theta[NP];
+  __shared__ uint16_t fresh[HS][HD];
+  const int lane = threadIdx.x, x = lane % NP, sub = lane / NP, KH = A.p.KH;
+  const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, half = A.e.n / 2;
+  const PageEntry E = entry_of(U, row);
+  const int p = E.pos + row - E.row0, off = p & (A.p.page - 1);
+  const Pair pr(A.e, x);
+  const int q_parts = A.parts - (KH + HS - 1) / HS;
+  const bool isq = part < q_parts;
+  const int h0 = isq ? part * A.each : (part - q_parts) * HS;
+  const float freq = A.e.freqs && x < half ? A.e.freqs[x] : 1.f;
+  // loads first, then the angles
+  float2 v[HMAX / HS], w = make_float2(0.f, 0.f);
+  int id = -1;
+  if (isq) {
+#pragma unroll
+    for (int e = 0; e < HMAX / HS; e++) {
+      const int h = h0 + e * HS + sub;
+      if (e * HS < A.each && h < A.H && e * HS + sub < A.each) v[e] = pr.load(A.q + ((int64_t)row * A.H + h) * HD);
+    }
+  } else {
+    id = A.p.id(E.seq, p >> A.p.shift);
+    const int64_t r = ((int64_t)row * KH + (h0 + sub < KH ? h0 + sub : KH - 1)) * HD;
+    v[0] = pr.load(A.k + r);
+    w = make_float2(A.v[r + 2 * x], A.v[r + 2 * x + 1]);
+  }
+  float c = 1.f, s = 0.f;
+  if (half) {
+    if (lane == 0) rope_chain<1>(theta, 0, p, half, A.e.theta_scale, A.e.freq_scale);
+    __syncthreads();
+    rope_cs_of(theta[x < half ? x : 0], freq, A.e.freqs != nullptr, c, s);
+  }
+  if (isq) {
+#pragma unroll
+    for (int e = 0; e < HMAX / HS; e++) {
+      const int h = h0 + e * HS + sub;
+      if (e * HS < A.each && h < A.H && e * HS + sub < A.each) {
+        const float2 y = pr.turn(v[e], c, s);
+        float *o = A.qr + ((int64_t)row * A.H + h) * HD;
+        o[pr.a] = y.x;
+        o[pr.b] = y.y;
+      }
+    }
+    return;
+  }
+  if (id < 0) return;  // uniform
+  const float2 y = pr.turn(v[0], c, s);
+  fresh[sub][pr.a] = half_of(y.x);
+  fresh[sub][pr.b] = half_of(y.y);
+  if (h0 + sub < KH) {
+    const int64_t at = A.p.at(id, h0 + sub);
+    A.p.K[at + pg_key(off, pr.a, HD)] = half_of(y.x);
+    A.p.K[at + pg_key(off, pr.b, HD)] = half_of(y.y);
+    A.p.V[at + pg_val(off, 2 * x, HD)] = half_of(w.x);
+    A.p.V[at + pg_val(off, 2 * x + 1, HD)] = half_of(w.y);
+  }
+  if (!A.p.bounds) return;
   __syncthreads();
-  auto turned = [&](const float *x, int d) {
-    if (d >= A.e.n) return x[d];
-    const int j = A.e.neox ? d % half : d / 2;
-    const int a = A.e.neox ? j : 2 * j, b = A.e.neox ? j + half : 2 * j + 1;
-    const float2 cs = angle[j];
-    return d == a ? x[a] * cs.x - x[b] * cs.y : x[a] * cs.y + x[b] * cs.x;
-  };
-  // a pair per thread, so that q may be rotated in place
-  for (int j = tid; j < A.H * HD / 2; j += 256) {
-    const int h = j / (HD / 2), x = j % (HD / 2);
-    const int a = x < half ? (A.e.neox ? x : 2 * x) : 2 * x, b = x < half ? (A.e.neox ? x + half : 2 * x + 1) : 2 * x + 1;
-    const float *xp = A.q + ((int64_t)row * A.H + h) * HD;
-    float *o = A.qr + ((int64_t)row * A.H + h) * HD;
-    const float ya = turned(xp, a), yb = turned(xp, b);
-    o[a] = ya;
-    o[b] = yb;
+  // the page's positions before this one, 16 bytes a lane: eight channels lane / 8 (+ 8 for every other piece of a head of 128)
+  constexpr int SETS = HD / 64;
+  for (int g = 0; g < HS && h0 + g < KH; g++) {
+    const uint16_t *K = A.p.K + A.p.at(id, h0 + g);
+    fh8 lo[SETS], hi[SETS];
+#pragma unroll
+    for (int e = 0; e < SETS; e++) lo[e] = hi[e] = *reinterpret_cast<const fh8 *>(&fresh[g][64 * e + lane / 8 * 8]);
+    const int slot = (lane >> 2 & 1) * 8 + (lane & 3);
+    for (int u = 0; 16 * u < off; u++) {
+#pragma unroll
+      for (int e = 0; e < 2 * SETS; e++) {
+        const int t = e / SETS;
+        if (16 * u + slot + 4 * t >= off) continue;
+        const fh8 b = *reinterpret_cast<const fh8 *>(K + u * 16 * HD + e * 512 + lane * 8);
+        lo[e % SETS] = least(lo[e % SETS], b);
+        hi[e % SETS] = most(hi[e % SETS], b);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < SETS; e++) {
+#pragma unroll
+      for (int m = 1; m <= 4; m <<= 1) {
+        lo[e] = least(lo[e], lane_swap(lo[e], m));
+        hi[e] = most(hi[e], lane_swap(hi[e], m));
+      }
+      uint16_t *b = A.p.bounds + ((int64_t)id * KH + h0 + g) * 2 * HD + 64 * e + lane / 8 * 8;
+      if ((lane & 7) == 0) *reinterpret_cast<fh8 *>(b) = lo[e];
+      if ((lane & 7) == 1) *reinterpret_cast<fh8 *>(b + HD) = hi[e];
+    }
   }
-  if (id < 0) return;
-  for (int j = tid; j < KH * HD; j += 256) {
-    const int kvh = j / HD, d = j % HD;
-    const int64_t at = A.p.at(id, kvh), r = (int64_t)row * KH * HD;
-    A.p.K[at + pg_key(off, d, HD)] = half_of(turned(A.k + r + kvh * HD, d));
-    A.p.V[at + pg_val(off, d, HD)] = half_of(A.v[r + j]);
+}
+
+// Prompts: a workgroup per part of a unit of 16 positions, a wave per position. The products of the angles once (a lane per
+// position), the heads' rows by their waves; keys and values of two KV heads at a time go through LDS and leave as whole pieces of the
+// page, a value's eight positions together.
+template <int HD>
+__global__ __launch_bounds__(1024) void paged_units_kernel(StoreArgs A, PageItems U) {
+  constexpr int NP = HD / 2, HS = 64 / NP, LD = HD + 8, PIECES = 2 * HD;  // 16-byte pieces of a unit's keys
+  __shared__ double theta[64 * 16];
+  __shared__ __attribute__((aligned(16))) uint16_t ks[2][16 * LD], vs[2][16 * LD];
+  const int tid = threadIdx.x, lane = tid & 63, r = __builtin_amdgcn_readfirstlane(tid >> 6), x = lane % NP, sub = lane / NP;
+  const int KH = A.p.KH, half = A.e.n / 2;
+  const int item = blockIdx.x / A.parts, part = blockIdx.x % A.parts;
+  const PageEntry E = entry_of(U, item);
+  const int u = (E.pos >> 4) + item - E.off, p = 16 * u + r;
+  const bool on = p >= E.pos && p < E.pos + E.rows;
+  const int64_t row = (int64_t)E.row0 + (on ? p - E.pos : 0);
+  const int id = A.p.id(E.seq, 16 * u >> A.p.shift);
+  const Pair pr(A.e, x);
+  const float freq = A.e.freqs && x < half ? A.e.freqs[x] : 1.f;
+  float c = 1.f, s = 0.f;
+  if (half) {
+    if (tid < 16) rope_chain<16>(theta, tid, 16 * u + tid, half, A.e.theta_scale, A.e.freq_scale);
+    __syncthreads();
+    rope_cs_of(theta[(x < half ? x : 0) * 16 + r], freq, A.e.freqs != nullptr, c, s);
+  }
+  if (on) {
+    const int h1 = (part + 1) * A.each < A.H ? (part + 1) * A.each : A.H;
+    for (int h = part * A.each + sub; h < h1; h += 4 * HS) {
+      float2 v[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (h + e * HS < h1) v[e] = pr.load(A.q + (row * A.H + h + e * HS) * HD);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (h + e * HS < h1) {
+          const float2 y = pr.turn(v[e], c, s);
+          float *o = A.qr + (row * A.H + h + e * HS) * HD;
+          o[pr.a] = y.x;
+          o[pr.b] = y.y;
+        }
+    }
+  }
+  if (id < 0) return;  // uniform over the workgroup
+  const int k1 = (int)((int64_t)(part + 1) * KH / A.parts);
+  for (int h0 = (int)((int64_t)part * KH / A.parts); h0 < k1; h0 += 2) {
+    __syncthreads();  // the heads before are written
+    if (on)
+      for (int g = sub; g < 2; g += HS)
+        if (h0 + g < k1) {
+          const int64_t at = (row * KH + h0 + g) * HD;
+          const float2 y = pr.turn(pr.load(A.k + at), c, s);
+          ks[g][r * LD + pr.a] = half_of(y.x);
+          ks[g][r * LD + pr.b] = half_of(y.y);
+          *reinterpret_cast<uint32_t *>(&vs[g][r * LD + 2 * x]) = halves_of(A.v[at + 2 * x], A.v[at + 2 * x + 1]);
+        }
+    __syncthreads();
+    // pieces of the first head's keys, its values, and so the second's
+    for (int e = tid; e < 4 * PIECES; e += 1024) {
+      const int g = e / (2 * PIECES), c8 = e % PIECES;
+      if (h0 + g >= k1) break;
+      const int64_t to = A.p.at(id, h0 + g) + (int64_t)(u & ((A.p.page >> 4) - 1)) * 16 * HD + c8 * 8;
+      if (e / PIECES % 2 == 0) {
+        const int off = (c8 >> 2 & 1) * 8 + c8 / HD * 4 + (c8 & 3), oct = c8 / 8 % (HD / 8), at = 16 * u + off;
+        if (at >= E.pos && at < E.pos + E.rows)
+          *reinterpret_cast<u32x4_t *>(A.p.K + to) = *reinterpret_cast<const u32x4_t *>(&ks[g][off * LD + oct * 8]);
+      } else {
+        const int o8 = c8 / HD * 8, d = c8 % HD, at = 16 * u + o8;
+        uint16_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = vs[g][(o8 + j) * LD + d];
+        if (at >= E.pos && at <= E.pos + E.rows - 8) {
+          u32x4_t y;
+#pragma unroll
+          for (int j = 0; j < 4; j++) y[j] = w[2 * j] | (uint32_t)w[2 * j + 1] << 16;
+          *reinterpret_cast<u32x4_t *>(A.p.V + to) = y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (at + j >= E.pos && at + j < E.pos + E.rows) A.p.V[to + j] = w[j];
+        }
+      }
+    }
   }
 }
 
 // The bounds of the pages written to: a workgroup per page and KV head, 16 bytes of keys a thread and step.
-struct BoundsItems {
-  int off[kPgRows + 1];  // pages before entry i's
-};
-__global__ __launch_bounds__(256) void paged_bounds_kernel(PagePool P, PageRows R, BoundsItems B) {
-  __shared__ _Float16 lo[4][128], hi[4][128];
+__global__ __launch_bounds__(256) void paged_bounds_kernel(PagePool P, PageItems U) {
+  __shared__ fh8 lo[4][16], hi[4][16];
   const int kvh = blockIdx.x % P.KH, item = blockIdx.x / P.KH, tid = threadIdx.x, HD = P.HD, oct = tid / 8 % (HD / 8);
-  const int i = entry_of(B.off, R.n, item);
-  const int j = (R.pos[i] >> P.shift) + item - B.off[i];
-  const int id = P.id(R.seq[i], j);
+  const PageEntry E = entry_of(U, item);
+  const int j = (E.pos >> P.shift) + item - E.off;
+  const int id = P.id(E.seq, j);
   if (id < 0) return;  // uniform
-  const int last = R.pos[i] + R.rows(i) - 1 - (j << P.shift);  // of the page; past it where the page is full
+  const int last = E.pos + E.rows - 1 - (j << P.shift);  // of the page; past it where the page is full
   const uint16_t *K = P.K + P.at(id, kvh);
-  _Float16 l[8], h[8];
   const _Float16 inf = (_Float16)INFINITY;
+  fh8 l, h;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     l[e] = inf;
     h[e] = -inf;
   }
-  auto take = [](_Float16 &m, _Float16 x, bool less) {  // a NaN stays
-    m = (less ? x < m : x > m) || x != x ? x : m;
-  };
   for (int c = tid; c < P.page * HD / 8; c += 256) {
     const int u = c / (2 * HD), t = c / HD & 1, s = c & 7;
     if (16 * u + 8 * (s >> 2) + 4 * t + (s & 3) > last) continue;
     const fh8 x = *reinterpret_cast<const fh8 *>(K + 8 * c);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      take(l[e], x[e], true);
-      take(h[e], x[e], false);
-    }
+    l = least(l, x);
+    h = most(h, x);
   }
-  // the eight positions of a piece, then the waves that hold the same channels
+  // the eight positions of a piece, then the threads that hold the same channels (2 or 4 of each)
 #pragma unroll
-  for (int m = 1; m <= 4; m <<= 1)
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      take(l[e], (_Float16)__shfl_xor((float)l[e], m, 64), true);
-      take(h[e], (_Float16)__shfl_xor((float)h[e], m, 64), false);
-    }
-  const int part = tid / HD;  // 2 or 4 threads a piece
-  if ((tid & 7) == 0)
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      lo[part][8 * oct + e] = l[e];
-      hi[part][8 * oct + e] = h[e];
-    }
+  for (int m = 1; m <= 4; m <<= 1) {
+    l = least(l, lane_swap(l, m));
+    h = most(h, lane_swap(h, m));
+  }
+  if ((tid & 7) == 0) {
+    lo[tid / HD][oct] = l;
+    hi[tid / HD][oct] = h;
+  }
   __syncthreads();
-  if (tid >= 2 * HD) return;
-  const int d = tid % HD;
-  const bool up = tid >= HD;
-  _Float16 m = up ? hi[0][d] : lo[0][d];
-  for (int e = 1; e < 256 / HD; e++) take(m, up ? hi[e][d] : lo[e][d], !up);
-  P.bounds[(((int64_t)id * P.KH + kvh) * 2 + up) * HD + d] = __builtin_bit_cast(uint16_t, m);
+  if (tid >= HD / 4) return;
+  const int o = tid % (HD / 8);
+  const bool up = tid >= HD / 8;
+  fh8 m = up ? hi[0][o] : lo[0][o];
+  for (int e = 1; e < 256 / HD; e++) m = up ? most(m, hi[e][o]) : least(m, lo[e][o]);
+  *reinterpret_cast<fh8 *>(P.bounds + (((int64_t)id * P.KH + kvh) * 2 + up) * HD + 8 * o) = m;
 }
 
 __global__ __launch_bounds__(256) void paged_read_kernel(PagePool P, int seq, int pos0, int T, float *__restrict__ k,
@@ -136,14 +291,39 @@ hipError_t paged_store_launch(const PagePool &p, const PageRows &r, const float 
                               const PageRope &rope, float *qr, hipStream_t st) {
   const int rows = r.row0[r.n];
   if (rows <= 0) return hipSuccess;
-  hipLaunchKernelGGL(paged_store_kernel, dim3(rows), dim3(256), 0, st, StoreArgs{p, rope, q, k, v, qr, H}, r);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !p.bounds) return e;
-  BoundsItems b;
-  b.off[0] = 0;
-  for (int i = 0; i < r.n; i++)
-    b.off[i + 1] = b.off[i] + (r.rows(i) ? ((r.pos[i] + r.rows(i) - 1) >> p.shift) - (r.pos[i] >> p.shift) + 1 : 0);
-  hipLaunchKernelGGL(paged_bounds_kernel, dim3(b.off[r.n] * p.KH), dim3(256), 0, st, p, r, b);
+  PageItems each, units, pages;
+  int T = 0;
+  for (int i = 0; i < r.n; i++) {
+    const int t = r.rows(i), last = r.pos[i] + t - 1;
+    T = T > t ? T : t;
+    each.add(r, i, t);
+    units.add(r, i, t ? (last >> 4) - (r.pos[i] >> 4) + 1 : 0);
+    pages.add(r, i, t ? (last >> p.shift) - (r.pos[i] >> p.shift) + 1 : 0);
+  }
+  StoreArgs A{p, rope, q, k, v, qr, H, 0, 0};
+  if (T < kPgUnitRows) {
+    if (T > 1) A.p.bounds = nullptr;  // rows of a page, by several waves
+    const int hs = 128 / p.HD;  // heads of a wave at once
+    // enough waves for every SIMD, no more than eight heads each
+    A.each = hs;
+    while (A.each < 8 && (int64_t)rows * (H / A.each) > 2048) A.each *= 2;
+    A.parts = (H + A.each - 1) / A.each + (p.KH + hs - 1) / hs;
+    const dim3 grid((unsigned)((int64_t)rows * A.parts));
+    if (p.HD == 64) hipLaunchKernelGGL(paged_rows_kernel<64>, grid, dim3(64), 0, st, A, each);
+    else hipLaunchKernelGGL(paged_rows_kernel<128>, grid, dim3(64), 0, st, A, each);
+  } else {
+    // parts of a unit: as many as give every CU two workgroups, of a KV head or a query head at least
+    const int most = p.KH > H ? p.KH : H;
+    A.parts = 512 / units.items;
+    A.parts = A.parts < 1 ? 1 : A.parts > most ? most : A.parts;
+    A.each = (H + A.parts - 1) / A.parts;
+    const dim3 grid((unsigned)((int64_t)units.items * A.parts));
+    if (p.HD == 64) hipLaunchKernelGGL(paged_units_kernel<64>, grid, dim3(1024), 0, st, A, units);
+    else hipLaunchKernelGGL(paged_units_kernel<128>, grid, dim3(1024), 0, st, A, units);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !p.bounds || T == 1) return e;
+  hipLaunchKernelGGL(paged_bounds_kernel, dim3(pages.items * p.KH), dim3(256), 0, st, p, pages);
   return hipGetLastError();
 }
 

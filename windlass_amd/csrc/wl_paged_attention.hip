@@ -25,10 +25,10 @@ constexpr int kManyWaves = 4, kManyCols = 32 * kManyWaves, kManyUnits = 4;  // u
 constexpr int kPgRuns = 256;  // of a row at most
 constexpr uint32_t kNowhere = 0xfffffff0u;  // the position of a unit that no row sees
 
-// A launch's items: entry i's begin at off[i], column block by column block, `per` tiles or steps each. Its rows' records, a run
-// after the other for each (row, head), begin H * rec[i] records into `part`; alone: a row of one run is the output itself.
+// A launch's items go entry by entry, column block by column block, run by run of `per` tiles or steps each. An entry's records, a
+// run after the other for each (row, head), begin H * rec records into `part`; alone: a row of one run is the output itself.
 struct PagedPlan {
-  int off[kPgRows + 1], per[kPgRows], rec[kPgRows];
+  PageItems it;
   int inc, base;  // a row's positions end at pos + row * inc; units before base are not read
   int alone;
 };
@@ -96,7 +96,7 @@ struct FewTile {
 };
 
 template <int HD, bool SPARSE>
-__global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_kernel(PagePool P, PageRows R, PagedPlan U,
+__global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_kernel(PagePool P, PagedPlan U,
                                                                       const float *__restrict__ q, int G,
                                                                       const int32_t *__restrict__ blocks, int nblocks,
                                                                       float scale, float *__restrict__ part,
@@ -109,27 +109,16 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kq = lane >> 4, KH = P.KH, H = G * KH, us = P.shift - 4;
   const int kvh = blockIdx.x % KH, item = blockIdx.x / KH;
-  int i, row0, T, pos, cb, run, runs, per;
+  const PageEntry E = entry_of(U.it, item);
+  const int runs = E.runs, per = E.per, run = (item - E.off) % runs;
+  int cb = (item - E.off) / runs, t0 = 0, T = E.rows;  // the block's rows: T from the entry's t0
   if constexpr (SPARSE) {
     const int nb = (G + kFewCols - 1) / kFewCols;
-    runs = U.off[1];
-    per = U.per[0];
-    run = item % runs;
-    cb = item / runs % nb;
-    row0 = item / runs / nb;
-    i = entry_of(R.row0, R.n, row0);
+    t0 = cb / nb;
+    cb %= nb;
     T = 1;
-    pos = R.pos[i] + row0 - R.row0[i];
-  } else {
-    i = entry_of(U.off, R.n, item);
-    row0 = R.row0[i];
-    T = R.rows(i);
-    pos = R.pos[i];
-    per = U.per[i];
-    runs = (U.off[i + 1] - U.off[i]) / ((T * G + kFewCols - 1) / kFewCols);
-    run = (item - U.off[i]) % runs;
-    cb = (item - U.off[i]) / runs;
   }
+  const int row0 = E.row0 + t0, pos = E.pos + t0;
   const int NC = T * G, c0 = cb * kFewCols, c = c0 + col < NC ? c0 + col : NC - 1;
   const int t = c / G, h = kvh * G + c % G;
   const int p = pos + t * U.inc, pa = pos + c0 / G * U.inc;
@@ -156,7 +145,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
       u = U.base + j;
       b = u >> us;
     }
-    const int id = P.id(R.seq[i], b);
+    const int id = P.id(E.seq, b);
     if (id < 0) return;
     off = P.at(id, kvh) + (int64_t)(u & ((1 << us) - 1)) * 16 * HD;
     up = 16u * (uint32_t)u;
@@ -303,7 +292,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
       for (int x = 0; x < 32; x++) {
         const uint32_t w = (x >> 4 ? a.up[1] : a.up[0]) + (x & 15);
         if (w <= (uint32_t)pa || w > (uint32_t)pb) continue;  // uniform
-        const uint16_t *vp = P.V + P.at(P.id(R.seq[i], (int)(w >> P.shift)), kvh);
+        const uint16_t *vp = P.V + P.at(P.id(E.seq, (int)(w >> P.shift)), kvh);
         const int o = (int)(w & (P.page - 1));
 #pragma unroll
         for (int d = 0; d < ND; d++)
@@ -342,15 +331,14 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
       o += so[w][g][four] * f;
       l += sl[w][g] * (double)f;
     }
-    const int64_t at = (int64_t)(cc / G) * H + kvh * G + cc % G, row = (int64_t)row0 * H + at;
+    const int64_t at = (int64_t)(t0 + cc / G) * H + kvh * G + cc % G, row = (int64_t)E.row0 * H + at;
     if (whole) {
       const double r = (1.0 / kSpUp) / l;
 #pragma unroll
       for (int j = 0; j < 4; j++) o[j] = l == 0.0 ? 0.f : (float)((double)o[j] * r);
       *reinterpret_cast<f4a4 *>(out + row * HD + 4 * four) = o;
     } else {
-      const int64_t from = SPARSE ? (int64_t)row0 * H * runs : (int64_t)U.rec[i] * H;
-      float *rec = part + (from + at * runs + run) * (HD + 4);
+      float *rec = part + ((int64_t)E.rec * H + at * runs + run) * (HD + 4);
       *reinterpret_cast<sf4 *>(rec + 4 * four) = o;
       if (four == 0) {
         rec[HD] = m;
@@ -372,7 +360,7 @@ __device__ __forceinline__ void to_lds(const uint16_t *from, uint32_t to) {
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <int HD>
-__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool P, PageRows R, PagedPlan U,
+__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool P, PagedPlan U,
                                                                         const float *__restrict__ q, int G, float scale,
                                                                         float *__restrict__ part, float *__restrict__ out) {
   constexpr int NK = HD / 16, ND = HD / 32, UN = 16 * HD;  // halves of a unit
@@ -380,10 +368,10 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, col = lane & 31, KH = P.KH, H = G * KH, us = P.shift - 4;
   const int kvh = blockIdx.x % KH, item = blockIdx.x / KH;
-  const int i = entry_of(U.off, R.n, item), row0 = R.row0[i], T = R.rows(i), pos = R.pos[i], per = U.per[i];
+  const PageEntry E = entry_of(U.it, item);
+  const int row0 = E.row0, T = E.rows, pos = E.pos, per = E.per, runs = E.runs;
   const int64_t NC = (int64_t)T * G;
-  const int nz = (int)((NC + kManyCols - 1) / kManyCols), runs = (U.off[i + 1] - U.off[i]) / nz;
-  const int run = (item - U.off[i]) % runs, r = (item - U.off[i]) / runs;
+  const int nz = (int)((NC + kManyCols - 1) / kManyCols), run = (item - E.off) % runs, r = (item - E.off) / runs;
   // longest and shortest rows in turn: the workgroups that share a CU (the grid's halves) add up
   const int z = r < (nz + 1) / 2 ? nz - 1 - r : r - (nz + 1) / 2;
   const int64_t z0 = (int64_t)z * kManyCols, w0 = z0 + 32 * wv, u = w0 + col, uc = u < NC ? u : NC - 1;
@@ -397,7 +385,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   // The pages of 16 steps: lane l has unit l of theirs; those of the 16 after them are loaded ahead.
   auto page_of = [&](int first) __attribute__((always_inline)) {
     const int j = kManyUnits * first + lane;
-    return j < nu && first < i1 ? P.id(R.seq[i], (U.base + j) >> us) : -1;
+    return j < nu && first < i1 ? P.id(E.seq, (U.base + j) >> us) : -1;
   };
   int ids = page_of(i0), ahead = page_of(i0 + 16);
   uint64_t there = __ballot(ids >= 0);
@@ -577,7 +565,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   if (u >= NC) return;
   const int64_t at = (int64_t)t * H + h;
   const bool whole = U.alone && runs == 1;
-  float *op = whole ? out + ((int64_t)row0 * H + at) * HD : part + ((int64_t)U.rec[i] * H + at * runs + run) * (HD + 4);
+  float *op = whole ? out + ((int64_t)row0 * H + at) * HD : part + ((int64_t)E.rec * H + at * runs + run) * (HD + 4);
   const double f = whole ? 1.0 / L / kSpUp : 1.0;
 #pragma unroll
   for (int d = 0; d < ND; d++)
@@ -597,27 +585,26 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
 
 // ------------------------------------------------------------------------------- runs
 
-// The runs of a row of each entry (1 and alone: the output itself), where its records are, and the prefix' runs of every row.
+// The entries whose rows have records, a row an item, and the prefix' runs of every row.
 struct PagedRuns {
-  int n[kPgRows], rec[kPgRows];
-  int pre, pre_rec, alone, sparse;
+  PageItems it;
+  int pre, pre_rec;
 };
 
 // The records of a row's runs under their largest maximum. A workgroup per (row, head): the runs' factors once, into LDS; then
 // HD / 4 threads to a record, the records over the groups in turn, each group's sum in order and the groups' in order.
 template <int HD>
-__global__ __launch_bounds__(256) void paged_join_kernel(const float *__restrict__ part, int H, PageRows R, PagedRuns U,
+__global__ __launch_bounds__(256) void paged_join_kernel(const float *__restrict__ part, int H, PagedRuns U,
                                                          float *__restrict__ out) {
   constexpr int TH = HD / 4, NG = 256 / TH;
   __shared__ float f[kPgRuns], sm[4];
   __shared__ double sl[4];
   __shared__ sf4 so[NG][TH];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, i = U.sparse ? 0 : entry_of(R.row0, R.n, (int)(row / H));
-  const int own = U.n[i], n = U.pre + own;
-  if (own == 1 && U.alone) return;
+  const PageEntry E = entry_of(U.it, blockIdx.x / H);
+  const int64_t at = (int64_t)blockIdx.x - (int64_t)E.off * H, row = (int64_t)E.row0 * H + at;  // (row, head) pairs
+  const int tid = threadIdx.x, n = U.pre + E.runs;
   const float *pre = part + ((int64_t)U.pre_rec * H + row * U.pre) * (HD + 4);
-  const float *ours = part + ((int64_t)U.rec[i] * H + (row - (U.sparse ? 0 : (int64_t)R.row0[i] * H)) * own) * (HD + 4);
+  const float *ours = part + ((int64_t)E.rec * H + at * E.runs) * (HD + 4);
   auto record = [&](int k) { return k < U.pre ? pre + k * (HD + 4) : ours + (k - U.pre) * (HD + 4); };
   static_assert(kPgRuns == 256, "a thread per run");
   const float *mine = record(tid < n ? tid : n - 1);
@@ -675,7 +662,7 @@ static int few_per(int n, int units) {
 
 // Steps of each run of an entry whose longest columns take n steps, in nz workgroups of columns a KV head.
 static int many_per(int n, int64_t wgs) {
-  int64_t S = wgs >= 256 ? 1 : (512 + wgs - 1) / wgs;
+  int64_t S = wgs >= 256 ? 1 : 512 / wgs;  // two workgroups fit a CU: one more than that is a second round
   S = S > n ? n : S;
   S = S > kPgRuns / 2 ? kPgRuns / 2 : S;
   return ceil_div(n, S);
@@ -684,75 +671,63 @@ static int many_per(int n, int64_t wgs) {
 // The launches of a call: the prefix (few or many columns), the entries of few columns, those of many.
 struct PagedLaunches {
   PagedPlan pre, few, many;
-  PageRows all;  // the rows of the prefix, as one entry
   bool pre_few = false;
   PagedRuns runs;
   int records = 0;  // of a head
 };
 
-// most, chosen: the pages that a row may take, and those that any row of the call has.
-static void paged_launches(const PagePool &p, const PageRows &r, int H, int prefix, int most, int chosen, PagedLaunches &L) {
-  const int G = H / p.KH, rows = r.row0[r.n], base = prefix / kPgUnit;
+// most: the pages that a row may take (0: all positions).
+static void paged_launches(const PagePool &p, const PageRows &r, int H, int prefix, int most, PagedLaunches &L) {
+  const int G = H / p.KH, rows = r.row0[r.n], base = prefix / kPgUnit, upp = p.page / kPgUnit;
   L.runs.pre = L.runs.pre_rec = 0;
-  L.runs.alone = L.few.alone = L.many.alone = !prefix;
-  L.runs.sparse = most > 0;
+  L.few.alone = L.many.alone = !prefix;
   L.few.inc = L.many.inc = 1;
   L.few.base = L.many.base = base;
-  L.few.off[0] = L.many.off[0] = 0;
-  if (most) {  // rows one by one, cut by a rule on the choice alone, all with as many runs
-    L.few.per[0] = few_per(ceil_div((int64_t)most << (p.shift - 4), 2), p.KH * ceil_div(G, kFewCols));
-    L.few.off[1] = L.runs.n[0] = ceil_div(ceil_div((int64_t)chosen << (p.shift - 4), 2), L.few.per[0]);
-    L.few.rec[0] = L.runs.rec[0] = 0;
-    if (L.runs.n[0] > 1) L.records = rows * L.runs.n[0];
-    return;
-  }
   if (prefix) {
+    PageRows all;  // the rows of all entries, without a mask
+    all.n = 1;
+    all.seq[0] = r.seq[0];
+    all.pos[0] = prefix - 1;
+    all.row0[0] = 0;
+    all.row0[1] = rows;
     const int64_t NC = (int64_t)rows * G;
-    L.all.n = 1;
-    L.all.seq[0] = r.seq[0];
-    L.all.pos[0] = prefix - 1;
-    L.all.row0[0] = 0;
-    L.all.row0[1] = rows;
     L.pre_few = is_few(NC);
     const int blocks = ceil_div(NC, L.pre_few ? kFewCols : kManyCols);
     const int n = ceil_div(prefix / kPgUnit, L.pre_few ? 2 : kManyUnits);
-    L.pre.per[0] = L.pre_few ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
-    L.runs.pre = ceil_div(n, L.pre.per[0]);
-    L.pre.off[0] = L.pre.inc = L.pre.base = L.pre.rec[0] = L.pre.alone = 0;
-    L.pre.off[1] = L.runs.pre * blocks;
+    const int per = L.pre_few ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
+    L.runs.pre = ceil_div(n, per);
+    L.pre.inc = L.pre.base = L.pre.alone = 0;
+    L.pre.it.add(all, 0, L.runs.pre * blocks, per, 0, L.runs.pre);
     L.records = rows * L.runs.pre;
   }
   for (int i = 0; i < r.n; i++) {
-    const int T = r.rows(i);
-    L.few.off[i + 1] = L.few.off[i];
-    L.many.off[i + 1] = L.many.off[i];
-    L.few.rec[i] = L.many.rec[i] = L.runs.rec[i] = L.records;
-    L.runs.n[i] = 1;
+    const int T = r.rows(i), last = r.pos[i] + T - 1;
     if (!T) continue;
     const int64_t NC = (int64_t)T * G;
-    const int units = ((r.pos[i] + T - 1) >> 4) - base + 1;
-    const bool f = is_few(NC);
-    PagedPlan &U = f ? L.few : L.many;
-    const int blocks = ceil_div(NC, f ? kFewCols : kManyCols), n = ceil_div(units, f ? 2 : kManyUnits);
-    U.per[i] = f ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
-    L.runs.n[i] = ceil_div(n, U.per[i]);
-    U.off[i + 1] += L.runs.n[i] * blocks;
-    if (L.runs.n[i] > 1 || prefix) L.records += T * L.runs.n[i];
+    const bool f = most || is_few(NC);
+    int blocks, per, runs;
+    if (most) {  // rows one by one, cut by a rule on the choice alone
+      const int took = std::min((last >> p.shift) + 1, most);
+      blocks = T * ceil_div(G, kFewCols);
+      per = few_per(ceil_div((int64_t)most * upp, 2), p.KH * ceil_div(G, kFewCols));
+      runs = ceil_div(ceil_div((int64_t)took * upp, 2), per);
+    } else {
+      const int units = (last >> 4) - base + 1, n = ceil_div(units, f ? 2 : kManyUnits);
+      blocks = ceil_div(NC, f ? kFewCols : kManyCols);
+      per = f ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
+      runs = ceil_div(n, per);
+    }
+    (f ? L.few : L.many).it.add(r, i, runs * blocks, per, L.records, runs);
+    if (runs == 1 && !prefix) continue;
+    L.runs.it.add(r, i, T, 0, L.records, runs);
+    L.records += T * runs;
   }
-}
-
-// Pages of a choice that any row of a call has: of a short context fewer than the choice takes.
-static int chosen(const PagePool &p, const PageRows &r, int most) {
-  int n = 1;
-  for (int i = 0; i < r.n; i++)
-    if (r.rows(i)) n = std::max(n, ((r.pos[i] + r.rows(i) - 1) >> p.shift) + 1);
-  return std::min(n, most);
 }
 
 int64_t paged_attention_scratch_floats(const PagePool &p, const PageRows &r, int H, int prefix, int most) {
   if (r.row0[r.n] <= 0) return 0;
   PagedLaunches L;
-  paged_launches(p, r, H, prefix, most, chosen(p, r, most), L);
+  paged_launches(p, r, H, prefix, most, L);
   return (int64_t)L.records * H * (p.HD + 4);
 }
 
@@ -760,31 +735,28 @@ template <int HD>
 static hipError_t paged_attend(const PagePool &p, const PageRows &r, const float *q, int H, int prefix, const int32_t *blocks,
                                int most, float scale, float *part, float *out, hipStream_t st) {
   PagedLaunches L;
-  paged_launches(p, r, H, prefix, most, chosen(p, r, most), L);
-  const int G = H / p.KH, rows = r.row0[r.n];
+  paged_launches(p, r, H, prefix, most, L);
+  const int G = H / p.KH;
   hipError_t e = hipSuccess;
-  auto few = [&](const PageRows &R, const PagedPlan &U, int items) {
-    hipLaunchKernelGGL((paged_few_kernel<HD, false>), dim3((unsigned)items * p.KH), dim3(64 * kFewWaves), 0, st, p, R, U, q,
-                       G, nullptr, 0, scale, part, out);
+  auto few = [&](const PagedPlan &U) {
+    const dim3 grid((unsigned)U.it.items * p.KH), block(64 * kFewWaves);
+    if (blocks)
+      hipLaunchKernelGGL((paged_few_kernel<HD, true>), grid, block, 0, st, p, U, q, G, blocks, most, scale, part, out);
+    else
+      hipLaunchKernelGGL((paged_few_kernel<HD, false>), grid, block, 0, st, p, U, q, G, nullptr, 0, scale, part, out);
     e = hipGetLastError();
   };
-  auto many = [&](const PageRows &R, const PagedPlan &U, int items) {
-    hipLaunchKernelGGL(paged_many_kernel<HD>, dim3((unsigned)items * p.KH), dim3(64 * kManyWaves), 0, st, p, R, U, q, G,
+  auto many = [&](const PagedPlan &U) {
+    hipLaunchKernelGGL(paged_many_kernel<HD>, dim3((unsigned)U.it.items * p.KH), dim3(64 * kManyWaves), 0, st, p, U, q, G,
                        scale, part, out);
     e = hipGetLastError();
   };
-  if (blocks) {
-    const int64_t items = (int64_t)rows * ceil_div(G, kFewCols) * L.few.off[1];
-    hipLaunchKernelGGL((paged_few_kernel<HD, true>), dim3((unsigned)(items * p.KH)), dim3(64 * kFewWaves), 0, st, p, r, L.few,
-                       q, G, blocks, most, scale, part, out);
-    e = hipGetLastError();
-  } else {
-    if (prefix) (L.pre_few ? few(L.all, L.pre, L.pre.off[1]) : many(L.all, L.pre, L.pre.off[1]));
-    if (e == hipSuccess && L.many.off[r.n]) many(r, L.many, L.many.off[r.n]);
-    if (e == hipSuccess && L.few.off[r.n]) few(r, L.few, L.few.off[r.n]);
-  }
+  if (prefix) L.pre_few ? few(L.pre) : many(L.pre);
+  if (e == hipSuccess && L.many.it.n) many(L.many);
+  if (e == hipSuccess && L.few.it.n) few(L.few);
   if (e != hipSuccess || !L.records) return e;
-  hipLaunchKernelGGL(paged_join_kernel<HD>, dim3((unsigned)((int64_t)rows * H)), dim3(256), 0, st, part, H, r, L.runs, out);
+  hipLaunchKernelGGL(paged_join_kernel<HD>, dim3((unsigned)((int64_t)L.runs.it.items * H)), dim3(256), 0, st, part, H, L.runs,
+                     out);
   return hipGetLastError();
 }
 

@@ -26,11 +26,6 @@ struct OpenPages {
   }
 };
 
-// Entry i's items begin at off[i], per[i] workgroups for each of its rows.
-struct ScorePlan {
-  int off[kPgRows + 1], per[kPgRows];
-};
-
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // A whole number in the order of x, a score that is not finite as +inf; 0 is no page.
@@ -44,16 +39,17 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 // and lane l has the channels l / 16 * HD / 4 on of both, so that its loads are whole and the largest of a column is the page's
 // score in whatever order the rows come out.
 template <int HD>
-__global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageRows R, ScorePlan U, PageSelect S,
+__global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
                                                           const float *__restrict__ q, int G, uint64_t *__restrict__ keys,
                                                           int64_t width) {
   constexpr int N = HD / 4;
   const int lane = threadIdx.x & 63, x = lane & 15, k = lane >> 4;
   const int kvh = blockIdx.x % P.KH, item = blockIdx.x / P.KH, H = G * P.KH;
-  const int i = entry_of(U.off, R.n, item), t = (item - U.off[i]) / U.per[i], row = R.row0[i] + t;
-  const OpenPages o(S, (R.pos[i] + t) >> P.shift);
-  const int j = o.from + (item - U.off[i]) % U.per[i] * kScorePages + (threadIdx.x >> 6) * 16 + x;
-  const int id = j < o.to ? P.id(R.seq[i], j) : -1;
+  const PageEntry E = entry_of(U, item);  // per workgroups for each of its rows
+  const int t = (item - E.off) / E.per, row = E.row0 + t;
+  const OpenPages o(S, (E.pos + t) >> P.shift);
+  const int j = o.from + (item - E.off) % E.per * kScorePages + (threadIdx.x >> 6) * 16 + x;
+  const int id = j < o.to ? P.id(E.seq, j) : -1;
   const uint16_t *b = P.bounds + ((int64_t)(id < 0 ? 0 : id) * P.KH + kvh) * 2 * HD + k * N;
   fh8 lo[N / 8], hi[N / 8];
 #pragma unroll
@@ -102,15 +98,15 @@ __device__ __forceinline__ int block_scan(int v, int *sh, int &all) {
 
 // A workgroup per row and KV head. Thread t has pages t * m .. of the m = ceil(n / 256) each has, in registers up to kOwn of them.
 template <int kOwn>
-__global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageRows R, PageSelect S,
+__global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageItems U, PageSelect S,
                                                          const uint64_t *__restrict__ keys, int64_t width,
                                                          int32_t *__restrict__ blocks) {
   constexpr int BINS = 1024;
   __shared__ int bins[BINS], sh[4], pick[3];
   __shared__ uint64_t ends[2][4];
   const int kvh = blockIdx.x % P.KH, row = blockIdx.x / P.KH, tid = threadIdx.x;
-  const int i = entry_of(R.row0, R.n, row);
-  const int cur = (R.pos[i] + row - R.row0[i]) >> P.shift;
+  const PageEntry E = entry_of(U, row);
+  const int cur = (E.pos + row - E.row0) >> P.shift;
   const OpenPages o(S, cur);
   const int n = o.to - o.from, m = (n + 255) / 256;
   const uint64_t *kp = keys + ((int64_t)row * P.KH + kvh) * width;
@@ -237,24 +233,24 @@ hipError_t paged_select_launch(const PagePool &p, const PageRows &r, const float
   if (rows <= 0) return hipSuccess;
   const int64_t width = open_width(p, r, s);
   uint64_t *keys = (uint64_t *)scratch;
-  ScorePlan U;
-  U.off[0] = 0;
+  PageItems U, each;
   for (int i = 0; i < r.n; i++) {
     const int T = r.rows(i);
     const OpenPages o(s, T ? (r.pos[i] + T - 1) >> p.shift : 0);
-    U.per[i] = T ? std::max(0, (o.to - o.from + kScorePages - 1) / kScorePages) : 0;
-    U.off[i + 1] = U.off[i] + T * U.per[i];
+    const int per = (o.to - o.from + kScorePages - 1) / kScorePages;
+    U.add(r, i, T * per, per);
+    each.add(r, i, T);
   }
-  if (U.off[r.n]) {
-    const dim3 grid((unsigned)((int64_t)U.off[r.n] * p.KH));
-    if (p.HD == 64) hipLaunchKernelGGL(paged_score_kernel<64>, grid, dim3(256), 0, st, p, r, U, s, q, G, keys, width);
-    else hipLaunchKernelGGL(paged_score_kernel<128>, grid, dim3(256), 0, st, p, r, U, s, q, G, keys, width);
+  if (U.n) {
+    const dim3 grid((unsigned)((int64_t)U.items * p.KH));
+    if (p.HD == 64) hipLaunchKernelGGL(paged_score_kernel<64>, grid, dim3(256), 0, st, p, U, s, q, G, keys, width);
+    else hipLaunchKernelGGL(paged_score_kernel<128>, grid, dim3(256), 0, st, p, U, s, q, G, keys, width);
     if (const hipError_t e = hipGetLastError()) return e;
   }
   const dim3 grid((unsigned)(rows * p.KH));
-  if (width <= 256 * 4) hipLaunchKernelGGL(paged_take_kernel<4>, grid, dim3(256), 0, st, p, r, s, keys, width, blocks);
-  else if (width <= 256 * 16) hipLaunchKernelGGL(paged_take_kernel<16>, grid, dim3(256), 0, st, p, r, s, keys, width, blocks);
-  else hipLaunchKernelGGL(paged_take_kernel<0>, grid, dim3(256), 0, st, p, r, s, keys, width, blocks);
+  if (width <= 256 * 4) hipLaunchKernelGGL(paged_take_kernel<4>, grid, dim3(256), 0, st, p, each, s, keys, width, blocks);
+  else if (width <= 256 * 16) hipLaunchKernelGGL(paged_take_kernel<16>, grid, dim3(256), 0, st, p, each, s, keys, width, blocks);
+  else hipLaunchKernelGGL(paged_take_kernel<0>, grid, dim3(256), 0, st, p, each, s, keys, width, blocks);
   return hipGetLastError();
 }
 

@@ -24,4 +24,22 @@ __device__ __forceinline__ void rope_cs(int p, int i, int half, double theta_sca
   s = (float)sin(a);
 }
 
+// The same in two steps, for many positions at once. Lane r of a wave makes the products of position p, theta[i][r] after i steps
+// (ROWS positions a step, i below half); the cosine and sine of a pair from its product.
+template <int ROWS>
+__device__ __forceinline__ void rope_chain(double *theta, int r, int p, int half, double theta_scale, double freq_scale) {
+#pragma clang fp contract(off)
+  double t = (double)p * freq_scale;
+  for (int i = 0; i < half; i++) {
+    theta[i * ROWS + r] = t;
+    t *= theta_scale;
+  }
+}
+__device__ __forceinline__ void rope_cs_of(double theta, float freq, bool has, float &c, float &s) {
+#pragma clang fp contract(off)
+  const double a = has ? theta / (double)freq : theta;
+  c = (float)cos(a);
+  s = (float)sin(a);
+}
+
 }  // namespace wl
