@@ -1,9 +1,9 @@
 // wl_paged_select.hip - the pages that a row and KV head attends to, by a bound of their scores (wl_paged.h).
 //
 // The score of a page is the largest, over the heads g of the group, of sum_d max(q_gd, 0) hi_d + min(q_gd, 0) lo_d: a product
-// of the heads' [2 HD] halves with the pages', in 64 bits on v_mfma_f64_16x16x4_f64, since which page is taken must not hang on
-// a rounding (a product of a 24-bit query and an 11-bit bound is exact, a sum of 256 of them off by 2^-45 of its terms). Scores
-// are kept as whole numbers of the same order, and the pages taken are those from a border (score, page) on, found by
+// of the heads' [2 HD] halves with the pages', in 64 bits on v_mfma_f64_4x4x4_f64 (four heads to 16 pages), since which page is
+// taken must not hang on a rounding (a product of a 24-bit query and an 11-bit bound is exact, a sum of 256 of them off by 2^-45
+// of its terms). Scores are kept as whole numbers of the same order, and the pages taken are those from a border (score, page) on, found by
 // histograms of a narrowing range.
 #include "wl_paged.h"
 
@@ -26,8 +26,6 @@ struct OpenPages {
   }
 };
 
-typedef double f64x4 __attribute__((ext_vector_type(4)));
-
 // A whole number in the order of x, a score that is not finite as +inf; 0 is no page.
 __device__ __forceinline__ uint64_t score_key(double x) {
   x = __builtin_isfinite(x) ? x : INFINITY;
@@ -35,14 +33,16 @@ __device__ __forceinline__ uint64_t score_key(double x) {
   return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-// A wave makes the scores of 16 pages: operand column l % 16 is a page, row l % 16 a head (past the group's last the last again),
-// and lane l has the channels l / 16 * HD / 4 on of both, so that its loads are whole and the largest of a column is the page's
-// score in whatever order the rows come out.
-template <int HD>
-__global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
+// A wave makes the scores of 16 pages: column l % 16 is a page, row l % 4 of four a head (past the group's last the last again),
+// and lane l has the channels l / 16 * HD / 4 on of both, so that its loads are whole. The rows come out in lanes l / 16; the
+// largest of a column is the page's score. The heads' halves lie in LDS in 64 bits: converting them in each wave took as long
+// as the products.
+template <int HD, int NB>
+__global__ __launch_bounds__(256, 4) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
                                                           const float *__restrict__ q, int G, uint64_t *__restrict__ keys,
                                                           int64_t width) {
   constexpr int N = HD / 4;
+  __shared__ double2 qs[NB * N * 16];  // [four heads][channel of a quarter][quarter][head]: (larger than 0, smaller)
   const int lane = threadIdx.x & 63, x = lane & 15, k = lane >> 4;
   const int kvh = blockIdx.x % P.KH, item = blockIdx.x / P.KH, H = G * P.KH;
   const PageEntry E = entry_of(U, item);  // per workgroups for each of its rows
@@ -58,21 +58,32 @@ __global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems 
     hi[e] = *reinterpret_cast<const fh8 *>(b + HD + 8 * e);
   }
   double best = -INFINITY;
-  for (int g0 = 0; g0 < G; g0 += 16) {
-    const int g = g0 + x < G ? g0 + x : G - 1;
-    const float *qp = q + ((int64_t)row * H + kvh * G + g) * HD + k * N;
-    f64x4 a0 = {0.0, 0.0, 0.0, 0.0}, a1 = a0;
+  for (int g0 = 0; g0 < G; g0 += 4 * NB) {
+    if (g0) __syncthreads();
+#pragma unroll
+    for (int e = threadIdx.x; e < 4 * NB * HD; e += 256) {
+      const int g = e / HD, d = e % HD;
+      const float v = q[((int64_t)row * H + kvh * G + (g0 + g < G ? g0 + g : G - 1)) * HD + d];
+      // a NaN goes with both
+      qs[(g / 4 * N + d % N) * 16 + d / N * 4 + g % 4] = make_double2((double)(v < 0.f ? 0.f : v), (double)(v > 0.f ? 0.f : v));
+    }
+    __syncthreads();
+    double up[NB], down[NB];
+#pragma unroll
+    for (int h = 0; h < NB; h++) up[h] = down[h] = 0.0;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      const float v = qp[e];
-      // a NaN goes with both
-      const double up = (double)(v < 0.f ? 0.f : v), down = (double)(v > 0.f ? 0.f : v);
-      a0 = __builtin_amdgcn_mfma_f64_16x16x4f64(up, (double)(float)hi[e / 8][e % 8], a0, 0, 0, 0);
-      a1 = __builtin_amdgcn_mfma_f64_16x16x4f64(down, (double)(float)lo[e / 8][e % 8], a1, 0, 0, 0);
+      const double bh = (double)(float)hi[e / 8][e % 8], bl = (double)(float)lo[e / 8][e % 8];
+#pragma unroll
+      for (int h = 0; h < NB; h++) {
+        const double2 a = qs[(h * N + e) * 16 + k * 4 + (lane & 3)];
+        up[h] = __builtin_amdgcn_mfma_f64_4x4x4f64(a.x, bh, up[h], 0, 0, 0);
+        down[h] = __builtin_amdgcn_mfma_f64_4x4x4f64(a.y, bl, down[h], 0, 0, 0);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const double s = a0[e] + a1[e];
+    for (int h = 0; h < NB; h++) {
+      const double s = up[h] + down[h];
       best = fmax(best, __builtin_isfinite(s) ? s : INFINITY);
     }
   }
@@ -81,19 +92,40 @@ __global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems 
   if (k == 0 && j < o.to) keys[((int64_t)row * P.KH + kvh) * width + j - o.from] = id < 0 ? 0 : score_key(best);
 }
 
+template <int HD>
+static void score_launch(dim3 grid, const PagePool &p, const PageItems &U, const PageSelect &s, const float *q, int G,
+                         uint64_t *keys, int64_t width, hipStream_t st) {
+  auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p, U, s, q, G, keys, width); };
+  if (G <= 4) run(paged_score_kernel<HD, 1>);
+  else if (G <= 8) run(paged_score_kernel<HD, 2>);
+  else run(paged_score_kernel<HD, 4>);
+}
+
 // Sum over the workgroup's 256 threads up to and with this one, and of all.
 __device__ __forceinline__ int block_scan(int v, int *sh, int &all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int o = __shfl_up(v, m, 64);
-    v += lane >= m ? o : 0;
-  }
+  // within rows of 16 lanes by shifts, then each row's last into the rows after it
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31), r2 = __builtin_amdgcn_readlane(v, 47);
+  v += (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
   __syncthreads();
   if (lane == 63) sh[w] = v;
   __syncthreads();
   all = (sh[0] + sh[1]) + (sh[2] + sh[3]);
   return v + (w > 0 ? sh[0] : 0) + (w > 1 ? sh[1] : 0) + (w > 2 ? sh[2] : 0);
+}
+
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+  auto up = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  v = up(v, dpp32<0xB1>(v));
+  v = up(v, dpp32<0x4E>(v));
+  v = up(v, dpp32<0x124>(v));
+  v = up(v, dpp32<0x128>(v));
+  auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+  return up(up(at(0), at(16)), up(at(32), at(48)));
 }
 
 // A workgroup per row and KV head. Thread t has pages t * m .. of the m = ceil(n / 256) each has, in registers up to kOwn of them.
@@ -103,7 +135,7 @@ __global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageItems U
                                                          int32_t *__restrict__ blocks) {
   constexpr int BINS = 1024;
   __shared__ int bins[BINS], sh[4], pick[3];
-  __shared__ uint64_t ends[2][4];
+  __shared__ uint32_t ends[2][4];
   const int kvh = blockIdx.x % P.KH, row = blockIdx.x / P.KH, tid = threadIdx.x;
   const PageEntry E = entry_of(U, row);
   const int cur = (E.pos + row - E.row0) >> P.shift;
@@ -128,27 +160,24 @@ __global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageItems U
     }
   };
   int all = 0;
-  uint64_t lo = ~0ull, hi = 0;
+  uint32_t least = ~0u, most = 0;  // of the keys' high words
   each([&](uint64_t v, int) {
     all++;
-    lo = v < lo ? v : lo;
-    hi = v > hi ? v : hi;
+    least = (uint32_t)(v >> 32) < least ? (uint32_t)(v >> 32) : least;
+    most = (uint32_t)(v >> 32) > most ? (uint32_t)(v >> 32) : most;
   });
-#pragma unroll
-  for (int x = 32; x; x >>= 1) {
-    const uint64_t a = __shfl_xor(lo, x, 64), b = __shfl_xor(hi, x, 64);
-    lo = a < lo ? a : lo;
-    hi = b > hi ? b : hi;
-  }
+  least = ~wave_max_u(~least);
+  most = wave_max_u(most);
   if ((tid & 63) == 0) {
-    ends[0][tid >> 6] = lo;
-    ends[1][tid >> 6] = hi;
+    ends[0][tid >> 6] = least;
+    ends[1][tid >> 6] = most;
   }
   (void)block_scan(all, sh, all);  // its barriers also order the ends
   for (int w = 0; w < 4; w++) {
-    lo = ends[0][w] < lo ? ends[0][w] : lo;
-    hi = ends[1][w] > hi ? ends[1][w] : hi;
+    least = ends[0][w] < least ? ends[0][w] : least;
+    most = ends[1][w] > most ? ends[1][w] : most;
   }
+  uint64_t lo = (uint64_t)least << 32, hi = (uint64_t)most << 32 | 0xffffffffu;
   // The border: pages of a key above `key`, and those of that key up to page `upto`. `need` of the pages in lo .. hi (by key, then,
   // among equal keys, by page from the last) are taken, and all above hi.
   uint64_t key = 0;
@@ -243,8 +272,8 @@ hipError_t paged_select_launch(const PagePool &p, const PageRows &r, const float
   }
   if (U.n) {
     const dim3 grid((unsigned)((int64_t)U.items * p.KH));
-    if (p.HD == 64) hipLaunchKernelGGL(paged_score_kernel<64>, grid, dim3(256), 0, st, p, U, s, q, G, keys, width);
-    else hipLaunchKernelGGL(paged_score_kernel<128>, grid, dim3(256), 0, st, p, U, s, q, G, keys, width);
+    if (p.HD == 64) score_launch<64>(grid, p, U, s, q, G, keys, width, st);
+    else score_launch<128>(grid, p, U, s, q, G, keys, width, st);
     if (const hipError_t e = hipGetLastError()) return e;
   }
   const dim3 grid((unsigned)(rows * p.KH));
