@@ -447,6 +447,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
   const float past = past_of(c2);
   double L = 0.0;
+  if (__builtin_amdgcn_s_getreg((4 - 1) << 11 | 0 << 6 | 4) & 1) __builtin_amdgcn_s_setprio(1);
   landed();
   __syncthreads();
 #pragma unroll 1
@@ -708,16 +709,20 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Columns that paged_few_kernel takes.
 static bool is_few(int64_t columns) { return columns <= 64; }
 
-// Tiles of each run of a row of n tiles, of `units` workgroups a run (a rule on the entry alone).
-static int few_per(int n, int units) {
-  if (n <= 16) return n;
-  const int64_t all = (int64_t)n * units;
-  int64_t per = 4 * kFewWaves, one = (all + 255) / 256, two = (all + 511) / 512;
-  if (n <= 160) per = one < kFewWaves ? kFewWaves : one < per ? one : per;
-  per = per < two ? two : per;
-  const int most = ceil_div(n, kPgRuns / 2);
-  return per < most ? most : (int)per;
+// Tiles of each run of an entry of n tiles, of `units` workgroups a run: a rule on the entry alone, so that its bits do not depend
+// on the others. Up to `whole` tiles one run, and no second launch; then runs of `least` tiles (four waves of two or four), for what a
+// run costs beside its tiles (the query's parts, the waves' sums, its record) weighs in a batch: 64 rows of up to 1,000 (70B) 33.5
+// us whole and 52.4 with a tile a wave, 32 rows of up to 3,000 54.6 and 67.3; a lone row of 1,000 or 2,000 pays 1.9-2.1 us for it
+// (11.2 and 9.3, 11.8 and 9.8), of 4,000 1.2. Long rows take no more runs than give every CU two workgroups.
+static int few_per(int n, int units, int whole, int least) {
+  if (n <= whole) return n;
+  const int two = (int)(((int64_t)n * units + 511) / 512), most = ceil_div(n, kPgRuns / 2);
+  return std::max({least, two, most});
 }
+constexpr int kFewWhole = 32, kFewLeast = 16;
+// Chosen pages: 16 rows of 32 pages of 64 (70B) 53.5 us with two tiles a wave, 49.8 with four and 58.6 with one; a lone row of 64
+// pages 25.6, 26.8 and 24.8.
+constexpr int kChosenWhole = 16, kChosenLeast = 8;
 
 // Steps of each run of an entry whose longest columns take n steps, in nz workgroups of columns a KV head.
 static int many_per(int n, int64_t wgs) {
@@ -753,7 +758,7 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
     L.pre_few = is_few(NC);
     const int blocks = ceil_div(NC, L.pre_few ? kFewCols : kManyCols);
     const int n = ceil_div(prefix / kPgUnit, L.pre_few ? 2 : kManyUnits);
-    const int per = L.pre_few ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
+    const int per = L.pre_few ? few_per(n, p.KH * blocks, kFewWaves, kFewWaves) : many_per(n, (int64_t)p.KH * blocks);
     L.runs.pre = ceil_div(n, per);
     L.pre.inc = L.pre.base = L.pre.alone = 0;
     L.pre.it.add(all, 0, L.runs.pre * blocks, per, 0, L.runs.pre);
@@ -768,12 +773,12 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
     if (most) {  // rows one by one, cut by a rule on the choice alone
       const int took = std::min((last >> p.shift) + 1, most);
       blocks = T * ceil_div(G, kFewCols);
-      per = few_per(ceil_div((int64_t)most * upp, 2), p.KH * ceil_div(G, kFewCols));
+      per = few_per(ceil_div((int64_t)most * upp, 2), p.KH * ceil_div(G, kFewCols), kChosenWhole, kChosenLeast);
       runs = ceil_div(ceil_div((int64_t)took * upp, 2), per);
     } else {
       const int units = (last >> 4) - base + 1, n = ceil_div(units, f ? 2 : kManyUnits);
       blocks = ceil_div(NC, f ? kFewCols : kManyCols);
-      per = f ? few_per(n, p.KH * blocks) : many_per(n, (int64_t)p.KH * blocks);
+      per = f ? few_per(n, p.KH * blocks, kFewWhole, kFewLeast) : many_per(n, (int64_t)p.KH * blocks);
       runs = ceil_div(n, per);
     }
     (f ? L.few : L.many).it.add(r, i, runs * blocks, per, L.records, runs);
