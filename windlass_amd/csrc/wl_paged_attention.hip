@@ -48,6 +48,18 @@ __device__ __forceinline__ void query_parts(float x, float f, _Float16 &hi, _Flo
   lo = (_Float16)(__builtin_isinf(X) ? 0.f : X - (float)hi);  // an infinity is all in its high part
 }
 
+// Weights are exp2 of a score's difference from the column's maximum M, times 2^8: all that follows is by their sum. M is one of
+// the scores seen, and is raised only where a step's weights would pass 2^15 (fp16 parts end at 2^16) or a column has none yet, so
+// that no step looks for its maximum. The largest weighs 2^8 at least; two parts are 22 bits of a weight down to 2^-14, and 2^-25 below.
+constexpr float kUp = 8.f, kFull = 0x1p15f;
+__device__ __forceinline__ float weight(float s, float M, float c2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s - M, c2, kUp)); }
+// Two weights as their fp16 parts: the high ones cut, the low ones what is left, rounded.
+__device__ __forceinline__ void weight_parts(float a, float b, uint32_t &hi, uint32_t &lo) {
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  asm("" : "+v"(hi));
+  lo = __builtin_bit_cast(uint32_t, fh2{(_Float16)__builtin_fmaf(a, 1.f, -half_lo(hi)), (_Float16)__builtin_fmaf(b, 1.f, -half_hi(hi))});
+}
+
 // Bits 15 and 31 set where a half of w is an infinity or NaN: its exponent's ones carry.
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
 
@@ -206,8 +218,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
   sf4 O[ND];
 #pragma unroll
   for (int d = 0; d < ND; d++) O[d] = sf4{0.f, 0.f, 0.f, 0.f};
-  float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
-  const float past = past_of(c2);
+  float M = -INFINITY;
   double L = 0.0;
 #pragma unroll 1
   for (; tile < i1; tile += W) {
@@ -247,42 +258,47 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
       for (int d = 0; d < ND; d++) bad |= clear_unseen(a.v[d], at, pa, pb);
       bad = __any(bad);
     }
-    float mt = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
-                     fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
-    if (__any(mt > top)) {
+    float e[8], ts;
+    auto weigh = [&]() __attribute__((always_inline)) {
+      const float Mu = M == -INFINITY ? 0.f : M;  // no score of this column yet: all are -inf
+#pragma unroll
+      for (int j = 0; j < 8; j++) e[j] = weight(S[j >> 2][j & 3], Mu, c2);
+      ts = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    };
+    weigh();
+    if (__any(!(ts < kFull) || M == -INFINITY)) {
+      asm volatile("");
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < 8; j++) odd |= S[j >> 2][j & 3] != S[j >> 2][j & 3];
+      if (__any(odd)) {  // past an infinity the low parts' product means nothing: a score of -inf may be NaN here
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          sf4 A1 = sf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < NK; s++)
+            A1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.k[x][s]), qh[s], A1, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; j++) S[x][j] = A1[j] == -INFINITY && S[x][j] != S[x][j] ? -INFINITY : S[x][j];
+        }
+      }
+      float mt = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
+                       fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
       mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-      const bool raise = mt > top;
+      const bool raise = mt > M;
       const float al = raise ? __builtin_amdgcn_exp2f((M - mt) * c2) : 1.f;
       L *= (double)al;
 #pragma unroll
       for (int d = 0; d < ND; d++) O[d] *= al;
       M = raise ? mt : M;
-      top = M + past;
-    }
-    const float Mu = M == -INFINITY ? 0.f : M;  // no position of this column yet: every score is -inf
-    float e[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f((S[j >> 2][j & 3] - Mu) * c2);
-    float ts = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-    if (__any(ts != ts)) {  // past an infinity the low parts' product means nothing: a score of -inf may be NaN here
-      asm volatile("");
-#pragma unroll
-      for (int x = 0; x < 2; x++) {
-        sf4 A1 = sf4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < NK; s++)
-          A1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.k[x][s]), qh[s], A1, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 4; j++) e[4 * x + j] = A1[j] == -INFINITY && S[x][j] != S[x][j] ? 0.f : e[4 * x + j];
-      }
-      ts = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      weigh();
     }
     if (more) a.keys(P, oa, ob, lane);
     L += (double)ts;
     uint32_t ph[4], pl[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) split_pair(e[2 * j], e[2 * j + 1], ph[j], pl[j]);
+    for (int j = 0; j < 4; j++) weight_parts(e[2 * j], e[2 * j + 1], ph[j], pl[j]);
     const fh8 eh = as_fh8(ph[0], ph[1], ph[2], ph[3]), el = as_fh8(pl[0], pl[1], pl[2], pl[3]);
 #pragma unroll
     for (int d = 0; d < ND; d++) O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fh8, a.v[d]), el, O[d], 0, 0, 0);
@@ -333,7 +349,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
     }
     const int64_t at = (int64_t)(t0 + cc / G) * H + kvh * G + cc % G, row = (int64_t)E.row0 * H + at;
     if (whole) {
-      const double r = (1.0 / kSpUp) / l;
+      const double r = 1.0 / l;
 #pragma unroll
       for (int j = 0; j < 4; j++) o[j] = l == 0.0 ? 0.f : (float)((double)o[j] * r);
       *reinterpret_cast<f4a4 *>(out + row * HD + 4 * four) = o;
@@ -444,8 +460,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   for (int d = 0; d < ND; d++)
 #pragma unroll
     for (int e = 0; e < 16; e++) O[d][e] = 0.f;
-  float M = -INFINITY, top = -INFINITY;  // the running maximum, and what raises it
-  const float past = past_of(c2);
+  float M = -INFINITY;
   double L = 0.0;
   if (__builtin_amdgcn_s_getreg((4 - 1) << 11 | 0 << 6 | 4) & 1) __builtin_amdgcn_s_setprio(1);
   landed();
@@ -480,12 +495,38 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
 #pragma unroll
           for (int e = 0; e < 16; e++) S[e] = up[e >> 3] + 8 * hf + (e & 7) > (uint32_t)p ? -INFINITY : S[e];
         }
-        float mt = S[0];
+        float w[16], tt;
+        auto weigh = [&]() __attribute__((always_inline)) {
+          const float Mu = M == -INFINITY ? 0.f : M;  // no score of this column yet: all are -inf
+          float tx[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 1; e < 16; e++) mt = fmaxf(mt, S[e]);
-        if (__any(mt > top)) {
+          for (int e = 0; e < 16; e++) {
+            w[e] = weight(S[e], Mu, c2);
+            tx[e & 3] += w[e];
+          }
+          tt = (tx[0] + tx[1]) + (tx[2] + tx[3]);
+        };
+        weigh();
+        if (__any(!(tt < kFull) || M == -INFINITY)) {
+          asm volatile("");
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 16; e++) odd |= S[e] != S[e];
+          if (__any(odd)) {  // past an infinity the low parts' product means nothing: a score of -inf may be NaN here
+            sf16 A;
+#pragma unroll
+            for (int e = 0; e < 16; e++) A[e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+              A = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kb + 256 * k), qh[k], A, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 16; e++) S[e] = A[e] == -INFINITY && S[e] != S[e] ? -INFINITY : S[e];
+          }
+          float mt = S[0];
+#pragma unroll
+          for (int e = 1; e < 16; e++) mt = fmaxf(mt, S[e]);
           mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-          const bool raise = mt > top;
+          const bool raise = mt > M;
           const float al = raise ? __builtin_amdgcn_exp2f((M - mt) * c2) : 1.f;
           L *= (double)al;
           ts *= al;
@@ -494,31 +535,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
 #pragma unroll
             for (int e = 0; e < 16; e++) O[d][e] *= al;
           M = raise ? mt : M;
-          top = M + past;
-        }
-        const float Mu = M == -INFINITY ? 0.f : M;  // no position of this column yet: every score is -inf
-        float tx[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float w = __builtin_amdgcn_exp2f((S[e] - Mu) * c2);
-          tx[e & 3] += w;
-          S[e] = w;
-        }
-        float tt = (tx[0] + tx[1]) + (tx[2] + tx[3]);
-        if (__any(tt != tt)) {  // past an infinity the low parts' product means nothing: a score of -inf may be NaN here
-          asm volatile("");
-          sf16 A;
-#pragma unroll
-          for (int e = 0; e < 16; e++) A[e] = 0.f;
-#pragma unroll
-          for (int k = 0; k < NK; k++)
-            A = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const fh8 *>(kb + 256 * k), qh[k], A, 0, 0, 0);
-          tt = 0.f;
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            S[e] = A[e] == -INFINITY && S[e] != S[e] ? 0.f : S[e];
-            tt += S[e];
-          }
+          weigh();
         }
         ts += tt;
         bool bad = false;
@@ -526,7 +543,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
         for (int k = 0; k < 2; k++) {
           uint32_t ph[4], pl[4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) split_pair(S[8 * k + 2 * e], S[8 * k + 2 * e + 1], ph[e], pl[e]);
+          for (int e = 0; e < 4; e++) weight_parts(w[8 * k + 2 * e], w[8 * k + 2 * e + 1], ph[e], pl[e]);
           const fh8 eh = as_fh8(ph[0], ph[1], ph[2], ph[3]), el = as_fh8(pl[0], pl[1], pl[2], pl[3]);
           const uint16_t *vb = lv[b] + (2 * x + k) * UN + hf * 8 * HD + col * 8;
           u32x4_t a[ND];
@@ -567,7 +584,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   const int64_t at = (int64_t)t * H + h;
   const bool whole = U.alone && runs == 1;
   float *op = whole ? out + ((int64_t)row0 * H + at) * HD : part + ((int64_t)E.rec * H + at * runs + run) * (HD + 4);
-  const double f = whole ? 1.0 / L / kSpUp : 1.0;
+  const double f = whole ? 1.0 / L : 1.0;
 #pragma unroll
   for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -636,7 +653,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const float *__restrict
     sf4 s = so[0][tid];
 #pragma unroll
     for (int k = 1; k < NG; k++) s += so[k][tid];
-    const double all = (sl[0] + sl[1]) + (sl[2] + sl[3]), r = (1.0 / kSpUp) / all;
+    const double all = (sl[0] + sl[1]) + (sl[2] + sl[3]), r = 1.0 / all;
 #pragma unroll
     for (int e = 0; e < 4; e++) s[e] = all == 0.0 ? 0.f : (float)((double)s[e] * r);
     *reinterpret_cast<f4a4 *>(out + row * HD + 4 * tid) = s;
@@ -696,7 +713,7 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(const float *__res
       for (int e = 0; e < 4; e++) w[e] = __shfl(o[k][e], a * TH + x, 64);
       s = k + a ? s + w : w;
     }
-  const double r = (1.0 / kSpUp) / all;
+  const double r = 1.0 / all;
 #pragma unroll
   for (int e = 0; e < 4; e++) s[e] = all == 0.0 ? 0.f : (float)((double)s[e] * r);
   if (g == 0) *reinterpret_cast<f4a4 *>(out + row * HD + 4 * x) = s;
