@@ -495,6 +495,8 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
 #pragma unroll
           for (int e = 0; e < 16; e++) S[e] = up[e >> 3] + 8 * hf + (e & 7) > (uint32_t)p ? -INFINITY : S[e];
         }
+        // weights before the other wave's work: 191.7 -> 188.3 us for 80 rows of a prefix of 60,000
+        __builtin_amdgcn_s_setprio(1);
         float w[16], tt;
         auto weigh = [&]() __attribute__((always_inline)) {
           const float Mu = M == -INFINITY ? 0.f : M;  // no score of this column yet: all are -inf
@@ -559,6 +561,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
 #pragma unroll
           for (int d = 0; d < ND; d++) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fh8, a[d]), el, O[d], 0, 0, 0);
         }
+        __builtin_amdgcn_s_setprio(0);
         if (__any(bad)) {  // infinite and NaN values into the columns that see them
           for (int y = 0; y < 32; y++) {
             const uint32_t w = (y >> 4 ? up[1] : up[0]) + (y & 15);

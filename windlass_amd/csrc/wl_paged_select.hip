@@ -38,7 +38,7 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 // largest of a column is the page's score. The heads' halves lie in LDS in 64 bits: converting them in each wave took as long
 // as the products.
 template <int HD, int NB>
-__global__ __launch_bounds__(256, 4) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
+__global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
                                                           const float *__restrict__ q, int G, uint64_t *__restrict__ keys,
                                                           int64_t width) {
   constexpr int N = HD / 4;
