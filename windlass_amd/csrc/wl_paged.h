@@ -16,7 +16,7 @@
 
 namespace wl {
 
-constexpr int kPgRows = 112;      // entries of a call that one launch takes: its arguments are 4 KB at most
+constexpr int kPgRows = 111;      // entries of a call that one launch takes, and one more: its arguments are 4 KB at most
 constexpr int kPgUnit = 16;       // positions of a unit: a page holds whole ones
 constexpr int kPgValues = 1 << 24;  // values of a row at most
 

@@ -25,13 +25,15 @@ constexpr int kManyWaves = 4, kManyCols = 32 * kManyWaves, kManyUnits = 4;  // u
 constexpr int kPgRuns = 256;  // of a row at most
 constexpr uint32_t kNowhere = 0xfffffff0u;  // the position of a unit that no row sees
 
-// A launch's items go entry by entry, column block by column block, run by run of `per` tiles or steps each. An entry's records, a
-// run after the other for each (row, head), begin H * rec records into `part`; alone: a row of one run is the output itself.
+// A launch's items go entry by entry, column block by column block, run by run of `per` tiles or steps each. An entry's records, a run after the other for each (row, head), begin H * rec records into `part`; alone: a row of one run is
+// the output itself. Of the items flat0 .. flat1 - 1, a prefix', all rows see what the entry's position does.
 struct PagedPlan {
   PageItems it;
-  int inc, base;  // a row's positions end at pos + row * inc; units before base are not read
+  int flat0, flat1;
+  int base;          // units before base are not read (but by a prefix' items)
   int alone;
 };
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // What a column needs of its query: the factor of its parts, and of its scores in units of log2.
 __device__ __forceinline__ void query_scale(float m, float scale, float &f, float &c2) {
@@ -107,12 +109,13 @@ struct FewTile {
   }
 };
 
-template <int HD, bool SPARSE>
+template <int HD, bool CHOSEN>
 __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_kernel(PagePool P, PagedPlan U,
-                                                                      const float *__restrict__ q, int G,
-                                                                      const int32_t *__restrict__ blocks, int nblocks,
-                                                                      float scale, float *__restrict__ part,
-                                                                      float *__restrict__ out) {
+                                                                                    const float *__restrict__ q, int G,
+                                                                                    const int32_t *__restrict__ blocks,
+                                                                                    int nblocks, float scale,
+                                                                                    float *__restrict__ part,
+                                                                                    float *__restrict__ out) {
   constexpr int NK = HD / 32, ND = HD / 16, W = kFewWaves;
   __shared__ sf4 so[W][kFewCols][HD / 4 + 1];
   __shared__ float sm[W][kFewCols], sc2[kFewCols];
@@ -122,22 +125,24 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
   const int col = lane & 15, kq = lane >> 4, KH = P.KH, H = G * KH, us = P.shift - 4;
   const int kvh = blockIdx.x % KH, item = blockIdx.x / KH;
   const PageEntry E = entry_of(U.it, item);
-  const int runs = E.runs, per = E.per, run = (item - E.off) % runs;
-  int cb = (item - E.off) / runs, t0 = 0, T = E.rows;  // the block's rows: T from the entry's t0
-  if constexpr (SPARSE) {
+  const bool flat = item >= U.flat0 && item < U.flat1;
+  const int inc = flat ? 0 : 1, base = flat ? 0 : U.base;
+  const int runs = E.runs, per = E.per, run = uniform((item - E.off) % runs);
+  int cb = uniform((item - E.off) / runs), t0 = 0, T = E.rows;  // the block's rows: T from the entry's t0
+  if constexpr (CHOSEN) {
     const int nb = (G + kFewCols - 1) / kFewCols;
-    t0 = cb / nb;
-    cb %= nb;
+    t0 = uniform(cb / nb);
+    cb = uniform(cb % nb);
     T = 1;
   }
   const int row0 = E.row0 + t0, pos = E.pos + t0;
   const int NC = T * G, c0 = cb * kFewCols, c = c0 + col < NC ? c0 + col : NC - 1;
   const int t = c / G, h = kvh * G + c % G;
-  const int p = pos + t * U.inc, pa = pos + c0 / G * U.inc;
-  const int pb = pos + (c0 + kFewCols - 1 < NC ? c0 + kFewCols - 1 : NC - 1) / G * U.inc;
+  const int p = pos + t * inc, pa = uniform(pos + c0 / G * inc);
+  const int pb = uniform(pos + (c0 + kFewCols - 1 < NC ? c0 + kFewCols - 1 : NC - 1) / G * inc);
   int nu;  // units
-  if constexpr (SPARSE) nu = ((pos >> P.shift) + 1 < nblocks ? (pos >> P.shift) + 1 : nblocks) << us;
-  else nu = (pb >> 4) - U.base + 1;
+  if constexpr (CHOSEN) nu = ((pos >> P.shift) + 1 < nblocks ? (pos >> P.shift) + 1 : nblocks) << us;
+  else nu = (pb >> 4) - base + 1;
   const int nt = (nu + 1) / 2, i0 = run * per, i1 = i0 + per < nt ? i0 + per : nt;
 
   // The wave's units, 64 (32 tiles) at a time: lane 2 k + x has unit x of its k-th tile.
@@ -149,12 +154,12 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
     up = kNowhere;
     if (tile >= i1 || j >= nu) return;
     int b, u;
-    if constexpr (SPARSE) {
+    if constexpr (CHOSEN) {
       b = blocks[((int64_t)row0 * KH + kvh) * nblocks + (j >> us)];
       if (b < 0) return;
       u = (b << us) + (j & ((1 << us) - 1));
     } else {
-      u = U.base + j;
+      u = base + j;
       b = u >> us;
     }
     const int id = P.id(E.seq, b);
@@ -294,7 +299,9 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
       M = raise ? mt : M;
       weigh();
     }
+    __builtin_amdgcn_sched_barrier(0);
     if (more) a.keys(P, oa, ob, lane);
+    __builtin_amdgcn_sched_barrier(0);
     L += (double)ts;
     uint32_t ph[4], pl[4];
 #pragma unroll
@@ -316,6 +323,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
           for (int j = 0; j < 4; j++) {
             const uint16_t y = vp[pg_val(o, 16 * d + 4 * kq + j, HD)];
             if ((y & 0x7c00u) == 0x7c00u && w <= (uint32_t)p) O[d][j] += (float)__builtin_bit_cast(_Float16, y);
+            __builtin_amdgcn_sched_barrier(0);  // one value at a time: this is rare, and its registers all the loop's
           }
       }
     }
@@ -332,7 +340,7 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
     sc2[col] = c2;
   }
   __syncthreads();
-  const bool whole = U.alone && runs == 1;
+  const bool whole = U.alone && !flat && runs == 1;
   for (int e = threadIdx.x; e < kFewCols * HD / 4; e += 64 * W) {
     const int g = e / (HD / 4), four = e % (HD / 4), cc = c0 + g;
     if (cc >= NC) break;
@@ -376,32 +384,34 @@ __device__ __forceinline__ void to_lds(const uint16_t *from, uint32_t to) {
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <int HD>
-__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool P, PagedPlan U,
-                                                                        const float *__restrict__ q, int G, float scale,
-                                                                        float *__restrict__ part, float *__restrict__ out) {
+__global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool P, PagedPlan U, const float *__restrict__ q,
+                                                                        int G, float scale, float *__restrict__ part,
+                                                                        float *__restrict__ out) {
   constexpr int NK = HD / 16, ND = HD / 32, UN = 16 * HD;  // halves of a unit
   __shared__ __attribute__((aligned(1024))) uint16_t lk[2][kManyUnits * UN], lv[2][kManyUnits * UN];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, col = lane & 31, KH = P.KH, H = G * KH, us = P.shift - 4;
   const int kvh = blockIdx.x % KH, item = blockIdx.x / KH;
   const PageEntry E = entry_of(U.it, item);
+  const bool flat = item >= U.flat0 && item < U.flat1;
+  const int inc = flat ? 0 : 1, base = flat ? 0 : U.base;
   const int row0 = E.row0, T = E.rows, pos = E.pos, per = E.per, runs = E.runs;
   const int64_t NC = (int64_t)T * G;
-  const int nz = (int)((NC + kManyCols - 1) / kManyCols), run = (item - E.off) % runs, r = (item - E.off) / runs;
+  const int nz = (int)((NC + kManyCols - 1) / kManyCols), run = uniform((item - E.off) % runs), r = uniform((item - E.off) / runs);
   // longest and shortest rows in turn: the workgroups that share a CU (the grid's halves) add up
   const int z = r < (nz + 1) / 2 ? nz - 1 - r : r - (nz + 1) / 2;
   const int64_t z0 = (int64_t)z * kManyCols, w0 = z0 + 32 * wv, u = w0 + col, uc = u < NC ? u : NC - 1;
-  auto position = [&](int64_t c) __attribute__((always_inline)) { return pos + (int)((c < NC ? c : NC - 1) / G) * U.inc; };
-  const int t = (int)(uc / G), h = kvh * G + (int)(uc % G), p = pos + t * U.inc;
-  const int pa = position(w0), pb = position(w0 + 31), last = position(z0 + kManyCols - 1);
+  auto position = [&](int64_t c) __attribute__((always_inline)) { return pos + (int)((c < NC ? c : NC - 1) / G) * inc; };
+  const int t = (int)(uc / G), h = kvh * G + (int)(uc % G), p = pos + t * inc;
+  const int pa = uniform(position(w0)), pb = uniform(position(w0 + 31)), last = uniform(position(z0 + kManyCols - 1));
   const bool idle = w0 >= NC;
-  const int nu = (last >> 4) - U.base + 1, ns = (nu + kManyUnits - 1) / kManyUnits;
+  const int nu = (last >> 4) - base + 1, ns = (nu + kManyUnits - 1) / kManyUnits;
   const int i0 = run * per, i1 = i0 + per < ns ? i0 + per : ns;
 
   // The pages of 16 steps: lane l has unit l of theirs; those of the 16 after them are loaded ahead.
   auto page_of = [&](int first) __attribute__((always_inline)) {
     const int j = kManyUnits * first + lane;
-    return j < nu && first < i1 ? P.id(E.seq, (U.base + j) >> us) : -1;
+    return j < nu && first < i1 ? P.id(E.seq, (base + j) >> us) : -1;
   };
   int ids = page_of(i0), ahead = page_of(i0 + 16);
   uint64_t there = __ballot(ids >= 0);
@@ -414,7 +424,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
       there = __ballot(ids >= 0);
     }
     const int l = (x & 15) * kManyUnits, id = __builtin_amdgcn_readlane(ids, l + wv);
-    const int unit = U.base + kManyUnits * s + wv;
+    const int unit = base + kManyUnits * s + wv;
     const int64_t off = P.at(id < 0 ? 0 : id, kvh) + (int64_t)(unit & ((1 << us) - 1)) * UN;
     // keys lie in LDS as [HD / 8][16 rows of the products][8]
     const uint16_t *kp = P.K + off + (lane >> 3 & 1) * 8 * HD + (lane >> 4) * 64 + (lane & 7) * 8;
@@ -469,7 +479,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   for (int s = i0; s < i1; s++) {
     const int b = (s - i0) & 1, here = have;
     if (s + 1 < i1) have = stage(b ^ 1, s + 1);
-    const uint32_t s0 = 16u * (uint32_t)(U.base + kManyUnits * s);  // the step's first position
+    const uint32_t s0 = 16u * (uint32_t)(base + kManyUnits * s);  // the step's first position
     const bool on = !idle && s0 <= (uint32_t)pb;
     if (on) {
       float ts = 0.f;
@@ -573,6 +583,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
               for (int e = 0; e < 16; e++) {
                 const uint16_t o = vp[pg_val(y & 15, 32 * d + 8 * (e >> 2) + 4 * hf + (e & 3), HD)];
                 if ((o & 0x7c00u) == 0x7c00u && w <= (uint32_t)p) O[d][e] += (float)__builtin_bit_cast(_Float16, o);
+                __builtin_amdgcn_sched_barrier(0);
               }
           }
         }
@@ -585,7 +596,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
   L += __shfl_xor(L, 32, 64);
   if (u >= NC) return;
   const int64_t at = (int64_t)t * H + h;
-  const bool whole = U.alone && runs == 1;
+  const bool whole = U.alone && !flat && runs == 1;
   float *op = whole ? out + ((int64_t)row0 * H + at) * HD : part + ((int64_t)E.rec * H + at * runs + run) * (HD + 4);
   const double f = whole ? 1.0 / L : 1.0;
 #pragma unroll
@@ -603,6 +614,8 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
     *reinterpret_cast<double *>(op + HD + 2) = L;
   }
 }
+
+// ------------------------------------------------------------------------------- launches
 
 // ------------------------------------------------------------------------------- runs
 
@@ -752,21 +765,20 @@ static int many_per(int n, int64_t wgs) {
   return ceil_div(n, S);
 }
 
-// The launches of a call: the prefix (few or many columns), the entries of few columns, those of many.
+// The launches of a call.
 struct PagedLaunches {
-  PagedPlan pre, few, many;
-  bool pre_few = false;
+  PagedPlan few, many;
   PagedRuns runs;
   int records = 0, most_runs = 0;  // records of a head, runs of a row that has some
 };
 
 // most: the pages that a row may take (0: all positions).
 static void paged_launches(const PagePool &p, const PageRows &r, int H, int prefix, int most, PagedLaunches &L) {
-  const int G = H / p.KH, rows = r.row0[r.n], base = prefix / kPgUnit, upp = p.page / kPgUnit;
-  L.runs.pre = L.runs.pre_rec = 0;
+  const int G = H / p.KH, rows = r.row0[r.n], upp = p.page / kPgUnit;
   L.few.alone = L.many.alone = !prefix;
-  L.few.inc = L.many.inc = 1;
-  L.few.base = L.many.base = base;
+  L.few.base = L.many.base = prefix / kPgUnit;
+  L.few.flat0 = L.few.flat1 = L.many.flat0 = L.many.flat1 = 0;
+  L.runs.pre = L.runs.pre_rec = 0;
   if (prefix) {
     PageRows all;  // the rows of all entries, without a mask
     all.n = 1;
@@ -774,14 +786,13 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
     all.pos[0] = prefix - 1;
     all.row0[0] = 0;
     all.row0[1] = rows;
-    const int64_t NC = (int64_t)rows * G;
-    L.pre_few = is_few(NC);
-    const int blocks = ceil_div(NC, L.pre_few ? kFewCols : kManyCols);
-    const int n = ceil_div(prefix / kPgUnit, L.pre_few ? 2 : kManyUnits);
-    const int per = L.pre_few ? few_per(n, p.KH * blocks, kFewWaves, kFewWaves) : many_per(n, (int64_t)p.KH * blocks);
+    const bool f = is_few((int64_t)rows * G);
+    PagedPlan &U = f ? L.few : L.many;
+    const int blocks = ceil_div((int64_t)rows * G, f ? kFewCols : kManyCols), n = ceil_div(prefix / kPgUnit, f ? 2 : kManyUnits);
+    const int per = f ? few_per(n, p.KH * blocks, kFewWaves, kFewWaves) : many_per(n, (int64_t)p.KH * blocks);
     L.runs.pre = ceil_div(n, per);
-    L.pre.inc = L.pre.base = L.pre.alone = 0;
-    L.pre.it.add(all, 0, L.runs.pre * blocks, per, 0, L.runs.pre);
+    U.it.add(all, 0, L.runs.pre * blocks, per, 0, L.runs.pre);
+    U.flat1 = U.it.items;
     L.records = rows * L.runs.pre;
   }
   for (int i = 0; i < r.n; i++) {
@@ -796,7 +807,7 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
       per = few_per(ceil_div((int64_t)most * upp, 2), p.KH * ceil_div(G, kFewCols), kChosenWhole, kChosenLeast);
       runs = ceil_div(ceil_div((int64_t)took * upp, 2), per);
     } else {
-      const int units = (last >> 4) - base + 1, n = ceil_div(units, f ? 2 : kManyUnits);
+      const int units = (last >> 4) - prefix / kPgUnit + 1, n = ceil_div(units, f ? 2 : kManyUnits);
       blocks = ceil_div(NC, f ? kFewCols : kManyCols);
       per = f ? few_per(n, p.KH * blocks, kFewWhole, kFewLeast) : many_per(n, (int64_t)p.KH * blocks);
       runs = ceil_div(n, per);
@@ -804,8 +815,8 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
     (f ? L.few : L.many).it.add(r, i, runs * blocks, per, L.records, runs);
     if (runs == 1 && !prefix) continue;
     L.runs.it.add(r, i, T, 0, L.records, runs);
-    L.most_runs = std::max(L.most_runs, L.runs.pre + runs);
     L.records += T * runs;
+    L.most_runs = std::max(L.most_runs, L.runs.pre + runs);
   }
 }
 
@@ -823,22 +834,19 @@ static hipError_t paged_attend(const PagePool &p, const PageRows &r, const float
   paged_launches(p, r, H, prefix, most, L);
   const int G = H / p.KH;
   hipError_t e = hipSuccess;
-  auto few = [&](const PagedPlan &U) {
-    const dim3 grid((unsigned)U.it.items * p.KH), block(64 * kFewWaves);
+  if (L.many.it.n) {
+    hipLaunchKernelGGL(paged_many_kernel<HD>, dim3((unsigned)L.many.it.items * p.KH), dim3(64 * kManyWaves), 0, st, p, L.many, q,
+                       G, scale, part, out);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && L.few.it.n) {
+    const dim3 grid((unsigned)L.few.it.items * p.KH), block(64 * kFewWaves);
     if (blocks)
-      hipLaunchKernelGGL((paged_few_kernel<HD, true>), grid, block, 0, st, p, U, q, G, blocks, most, scale, part, out);
+      hipLaunchKernelGGL((paged_few_kernel<HD, true>), grid, block, 0, st, p, L.few, q, G, blocks, most, scale, part, out);
     else
-      hipLaunchKernelGGL((paged_few_kernel<HD, false>), grid, block, 0, st, p, U, q, G, nullptr, 0, scale, part, out);
+      hipLaunchKernelGGL((paged_few_kernel<HD, false>), grid, block, 0, st, p, L.few, q, G, nullptr, 0, scale, part, out);
     e = hipGetLastError();
-  };
-  auto many = [&](const PagedPlan &U) {
-    hipLaunchKernelGGL(paged_many_kernel<HD>, dim3((unsigned)U.it.items * p.KH), dim3(64 * kManyWaves), 0, st, p, U, q, G,
-                       scale, part, out);
-    e = hipGetLastError();
-  };
-  if (prefix) L.pre_few ? few(L.pre) : many(L.pre);
-  if (e == hipSuccess && L.many.it.n) many(L.many);
-  if (e == hipSuccess && L.few.it.n) few(L.few);
+  }
   if (e != hipSuccess || !L.records) return e;
   // many rows of few runs: a workgroup each would be idle for the most part (667 rows of
   // 32 heads and 3 runs among others 34.0 -> 16.2 us)

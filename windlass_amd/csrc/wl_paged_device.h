@@ -11,7 +11,7 @@ struct __attribute__((aligned(16))) PageEntry {
   int rows, per, rec, runs;
 };
 struct PageItems {
-  PageEntry e[kPgRows];
+  PageEntry e[kPgRows + 1];  // a prefix' rows are one more
   int n = 0, items = 0;
   // The next entry, of `count` items.
   void add(const PageRows &r, int i, int count, int per = 0, int rec = 0, int runs = 0) {
@@ -27,7 +27,7 @@ struct PageItems {
 __device__ __forceinline__ PageEntry entry_of(const PageItems &I, int x) {
   if (I.n == 1) return I.e[0];
   typedef int i32x4 __attribute__((ext_vector_type(4)));
-  static_assert(kPgRows <= 128, "two lanes' worth");
+  static_assert(kPgRows < 128, "two lanes' worth");
   const int lane = threadIdx.x & 63, n = I.n;
   const i32x4 *p = reinterpret_cast<const i32x4 *>(I.e + (lane < n ? lane : n - 1));
   i32x4 a = p[0], b = p[1];
