@@ -739,8 +739,14 @@ __global__ __launch_bounds__(256) void paged_join_rows_kernel(const float *__res
 
 static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Columns that paged_few_kernel takes.
-static bool is_few(int64_t columns) { return columns <= 64; }
+// Whether paged_few_kernel takes an entry: one that its keys and values pass once anyway, or one of so few products (columns times
+// the positions that they see on average, in all KV heads) that the other's 128 columns a workgroup leave CUs idle. At the border, in
+// us, few and many: 8B, 700 rows from 0 25.6 and 43.5, 300 up to 1,000 20.3 and 31.3, 4 up to 60,000 44.1 and 49.2, 60 up to 4,000 29.5
+// and 29.0; past it, 16 up to 20,000 40.0 and 32.4, 8 up to 60,000 77.1 and 49.5; 70B, 700 from 0 48.6 and 38.7, but 300 up to 1,000
+// 32.1 and 44.2; 16 rows on a prefix of 5,000 21.1 and 34.4.
+static bool is_few(int64_t columns, int first, int last, int KH) {
+  return columns <= kFewCols || (double)columns * (0.5 * ((double)first + last) + 1.0) * KH <= 0x1p23;
+}
 
 // Tiles of each run of an entry of n tiles, of `units` workgroups a run: a rule on the entry alone, so that its bits do not depend
 // on the others. Up to `whole` tiles one run, and no second launch; then runs of `least` tiles (four waves of two or four), for what a
@@ -786,7 +792,7 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
     all.pos[0] = prefix - 1;
     all.row0[0] = 0;
     all.row0[1] = rows;
-    const bool f = is_few((int64_t)rows * G);
+    const bool f = is_few((int64_t)rows * G, prefix, prefix, p.KH);
     PagedPlan &U = f ? L.few : L.many;
     const int blocks = ceil_div((int64_t)rows * G, f ? kFewCols : kManyCols), n = ceil_div(prefix / kPgUnit, f ? 2 : kManyUnits);
     const int per = f ? few_per(n, p.KH * blocks, kFewWaves, kFewWaves) : many_per(n, (int64_t)p.KH * blocks);
@@ -799,7 +805,7 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
     const int T = r.rows(i), last = r.pos[i] + T - 1;
     if (!T) continue;
     const int64_t NC = (int64_t)T * G;
-    const bool f = most || is_few(NC);
+    const bool f = most || is_few(NC, r.pos[i] - prefix, last - prefix, p.KH);
     int blocks, per, runs;
     if (most) {  // rows one by one, cut by a rule on the choice alone
       const int took = std::min((last >> p.shift) + 1, most);
