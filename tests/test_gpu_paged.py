@@ -421,7 +421,7 @@ def test_chosen_pages(ctx, H, KH, HD, page, opts):
     assert same(one, got[1:2]) and np.array_equal(t1, taken[1:2])
 
 
-@pytest.mark.parametrize("page,n,top", [(16, 20000, 100), (16, 70000, 2000), (64, 40000, 7)])
+@pytest.mark.parametrize("page,n,top", [(16, 20000, 100), (16, 70000, 2000), (64, 40000, 7), (16, 140000, 300)])
 def test_chosen_pages_of_long_contexts(ctx, page, n, top):
     rng = np.random.default_rng(n)
     H, KH, HD = 4, 1, 64

@@ -101,7 +101,8 @@ static void score_launch(dim3 grid, const PagePool &p, const PageItems &U, const
   else run(paged_score_kernel<HD, 4>);
 }
 
-// Sum over the workgroup's 256 threads up to and with this one, and of all.
+// Sum over the workgroup's threads up to and with this one, and of all.
+template <int THREADS>
 __device__ __forceinline__ int block_scan(int v, int *sh, int &all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   // within rows of 16 lanes by shifts, then each row's last into the rows after it
@@ -114,8 +115,14 @@ __device__ __forceinline__ int block_scan(int v, int *sh, int &all) {
   __syncthreads();
   if (lane == 63) sh[w] = v;
   __syncthreads();
-  all = (sh[0] + sh[1]) + (sh[2] + sh[3]);
-  return v + (w > 0 ? sh[0] : 0) + (w > 1 ? sh[1] : 0) + (w > 2 ? sh[2] : 0);
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; i++) {
+    const int s = sh[i];
+    v += i < w ? s : 0;
+    all += s;
+  }
+  return v;
 }
 
 __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
@@ -128,19 +135,22 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
   return up(up(at(0), at(16)), up(at(32), at(48)));
 }
 
-// A workgroup per row and KV head. Thread t has pages t * m .. of the m = ceil(n / 256) each has, in registers up to kOwn of them.
-template <int kOwn>
-__global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageItems U, PageSelect S,
-                                                         const uint64_t *__restrict__ keys, int64_t width,
-                                                         int32_t *__restrict__ blocks) {
+// A workgroup per row and KV head. Thread t has pages t * m .. of the m = ceil(n / THREADS) each has, in registers up to kOwn of
+// them. Its time is its passes' latency, so each thread has few: the whole call of a row with 8 KV heads takes 23.6 us on 4,096 pages
+// and 31.9 on 8,190 by 1,024 threads of 8 pages each, 25.9 by 256 of 16, 26.0 and 38.1 where 1,024 read them again each pass; up to
+// 1,024 pages 256 threads do as well (20.5 us on 940; 21.5 by 1,024).
+template <int THREADS, int kOwn>
+__global__ __launch_bounds__(THREADS) void paged_take_kernel(PagePool P, PageItems U, PageSelect S,
+                                                             const uint64_t *__restrict__ keys, int64_t width,
+                                                             int32_t *__restrict__ blocks) {
   constexpr int BINS = 1024;
-  __shared__ int bins[BINS], sh[4], pick[3];
-  __shared__ uint32_t ends[2][4];
+  __shared__ int bins[BINS], sh[THREADS / 64], pick[3];
+  __shared__ uint32_t ends[2][THREADS / 64];
   const int kvh = blockIdx.x % P.KH, row = blockIdx.x / P.KH, tid = threadIdx.x;
   const PageEntry E = entry_of(U, row);
   const int cur = (E.pos + row - E.row0) >> P.shift;
   const OpenPages o(S, cur);
-  const int n = o.to - o.from, m = (n + 255) / 256;
+  const int n = o.to - o.from, m = (n + THREADS - 1) / THREADS;
   const uint64_t *kp = keys + ((int64_t)row * P.KH + kvh) * width;
   int32_t *out = blocks + ((int64_t)row * P.KH + kvh) * S.most();
   uint64_t mine[kOwn > 0 ? kOwn : 1];
@@ -172,8 +182,8 @@ __global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageItems U
     ends[0][tid >> 6] = least;
     ends[1][tid >> 6] = most;
   }
-  (void)block_scan(all, sh, all);  // its barriers also order the ends
-  for (int w = 0; w < 4; w++) {
+  (void)block_scan<THREADS>(all, sh, all);  // its barriers also order the ends
+  for (int w = 0; w < THREADS / 64; w++) {
     least = ends[0][w] < least ? ends[0][w] : least;
     most = ends[1][w] > most ? ends[1][w] : most;
   }
@@ -191,22 +201,23 @@ __global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageItems U
     for (;;) {
       const uint64_t span = hi - lo;
       const int shift = span >> 10 ? 54 - __builtin_clzll(span) : 0;  // span >> shift is below 1024
-      for (int e = tid; e < BINS; e += 256) bins[e] = 0;
+      for (int e = tid; e < BINS; e += THREADS) bins[e] = 0;
       __syncthreads();
       each([&](uint64_t v, int page) {
         const uint64_t w = ties ? ~(uint32_t)page : v;
         if ((!ties || v == key) && w >= lo && w <= hi) atomicAdd(&bins[(w - lo) >> shift], 1);
       });
       __syncthreads();
-      // from the top: thread t has bins 1023 - 4 t down to 1020 - 4 t
-      int c[4], sum = 0, total;
+      // from the top: a thread has EACH bins
+      constexpr int EACH = BINS / THREADS;
+      int c[EACH], sum = 0, total;
 #pragma unroll
-      for (int e = 0; e < 4; e++) sum += c[e] = bins[BINS - 1 - 4 * tid - e];
-      int before = block_scan(sum, sh, total) - sum;
+      for (int e = 0; e < EACH; e++) sum += c[e] = bins[BINS - 1 - EACH * tid - e];
+      int before = block_scan<THREADS>(sum, sh, total) - sum;
       if (before < need && before + sum >= need) {  // one thread
         int e = 0;
         while (before + c[e] < need) before += c[e++];
-        pick[0] = BINS - 1 - 4 * tid - e;
+        pick[0] = BINS - 1 - EACH * tid - e;
         pick[1] = before;
         pick[2] = c[e];
       }
@@ -232,13 +243,13 @@ __global__ __launch_bounds__(256) void paged_take_kernel(PagePool P, PageItems U
   auto taken = [&](uint64_t v, int page) { return v > key || (v == key && page <= upto); };
   int count = 0, total;
   each([&](uint64_t v, int page) { count += taken(v, page); });
-  int at = o.from + block_scan(count, sh, total) - count;
+  int at = o.from + block_scan<THREADS>(count, sh, total) - count;
   each([&](uint64_t v, int page) {
     if (taken(v, page)) out[at++] = o.from + page;
   });
-  for (int e = tid; e < o.from; e += 256) out[e] = e;
+  for (int e = tid; e < o.from; e += THREADS) out[e] = e;
   const int rest = o.from + total, last = rest + cur + 1 - o.to;
-  for (int e = rest + tid; e < S.most(); e += 256) out[e] = e < last ? o.to + e - rest : -1;
+  for (int e = rest + tid; e < S.most(); e += THREADS) out[e] = e < last ? o.to + e - rest : -1;
 }
 
 // Pages open to choice of any row of a call.
@@ -277,9 +288,12 @@ hipError_t paged_select_launch(const PagePool &p, const PageRows &r, const float
     if (const hipError_t e = hipGetLastError()) return e;
   }
   const dim3 grid((unsigned)(rows * p.KH));
-  if (width <= 256 * 4) hipLaunchKernelGGL(paged_take_kernel<4>, grid, dim3(256), 0, st, p, each, s, keys, width, blocks);
-  else if (width <= 256 * 16) hipLaunchKernelGGL(paged_take_kernel<16>, grid, dim3(256), 0, st, p, each, s, keys, width, blocks);
-  else hipLaunchKernelGGL(paged_take_kernel<0>, grid, dim3(256), 0, st, p, each, s, keys, width, blocks);
+  auto take = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, p, each, s, keys, width, blocks);
+  };
+  if (width <= 256 * 4) take(paged_take_kernel<256, 4>, 256);
+  else if (width <= 1024 * 8) take(paged_take_kernel<1024, 8>, 1024);
+  else take(paged_take_kernel<1024, 0>, 1024);
   return hipGetLastError();
 }
 
