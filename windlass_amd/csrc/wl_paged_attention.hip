@@ -25,8 +25,9 @@ constexpr int kManyWaves = 4, kManyCols = 32 * kManyWaves, kManyUnits = 4;  // u
 constexpr int kPgRuns = 256;  // of a row at most
 constexpr uint32_t kNowhere = 0xfffffff0u;  // the position of a unit that no row sees
 
-// A launch's items go entry by entry, column block by column block, run by run of `per` tiles or steps each. An entry's records, a run after the other for each (row, head), begin H * rec records into `part`; alone: a row of one run is
-// the output itself. Of the items flat0 .. flat1 - 1, a prefix', all rows see what the entry's position does.
+// A launch's items go entry by entry, column block by column block, run by run of `per` tiles or steps each. An entry's records,
+// a run after the other for each (row, head), begin H * rec records into `part`; alone: a row of one run is the output itself. Of
+// the items flat0 .. flat1 - 1, a prefix', all rows see what the entry's position does.
 struct PagedPlan {
   PageItems it;
   int flat0, flat1;
@@ -472,7 +473,6 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
     for (int e = 0; e < 16; e++) O[d][e] = 0.f;
   float M = -INFINITY;
   double L = 0.0;
-  if (__builtin_amdgcn_s_getreg((4 - 1) << 11 | 0 << 6 | 4) & 1) __builtin_amdgcn_s_setprio(1);
   landed();
   __syncthreads();
 #pragma unroll 1
@@ -614,8 +614,6 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool
     *reinterpret_cast<double *>(op + HD + 2) = L;
   }
 }
-
-// ------------------------------------------------------------------------------- launches
 
 // ------------------------------------------------------------------------------- runs
 
