@@ -480,9 +480,10 @@ int64_t wl_page_bounds_bytes(int32_t kv_heads, int32_t head_dim);
 int wl_paged_assign_dev(wl_ctx *ctx, const wl_pages *p, int32_t seq, int32_t first, int32_t n, const int32_t *ids);
 
 /* wl_rope_dev's rotation of q [rows][heads * head_dim] into d_q_out (which may be d_q) and of k, and k and v
- * [rows][kv_heads * head_dim] into the pages, in one launch; with d_bounds also the bounds of the pages written to. rope_dims 0
- * rotates nothing; heads 0 (and null d_q, d_q_out) leaves the queries out. d_k and d_v stay as they were. The entries'
- * sequences are distinct, and no page that is written to belongs to two of them. */
+ * [rows][kv_heads * head_dim] into the pages, and with d_bounds the bounds of the pages written to (one launch, two where a
+ * sequence with bounds has several rows). rope_dims 0 rotates nothing; heads 0 (and null d_q, d_q_out) leaves the queries
+ * out. d_k and d_v stay as they were. The entries' sequences are distinct, and no page that is written to belongs to two
+ * of them. */
 int wl_paged_store_dev(wl_ctx *ctx, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
                        const float *d_k, const float *d_v, int32_t rope_dims, int32_t neox, double base,
                        double freq_scale, const float *d_freqs, float *d_q_out);

@@ -7,7 +7,7 @@ import pytest
 
 from paged_ref import F32, Pool, attend_ref, blocks_ref, key_at, rope_ref, val_at
 from windlass_amd._lib import check, load
-from windlass_amd.backend import Context
+from windlass_amd.backend import Context, PageRows
 
 pytestmark = pytest.mark.gpu
 
@@ -540,3 +540,78 @@ def test_other_streams_and_two_contexts(ctx):
         ctx.sync()
         other.sync()
     assert same(out[0].cpu().numpy(), want[0]) and same(out[1].cpu().numpy(), want[1])
+
+
+# ------------------------------------------------------------------------------------- large calls
+
+
+def test_more_rows_than_a_launch_takes(ctx):
+    """16,400 rows of 256 heads: two launches, the second of 16 rows."""
+    import torch
+    H, HD, page, n = 256, 64, 64, 16400
+    pool = Pool(ctx, [n], 1, HD, page, seed=2)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn((n, H, HD), generator=g, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    one = torch.full_like(q[:16], float("nan"))
+    torch.cuda.synchronize()
+    for r, a, o in ((PageRows([0], [0], [n]), q, out), (PageRows([0], [16384], [16]), q[16384:], one)):
+        check(load().wl_paged_attention_dev(ctx.handle, ctypes.byref(pool.desc), ctypes.byref(r), a.data_ptr(), H, 0, HD ** -0.5,
+                                            o.data_ptr()))
+    ctx.sync()
+    assert same(out[16384:].cpu().numpy(), one.cpu().numpy())
+    for row in (0, 5, 8000, 16383, 16384, 16399):
+        want, tol = attend_ref(q[row:row + 1].cpu().numpy(), pool.K[0], pool.V[0], [[np.arange(row + 1)]], HD ** -0.5)
+        near(out[row:row + 1].cpu().numpy(), want, tol, "row %d" % row)
+
+
+def test_reading_more_values_than_a_launch_takes(ctx):
+    """2^32 + 2^16 values of keys: positions that all name the same pages."""
+    import torch
+    KH, HD, page, T = 8, 128, 256, (1 << 22) + 64
+    pool = Pool(ctx, [4 * page], KH, HD, page, seed=3)
+    width = T // page + 1
+    table = torch.from_numpy(np.tile(pool.table[0, :4], width // 4 + 1)[:width].copy()).to("cuda")
+    pool.desc.d_table, pool.desc.sequences, pool.desc.table_pages = table.data_ptr(), 1, width
+    k, v = (torch.full((T, KH, HD), float("nan"), device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    check(load().wl_paged_read_dev(ctx.handle, ctypes.byref(pool.desc), 0, 0, T, k.data_ptr(), v.data_ptr()))
+    ctx.sync()
+    for row in (0, 1500, (1 << 21) - 1, 1 << 21, (1 << 21) + 1025, (1 << 22) + 63):
+        assert same(k[row].cpu().numpy(), pool.K[0][row % (4 * page)]) and same(v[row].cpu().numpy(), pool.V[0][row % (4 * page)])
+
+
+def test_chosen_pages_of_many_rows(ctx):
+    """Rows of many runs, whose records come a part of the rows at a time."""
+    H, KH, HD, page, n, T = 32, 8, 128, 256, 40000, 1100
+    pool = Pool(ctx, [n], KH, HD, page, seed=4, bounds=True)
+    q = normal(np.random.default_rng(5), T, H, HD)
+    opts = (1, 2, 125)
+    got, taken = pool.attend([0], [n - T], [T], q, sparse=opts)
+    for row in (0, 777, 1000, T - 1):
+        one, t1 = pool.attend([0], [n - T + row], [1], q[row:row + 1], sparse=opts)
+        assert same(one, got[row:row + 1]) and np.array_equal(t1, taken[row:row + 1])
+    want, tol, blocks = sparse_ref(pool, [0], [n - 1], [1], q[T - 1:], opts, HD ** -0.5)
+    assert np.array_equal(taken[T - 1:], blocks)
+    near(got[T - 1:], want, tol, "the last row")
+
+
+@pytest.mark.parametrize("T", [3, 60])
+def test_a_query_that_is_not_a_number(ctx, T):
+    """Gives a row that is not, beside others that are what they were."""
+    H, KH, HD, page, n = 8, 2, 64, 32, 700
+    pool = Pool(ctx, [n], KH, HD, page, seed=6, bounds=True)
+    q = normal(np.random.default_rng(7), T, H, HD)
+    bad = q.copy()
+    bad[1, 3, 5] = np.nan
+    want, tol = entries_ref(pool, [0], [n - T], [T], q, HD ** -0.5)
+    for prefix in (0, 128):
+        got = pool.attend([0], [n - T], [T], bad, prefix=prefix)
+        assert np.isnan(got[1, 3]).all()
+        got[1, 3] = want[1, 3]
+        near(got, want, tol, "prefix %d" % prefix)
+    want, tol, _ = sparse_ref(pool, [0], [n - T], [T], q, (1, 1, 4), HD ** -0.5)
+    got, _ = pool.attend([0], [n - T], [T], bad, sparse=(1, 1, 4))
+    assert np.isnan(got[1, 3]).all()
+    got[1, :4] = want[1, :4]  # its group's choice may be another
+    near(got, want, tol, "sparse")

@@ -2090,8 +2090,8 @@ static int paged_sparse(const char *who, const wl_pages *p, const wl_sparse_opts
   return WL_OK;
 }
 
-// Rows of a launch: a (row, head) pair is a workgroup of one of them.
-static int paged_most_rows(int heads) { return std::max(1, (1 << 24) / std::max(heads, 1)); }
+// Rows of a launch: a (row, head) pair is a workgroup of up to 512 threads of one of them, and a grid has fewer than 2^32.
+static int paged_most_rows(int heads) { return std::max(1, (1 << 22) / heads); }
 
 // f(rows, first row) for a call's entries, kPgRows and `most` rows at a time; entries without rows are left out.
 template <class F>
@@ -2139,7 +2139,7 @@ extern "C" int wl_paged_assign_dev(wl_ctx *c, const wl_pages *p, int32_t seq, in
 static int paged_store(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
                        const float *d_k, const float *d_v, const wl::PageRope &rope, float *d_q_out) {
   const int64_t qd = (int64_t)heads * pool.HD, kd = (int64_t)pool.KH * pool.HD;
-  return each_page_rows(r, paged_most_rows(heads), [&](const wl::PageRows &R, int r0) -> int {
+  return each_page_rows(r, paged_most_rows(std::max(heads, pool.KH)), [&](const wl::PageRows &R, int r0) -> int {
     WL_HIP(wl::paged_store_launch(pool, R, heads ? d_q + r0 * qd : nullptr, heads, d_k + r0 * kd, d_v + r0 * kd, rope,
                                   heads ? d_q_out + r0 * qd : nullptr, c->stream), "paged store");
     return WL_OK;
@@ -2170,7 +2170,10 @@ extern "C" int wl_paged_read_dev(wl_ctx *c, const wl_pages *p, int32_t seq, int3
   if ((rc = paged_pool("wl_paged_read_dev", p, &pool)) || (rc = paged_rows("wl_paged_read_dev", p, &r, false, &rows)))
     return rc;
   WL_ON_DEVICE(c);
-  WL_HIP(wl::paged_read_launch(pool, seq, pos0, T, d_k, d_v, c->stream), "paged read");
+  const int64_t kd = (int64_t)pool.KH * pool.HD;
+  const int most = (int)std::min((int64_t)1 << 24, ((int64_t)1 << 31) / kd);  // a value is a thread
+  for (int t = 0; t < T; t += most)
+    WL_HIP(wl::paged_read_launch(pool, seq, pos0 + t, std::min(T - t, most), d_k + t * kd, d_v + t * kd, c->stream), "paged read");
   return WL_OK;
 }
 
@@ -2201,19 +2204,26 @@ extern "C" int wl_paged_attention_dev(wl_ctx *c, const wl_pages *p, const wl_pag
   return paged_attention(c, pool, r, d_q, heads, prefix, scale, d_out);
 }
 
-// Rows of a choice of pages at a time: as many as 256 MB of scores and of pages chosen take.
-static int sparse_rows(const wl::PagePool &pool, const wl_page_rows *r, const wl::PageSelect &s) {
-  int64_t pages = s.most();
-  for (int i = 0; i < r->n; i++)
-    pages = std::max(pages, ((int64_t)r->pos[i] + (r->rows ? r->rows[i] : 1) + pool.page - 1) >> pool.shift);
-  return (int)std::clamp(((int64_t)32 << 20) / (pages * pool.KH), (int64_t)1, (int64_t)32768);
+// Rows of a choice of pages at a time: as many as 256 MB of scores, of pages chosen and 1 GB of their runs' records take.
+static int sparse_rows(const wl::PagePool &pool, const wl_page_rows *r, int heads, const wl::PageSelect &s) {
+  int64_t end = 1;
+  for (int i = 0; i < r->n; i++) end = std::max(end, (int64_t)r->pos[i] + (r->rows ? r->rows[i] : 1));
+  const int64_t pages = std::max((int64_t)s.most(), (end + pool.page - 1) >> pool.shift);
+  wl::PageRows last;
+  last.n = 1;
+  last.seq[0] = last.row0[0] = 0;
+  last.pos[0] = (int)end - 1;
+  last.row0[1] = 1;
+  const int64_t record = std::max((int64_t)1, wl::paged_attention_scratch_floats(pool, last, heads, 0, s.most()));
+  return (int)std::clamp(std::min(((int64_t)32 << 20) / (pages * pool.KH), ((int64_t)256 << 20) / record), (int64_t)1,
+                         (int64_t)paged_most_rows(heads));
 }
 
 static int paged_sparse_attention(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
                                   const wl_sparse_opts *o, float scale, float *d_out, int32_t *d_blocks) {
   const int64_t qd = (int64_t)heads * pool.HD;
   const wl::PageSelect s{o->first, o->recent, o->top};
-  return each_page_rows(r, std::min(sparse_rows(pool, r, s), paged_most_rows(heads)), [&](const wl::PageRows &R, int r0) -> int {
+  return each_page_rows(r, sparse_rows(pool, r, heads, s), [&](const wl::PageRows &R, int r0) -> int {
     int rc;
     const size_t blocks = (size_t)R.row0[R.n] * pool.KH * s.most();
     if ((rc = ensure(c, S_SEL, (size_t)wl::paged_select_scratch_bytes(pool, R, s))) ||
