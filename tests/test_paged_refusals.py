@@ -159,3 +159,16 @@ def test_every_entry_is_bound():
     assert {n for n in _lib.SIGNATURES if "page" in n} == {
         "wl_page_bytes", "wl_page_bounds_bytes", "wl_paged_assign_dev", "wl_paged_store_dev", "wl_paged_read_dev",
         "wl_paged_attention_dev", "wl_paged_sparse_dev", "wl_layer_paged_dev"}
+
+
+@pytest.mark.parametrize("make", [
+    lambda v: PageRows([v], [0]), lambda v: PageRows([0], [v]), lambda v: PageRows([0], [0], [v]),
+    lambda v: SparseOpts(v, 1, 1), lambda v: SparseOpts(1, v, 1), lambda v: SparseOpts(1, 1, v),
+    lambda v: desc(pages=v), lambda v: desc(page=v), lambda v: desc(kv_heads=v), lambda v: desc(head_dim=v),
+    lambda v: desc(sequences=v), lambda v: desc(table_pages=v)])
+def test_numbers_past_32_bits(make):
+    """2^32 + 1 would reach the library as 1."""
+    for v in ((1 << 32) + 1, 1 << 31, -(1 << 31) - 1):
+        with pytest.raises(ShapeError):
+            make(v)
+    make((1 << 31) - 1)

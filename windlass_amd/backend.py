@@ -369,10 +369,23 @@ class KvOpts(ctypes.Structure):
                 ("positions", ctypes.c_int32)]
 
 
+def _int32s(what, values):
+    """The values as they are; past 32 bits ctypes would cut them without a word."""
+    for v in values:
+        if not -(1 << 31) <= v < 1 << 31:
+            raise ShapeError("%s of %d." % (what, v))
+    return values
+
+
 class Pages(ctypes.Structure):
     """wl_pages: a pool of pages of keys and values, the table of the sequences' pages, and their shapes."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("d_K", "d_V", "d_bounds", "d_table")] + [
         (n, ctypes.c_int32) for n in ("pages", "page", "kv_heads", "head_dim", "sequences", "table_pages")]
+
+    def __init__(self, d_K=None, d_V=None, d_bounds=None, d_table=None, pages=0, page=0, kv_heads=0, head_dim=0, sequences=0,
+                 table_pages=0):
+        super().__init__(d_K, d_V, d_bounds, d_table,
+                         *_int32s("Pages", (pages, page, kv_heads, head_dim, sequences, table_pages)))
 
 
 class PageRows(ctypes.Structure):
@@ -384,13 +397,16 @@ class PageRows(ctypes.Structure):
         if len(pos) != n or (rows is not None and len(rows) != n):
             raise ShapeError("Entries of %d sequences, %d positions and %s rows." % (n, len(pos), rows and len(rows)))
         a = ctypes.c_int32 * n
-        super().__init__(n, a(*seq), a(*pos), None if rows is None else a(*rows))  # ctypes keeps the arrays alive
+        super().__init__(n, *(None if x is None else a(*_int32s("Entries", x)) for x in (seq, pos, rows)))  # ctypes keeps the arrays
 
 
 class SparseOpts(ctypes.Structure):
     """wl_sparse_opts: the pages a row attends to: the `first` first, the `recent` last, and the `top` others of largest
     score."""
     _fields_ = [(n, ctypes.c_int32) for n in ("first", "recent", "top")]
+
+    def __init__(self, first=0, recent=0, top=0):
+        super().__init__(*_int32s("Chosen pages", (first, recent, top)))
 
 
 class SampleParams(ctypes.Structure):
