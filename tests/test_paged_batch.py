@@ -141,3 +141,33 @@ def test_nothing_stays_queued_after_a_failure(fails, after):
     with pytest.raises(ArgumentOutOfRangeError):
         b.generate([[1] * 20, [1] * 20], 5, [SampleParams()] * 2, [0.5] * 10, shared=18)
     assert m.log[-1] == "sync"
+
+
+def test_a_sequence_set_back_does_not_write_into_pages_that_others_hold():
+    m = model()
+    b = batch(m)
+    b.prefill(0, [1] * 40)
+    b.share(0, 1, 32)
+    b.length[0] = 20
+    del m.log[:]
+    for call in (lambda: b.prefill(0, [1]), lambda: b.step([0], torch.zeros(1, dtype=torch.int32))):
+        with pytest.raises(ShapeError):
+            call()
+    assert not m.log
+    b.length[0] = 33
+    b.prefill(0, [1])
+    b.release(1)
+    b.length[0] = 20
+    b.prefill(0, [1])
+    assert b.length[0] == 21 and len(b.held[0]) == 3
+
+
+def test_a_shared_beginning_for_sequences_that_hold_pages_is_refused():
+    m = model()
+    b = batch(m)
+    b.prefill(1, [1] * 16)
+    b.length[1] = 0
+    del m.log[:]
+    with pytest.raises(ShapeError):
+        b.generate([[1] * 20, [1] * 20], 2, [SampleParams()] * 2, [0.5] * 4, shared=16)
+    assert not queued(m)

@@ -40,5 +40,5 @@ from .model import DeviceBatch, DeviceTransformer, KvCaches, ModelConfig, PagedB
 
 __all__ = ["ArgumentOutOfRangeError", "BackendError", "NotSupportedError", "ShapeError",
            "library_path", "load", "Context", "FastMath", "GgmlType", "Graph", "HostBuffer", "KvCaches", "KvOpts",
-           "LayerDesc", "PageRows", "Pages", "QActs", "Quants", "SampleParams", "SparseOpts", "Stage", "Transformer", "WeightView", "layout", "DeviceBatch",
-           "DeviceTransformer", "ModelConfig", "PagedBatch", "StageStream"]
+           "LayerDesc", "PageRows", "Pages", "QActs", "Quants", "SampleParams", "SparseOpts", "Stage", "Transformer",
+           "WeightView", "layout", "DeviceBatch", "DeviceTransformer", "ModelConfig", "PagedBatch", "StageStream"]

@@ -570,6 +570,8 @@ class PagedBatch(DeviceBatch):
         for s, n in zip(slots, counts):
             if n <= 0 or self.length[s] + n > self.cap:
                 raise ShapeError("The prompt and reply need %d positions; the context is %d." % (self.length[s] + n, self.cap))
+            if any(self.users[i] > 1 for i in self.held[s][self.length[s] // self.page:]):
+                raise ShapeError("Position %d of sequence %d is in a page that others hold." % (self.length[s], s))
         need = [self._need(s, self.length[s] + n) for s, n in zip(slots, counts)]
         if sum(need) > len(self.free_pages):
             raise ShapeError("%d more pages are needed; %d are free." % (sum(need), len(self.free_pages)))
@@ -658,7 +660,7 @@ class PagedBatch(DeviceBatch):
         k = min([shared] + [len(p) - 1 for p in prompts]) // self.page * self.page if N > 1 else 0  # each runs a token of its own
         if N > self.slots:
             raise ShapeError("%d sequences for %d slots." % (N, self.slots))
-        if k and any(self.length[:N]):
+        if k and (any(self.length[:N]) or any(self.held[:N])):
             raise ShapeError("A shared beginning for sequences that hold positions.")
         if len(params) != N or np.size(u) != steps * N:
             raise ShapeError("%d settings and %d numbers for %d sequences of %d tokens." % (len(params), np.size(u), N, steps))
