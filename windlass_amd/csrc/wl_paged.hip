@@ -10,14 +10,19 @@
 
 namespace wl {
 
-constexpr int kPgUnitRows = 8;  // rows of a sequence from which units pay
+// Values (of q and k) up to which a call's rows go by themselves, past which by units: 8B in us 20.2 and 23.1 at 1,536 rows, 24.8 and
+// 24.6 at 2,048; 70B 20.8 and 22.5 at 1,024, 28.2 and 30.5 at 1,536 of 64 sequences, 26.6 and 25.3 at 1,500 of one; 1B 13.3 and 20.1
+// at 2,000.
+constexpr int64_t kPgRowValues = (int64_t)8 << 20;
+// Query heads of a row that share a wave and its angles: one row of 8B takes 5.2 us as with two each, 110 rows of 70B 8.5 (12.5).
+constexpr int kPgRowHeads = 8;
 
 struct StoreArgs {
   PagePool p;
   PageRope e;
   const float *q, *k, *v;
   float *qr;
-  int H, parts, each;  // parts of a row or unit, query heads each
+  int H, parts, each;  // parts of a row or unit, query heads of a unit's each
 };
 
 __device__ __forceinline__ uint16_t half_of(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
@@ -48,12 +53,12 @@ __device__ __forceinline__ fh8 lane_swap(fh8 v, int m) {
   return __builtin_bit_cast(fh8, w);
 }
 
-// Few rows of each sequence: a wave per part of a row, `each` query heads or the keys and values of one KV head (two of 64), a
-// lane per pair, so that the heads of a part share its angles. With one row of each sequence the
-// waves of the keys also make their page's bounds.
+// Few rows: a wave per part of a row, kPgRowHeads query heads or the keys and values of one KV head (two of 64), a lane per pair, so
+// that the heads of a part share its angles. With one row of each sequence the waves of the keys also make their page's bounds.
+// Latency bounds it: one row of 32 + 8 heads of 128 5.2 us, of which a launch takes 4.9; 64 rows of 64 + 8 with bounds 7.5.
 template <int HD>
 __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U) {
-  constexpr int NP = HD / 2, HS = 64 / NP, HMAX = 8;  // pairs, heads at once, query heads a part at most (in steps of HS)
+  constexpr int NP = HD / 2, HS = 64 / NP, N = kPgRowHeads / HS;  // pairs, heads at once, and of a part one after the other
   __shared__ double theta[NP];
   __shared__ uint16_t fresh[HS][HD];
   const int lane = threadIdx.x, x = lane % NP, sub = lane / NP, KH = A.p.KH;
@@ -63,16 +68,16 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U
   const Pair pr(A.e, x);
   const int q_parts = A.parts - (KH + HS - 1) / HS;
   const bool isq = part < q_parts;
-  const int h0 = isq ? part * A.each : (part - q_parts) * HS;
+  const int h0 = isq ? part * kPgRowHeads : (part - q_parts) * HS;
   const float freq = A.e.freqs && x < half ? A.e.freqs[x] : 1.f;
   // loads first, then the angles
-  float2 v[HMAX / HS], w = make_float2(0.f, 0.f);
+  float2 v[N], w = make_float2(0.f, 0.f);
   int id = -1;
   if (isq) {
 #pragma unroll
-    for (int e = 0; e < HMAX / HS; e++) {
+    for (int e = 0; e < N; e++) {
       const int h = h0 + e * HS + sub;
-      if (e * HS < A.each && h < A.H && e * HS + sub < A.each) v[e] = pr.load(A.q + ((int64_t)row * A.H + h) * HD);
+      if (h < A.H) v[e] = pr.load(A.q + ((int64_t)row * A.H + h) * HD);
     }
   } else {
     id = A.p.id(E.seq, p >> A.p.shift);
@@ -88,9 +93,9 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U
   }
   if (isq) {
 #pragma unroll
-    for (int e = 0; e < HMAX / HS; e++) {
+    for (int e = 0; e < N; e++) {
       const int h = h0 + e * HS + sub;
-      if (e * HS < A.each && h < A.H && e * HS + sub < A.each) {
+      if (h < A.H) {
         const float2 y = pr.turn(v[e], c, s);
         float *o = A.qr + ((int64_t)row * A.H + h) * HD;
         o[pr.a] = y.x;
@@ -301,13 +306,10 @@ hipError_t paged_store_launch(const PagePool &p, const PageRows &r, const float 
     pages.add(r, i, t ? (last >> p.shift) - (r.pos[i] >> p.shift) + 1 : 0);
   }
   StoreArgs A{p, rope, q, k, v, qr, H, 0, 0};
-  if (T < kPgUnitRows) {
+  if (T == 1 || (int64_t)rows * (H + p.KH) * p.HD <= kPgRowValues) {
     if (T > 1) A.p.bounds = nullptr;  // rows of a page, by several waves
     const int hs = 128 / p.HD;  // heads of a wave at once
-    // enough waves for every SIMD, no more than eight heads each
-    A.each = hs;
-    while (A.each < 8 && (int64_t)rows * (H / A.each) > 2048) A.each *= 2;
-    A.parts = (H + A.each - 1) / A.each + (p.KH + hs - 1) / hs;
+    A.parts = (H + kPgRowHeads - 1) / kPgRowHeads + (p.KH + hs - 1) / hs;
     const dim3 grid((unsigned)((int64_t)rows * A.parts));
     if (p.HD == 64) hipLaunchKernelGGL(paged_rows_kernel<64>, grid, dim3(64), 0, st, A, each);
     else hipLaunchKernelGGL(paged_rows_kernel<128>, grid, dim3(64), 0, st, A, each);
