@@ -495,9 +495,9 @@ int wl_paged_read_dev(wl_ctx *ctx, const wl_pages *p, int32_t seq, int32_t pos0,
 /* wl_attention_dev over pages: d_q, d_out [rows][heads * head_dim], each row over positions 0 .. its own of its sequence. A
  * score of -inf weighs nothing; a row without a score above -inf (or that sees no page) gives zeros. A visible value that is
  * infinite or NaN makes its column of the rows that see it infinite or NaN.
- * prefix > 0 (whole pages): the entries' sequences have the same pages for the positions below it, which are read from the
- * first entry's and once for all rows; every pos[i] is at least prefix. With prefix 0 a row's bits do not depend on the other
- * entries; with one they differ from those in the last places. */
+ * prefix > 0 (whole pages): the entries' sequences have the same pages for the positions below it, which are read once for
+ * all rows, from an entry's, where that takes less time (long prefixes of many rows); every pos[i] is at least prefix. With
+ * prefix 0 a row's bits do not depend on the other entries; with one they may differ from those in the last places. */
 int wl_paged_attention_dev(wl_ctx *ctx, const wl_pages *p, const wl_page_rows *r, const float *d_q, int32_t heads,
                            int32_t prefix, float scale, float *d_out);
 

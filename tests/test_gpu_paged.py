@@ -339,9 +339,26 @@ def test_shared_prefix(ctx, H, KH, HD, page, prefix, N, T):
     assert same(got, pool.attend(seq, pos, rows, q, prefix=prefix))
 
 
-def test_prefix_with_more_entries_than_a_launch_takes(ctx):
+@pytest.mark.parametrize("H,KH,HD,page", [(8, 2, 64, 32), (16, 2, 128, 256), (5, 1, 128, 16)])
+@pytest.mark.parametrize("prefix,N,T", [(8192, 36, 1), (16384, 20, 3), (8192, 4, 50), (65536, 5, 1)])
+def test_shared_prefix_that_is_read_once(ctx, H, KH, HD, page, prefix, N, T):
+    rng = np.random.default_rng(prefix + H)
+    lengths = [prefix + T + (13 * i) % 90 for i in range(N)]
+    pool = Pool(ctx, lengths, KH, HD, page, seed=6, shared=prefix, room=1)
+    pos = [n - T for n in lengths]
+    q = normal(rng, N * T, H, HD, scale=2)
+    got = pool.attend(list(range(N)), pos, [T] * N, q, prefix=prefix)
+    for r in sorted({0, N * T - 1, *rng.permutation(N * T)[:6].tolist()}):
+        p = pos[r // T] + r % T
+        want, tol = attend_ref(q[r:r + 1], pool.K[r // T], pool.V[r // T], [[np.arange(p + 1)] * KH], HD ** -0.5)
+        near(got[r:r + 1], want, tol, "row %d" % r)
+    assert same(got, pool.attend(list(range(N)), pos, [T] * N, q, prefix=prefix))
+
+
+@pytest.mark.parametrize("prefix", [320, 3200])
+def test_prefix_with_more_entries_than_a_launch_takes(ctx, prefix):
     rng = np.random.default_rng(1)
-    H, KH, HD, page, N, prefix = 4, 1, 64, 16, 200, 320
+    H, KH, HD, page, N = 4, 1, 64, 16, 200
     pool = Pool(ctx, [prefix + 1 + i % 20 for i in range(N)], KH, HD, page, shared=prefix, room=1)
     seq, pos = list(range(N)), [prefix + i % 20 for i in range(N)]
     q = normal(rng, N, H, HD)
@@ -349,19 +366,19 @@ def test_prefix_with_more_entries_than_a_launch_takes(ctx):
     near(pool.attend(seq, pos, None, q, prefix=prefix), want, tol, "prefix")
 
 
-@pytest.mark.parametrize("N,T", [(3, 1), (4, 40)])
-def test_prefix_with_missing_and_odd_pages(ctx, N, T):
+@pytest.mark.parametrize("N,T,prefix", [(3, 1, 128), (4, 40, 128), (9, 1, 16384), (4, 40, 4096)])
+def test_prefix_with_missing_and_odd_pages(ctx, N, T, prefix):
     """A prefix whose pages are missing in part or all, an infinity in it, and rows that then see little."""
     import torch
     rng = np.random.default_rng(N)
-    H, KH, HD, page, prefix = 8, 2, 128, 32, 128
+    H, KH, HD, page = 8, 2, 128, 32
 
     def values(s, k, v):
         v[70, :, 4] = np.inf
     pool = Pool(ctx, [prefix + 60] * N, KH, HD, page, shared=prefix, values=values)
     q = normal(rng, N * T, H, HD)
     seq, pos, rows = list(range(N)), [prefix + 60 - T] * N, [T] * N
-    for gone in ([1], [0, 1, 2, 3], list(range(pool.table.shape[1]))):
+    for gone in ([1], list(range(prefix // page)), list(range(pool.table.shape[1]))):
         pool.d_table[:, gone] = -1
         torch.cuda.synchronize()
         got = pool.attend(seq, pos, rows, q, prefix=prefix)

@@ -62,8 +62,8 @@ hipError_t paged_store_launch(const PagePool &p, const PageRows &r, const float 
 // Positions pos0 .. pos0 + T - 1 of a sequence as rows k, v [T][KH * HD]; zeros where there is no page.
 hipError_t paged_read_launch(const PagePool &p, int seq, int pos0, int T, float *k, float *v, hipStream_t st);
 
-// Attention of the rows q [rows][H * HD]. prefix > 0: positions below it are read once, from the pages of the first
-// entry's sequence, for all rows. blocks [rows][KH][most] (or null): the pages that a row and KV head reads, in order, -1
+// Attention of the rows q [rows][H * HD]. prefix > 0: positions below it are the same pages for all entries, and may
+// be read once for all rows. blocks [rows][KH][most] (or null): the pages that a row and KV head reads, in order, -1
 // after the last.
 int64_t paged_attention_scratch_floats(const PagePool &p, const PageRows &r, int H, int prefix, int most);
 hipError_t paged_attention_launch(const PagePool &p, const PageRows &r, const float *q, int H, int prefix,

@@ -13,6 +13,7 @@
 #include "wl_paged_device.h"
 
 #include <algorithm>
+#include <math.h>
 
 #pragma clang fp contract(off)
 
@@ -761,12 +762,44 @@ constexpr int kFewWhole = 32, kFewLeast = 16;
 // pages 25.6, 26.8 and 24.8.
 constexpr int kChosenWhole = 16, kChosenLeast = 8;
 
-// Steps of each run of an entry whose longest columns take n steps, in nz workgroups of columns a KV head.
-static int many_per(int n, int64_t wgs) {
-  int64_t S = wgs >= 256 ? 1 : 512 / wgs;  // two workgroups fit a CU: one more than that is a second round
-  S = S > n ? n : S;
-  S = S > kPgRuns / 2 ? kPgRuns / 2 : S;
-  return ceil_div(n, S);
+// Steps of each run of an entry in wgs workgroups of columns, whose shortest columns take n0 steps and whose longest n. A CU takes
+// two workgroups at once, in 1.2 times the time of two halves' sum alone, and a run costs five steps beside its own; the runs go
+// round by round over the CUs. In us, with as many runs as 512 workgroups make and with the rule's: 8B, 700 rows up to 20,000 478 and
+// 455, 1,300 863 and 758, 2,500 1,579 and 1,403; 600 up to 3,000 94 and 79; 1B, 700 up to 9,000 164 and 136. Where most positions are
+// the rows' own, the workgroups, longest and shortest in turn, even out by themselves (1,300 from 0 59 us; in two runs 80).
+static int many_per(int n0, int n, int64_t wgs) {
+  if (2 * n0 < n) {
+    const int64_t S = wgs >= 256 ? 1 : 512 / wgs;
+    return ceil_div(n, std::min({S, (int64_t)n, (int64_t)kPgRuns / 2}));
+  }
+  constexpr double kRunSteps = 5, kAlone = 1.2;
+  const double work = 0.5 * ((double)n0 + n) * wgs;
+  int best = n;
+  double least = INFINITY;
+  for (int S = 1; S <= n && S <= kPgRuns / 2 && (S == 1 || S * wgs < 8 * 256); S++) {
+    const int per = ceil_div(n, S);
+    if (ceil_div(n, per) != S) continue;
+    const double runs = S == 1 ? wgs : 0.5 * wgs * (ceil_div(n0, per) + S);
+    const int64_t rounds = (int64_t)ceil(runs / 256);
+    const double t = (work / runs + kRunSteps) * (rounds == 1 ? kAlone : rounds & 1 ? rounds + 0.5 * (kAlone - 1) : rounds);
+    if (t < least) {
+      least = t;
+      best = per;
+    }
+  }
+  return best;
+}
+
+// Whether a prefix is read once for all rows: where what its entries would read of it, a pass for each 16 of their columns, is more
+// than 2^18 positions of keys and values (in all KV heads); else the join that it needs costs more, and each entry reads it for
+// itself, from the caches after the first. At the border, in us, read once and by each entry: 8B, 16 rows on 2,048 19.2 and 16.9, on
+// 4,096 20.8 and 28.1; 2 on 8,192 19.0 and 16.6, on 16,384 22.2 and 27.2; 64 on 512 24.4 and 19.7, on 1,024 26.4 and 33.0, but 110 on
+// 512 38.4 and 34.7, so 1,024 at least. Entries that fill the workgroups by themselves (four of 300 rows on 4,096: 243 and 204;
+// of 100 83 and 104) gain nothing.
+static bool prefix_pays(const PagePool &p, const PageRows &r, int G, int prefix) {
+  int64_t passes = 0;
+  for (int i = 0; i < r.n; i++) passes += ceil_div((int64_t)r.rows(i) * G, kFewCols);
+  return prefix >= 1024 && (double)passes * prefix * p.KH > 0x1p18 && (int64_t)r.row0[r.n] * G <= (int64_t)1024 * r.n;
 }
 
 // The launches of a call.
@@ -779,6 +812,7 @@ struct PagedLaunches {
 // most: the pages that a row may take (0: all positions).
 static void paged_launches(const PagePool &p, const PageRows &r, int H, int prefix, int most, PagedLaunches &L) {
   const int G = H / p.KH, rows = r.row0[r.n], upp = p.page / kPgUnit;
+  if (prefix && !prefix_pays(p, r, G, prefix)) prefix = 0;
   L.few.alone = L.many.alone = !prefix;
   L.few.base = L.many.base = prefix / kPgUnit;
   L.few.flat0 = L.few.flat1 = L.many.flat0 = L.many.flat1 = 0;
@@ -793,12 +827,17 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
     const bool f = is_few((int64_t)rows * G, prefix, prefix, p.KH);
     PagedPlan &U = f ? L.few : L.many;
     const int blocks = ceil_div((int64_t)rows * G, f ? kFewCols : kManyCols), n = ceil_div(prefix / kPgUnit, f ? 2 : kManyUnits);
-    const int per = f ? few_per(n, p.KH * blocks, kFewWaves, kFewWaves) : many_per(n, (int64_t)p.KH * blocks);
+    const int per = f ? few_per(n, p.KH * blocks, kFewWaves, kFewWaves) : many_per(n, n, (int64_t)p.KH * blocks);
     L.runs.pre = ceil_div(n, per);
     U.it.add(all, 0, L.runs.pre * blocks, per, 0, L.runs.pre);
     U.flat1 = U.it.items;
     L.records = rows * L.runs.pre;
   }
+  struct {
+    bool few;
+    int items, per, runs;
+  } e[kPgRows];
+  int order[kPgRows], n = 0, many = 0;
   for (int i = 0; i < r.n; i++) {
     const int T = r.rows(i), last = r.pos[i] + T - 1;
     if (!T) continue;
@@ -812,15 +851,24 @@ static void paged_launches(const PagePool &p, const PageRows &r, int H, int pref
       runs = ceil_div(ceil_div((int64_t)took * upp, 2), per);
     } else {
       const int units = (last >> 4) - prefix / kPgUnit + 1, n = ceil_div(units, f ? 2 : kManyUnits);
+      const int n0 = ceil_div((r.pos[i] >> 4) - prefix / kPgUnit + 1, kManyUnits);
       blocks = ceil_div(NC, f ? kFewCols : kManyCols);
-      per = f ? few_per(n, p.KH * blocks, kFewWhole, kFewLeast) : many_per(n, (int64_t)p.KH * blocks);
+      per = f ? few_per(n, p.KH * blocks, kFewWhole, kFewLeast) : many_per(n0, n, (int64_t)p.KH * blocks);
       runs = ceil_div(n, per);
     }
-    (f ? L.few : L.many).it.add(r, i, runs * blocks, per, L.records, runs);
-    if (runs == 1 && !prefix) continue;
-    L.runs.it.add(r, i, T, 0, L.records, runs);
-    L.records += T * runs;
-    L.most_runs = std::max(L.most_runs, L.runs.pre + runs);
+    e[i] = {f, runs * blocks, per, runs};
+    order[n++] = i;
+    many += !f;
+  }
+  // the longest runs first, so that the short ones fill the end (prompts of 2,001, 667 and 50 rows 505 -> 492 us)
+  if (many > 1) std::stable_sort(order, order + n, [&](int a, int b) { return e[a].per > e[b].per; });
+  for (int k = 0; k < n; k++) {
+    const int i = order[k], T = r.rows(i);
+    (e[i].few ? L.few : L.many).it.add(r, i, e[i].items, e[i].per, L.records, e[i].runs);
+    if (e[i].runs == 1 && !prefix) continue;
+    L.runs.it.add(r, i, T, 0, L.records, e[i].runs);
+    L.records += T * e[i].runs;
+    L.most_runs = std::max(L.most_runs, L.runs.pre + e[i].runs);
   }
 }
 
