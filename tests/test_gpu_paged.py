@@ -489,12 +489,13 @@ def test_missing_pages_are_not_taken(ctx):
 # ------------------------------------------------------------------------------------- together
 
 
-def test_a_recorded_step_and_its_replays(ctx):
+@pytest.mark.parametrize("prefix", [512, 24576])
+def test_a_recorded_step_and_its_replays(ctx, prefix):
     """Store, attention with and without a prefix and the sparse choice, recorded, replayed over other values, with eager calls
     between the replays."""
     import torch
     from windlass_amd.backend import PageRows, SparseOpts
-    L, H, KH, HD, page, prefix, N = load(), 16, 2, 128, 16, 512, 6
+    L, H, KH, HD, page, N = load(), 16, 2, 128, 16, 6
     rng = np.random.default_rng(3)
     lengths = [prefix + 20 + 31 * i for i in range(N)]
     pool = Pool(ctx, lengths, KH, HD, page, shared=prefix, bounds=True)

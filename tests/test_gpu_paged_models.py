@@ -95,6 +95,56 @@ def test_layer_equals_its_operations(ctx, HD, rd, neox, seq, pos, rows, prefix, 
     l.free()
 
 
+@pytest.mark.parametrize("seq,pos,rows,prefix,sparse", [
+    ([2, 0, 1], [90, 100, 41], None, 0, None), ([0, 1], [100, 200], None, 0, (1, 2, 3)), ([1, 2], [60, 90], [3, 40], 48, None)])
+def test_a_recorded_layer_reads_the_table_as_it_is(ctx, seq, pos, rows, prefix, sparse):
+    """Replays over other rows and after pages have moved, with eager calls between."""
+    rng = np.random.default_rng(11)
+    l = PagedLayer(ctx, 64, 64, 1)
+    l.pool(rng, [100, 200, 90])
+    if prefix:
+        l.t[3][2, :3] = l.t[3][1, :3]
+        torch.cuda.synchronize()
+    T = sum(rows) if rows else len(seq)
+    x = torch.zeros((T, E), device=DEV)
+    r, o = PageRows(seq, pos, rows), SparseOpts(*sparse) if sparse else None
+
+    def step():
+        check(load().wl_layer_paged_dev(ctx.handle, ctypes.byref(l.d), P(x), ctypes.byref(l.p), ctypes.byref(r), prefix,
+                                        ctypes.byref(o) if o else None))
+    step()
+    ctx.sync()
+    graph = ctx.capture(step)
+    free = sorted(set(range(l.p.pages)) - set(l.t[3].cpu().numpy().reshape(-1).tolist()))[0]
+    for i in range(3):
+        new = dev(rng.standard_normal((T, E), dtype=F32))
+        # the page before the last entry's own goes to a free place
+        j = pos[-1] // 16 - 1
+        old = int(l.t[3][seq[-1], j])
+        for t, n in ((l.t[0], KH * 16 * 64), (l.t[1], KH * 16 * 64), (l.t[2], KH * 2 * 64)):
+            t[free * n:free * n + n] = t[old * n:old * n + n]
+            t[old * n:old * n + n] = 3.0
+        torch.cuda.synchronize()
+        check(load().wl_paged_assign_dev(ctx.handle, ctypes.byref(l.p), seq[-1], j, 1, (ctypes.c_int32 * 1)(free)))
+        ctx.sync()
+        free = old
+        was = l.state()
+        x.copy_(new)
+        torch.cuda.synchronize()
+        step()
+        ctx.sync()
+        want, now = x.clone(), l.state()
+        for a, b in zip(l.t, was):
+            a.copy_(b)
+        x.copy_(new)
+        torch.cuda.synchronize()
+        graph.launch()
+        ctx.sync()
+        assert same(ctx, x, want) and all(same(ctx, a, b) for a, b in zip(l.t, now)), i
+    graph.free()
+    l.free()
+
+
 @pytest.mark.parametrize("N", [1, 5, 70, 140])
 @pytest.mark.parametrize("sparse", [None, (1, 1, 3)])
 def test_batch_rows_equal_single_tokens(ctx, N, sparse):
