@@ -759,7 +759,8 @@ static int few_per(int n, int units, int whole, int least) {
 }
 constexpr int kFewWhole = 32, kFewLeast = 16;
 // Chosen pages: 16 rows of 32 pages of 64 (70B) 53.5 us with two tiles a wave, 49.8 with four and 58.6 with one; a lone row of 64
-// pages 25.6, 26.8 and 24.8.
+// pages 25.6, 26.8 and 24.8. Whole up to 32 tiles as above, 64 rows of 32 pages of 32 (70B) would take 71 us, not 83, but 8 rows of 8B
+// 26.4, not 23.5, and rows of long contexts come in small batches.
 constexpr int kChosenWhole = 16, kChosenLeast = 8;
 
 // Steps of each run of an entry in wgs workgroups of columns, whose shortest columns take n0 steps and whose longest n. A CU takes
