@@ -171,3 +171,23 @@ def test_a_shared_beginning_for_sequences_that_hold_pages_is_refused():
     with pytest.raises(ShapeError):
         b.generate([[1] * 20, [1] * 20], 2, [SampleParams()] * 2, [0.5] * 4, shared=16)
     assert not queued(m)
+
+
+def test_what_all_of_the_sequences_share():
+    """Against its definition, over sequences that begin at one another."""
+    import random
+    rng = random.Random(0)
+    b = batch(model(), pages=200, slots=8, cap=200)
+    for s in range(8):
+        if s and rng.random() < 0.8:
+            src = rng.randrange(s)
+            b.share(src, s, rng.randrange(0, b.length[src] // 16 + 1) * 16)
+        b.prefill(s, [1] * rng.randrange(1, 80))
+    for _ in range(300):
+        slots = rng.sample(range(8), rng.randrange(1, 9))
+        n = 0
+        for ids in zip(*(b.held[s] for s in slots)):
+            if len(set(ids)) > 1:
+                break
+            n += 1
+        assert b._shared(slots) == (n * 16 if len(slots) > 1 else 0)

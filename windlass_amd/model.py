@@ -613,11 +613,12 @@ class PagedBatch(DeviceBatch):
         """The positions at the beginning that all of the sequences have in the same pages."""
         if len(slots) < 2:
             return 0
-        n = 0
-        for ids in zip(*(self.held[s] for s in slots)):
-            if any(i != ids[0] for i in ids):
-                break
+        first, n = self.held[slots[0]], 0
+        while n < len(first) and self.users[first[n]] >= len(slots):
             n += 1
+        for s in slots[1:]:
+            if self.held[s][:n] != first[:n]:  # pages that others hold too
+                n = next((i for i, (a, b) in enumerate(zip(first[:n], self.held[s])) if a != b), min(n, len(self.held[s])))
         return n * self.page
 
     def _pass(self, x, slots, counts, prefix, sparse):
@@ -641,7 +642,7 @@ class PagedBatch(DeviceBatch):
 
     def step(self, slots, d_ids):
         """One stacked decode step (DeviceBatch.step); pages that all of the sequences share at their beginning are read
-        once."""
+        once where that takes less time."""
         m, c, N = self.m, ctypes.c_void_p, len(slots)
         self._grow(slots, [1] * N)
         x = self._buf("x", N, m.cfg.embd)
