@@ -124,6 +124,49 @@ def test_stored_rows_have_the_other_caches_bits(ctx, T, HD, n, neox):
     assert same(gv, Vc[pos0:].float().reshape(T, KH, HD).cpu().numpy())
 
 
+@pytest.mark.parametrize("H,KH,HD,page,n,neox", [(32, 8, 128, 64, 128, 0), (63, 3, 64, 16, 64, 1), (48, 1, 128, 256, 96, 1),
+                                                 (64, 64, 64, 32, 0, 0)])
+def test_prompts_of_many_rows(ctx, H, KH, HD, page, n, neox):
+    """Past the rows that go by themselves: the formulas' values, and the bits of small calls."""
+    rng = np.random.default_rng(H)
+    every = (11 << 20) // ((H + KH) * HD)
+    seq, pos, rows = [2, 0, 4, 1, 3], [5, 300, 16, 0, 37], [every // 2 + 3, every // 4, 1, 0, every // 4 + 8]
+    lengths = [p + t + 1 for s, p, t in sorted(zip(seq, pos, rows))]
+    R = sum(rows)
+    assert R * (H + KH) * HD > 10 << 20
+    q, k, v = normal(rng, R, H, HD), normal(rng, R, KH, HD), normal(rng, R, KH, HD)
+    k[R // 3, 0, 3], k[R // 3 + 1, 0, 4] = np.nan, -np.inf
+    freqs = (1 + 7 * rng.random(n // 2)).astype(F32) if n == 128 else None
+    pools, got = [], []
+    for many in (True, False):
+        pool = Pool(ctx, [40] * 5, KH, HD, page, seed=3, bounds=True, room=max(lengths))
+        if many:
+            got.append(pool.store(seq, pos, rows, q, k, v, n, neox, 500000.0, 0.5, freqs))
+        else:
+            parts, at = [], 0
+            for s, p, t in zip(seq, pos, rows):
+                for i in range(0, t, 200):
+                    m = min(200, t - i)
+                    a = slice(at + i, at + i + m)
+                    parts.append(pool.store([s], [p + i], [m], q[a], k[a], v[a], n, neox, 500000.0, 0.5, freqs))
+                at += t
+            got.append(np.concatenate(parts))
+        pools.append(pool)
+    assert same(*got)
+    for x in ("dK", "dV", "dB"):
+        a, b = (getattr(p, x).cpu().numpy().view(np.uint16) for p in pools)
+        assert np.array_equal(a, b), x
+    some = sorted({0, R // 3, R - 1, *rng.permutation(R)[:40].tolist()})
+    places = np.concatenate([p + np.arange(t) for p, t in zip(pos, rows)])[some]
+    want, tol = rope_ref(q[some], places, n, neox, 500000.0, 0.5, freqs)
+    near(got[0][some], want, tol, "q")
+    at = 0
+    for s, p, t in zip(seq, pos, rows):
+        if t:
+            assert same(pools[0].read(s, p, t)[1], v[at:at + t].astype(np.float16).astype(F32))
+        at += t
+
+
 def test_more_entries_than_a_launch_takes(ctx):
     """300 sequences: stores, bounds and attention of entries past the first launch's."""
     rng = np.random.default_rng(5)

@@ -13,7 +13,7 @@ namespace wl {
 // Values (of q and k) up to which a call's rows go by themselves, past which by units: 8B in us 20.2 and 23.1 at 1,536 rows, 24.8 and
 // 24.6 at 2,048; 70B 20.8 and 22.5 at 1,024, 28.2 and 30.5 at 1,536 of 64 sequences, 26.6 and 25.3 at 1,500 of one; 1B 13.3 and 20.1
 // at 2,000.
-constexpr int64_t kPgRowValues = (int64_t)8 << 20;
+constexpr int64_t kPgRowValues = (int64_t)10 << 20;
 // Query heads of a row that share a wave and its angles: one row of 8B takes 5.2 us as with two each, 110 rows of 70B 8.5 (12.5).
 constexpr int kPgRowHeads = 8;
 
@@ -55,8 +55,9 @@ __device__ __forceinline__ fh8 lane_swap(fh8 v, int m) {
 
 // Few rows: a wave per part of a row, kPgRowHeads query heads or the keys and values of one KV head (two of 64), a lane per pair, so
 // that the heads of a part share its angles. With one row of each sequence the waves of the keys also make their page's bounds.
-// Latency bounds it: one row of 32 + 8 heads of 128 5.2 us, of which a launch takes 4.9; 64 rows of 64 + 8 with bounds 7.5.
-template <int HD>
+// Latency bounds it: one row of 32 + 8 heads of 128 5.2 us, of which a launch takes 4.9; 64 rows of 64 + 8 with bounds
+// 6.3, whose pages' keys are loaded beside the row (after it 7.9).
+template <int HD, bool BOUNDS>
 __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U) {
   constexpr int NP = HD / 2, HS = 64 / NP, N = kPgRowHeads / HS;  // pairs, heads at once, and of a part one after the other
   __shared__ double theta[NP];
@@ -73,6 +74,10 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U
   // loads first, then the angles
   float2 v[N], w = make_float2(0.f, 0.f);
   int id = -1;
+  // the page's keys, 16 bytes a lane: eight channels lane / 8 (+ 8 for every other piece of a head of 128) of position slot (+ 4)
+  constexpr int SETS = HD / 64, AHEAD = 4;  // units loaded before the angles are made
+  const int slot = (lane >> 2 & 1) * 8 + (lane & 3);
+  fh8 ahead[HS][AHEAD][2 * SETS];
   if (isq) {
 #pragma unroll
     for (int e = 0; e < N; e++) {
@@ -84,6 +89,17 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U
     const int64_t r = ((int64_t)row * KH + (h0 + sub < KH ? h0 + sub : KH - 1)) * HD;
     v[0] = pr.load(A.k + r);
     w = make_float2(A.v[r + 2 * x], A.v[r + 2 * x + 1]);
+    if (BOUNDS && id >= 0) {
+#pragma unroll
+      for (int g = 0; g < HS; g++) {
+        const uint16_t *K = A.p.K + A.p.at(id, h0 + g < KH ? h0 + g : KH - 1) + lane * 8;
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+          for (int e = 0; e < 2 * SETS; e++)
+            if (16 * u + slot + 4 * (e / SETS) < off) ahead[g][u][e] = *reinterpret_cast<const fh8 *>(K + u * 16 * HD + e * 512);
+      }
+    }
   }
   float c = 1.f, s = 0.f;
   if (half) {
@@ -115,26 +131,28 @@ __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U
     A.p.V[at + pg_val(off, 2 * x, HD)] = half_of(w.x);
     A.p.V[at + pg_val(off, 2 * x + 1, HD)] = half_of(w.y);
   }
-  if (!A.p.bounds) return;
+  if constexpr (!BOUNDS) return;
   __syncthreads();
-  // the page's positions before this one, 16 bytes a lane: eight channels lane / 8 (+ 8 for every other piece of a head of 128)
-  constexpr int SETS = HD / 64;
-  for (int g = 0; g < HS && h0 + g < KH; g++) {
-    const uint16_t *K = A.p.K + A.p.at(id, h0 + g);
+#pragma unroll
+  for (int g = 0; g < HS; g++) {
+    if (h0 + g >= KH) break;
+    const uint16_t *K = A.p.K + A.p.at(id, h0 + g) + lane * 8;
     fh8 lo[SETS], hi[SETS];
 #pragma unroll
     for (int e = 0; e < SETS; e++) lo[e] = hi[e] = *reinterpret_cast<const fh8 *>(&fresh[g][64 * e + lane / 8 * 8]);
-    const int slot = (lane >> 2 & 1) * 8 + (lane & 3);
-    for (int u = 0; 16 * u < off; u++) {
+    auto take = [&](fh8 k, int e) __attribute__((always_inline)) {
+      lo[e % SETS] = least(lo[e % SETS], k);
+      hi[e % SETS] = most(hi[e % SETS], k);
+    };
 #pragma unroll
-      for (int e = 0; e < 2 * SETS; e++) {
-        const int t = e / SETS;
-        if (16 * u + slot + 4 * t >= off) continue;
-        const fh8 b = *reinterpret_cast<const fh8 *>(K + u * 16 * HD + e * 512 + lane * 8);
-        lo[e % SETS] = least(lo[e % SETS], b);
-        hi[e % SETS] = most(hi[e % SETS], b);
-      }
-    }
+    for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+      for (int e = 0; e < 2 * SETS; e++)
+        if (16 * u + slot + 4 * (e / SETS) < off) take(ahead[g][u][e], e);
+    for (int u = AHEAD; 16 * u < off; u++)
+#pragma unroll
+      for (int e = 0; e < 2 * SETS; e++)
+        if (16 * u + slot + 4 * (e / SETS) < off) take(*reinterpret_cast<const fh8 *>(K + u * 16 * HD + e * 512), e);
 #pragma unroll
     for (int e = 0; e < SETS; e++) {
 #pragma unroll
@@ -309,12 +327,13 @@ hipError_t paged_store_launch(const PagePool &p, const PageRows &r, const float 
   }
   StoreArgs A{p, rope, q, k, v, qr, H, 0, 0};
   if (T == 1 || (int64_t)rows * (H + p.KH) * p.HD <= kPgRowValues) {
-    if (T > 1) A.p.bounds = nullptr;  // rows of a page, by several waves
     const int hs = 128 / p.HD;  // heads of a wave at once
     A.parts = (H + kPgRowHeads - 1) / kPgRowHeads + (p.KH + hs - 1) / hs;
     const dim3 grid((unsigned)((int64_t)rows * A.parts));
-    if (p.HD == 64) hipLaunchKernelGGL(paged_rows_kernel<64>, grid, dim3(64), 0, st, A, each);
-    else hipLaunchKernelGGL(paged_rows_kernel<128>, grid, dim3(64), 0, st, A, each);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64), 0, st, A, each); };
+    const bool bounds = p.bounds && T == 1;  // rows of a page, by several waves, cannot
+    if (p.HD == 64) bounds ? run(paged_rows_kernel<64, true>) : run(paged_rows_kernel<64, false>);
+    else bounds ? run(paged_rows_kernel<128, true>) : run(paged_rows_kernel<128, false>);
   } else {
     // Parts of a unit, of a KV head or a query head at least: as many as give every CU six workgroups (4,248 rows of 32 + 8 heads
     // of 128 39.5 us, 4.8 TB/s; two 52.2, eight 41.9, sixteen, whose angles are made as often, 59.6).
