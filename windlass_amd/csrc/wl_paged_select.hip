@@ -37,8 +37,9 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 // and lane l has the channels l / 16 * HD / 4 on of both, so that its loads are whole. The rows come out in lanes l / 16; the
 // largest of a column is the page's score. The heads' halves lie in LDS in 64 bits: converting them in each wave took as long
 // as the products. 16 rows of 70B on up to 500 pages of 64 take 13.5 us: 33 MB of bounds, and 6.6 us of products after them.
+// Waves a SIMD are named, as many as fit without what follows a sum that is not finite.
 template <int HD, int NB>
-__global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
+__global__ __launch_bounds__(256, HD == 64 ? 4 : NB <= 2 ? 3 : 2) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
                                                           const float *__restrict__ q, int G, uint64_t *__restrict__ keys,
                                                           int64_t width) {
   constexpr int N = HD / 4;
@@ -58,6 +59,7 @@ __global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems 
     hi[e] = *reinterpret_cast<const fh8 *>(b + HD + 8 * e);
   }
   double best = -INFINITY;
+  bool odd = false;
   for (int g0 = 0; g0 < G; g0 += 4 * NB) {
     if (g0) __syncthreads();
 #pragma unroll
@@ -84,6 +86,30 @@ __global__ __launch_bounds__(256) void paged_score_kernel(PagePool P, PageItems 
 #pragma unroll
     for (int h = 0; h < NB; h++) {
       const double s = up[h] + down[h];
+      odd |= !__builtin_isfinite(s);
+      best = fmax(best, __builtin_isfinite(s) ? s : INFINITY);
+    }
+  }
+  if (__any(odd && id >= 0)) {
+    // A bound or query is infinite or NaN, and the zero that stands for a query of the other sign makes NaN also of the infinite bound
+    // that max(q lo, q hi) does not take. So by that itself, head by head, a quarter of the channels a lane: rare, and its loops
+    // are small ones, since the products again would take twice the registers of all that is above.
+    best = -INFINITY;
+#pragma unroll 1
+    for (int g = 0; g < G; g++) {
+      const float *qp = q + ((int64_t)row * H + kvh * G + g) * HD + k * N;
+      double s = 0.0;
+#pragma unroll 1
+      for (int c = 0; c < N; c += 8) {
+        const fh8 l8 = *reinterpret_cast<const fh8 *>(b + c), h8 = *reinterpret_cast<const fh8 *>(b + HD + c);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const double x = (double)qp[c + e], low = x * (double)(float)l8[e], high = x * (double)(float)h8[e];
+          s += low != low || low > high ? low : high;  // a NaN of either
+        }
+      }
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
       best = fmax(best, __builtin_isfinite(s) ? s : INFINITY);
     }
   }
