@@ -2093,7 +2093,9 @@ static int paged_sparse(const char *who, const wl_pages *p, const wl_sparse_opts
 // Rows of a launch: a (row, head) pair is a workgroup of up to 512 threads of one of them, and a grid has fewer than 2^32.
 static int paged_most_rows(int heads) { return std::max(1, (1 << 22) / heads); }
 
-// f(rows, first row) for a call's entries, kPgRows and `most` rows at a time; entries without rows are left out.
+// f(rows, first row) for a call's entries, kPgRows and `most` rows at a time; entries without rows are left out. A launch ends
+// before an entry that it has no room for, and an entry of more than `most` rows is cut from its own first on: a row's bits
+// depend on where its entry is cut, and so not on the entries before.
 template <class F>
 static int each_page_rows(const wl_page_rows *r, int most, const F &f) {
   wl::PageRows R;
@@ -2107,8 +2109,10 @@ static int each_page_rows(const wl_page_rows *r, int most, const F &f) {
   };
   for (int i = 0; i < r->n; i++) {
     const int T = r->rows ? r->rows[i] : 1;
+    if (R.n && T > most - R.row0[R.n])
+      if (const int rc = flush()) return rc;
     for (int t = 0; t < T;) {
-      const int m = std::min(T - t, most - R.row0[R.n]);
+      const int m = std::min(T - t, most);
       R.seq[R.n] = r->seq[i];
       R.pos[R.n] = r->pos[i] + t;
       R.row0[R.n + 1] = R.row0[R.n] + m;
