@@ -31,7 +31,7 @@ extern "C" {
 #define WL_E_SHAPE (-2)       /* ArgumentException "MatMul shape mismatch" (src/Transformer.cs:486) */
 #define WL_E_DEVICE (-3)      /* HIP runtime failure; the server's BackendException 500 (src/Server.cs:756-761) */
 #define WL_E_ARG (-4)         /* ArgumentOutOfRangeException / null argument (src/LayerStream.cs:28) */
-#define WL_E_NOMEM (-5)       /* device allocation failed */
+#define WL_E_NOMEM (-5)       /* an allocation failed, on the device or for a paged call's entries */
 
 /* ggml type ids (enum GgmlType, src/Gguf.cs:19-25). */
 #define WL_TYPE_F32 0

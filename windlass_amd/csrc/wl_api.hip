@@ -11,7 +11,9 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -2059,9 +2061,11 @@ static int paged_rows(const char *who, const wl_pages *p, const wl_page_rows *r,
   }
   if (all > 1 << 24) return fail(WL_E_SHAPE, "%s: %lld rows", who, (long long)all);
   if (distinct) {
-    std::vector<int32_t> s(r->seq, r->seq + r->n);
-    std::sort(s.begin(), s.end());
-    if (std::adjacent_find(s.begin(), s.end()) != s.end())
+    const std::unique_ptr<int32_t[]> s(new (std::nothrow) int32_t[r->n]);
+    if (!s) return fail(WL_E_NOMEM, "%s: no host memory for %d entries", who, r->n);
+    std::copy(r->seq, r->seq + r->n, s.get());
+    std::sort(s.get(), s.get() + r->n);
+    if (std::adjacent_find(s.get(), s.get() + r->n) != s.get() + r->n)
       return fail(WL_E_ARG, "%s: a sequence can be one entry of a call that stores.", who);
   }
   *rows = (int)all;
