@@ -2094,7 +2094,8 @@ static int paged_sparse(const char *who, const wl_pages *p, const wl_sparse_opts
   return WL_OK;
 }
 
-// Rows of a launch: a (row, head) pair is a workgroup of up to 512 threads of one of them, and a grid has fewer than 2^32.
+// Rows of a launch, whose grid has fewer than 2^32 threads: its kernels have 256 for a (row, head) pair at most (the join of runs).
+// Chosen pages have 1,024 for a (row, KV head) pair, and rows of their own (sparse_rows).
 static int paged_most_rows(int heads) { return std::max(1, (1 << 22) / heads); }
 
 // f(rows, first row) for a call's entries, kPgRows and `most` rows at a time; entries without rows are left out. A launch ends
@@ -2223,8 +2224,9 @@ static int sparse_rows(const wl::PagePool &pool, const wl_page_rows *r, int head
   last.pos[0] = (int)end - 1;
   last.row0[1] = 1;
   const int64_t record = std::max((int64_t)1, wl::paged_attention_scratch_floats(pool, last, heads, 0, s.most()));
+  // and at most 2^31 threads of the choice, 1,024 for a row's KV head
   return (int)std::clamp(std::min(((int64_t)32 << 20) / (pages * pool.KH), ((int64_t)256 << 20) / record), (int64_t)1,
-                         (int64_t)paged_most_rows(heads));
+                         (int64_t)std::min(paged_most_rows(heads), std::max(1, (1 << 21) / pool.KH)));
 }
 
 static int paged_sparse_attention(wl_ctx *c, const wl::PagePool &pool, const wl_page_rows *r, const float *d_q, int heads,
