@@ -383,11 +383,15 @@ __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_ke
 // ------------------------------------------------------------------------------- many columns
 
 // 16 bytes a lane from memory to LDS, lane after lane from `to` on; complete after landed(). The compiler's own form made
-// every read of LDS after it wait for it, also reads of the buffer before.
+// every read of LDS after it wait for it, also reads of the buffer before. It writes m0, and says so: the compiler, which gives that
+// register to no value of its own, may set it for an instruction and use it again, and warns of the name in a list.
 typedef __attribute__((address_space(3))) uint16_t lds_u16;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_lds(const uint16_t *from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // 128 columns and a run of steps a workgroup, 32 columns a wave: the products of 32 keys (64 positions a step) with both parts of q
