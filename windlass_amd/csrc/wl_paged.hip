@@ -61,7 +61,7 @@ template <int HD, bool BOUNDS>
 __global__ __launch_bounds__(64) void paged_rows_kernel(StoreArgs A, PageItems U) {
   constexpr int NP = HD / 2, HS = 64 / NP, N = kPgRowHeads / HS;  // pairs, heads at once, and of a part one after the other
   __shared__ double theta[NP];
-  __shared__ uint16_t fresh[HS][HD];
+  __shared__ __attribute__((aligned(16))) uint16_t fresh[HS][HD];
   const int lane = threadIdx.x, x = lane % NP, sub = lane / NP, KH = A.p.KH;
   const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, half = A.e.n / 2;
   const PageEntry E = entry_of(U, row);
