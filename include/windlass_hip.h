@@ -505,9 +505,9 @@ int wl_paged_attention_dev(wl_ctx *ctx, const wl_pages *p, const wl_page_rows *r
  * `recent` last (its own among them), and of the others the `top` of largest score (of equals the lower): the largest, over
  * the query heads of the KV head, of the sum over channels of max(q lo, q hi) with the page's bounds lo and hi: no score
  * q k of the page is larger. Formed in double; a score that is infinite or NaN (as 0 times an infinite bound is) comes before
- * all others, and what has no page is not taken. d_blocks (or null) [rows][kv_heads][first + recent + top] receives the pages
- * taken (their numbers within the sequence, rising; -1 after the last). Scores below 0 and a negative scale change nothing in
- * the choice. */
+ * all others, and of these others what has no page is not taken (the first and last are named all the same). d_blocks (or
+ * null) [rows][kv_heads][first + recent + top] receives the pages taken (their numbers within the sequence, rising; -1 after
+ * the last). Scores below 0 and a negative scale change nothing in the choice. */
 typedef struct wl_sparse_opts {
   int32_t first, recent, top; /* recent >= 1 */
 } wl_sparse_opts;

@@ -7,7 +7,7 @@ namespace wl {
 
 typedef float sf4 __attribute__((ext_vector_type(4)));
 // A running maximum is raised only by scores more than 2^6 past it, so nearly never after a wave's first tile: the
-// exponentials reach 2^6, and 2^8 of them are fp16 parts (22 bits down to 2^-22 of the row's largest, 2^-33 of it below).
+// exponentials reach 2^6, and 2^8 of them are fp16 parts: 23 bits of what is 2^-10 or more, and off by 2^-33 at most below.
 constexpr float kSpUp = 0x1p8f, kSpPast = 6.f;
 // In the scores' units: finite where those are the smallest there are, so that a lane without a key yet keeps -inf as what
 // raises its maximum.

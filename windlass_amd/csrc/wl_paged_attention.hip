@@ -54,7 +54,8 @@ __device__ __forceinline__ void query_parts(float x, float f, _Float16 &hi, _Flo
 
 // Weights are exp2 of a score's difference from the column's maximum M, times 2^8: all that follows is by their sum. M is one of
 // the scores seen, and is raised only where a step's weights would pass 2^15 (fp16 parts end at 2^16) or a column has none yet, so
-// that no step looks for its maximum. The largest weighs 2^8 at least; two parts are 22 bits of a weight down to 2^-14, and 2^-25 below.
+// that no step looks for its maximum. The largest weighs 2^8 at least; two parts, the high one cut, are 22 bits of a weight down to
+// 2^-3, and off by 2^-25 at most below (half a step of the least fp16 numbers), 2^-33 of the largest.
 constexpr float kUp = 8.f, kFull = 0x1p15f;
 __device__ __forceinline__ float weight(float s, float M, float c2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s - M, c2, kUp)); }
 // Two weights as their fp16 parts: the high ones cut, the low ones what is left, rounded.
@@ -113,8 +114,8 @@ struct FewTile {
 
 // 16 columns and a run of tiles a workgroup: S^T = K Q^T of 32 positions by two products of 16 keys each per 32 channels and part of
 // q, the weights, O^T += V^T P^T by one product per 16 channels and part of the weights. A product of 16 columns is half empty with
-// the eight heads of 70B and no matter: keys and values pass once and memory bounds it (48 rows up to 9,001 of 70B 224-230 us, 5.7 TB/s,
-// what a large read reaches; matrix cores 7% busy, VALU 18%). So nothing is staged: a wave's loads are its operands, whole lines of
+// the eight heads of 70B and no matter: keys and values pass once and memory bounds it (48 rows up to 9,001 of 70B 224-230 us, 5.8 TB/s
+// of the 7.1 that a read can reach here; matrix cores 7% busy, VALU 18%). So nothing is staged: a wave's loads are its operands, whole lines of
 // pieces of 16 bytes, and its tiles go to no other wave. Small calls are a wave's tiles one after the other, about 1 us each.
 template <int HD, bool CHOSEN>
 __global__ __launch_bounds__(64 * kFewWaves, HD == 64 ? 4 : 3) void paged_few_kernel(PagePool P, PagedPlan U,
@@ -397,9 +398,10 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" :::
 // 128 columns and a run of steps a workgroup, 32 columns a wave: the products of 32 keys (64 positions a step) with both parts of q
 // from registers, and of 32 channels with both parts of the weights. The four waves share keys and values in LDS, where they lie
 // as in the page (a wave's 16-byte reads are whole lines: no bank conflicts), brought by direct loads a step ahead. Two workgroups
-// fit a CU (64 KB, 256 registers a lane), so that one wave's weights run beside the other's products. The SIMDs' issue bounds it:
-// prompts of 2,001, 2,001 and 667 rows (8B) take 436-447 us, 530 TFLOP/s of 4 HD flops a score and column (twice that in two
-// parts), matrix cores 41% and VALU 36% busy, waits 25% of the wave cycles.
+// fit a CU (64 KB, 256 registers a lane), so that one wave's weights run beside the other's products (64 rows of 70B on a prefix of
+// 8,192 are but one a CU: matrix cores 24% busy). The SIMDs' issue bounds it: prompts of 2,001, 2,001 and 667 rows (8B) take 436-447
+// us, 530 TFLOP/s of 4 HD flops a score and column (twice that in two parts), matrix cores 41% and VALU 36% busy, waits 25% of the
+// wave cycles.
 template <int HD>
 __global__ __launch_bounds__(64 * kManyWaves, 2) void paged_many_kernel(PagePool P, PagedPlan U, const float *__restrict__ q,
                                                                         int G, float scale, float *__restrict__ part,
@@ -809,7 +811,8 @@ static int many_per(int n0, int n, int64_t wgs) {
 
 // Whether a prefix is read once for all rows: where what its entries would read of it, a pass for each 16 of their columns, is more
 // than 2^18 positions of keys and values (in all KV heads); else the join that it needs costs more, and each entry reads it for
-// itself, from the caches after the first. At the border, in us, read once and by each entry: 8B, 16 rows on 2,048 19.2 and 16.9, on
+// itself, from the caches after the first (7 rows of 8B on 2,048: 72 MB asked of the L2, 17 MB not there, what all entries' pages
+// hold together). At the border, in us, read once and by each entry: 8B, 16 rows on 2,048 19.2 and 16.9, on
 // 4,096 20.8 and 28.1; 2 on 8,192 19.0 and 16.6, on 16,384 22.2 and 27.2; 64 on 512 24.4 and 19.7, on 1,024 26.4 and 33.0, but 110 on
 // 512 38.4 and 34.7, so 1,024 at least. Entries that fill the workgroups by themselves (four of 300 rows on 4,096: 243 and 204;
 // of 100 83 and 104) gain nothing.

@@ -36,7 +36,7 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 // A wave makes the scores of 16 pages: column l % 16 is a page, row l % 4 of four a head (past the group's last the last again),
 // and lane l has the channels l / 16 * HD / 4 on of both, so that its loads are whole. The rows come out in lanes l / 16; the
 // largest of a column is the page's score. The heads' halves lie in LDS in 64 bits: converting them in each wave took as long
-// as the products. 16 rows of 70B on up to 500 pages of 64 take 13.5 us: 33 MB of bounds, and 6.6 us of products after them.
+// as the products. 16 rows of 70B on up to 500 pages of 64 take 12.9 us: 33 MB of bounds, and 6.6 us of products after them.
 // Three waves a SIMD are named where the loops that follow a sum that is not finite would leave two.
 template <int HD, int NB>
 __global__ __launch_bounds__(256, HD == 64 ? 1 : NB == 2 ? 3 : 1) void paged_score_kernel(PagePool P, PageItems U, PageSelect S,
