@@ -69,3 +69,27 @@ def test_infinite_bounds(ctx, G, KH, HD, page, n):
                 want = blocks_by_maximum(q[t, g * G:(g + 1) * G], b[:, g], (n - T + t) // page, *opts)
                 want += [-1] * (sum(opts) - len(want))
                 assert taken[t, g].tolist() == want, (opts, t, g)
+
+
+@pytest.mark.parametrize("G,KH,HD", [(1, 1, 64), (8, 2, 128), (18, 1, 64)])
+def test_queries_that_are_infinite_or_nan(ctx, G, KH, HD):
+    """Of one head of a group, over finite bounds of both signs, of one sign and of zero, and over infinite ones."""
+    page, n, T = 16, 16 * 50 + 3, 5
+
+    def values(s, k, v):
+        k[5 * page:6 * page, :, 9] = np.abs(k[5 * page:6 * page, :, 9]) + 1  # lo above 0
+        k[7 * page:8 * page, :, 9] = 0
+        k[11 * page:12 * page, :, 9] = np.minimum(k[11 * page:12 * page, :, 9], 0)
+        k[11 * page, :, 9] = 0  # hi of 0
+        k[13 * page + 1, :, 9], k[17 * page + 1, :, 9], k[19 * page + 1, :, 30] = np.inf, -np.inf, -np.inf
+    pool = Pool(ctx, [n], KH, HD, page, bounds=True, values=values)
+    q = np.random.default_rng(HD).standard_normal((T, KH * G, HD)).astype(F32)
+    q[0, 0, 9], q[1, 0, 9], q[2, 0, 9] = np.inf, -np.inf, np.nan
+    q[3, :, 9], q[3, :, 30] = 3e38, 1e-45  # the largest and smallest numbers
+    b = pool.bounds_of(0, (n - 1) // page + 1)
+    for opts in ((0, 1, 4), (1, 2, 20)):
+        _, taken = pool.attend([0], [n - T], [T], q, sparse=opts)
+        for t in range(T):
+            for g in range(KH):
+                want = blocks_by_maximum(q[t, g * G:(g + 1) * G], b[:, g], (n - T + t) // page, *opts)
+                assert taken[t, g].tolist() == want + [-1] * (sum(opts) - len(want)), (opts, t, g)
